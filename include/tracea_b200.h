@@ -232,6 +232,77 @@ uint64_t tracea_gemm_prepack_b_bytes(TraceaTensorView b);
 TraceaStatus tracea_gemm_prepack_b(TraceaTensorView b, void *dst, uint64_t dst_bytes, int64_t packed_stride[2],
                                    void *stream);
 
+/* ---- 4-bit microscaled matrices (OCP MX: E2M1 elements, an E8M0 scale per 32 columns). No counterpart in the reference. -- */
+
+/* A rows x cols matrix in the 4-bit format, in device memory, 16-byte aligned. A row's columns are cut into blocks of 32; a block
+ * has one scale byte b, which stands for 2^(b - 127) (255: NaN, and so is the whole block), and 32 codes of 4 bits: sign, two
+ * exponent bits, one mantissa bit, i.e. 0, .5, 1, 1.5, 2, 3, 4, 6.
+ *   data    `rows` rows of 16 * ceil(cols / 32) bytes, the even column in a byte's low half; codes past `cols` are 0
+ *   scales  ceil(rows / 128) x ceil(cols / 128) tiles of 512 bytes: the byte of row r, block b is byte
+ *           16 * (r % 32) + 4 * (r % 128 / 32) + b % 4 of tile [r / 128][b / 4]; bytes of blocks past the last one are 0. Bytes of
+ *           rows past the last one may hold anything: no result depends on them, and entries that write a matrix may leave them.
+ * cols >= 1. Quantising a block with largest absolute value p (tracea_mx_quantize, and c_mx / y_mx below):
+ *   b = clamp(floor(log2 p) - 2, -127, 125) + 127,  code = v / 2^(b - 127) to the nearest, ties to even, at most 6 (p = 0: b = 0);
+ * a block with a NaN or an infinity becomes b = 255, codes 0. */
+typedef struct {
+  void *data;
+  void *scales;
+  uint64_t rows;
+  uint64_t cols;
+  int32_t device_id;
+} TraceaMxMatrix;
+
+/* Bytes of `data` and `scales` (0 when the extents are out of range). */
+uint64_t tracea_mx_data_bytes(uint64_t rows, uint64_t cols);
+uint64_t tracea_mx_scale_bytes(uint64_t rows, uint64_t cols);
+
+/* q = x in the 4-bit format / out = q's values. x and out: rank 2, FLOAT32, FLOAT16 or BFLOAT16, any strides, device memory. The
+ * values are exact in FLOAT32 and BFLOAT16; FLOAT16 rounds, and overflows to infinity. All bytes of q are written. */
+TraceaStatus tracea_mx_quantize(TraceaTensorView x, TraceaMxMatrix *q, void *stream);
+TraceaStatus tracea_mx_dequantize(TraceaMxMatrix q, TraceaTensorView *out, void *stream);
+
+/* c = epilogue(a w^T), a [M,K], w [N,K] (a Linear layer's weight as it lies), accumulated in fp32. Exactly one of c and c_mx is
+ * given: c [M,N] in FLOAT32, FLOAT16 or BFLOAT16 with contiguous columns and any row stride, rounded once; or c_mx, quantised from
+ * the fp32 results. Epilogue kinds, bias (fp32, or the dtype of c) and residual ([M,N], the dtype of c; not with c_mx) as
+ * tracea_gemm. The output may not overlap the inputs, except that c may be the residual. M = 0 is a no-op. */
+TraceaStatus tracea_mx_gemm(TraceaMxMatrix a, TraceaMxMatrix w, const TraceaTensorView *bias, const TraceaTensorView *residual,
+                            TraceaTensorView *c, TraceaMxMatrix *c_mx, TraceaGemmParams params);
+
+/* The same for an input that is not quantised yet: x [M,K] of any strides, FLOAT32, FLOAT16 or BFLOAT16, is quantised inside the
+ * call, in scratch. The result is that of tracea_mx_quantize followed by tracea_mx_gemm, up to the order of summation. */
+TraceaStatus tracea_mx_linear(TraceaTensorView x, TraceaMxMatrix w, const TraceaTensorView *bias, const TraceaTensorView *residual,
+                              TraceaTensorView *c, TraceaMxMatrix *c_mx, TraceaGemmParams params);
+
+/* ---- norms before and after a block. No counterpart in the reference. ------------------------------------------------------ */
+typedef enum {
+  TRACEA_NORM_NONE = 0,  /* v */
+  TRACEA_NORM_RMS = 1,   /* v / sqrt(mean(v^2) + eps) */
+  TRACEA_NORM_LAYER = 2  /* (v - mean) / sqrt(mean((v - mean)^2) + eps) */
+} TraceaNormKind;
+
+/* norm(v) * weight + bias, then * (1 + scale) + shift. weight and bias: [C]; scale and shift: [G, C] with G dividing the rows, of
+ * which M / G consecutive ones share a row of these (an image's conditioning, say). Each NULL or FLOAT32 or the rows' dtype, with
+ * contiguous columns. */
+typedef struct {
+  TraceaNormKind kind;
+  float eps;             /* >= 0 */
+  const TraceaTensorView *weight;
+  const TraceaTensorView *bias;
+  const TraceaTensorView *scale;
+  const TraceaTensorView *shift;
+} TraceaNorm;
+
+/* y = norm(x), x [M,C] with contiguous columns and any row stride, C <= 16384, computed in fp32; into y (the dtype of x) or, one
+ * of the two, into y_mx. y may be x itself. */
+TraceaStatus tracea_block_norm(TraceaTensorView x, const TraceaNorm *norm, TraceaTensorView *y, TraceaMxMatrix *y_mx, void *stream);
+
+/* r = residual_scale * x + gate * norm(h): joins a block's output h to the stream x it started from. h, x, r: [M,C], one dtype;
+ * gate: [G,C] as scale above, or NULL. With `following`, y (or y_mx) = following(r), of r as it is stored, in the same pass.
+ * r may be x or h itself; otherwise outputs overlap nothing. */
+TraceaStatus tracea_block_norm_add(TraceaTensorView h, TraceaTensorView x, const TraceaNorm *norm, const TraceaTensorView *gate,
+                                   float residual_scale, TraceaTensorView *r, const TraceaNorm *following, TraceaTensorView *y,
+                                   TraceaMxMatrix *y_mx, void *stream);
+
 /* Thread-local last error text: tracea-ffi/src/lib.rs:87-109. Returns bytes copied (without the
  * terminating NUL), -1 when buf is NULL or len is 0. */
 int32_t tracea_get_last_error(uint8_t *buf, size_t len);
@@ -278,7 +349,8 @@ uint64_t tracea_b200_launch_count(void);
 /* The same count for one kind of kernel: 0 the general implicit-GEMM conv kernel, 1 its instantiations that cut tiles
  * over K, 2 the resident-filter kernel (stride-1 small filters over 64-channel activations), 3 layout adapters,
  * 4 the row-band kernel (few-channel 16-bit images such as the RGB stem), 5 the small-tile kernel (problems of up to one
- * wave of 64-row tiles); and 6, those of 0, 1 and 5 that read a copied input by whole filter rows instead of tap by tap.
+ * wave of 64-row tiles); and 6, those of 0, 1 and 5 that read a copied input by whole filter rows instead of tap by tap; 7
+ * conversions to and from the 4-bit format, 8 its matrix product, 9 the form of that for few rows, 10 norms.
  * Lets tests and benchmarks see which path a call took. 0 for any other `kind`. No counterpart in the reference. */
 uint64_t tracea_b200_launch_count_of(int32_t kind);
 

@@ -618,7 +618,7 @@ __device__ __noinline__ void sk_dump_partial(uint32_t taddr0, int chunks, float4
 
 // Lane 0 waits until `expected` other pieces have counted themselves done on cnt[1], then zeroes the tile's two
 // counters (every party has passed both by then). False when the wait gave up.
-__device__ __noinline__ bool sk_wait_partials(uint32_t* cnt, uint32_t expected, volatile uint32_t* abort_flag,
+inline __device__ __noinline__ bool sk_wait_partials(uint32_t* cnt, uint32_t expected, volatile uint32_t* abort_flag,
                                               long long limit_cycles, int lane) {
   bool all_in = true;
   if (lane == 0) {
@@ -643,7 +643,7 @@ __device__ __noinline__ bool sk_wait_partials(uint32_t* cnt, uint32_t expected, 
 // Two pieces (a split region of more than one wave never cuts a tile into more): own + other, which is the same
 // number whichever of the two does the adding. `src` is this lane's first float4 of the other piece's values; the
 // block of the next chunk is in flight while this chunk is added and written back.
-__device__ __noinline__ void sk_reduce_two(uint32_t taddr0, int chunks, const float4* src) {
+inline __device__ __noinline__ void sk_reduce_two(uint32_t taddr0, int chunks, const float4* src) {
   using namespace ptx;
   float4 nb[8];
 #pragma unroll
@@ -676,7 +676,7 @@ __device__ __noinline__ void sk_reduce_two(uint32_t taddr0, int chunks, const fl
 // pieces me+1 .. from scratch. `first` is the worker of piece 0, `warp_off` the lane's float4 offset inside a slot.
 // (One block of 32 columns is fetched while the previous one is added; layers with fewer tiles than SMs, whose
 // tiles are cut into three or more pieces, come through here.)
-__device__ __noinline__ void sk_reduce_many(const ConvKernelArgs& a, uint32_t taddr0, int chunks, int first, int pieces,
+inline __device__ __noinline__ void sk_reduce_many(const ConvKernelArgs& a, uint32_t taddr0, int chunks, int first, int pieces,
                                             int me, long long warp_off) {
   using namespace ptx;
 #pragma unroll 1

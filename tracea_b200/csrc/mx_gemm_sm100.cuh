@@ -1,0 +1,420 @@
+// Matrix product of two operands in the 4-bit microscaled format (mx_format.cuh), out = epilogue(A W^T), on the block-scaled tensor
+// cores: TMA loads -> smem ring -> tcgen05.cp of the scales into TMEM -> tcgen05.mma kind::mxf4 -> TMEM -> fused epilogue.
+//
+// A k-step is 128 bytes of each row, 256 columns: four MMAs of 64, each with two scales a row. The scales of 128 rows x 4 blocks
+// lie in memory as the 512 bytes that tcgen05.cp spreads over 32 lanes x 4 columns (and repeats for the four lane quarters), so
+// a stage's scales are copied by the TMA unit beside its operands and never touched by a thread.
+//
+// What bounds it: an MMA of M rows x N columns takes N / 2 cycles whatever the format, and 4-bit operands bring four times as
+// many products a byte as 16-bit ones -- so a k-step takes as long as a 128-byte k-step of the 16-bit kernel, and the same tilings
+// are fed by the same bytes per cycle from L2 (all SMs together get about 87 B/cycle/SM).
+#pragma once
+#include "mx_format.cuh"
+
+namespace tb200 {
+
+enum : int { kMxStoreTma = 0, kMxStoreRows = 1, kMxStoreMx = 2 };
+
+constexpr int kMxMaxStages = 8;
+
+struct MxGemmArgs {
+  int M, N;
+  int k_iters;                 // ceil(K / 256)
+  int num_m_tiles, num_n_tiles;
+  int panel_width, panel_tiles;
+  int num_stages;
+  uint32_t idesc;
+  void* out;                   // kMxStoreRows, TMA stores go by their map; kMxStoreMx: the codes
+  long long out_stride;        // elements
+  int out_vec;                 // kMxStoreRows: bytes a lane may store at once
+  uint8_t* out_scales;         // kMxStoreMx
+  int out_blocks, out_k_tiles;
+  const void* bias;
+  int bias_is_f32;
+  const void* residual;        // same dtype as out
+  long long res_stride;
+  int res_vec;
+  int act;
+  uint32_t* status;
+  long long wait_limit;
+  int test_producer_stop;
+};
+
+// Bytes of a stage: rows of A, rows of W, scales of 128 rows of A, scales of the 128-row tiles that the columns touch.
+__host__ __device__ constexpr int mx_b_scale_tiles(int bn) { return bn <= 128 ? 1 : 2; }
+__host__ __device__ constexpr int mx_stage_bytes(int bn, bool pair) {
+  return kBlockM * kStageKBytes + (pair ? bn / 2 : bn) * kStageKBytes + (1 + mx_b_scale_tiles(bn)) * 2 * kMxTileBytes;
+}
+constexpr int kMxBarrierBytes = 256;
+__host__ __device__ constexpr int mx_smem_bytes(int bn, int stages, bool pair, int staging_depth) {
+  return 1024 + stages * mx_stage_bytes(bn, pair) + kNumEpilogueWarps * (staging_depth * kStagingBoxBytes + bn * 4) + kMxBarrierBytes;
+}
+
+// TMEM columns: two accumulators, then the scales of every stage (8 columns of A's, 8 per tile of W's). A stage's columns are
+// rewritten when its shared memory is, which the stage's empty barrier orders behind the MMAs that read them.
+__host__ __device__ constexpr int mx_scale_cols(int bn) { return 8 + 8 * mx_b_scale_tiles(bn); }
+
+template <typename OutT, int BN, bool kPair, int kStore>
+__global__ void __launch_bounds__(kNumThreads, 1)
+mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
+                     const __grid_constant__ CUtensorMap tmap_sa, const __grid_constant__ CUtensorMap tmap_sw,
+                     const __grid_constant__ CUtensorMap tmap_out, const __grid_constant__ MxGemmArgs args) {
+  using namespace ptx;
+  constexpr uint32_t kABytes = kBlockM * kStageKBytes;
+  constexpr uint32_t kBRows = kPair ? BN / 2 : BN;
+  constexpr uint32_t kBBytes = kBRows * kStageKBytes;
+  constexpr uint32_t kBTiles = mx_b_scale_tiles(BN);
+  constexpr uint32_t kSaOff = kABytes + kBBytes, kSbOff = kSaOff + 2 * kMxTileBytes;
+  constexpr uint32_t kStageBytes = mx_stage_bytes(BN, kPair);
+  constexpr int kTileM = kPair ? 2 * kBlockM : kBlockM;
+  constexpr uint32_t kScaleCols = mx_scale_cols(BN);
+  constexpr int kStagingDepth = kStore == kMxStoreTma ? 2 : (kStore == kMxStoreRows ? 1 : 0);
+  static_assert(BN % 64 == 0 && BN <= 192 && kStageBytes % 1024 == 0, "tile");
+  static_assert(2 * BN + kMxMaxStages * kScaleCols <= 512 || BN == 192, "TMEM columns (192: the host keeps to five stages)");
+  constexpr uint32_t kTmemCols = 512;
+  const uint32_t cta_rank = kPair ? __shfl_sync(0xffffffffu, cluster_ctarank(), 0) : 0u;
+  const bool leader = cta_rank == 0u;
+  const int worker = kPair ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
+  const int num_workers = kPair ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
+  const int lane = threadIdx.x & 31;
+
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem_base = __shfl_sync(0xffffffffu, (smem_u32(smem_raw) + 1023u) & ~1023u, 0);
+  uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
+  const int num_stages = args.num_stages;
+  const uint32_t ring_bytes = static_cast<uint32_t>(num_stages) * kStageBytes;
+  const uint32_t staging_base = smem_base + ring_bytes;
+  const uint32_t bias_off = ring_bytes + kNumEpilogueWarps * kStagingDepth * kStagingBoxBytes;
+  const uint32_t bar_off = bias_off + kNumEpilogueWarps * BN * 4;
+  const uint32_t bar_base = smem_base + bar_off;
+  const uint32_t full_bar0 = bar_base, empty_bar0 = bar_base + 8u * kMxMaxStages;
+  auto tfull_bar = [&](int b) { return bar_base + 8u * (2 * kMxMaxStages + b); };
+  auto tempty_bar = [&](int b) { return bar_base + 8u * (2 * kMxMaxStages + 2 + b); };
+  constexpr uint32_t kNumBars = 2 * kMxMaxStages + 4;
+  const uint32_t tmem_slot = bar_base + 8u * kNumBars;
+  volatile uint32_t* tmem_slot_p = reinterpret_cast<volatile uint32_t*>(smem_gen + bar_off + 8u * kNumBars);
+  volatile uint32_t* abort_p = tmem_slot_p + 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < num_stages; ++s) {
+      mbar_init(full_bar0 + 8u * s, 1);
+      mbar_init(empty_bar0 + 8u * s, 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(tfull_bar(b), 1);
+      mbar_init(tempty_bar(b), kPair ? 8 : 4);   // the four warps of the group that drains it, in both CTAs of a pair
+    }
+    *abort_p = 0u;
+    fence_mbar_init();
+    prefetch_tmap(&tmap_a);
+    prefetch_tmap(&tmap_w);
+    prefetch_tmap(&tmap_sa);
+    prefetch_tmap(&tmap_sw);
+    if constexpr (kStore == kMxStoreTma) prefetch_tmap(&tmap_out);
+  }
+  if (warp == 1) {
+    if constexpr (kPair) {
+      tmem_alloc_pair<kTmemCols>(tmem_slot);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc<kTmemCols>(tmem_slot);
+      tmem_relinquish();
+    }
+  }
+  tc_fence_before();
+  if constexpr (kPair) cluster_sync();
+  else __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot_p, 0);
+  griddep_launch_dependents();
+  griddep_wait();
+
+  const int tiles = args.num_m_tiles * args.num_n_tiles;
+  const int k_iters = args.k_iters;
+  // panels of `panel_width` column tiles, row by row inside a panel: see the convolution's general kernel
+  auto tile_coords = [&](int tile, int& mt, int& nt) {
+    const int panel = tile / args.panel_tiles;
+    const int rem = tile - panel * args.panel_tiles;
+    const int n0 = panel * args.panel_width;
+    const int width = min(args.panel_width, args.num_n_tiles - n0);
+    mt = rem / width;
+    nt = n0 + rem - mt * width;
+  };
+  const uint32_t full_leader0 = kPair ? __shfl_sync(0xffffffffu, mapa_cluster(full_bar0, 0u), 0) : full_bar0;
+  const uint32_t ring_end = smem_base + ring_bytes;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer (uniform control flow, one lane issues)
+    const uint32_t issue = elect_one_lane();
+    uint32_t stage_addr = smem_base, full_addr = full_bar0, empty_addr = empty_bar0, phase = 0;
+    bool ok = true, stopped = false;
+    int issued = 0;
+    for (int tile = worker; ok && !stopped && tile < tiles; tile += num_workers) {
+      int mt, nt;
+      tile_coords(tile, mt, nt);
+      const int a_row = mt * kTileM + static_cast<int>(cta_rank) * kBlockM;
+      const int w_row = nt * BN + static_cast<int>(cta_rank * kBRows);
+      const int sa_tile = a_row / kMxTileRows, sw_tile = nt * BN / kMxTileRows;
+      for (int it = 0; it < k_iters; ++it) {
+        if (issued == args.test_producer_stop) {   // test hook: go silent, leave normally
+          stopped = true;
+          break;
+        }
+        if (!mbar_wait_bounded_uniform(empty_addr, phase ^ 1u, abort_p, args.wait_limit)) {
+          if (issue) report_error_status(args.status, abort_p, kErrProducerWait, static_cast<uint32_t>(it));
+          ok = false;
+          break;
+        }
+        const uint32_t full = full_leader0 + (full_addr - full_bar0);
+        if (leader) mbar_arrive_expect_tx_if(issue, full_addr, kPair ? 2u * kStageBytes : kStageBytes);
+        if constexpr (kPair) {
+          tma_load_2d_pair_if(issue, stage_addr, &tmap_a, full, it * kStageKBytes, a_row);
+          tma_load_2d_pair_if(issue, stage_addr + kABytes, &tmap_w, full, it * kStageKBytes, w_row);
+          tma_load_3d_pair_if(issue, stage_addr + kSaOff, &tmap_sa, full, 0, 2 * it, sa_tile);
+          tma_load_3d_pair_if(issue, stage_addr + kSbOff, &tmap_sw, full, 0, 2 * it, sw_tile);
+        } else {
+          tma_load_2d_if(issue, stage_addr, &tmap_a, full, it * kStageKBytes, a_row);
+          tma_load_2d_if(issue, stage_addr + kABytes, &tmap_w, full, it * kStageKBytes, w_row);
+          tma_load_3d_if(issue, stage_addr + kSaOff, &tmap_sa, full, 0, 2 * it, sa_tile);
+          tma_load_3d_if(issue, stage_addr + kSbOff, &tmap_sw, full, 0, 2 * it, sw_tile);
+        }
+        ++issued;
+        stage_addr += kStageBytes; full_addr += 8u; empty_addr += 8u;
+        if (stage_addr == ring_end) { stage_addr = smem_base; full_addr = full_bar0; empty_addr = empty_bar0; phase ^= 1u; }
+      }
+    }
+    // never leave with copies in flight into this CTA's shared memory
+    if (ok) {
+      const int pending = issued < num_stages ? issued : num_stages;
+      if (issued < num_stages) { stage_addr = smem_base; empty_addr = empty_bar0; phase = 1u; }   // the oldest filled stage; its first release has parity 0
+      for (int i = 0; i < pending; ++i) {
+        if (!mbar_wait_bounded_uniform(empty_addr, phase ^ 1u, abort_p, args.wait_limit)) break;
+        stage_addr += kStageBytes; empty_addr += 8u;
+        if (stage_addr == ring_end) { stage_addr = smem_base; empty_addr = empty_bar0; phase ^= 1u; }
+      }
+    } else {
+      const long long t0 = clock64();
+      while (clock64() - t0 < 2000000LL) { __nanosleep(1000); }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer (uniform control flow, one lane issues)
+    if (leader) {
+      const uint32_t issue = elect_one_lane();
+      // operands: 128-byte swizzled rows, 8 rows to 1024 bytes; scales: 32 rows of 16 bytes, 8 rows to 128 bytes, not swizzled
+      constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+      constexpr uint32_t kScaleDescHi = (128u >> 4) | (1u << 14);
+      const uint32_t idesc0 = args.idesc, idesc2 = args.idesc | (2u << 4) | (2u << 29);   // scale words' lower and upper halves
+      const uint32_t base_units = smem_base >> 4;
+      constexpr uint32_t kStageUnits = kStageBytes >> 4;
+      const uint32_t scale_cols0 = tmem_base + 2u * BN;
+      int stage = 0, local = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      bool stage_ready = false;
+      for (int tile = worker; ok && tile < tiles; tile += num_workers, ++local) {
+        const int buf = local & 1;
+        if (!mbar_wait_bounded_uniform(tempty_bar(buf), ((local >> 1) & 1u) ^ 1u, abort_p, args.wait_limit)) {
+          if (issue) report_error_status(args.status, abort_p, kErrMmaWaitTmem, static_cast<uint32_t>(local));
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        int mt, nt;
+        tile_coords(tile, mt, nt);
+        const uint32_t sw_shift = static_cast<uint32_t>(nt * BN % kMxTileRows) / 32u;   // the tile may start inside a scale tile
+        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(buf) * BN;
+        for (int it = 0; it < k_iters; ++it) {
+          if (!stage_ready && !mbar_wait_bounded_uniform(full_bar0 + 8u * stage, phase, abort_p, args.wait_limit)) {
+            if (issue) report_error_status(args.status, abort_p, kErrMmaWaitFull, static_cast<uint32_t>(it));
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a = base_units + static_cast<uint32_t>(stage) * kStageUnits, b = a + (kABytes >> 4);
+          const uint32_t sa = a + (kSaOff >> 4), sb = a + (kSbOff >> 4);
+          const uint32_t ta = scale_cols0 + static_cast<uint32_t>(stage) * kScaleCols, tb = ta + 8u;
+          // [tile of rows][k tile] in shared memory -> [k tile][tile of rows] in tensor memory
+#pragma unroll
+          for (uint32_t k = 0; k < 2; ++k) {
+            tmem_cp_32x128b_if<kPair>(issue, ta + 4u * k, sa + k * (kMxTileBytes >> 4), kScaleDescHi);
+#pragma unroll
+            for (uint32_t r = 0; r < kBTiles; ++r)
+              tmem_cp_32x128b_if<kPair>(issue, tb + 4u * (k * kBTiles + r), sb + (2u * r + k) * (kMxTileBytes >> 4), kScaleDescHi);
+          }
+          const uint32_t empty = empty_bar0 + 8u * stage;
+          if (++stage == num_stages) { stage = 0; phase ^= 1u; }
+          const bool next = mx_mma_stage4_probe<kPair>(d_tmem, a, b, kDescHi, idesc0, idesc2, ta, ta + 4u, tb + sw_shift,
+                                                       tb + 4u * kBTiles + sw_shift, empty, full_bar0 + 8u * stage, phase,
+                                                       it > 0 ? 1u : 0u, issue);
+          stage_ready = __all_sync(0xffffffffu, next);
+        }
+        if (ok && issue) {
+          if constexpr (kPair) mma_commit_pair(tfull_bar(buf));
+          else mma_commit(tfull_bar(buf));
+        }
+        __syncwarp();
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue: two groups of four warps, alternate tiles
+    // (the last tile is shared: each group takes every second group of columns), a row a lane
+    const int ew = warp - 2, egroup = ew >> 2, quarter = warp & 3;
+    constexpr int kGroupCols = kStore == kMxStoreMx ? 64 : 128 / static_cast<int>(sizeof(OutT));
+    constexpr int kGroups = BN / kGroupCols;
+    constexpr int kLdPerGroup = kGroupCols / 32;
+    constexpr int kVec = 16 / sizeof(OutT);
+    constexpr int kChunksPerLd = 32 / kVec;
+    float* bias_w = reinterpret_cast<float*>(smem_gen + bias_off) + ew * BN;
+    const uint32_t bias_s = smem_base + bias_off + static_cast<uint32_t>(ew * BN) * 4u;
+    const uint32_t stg0 = staging_base + static_cast<uint32_t>(ew * kStagingDepth) * kStagingBoxBytes;
+    const uint32_t lane_row_off = static_cast<uint32_t>(lane) * 128u, lane_xor = static_cast<uint32_t>(lane) & 7u;
+    const OutT* res = static_cast<const OutT*>(args.residual);
+    const int my_tiles = worker < tiles ? (tiles - worker + num_workers - 1) / num_workers : 0;
+    uint32_t box = 0;
+    int bias_tile = -1;
+    bool ok = true;
+    for (int local = 0; ok && local < my_tiles; ++local) {
+      const bool shared = local == my_tiles - 1 && kGroups > 1;
+      if ((local & 1) != egroup && !shared) continue;
+      const int g_first = shared && (local & 1) != egroup ? 1 : 0, g_step = shared ? 2 : 1;
+      const int buf = local & 1;
+      int mt, nt;
+      tile_coords(worker + local * num_workers, mt, nt);
+      const int n_base = nt * BN;
+      const int m_row0 = mt * kTileM + static_cast<int>(cta_rank) * kBlockM + quarter * 32;
+      const int m = m_row0 + lane;
+      const bool row_ok = m < args.M;
+      if (nt != bias_tile) {
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < BN / 32; ++j) {
+          const int n = n_base + j * 32 + lane;
+          float b = 0.0f;
+          if (args.bias != nullptr && n < args.N)
+            b = args.bias_is_f32 ? ld_global_f32(static_cast<const float*>(args.bias) + n)
+                                 : OutTraits<OutT>::to_f(static_cast<const OutT*>(args.bias)[n]);
+          bias_w[j * 32 + lane] = b;
+        }
+        __syncwarp();
+        bias_tile = nt;
+      }
+      const bool ready = mbar_wait_bounded(tfull_bar(buf), (local >> 1) & 1u, abort_p, 2 * args.wait_limit);
+      if (!__all_sync(0xffffffffu, ready)) {
+        if (lane == 0) report_error_status(args.status, abort_p, kErrEpilogueWait, static_cast<uint32_t>(local));
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t taddr0 = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(buf) * BN;
+#pragma unroll 1
+      for (int g = g_first; g < kGroups; g += g_step) {
+        const int n0 = n_base + g * kGroupCols;
+        const bool live = n0 < args.N;
+        uint32_t v[kLdPerGroup][32];
+#pragma unroll
+        for (int h = 0; h < kLdPerGroup; ++h) tmem_ld_32x32(taddr0 + g * kGroupCols + h * 32, v[h]);
+        tmem_ld_wait();
+        if (g == kGroups - 1 && !shared) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (kPair) mbar_arrive_cluster(mapa_cluster(tempty_bar(buf), 0u));
+            else mbar_arrive(tempty_bar(buf));
+          }
+        }
+        if (!live) continue;
+        const uint32_t stg = stg0 + box * kStagingBoxBytes;
+        if constexpr (kStore == kMxStoreTma) {
+          if (lane == 0) bulk_wait_group_read<1>();   // this box's store, two groups ago, has been read out
+          __syncwarp();
+        }
+        if constexpr (kStore != kMxStoreMx) {
+          if (res != nullptr)
+            load_rows<OutT>(args.res_vec, stg, res + n0, static_cast<long long>(m) * args.res_stride, row_ok, args.N - n0, lane);
+        }
+        uint4 packed[8];
+        uint32_t scale_bytes = 0;
+#pragma unroll
+        for (int h = 0; h < kLdPerGroup; ++h) {
+          float f[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[h][j]);
+#pragma unroll
+          for (int j4 = 0; j4 < 8; ++j4) {
+            const float4 b4 = ld_shared_f4(bias_s + static_cast<uint32_t>(g * kGroupCols + h * 32 + j4 * 4) * 4u);
+            add2(f[j4 * 4 + 0], f[j4 * 4 + 1], b4.x, b4.y);
+            add2(f[j4 * 4 + 2], f[j4 * 4 + 3], b4.z, b4.w);
+          }
+          if constexpr (kStore == kMxStoreMx) {
+            apply_act32<true>(f, args.act);
+            // columns past N: their scales are whatever lies behind the last row of W, and may not reach the block's
+            if (n0 + h * 32 + 32 > args.N) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (n0 + h * 32 + j >= args.N) f[j] = 0.0f;
+            }
+            uint32_t byte;
+            packed[h] = mx_quantize32(f, byte);
+            scale_bytes |= byte << (8 * h);
+          } else {
+            if (res != nullptr) {
+#pragma unroll
+              for (int c = 0; c < kChunksPerLd; ++c) {
+                const uint32_t cc = static_cast<uint32_t>(h * kChunksPerLd + c);
+                add16<OutT>(f + c * kVec, ld_shared_v4(stg + lane_row_off + ((cc ^ lane_xor) << 4)));
+              }
+            }
+            if (args.act == kActRelu) {
+              finish32<OutT, true>(f, nullptr, false, packed + h * kChunksPerLd);
+            } else {
+              apply_act32<sizeof(OutT) == 2>(f, args.act);
+              finish32<OutT, false>(f, nullptr, false, packed + h * kChunksPerLd);
+            }
+          }
+        }
+        if constexpr (kStore == kMxStoreMx) {
+          // two blocks of this lane's row: up to 32 bytes of codes and half a word of scales
+          const int blk = n0 / kMxBlock;
+          if (row_ok) {
+            uint8_t* codes = static_cast<uint8_t*>(args.out) + static_cast<long long>(m) * (16LL * args.out_blocks) + 16LL * blk;
+            reinterpret_cast<uint4*>(codes)[0] = packed[0];
+            if (blk + 1 < args.out_blocks) reinterpret_cast<uint4*>(codes)[1] = packed[1];
+            uint8_t* sw = args.out_scales + mx_scale_word(m, blk >> 2, args.out_k_tiles) + (blk & 3);
+            // the last word is written whole: blocks past N are 0
+            if ((blk & 3) == 0 && blk + 2 >= args.out_blocks) *reinterpret_cast<uint32_t*>(sw) = scale_bytes;
+            else *reinterpret_cast<uint16_t*>(sw) = static_cast<uint16_t>(scale_bytes);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            st_shared_v4(stg + lane_row_off + ((static_cast<uint32_t>(c) ^ lane_xor) << 4), packed[c]);
+          if constexpr (kStore == kMxStoreTma) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&tmap_out, stg, n0, m_row0);
+              bulk_commit_group();
+            }
+            box ^= 1u;
+          } else {
+            store_rows<OutT>(args.out_vec, stg, static_cast<OutT*>(args.out) + n0, static_cast<long long>(m) * args.out_stride,
+                             row_ok, args.N - n0, lane);
+          }
+        }
+      }
+    }
+    if (kStore == kMxStoreTma && lane == 0) bulk_wait_group0();
+  }
+
+  tc_fence_before();
+  if constexpr (kPair) cluster_sync();
+  else __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    if constexpr (kPair) tmem_dealloc_pair<kTmemCols>(tmem_base);
+    else tmem_dealloc<kTmemCols>(tmem_base);
+  }
+}
+
+}  // namespace tb200

@@ -219,6 +219,15 @@ __device__ __forceinline__ void tma_load_3d_if(uint32_t issue, uint32_t dst, con
       : "memory");
 }
 // The same from either CTA of a pair, signalling the leader's barrier (a shared::cluster address).
+__device__ __forceinline__ void tma_load_2d_pair_if(uint32_t issue, uint32_t dst, const void* tmap, uint32_t bar, int c0, int c1) {
+  asm volatile(
+      "{\n"
+      ".reg .pred q;\n"
+      "setp.ne.b32 q, %5, 0;\n"
+      "@q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n"
+      "}\n" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(c0), "r"(c1), "r"(issue)
+      : "memory");
+}
 __device__ __forceinline__ void tma_load_3d_pair_if(uint32_t issue, uint32_t dst, const void* tmap, uint32_t bar, int c0, int c1,
                                                     int c2) {
   asm volatile(
@@ -596,6 +605,88 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
                    bar)
                : "memory");
+}
+
+// ------------------------------------------------------------------ block-scaled MMA (4-bit operands, a scale per 32 of K)
+// 32 rows of 16 bytes in shared memory -> 32 lanes x 4 columns of tensor memory, repeated for the four lane quarters (kPair: in
+// both CTAs, each from its own shared memory). Whole-warp code, predicated on `issue`; runs in order with the issuing thread's
+// later MMAs of the same cta_group. `desc_lo`, `desc_hi`: the shared memory descriptor.
+template <bool kPair>
+__device__ __forceinline__ void tmem_cp_32x128b_if(uint32_t issue, uint32_t taddr, uint32_t desc_lo, uint32_t desc_hi) {
+#define TB200_TMEM_CP(GROUP)                                                                  \
+  asm volatile(                                                                               \
+      "{\n"                                                                                   \
+      ".reg .pred q;\n"                                                                       \
+      ".reg .b64 d;\n"                                                                        \
+      "setp.ne.b32 q, %3, 0;\n"                                                               \
+      "mov.b64 d, {%1, %2};\n"                                                                \
+      "@q tcgen05.cp.cta_group::" GROUP ".32x128b.warpx4 [%0], d;\n"                          \
+      "}\n" ::"r"(taddr), "r"(desc_lo), "r"(desc_hi), "r"(issue)                              \
+      : "memory")
+  if constexpr (kPair) TB200_TMEM_CP("2");
+  else TB200_TMEM_CP("1");
+#undef TB200_TMEM_CP
+}
+
+// One 128-byte k-step of kind::mxf4 as a single block, after mma_stage4_probe: four MMAs of 64 columns of K, the operands' rows
+// 32 bytes further on each (`a`, `b`: descriptor low words of the first), the scales of MMAs 0, 1 in columns sa0 / sb0 and of 2, 3
+// in sa1 / sb1, in the lower (idesc0) and the upper (idesc2) half of their words.
+template <bool kPair>
+__device__ __forceinline__ bool mx_mma_stage4_probe(uint32_t tmem_d, uint32_t a, uint32_t b, uint32_t desc_hi, uint32_t idesc0,
+                                                    uint32_t idesc2, uint32_t sa0, uint32_t sa1, uint32_t sb0, uint32_t sb1,
+                                                    uint32_t empty_bar, uint32_t next_full_bar, uint32_t next_parity,
+                                                    uint32_t accumulate, uint32_t issue) {
+  uint32_t ready;
+#define TB200_MX_STAGE(GROUP, COMMIT)                                                                            \
+  asm volatile(                                                                                                  \
+      "{\n"                                                                                                      \
+      ".reg .pred pn, p0, p1, q;\n"                                                                              \
+      ".reg .b64 da, db;\n"                                                                                      \
+      ".reg .b32 a, b;\n"                                                                                        \
+      ".reg .b16 msk;\n"                                                                                         \
+      "mov.b16 msk, 3;\n"                                                                                        \
+      "mbarrier.test_wait.parity.shared::cta.b64 pn, [%12], %13;\n"                                              \
+      "setp.ne.b32 p0, %14, 0;\n"                                                                                \
+      "setp.eq.b32 p1, 0, 0;\n"                                                                                  \
+      "setp.ne.b32 q, %15, 0;\n"                                                                                 \
+      "mov.b64 da, {%2, %4};\n"                                                                                  \
+      "mov.b64 db, {%3, %4};\n"                                                                                  \
+      "@q tcgen05.mma.cta_group::" GROUP ".kind::mxf4.block_scale.scale_vec::2X [%1], da, db, %5, [%7], [%9], p0;\n"  \
+      "add.u32 a, %2, 2;\n"                                                                                      \
+      "add.u32 b, %3, 2;\n"                                                                                      \
+      "mov.b64 da, {a, %4};\n"                                                                                   \
+      "mov.b64 db, {b, %4};\n"                                                                                   \
+      "@q tcgen05.mma.cta_group::" GROUP ".kind::mxf4.block_scale.scale_vec::2X [%1], da, db, %6, [%7], [%9], p1;\n"  \
+      "add.u32 a, %2, 4;\n"                                                                                      \
+      "add.u32 b, %3, 4;\n"                                                                                      \
+      "mov.b64 da, {a, %4};\n"                                                                                   \
+      "mov.b64 db, {b, %4};\n"                                                                                   \
+      "@q tcgen05.mma.cta_group::" GROUP ".kind::mxf4.block_scale.scale_vec::2X [%1], da, db, %5, [%8], [%10], p1;\n" \
+      "add.u32 a, %2, 6;\n"                                                                                      \
+      "add.u32 b, %3, 6;\n"                                                                                      \
+      "mov.b64 da, {a, %4};\n"                                                                                   \
+      "mov.b64 db, {b, %4};\n"                                                                                   \
+      "@q tcgen05.mma.cta_group::" GROUP ".kind::mxf4.block_scale.scale_vec::2X [%1], da, db, %6, [%8], [%10], p1;\n" \
+      "@q tcgen05.commit.cta_group::" GROUP COMMIT                                                               \
+      "selp.u32 %0, 1, 0, pn;\n"                                                                                 \
+      "}\n"                                                                                                      \
+      : "=r"(ready)                                                                                              \
+      : "r"(tmem_d), "r"(a), "r"(b), "r"(desc_hi), "r"(idesc0), "r"(idesc2), "r"(sa0), "r"(sa1), "r"(sb0),       \
+        "r"(sb1), "r"(empty_bar), "r"(next_full_bar), "r"(next_parity), "r"(accumulate), "r"(issue)              \
+      : "memory")
+  if constexpr (kPair) {
+    TB200_MX_STAGE("2", ".mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%11], msk;\n");
+  } else {
+    TB200_MX_STAGE("1", ".mbarrier::arrive::one.shared::cluster.b64 [%11];\n");
+  }
+#undef TB200_MX_STAGE
+  return ready != 0;
+}
+// Instruction descriptor of kind::mxf4: E2M1 operands, K-major, power-of-two scales; accumulation is always in fp32.
+//   [4,6) B's scale half   [7,10) A format, [10,12) B format (1 = E2M1)   [17,23) N >> 3   [23] 1: E8M0 scales   [24,29) M >> 4
+//   [29,31) A's scale half
+__host__ __device__ constexpr uint32_t make_mx_idesc(uint32_t m, uint32_t n) {
+  return (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | ((m >> 4) << 24);
 }
 
 // 32 lanes x 32 consecutive 32-bit columns -> 32 registers per thread (thread i = lane i).

@@ -28,6 +28,8 @@ EXPORTED_SYMBOLS = (
     "tracea_b200_conv_transpose_plan",
     "tracea_gemm", "tracea_conv_transpose2d", "tracea_conv2d_prepack_bytes", "tracea_conv2d_prepack",
     "tracea_gemm_prepack_b_bytes", "tracea_gemm_prepack_b",
+    "tracea_mx_data_bytes", "tracea_mx_scale_bytes", "tracea_mx_quantize", "tracea_mx_dequantize", "tracea_mx_gemm",
+    "tracea_mx_linear", "tracea_block_norm", "tracea_block_norm_add",
 )
 
 
@@ -77,6 +79,21 @@ class ConvTranspose2dParams(ctypes.Structure):
         ("epilogue", ctypes.c_int),
         ("stream", ctypes.c_void_p),
     ]
+
+
+class MxMatrix(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("rows", ctypes.c_uint64), ("cols", ctypes.c_uint64),
+                ("device_id", ctypes.c_int32)]
+
+
+# TraceaNormKind
+NORM_NONE, NORM_RMS, NORM_LAYER = range(3)
+
+
+class Norm(ctypes.Structure):
+    _fields_ = [("kind", ctypes.c_int), ("eps", ctypes.c_float), ("weight", ctypes.POINTER(TensorView)),
+                ("bias", ctypes.POINTER(TensorView)), ("scale", ctypes.POINTER(TensorView)),
+                ("shift", ctypes.POINTER(TensorView))]
 
 
 class TraceaError(RuntimeError):
@@ -147,6 +164,19 @@ def load():
     lib.tracea_gemm_prepack_b.argtypes = [TensorView, ctypes.c_void_p, ctypes.c_uint64, ctypes.POINTER(ctypes.c_int64),
                                           ctypes.c_void_p]
     lib.tracea_gemm_prepack_b.restype = ctypes.c_int
+    pm, pn = ctypes.POINTER(MxMatrix), ctypes.POINTER(Norm)
+    for name in ("tracea_mx_data_bytes", "tracea_mx_scale_bytes"):
+        getattr(lib, name).argtypes = [ctypes.c_uint64, ctypes.c_uint64]
+        getattr(lib, name).restype = ctypes.c_uint64
+    lib.tracea_mx_quantize.argtypes = [TensorView, pm, ctypes.c_void_p]
+    lib.tracea_mx_dequantize.argtypes = [MxMatrix, pv, ctypes.c_void_p]
+    lib.tracea_mx_gemm.argtypes = [MxMatrix, MxMatrix, pv, pv, pv, pm, GemmParams]
+    lib.tracea_mx_linear.argtypes = [TensorView, MxMatrix, pv, pv, pv, pm, GemmParams]
+    lib.tracea_block_norm.argtypes = [TensorView, pn, pv, pm, ctypes.c_void_p]
+    lib.tracea_block_norm_add.argtypes = [TensorView, TensorView, pn, pv, ctypes.c_float, pv, pn, pv, pm, ctypes.c_void_p]
+    for name in ("tracea_mx_quantize", "tracea_mx_dequantize", "tracea_mx_gemm", "tracea_mx_linear", "tracea_block_norm",
+                 "tracea_block_norm_add"):
+        getattr(lib, name).restype = ctypes.c_int
     _lib = lib
     return lib
 
@@ -218,7 +248,7 @@ def conv_transpose2d_raw(x, w, bias, residual, out, stride=(1, 1), padding=(0, 0
 
 
 (KERNEL_GENERAL, KERNEL_SPLIT_K, KERNEL_RESIDENT_FILTER, KERNEL_LAYOUT, KERNEL_ROW_BAND,
- KERNEL_SMALL_TILE, FORM_FILTER_ROWS) = range(7)
+ KERNEL_SMALL_TILE, FORM_FILTER_ROWS, KERNEL_MX_COPY, KERNEL_MX_GEMM, KERNEL_MX_TOKENS, KERNEL_NORM) = range(11)
 
 
 def launch_count_of(kind):

@@ -232,6 +232,103 @@ def prepack_gemm_b(b):
     return torch.as_strided(buf, tuple(b.shape), (int(stride[0]), int(stride[1])))
 
 
+class MxTensor:
+    """A (rows, cols) matrix in the 4-bit microscaled format of include/tracea_b200.h (TraceaMxMatrix): ``data``, uint8 of shape
+    (rows, 16 * ceil(cols / 32)), and ``scales``, uint8 of shape (ceil(rows / 128), ceil(cols / 128), 512)."""
+
+    __slots__ = ("data", "scales", "shape")
+
+    def __init__(self, data, scales, shape):
+        self.data, self.scales, self.shape = data, scales, shape
+
+    @property
+    def device(self):
+        return self.data.device
+
+    def dequantize(self, dtype=torch.bfloat16):
+        return mx_dequantize(self, dtype)
+
+    def __repr__(self):
+        return "MxTensor(%d x %d, device=%s)" % (self.shape[0], self.shape[1], self.data.device)
+
+
+def mx_quantize(x):
+    """x (M, K), any strides -> MxTensor: blocks of 32 columns with a power-of-two scale and 4-bit elements, a quarter of the
+    memory of 16-bit values and a bit. The scale is the largest power of two whose quadruple does not pass the block's largest
+    value; elements are rounded to nearest, ties to even, and saturate at 6 scales. A block with a NaN or an infinity becomes
+    NaN."""
+    data, scales = _native().mx_quantize(x)
+    return MxTensor(data, scales, tuple(x.shape))
+
+
+def mx_dequantize(q, dtype=torch.bfloat16):
+    """The values of an MxTensor; exact in bfloat16 and float32."""
+    return _native().mx_dequantize(q.data, q.scales, q.shape[0], q.shape[1], _DTYPES.get(dtype, -1))
+
+
+def mx_gemm(a, w, bias=None, epilogue=None, residual=None, dtype=None, quantize=False):
+    """a (M, K) times the transpose of w (N, K) -> (M, N), with the epilogue of ``gemm``, on the block-scaled tensor cores.
+
+    w is an MxTensor, a Linear layer's weight as it lies; a is an MxTensor or a tensor that the call quantises first. The output
+    has ``dtype`` (default: the type of a, bfloat16 for an MxTensor), or with ``quantize`` is an MxTensor itself, quantised from
+    the fp32 results. ``bias`` (N): float32 or the output's type; ``residual`` (M, N): the output's type, not with ``quantize``."""
+    kind = parse_epilogue(epilogue, bias, residual)
+    if not isinstance(w, MxTensor):
+        raise TypeError("w must be an MxTensor")
+    n, k = w.shape
+    if len(a.shape) != 2:
+        raise ValueError("Expected a 2D tensor: a (M, K)")
+    m, k_a = a.shape
+    if k_a != k:
+        raise ValueError(f"Inner dimension mismatch: a({k_a}) vs w({k})")
+    if isinstance(a, MxTensor):
+        data, scales, out = a.data, a.scales, torch.bfloat16
+    else:
+        data, scales, out = a, None, a.dtype
+    if dtype is not None:
+        if quantize:
+            raise ValueError("either dtype or quantize")
+        out = dtype
+    r = _native().mx_gemm(data, scales, m, w.data, w.scales, n, k, bias, residual, kind, None if quantize else _DTYPES.get(out, -1))
+    return MxTensor(*r, (m, n)) if quantize else r
+
+
+_NORM_KINDS = {"none": ffi.NORM_NONE, "rms": ffi.NORM_RMS, "layer": ffi.NORM_LAYER}
+
+
+def _norm_kind(kind):
+    if kind not in _NORM_KINDS:
+        raise ValueError("Unknown norm: %s (supported: %s)" % (kind, ", ".join(_NORM_KINDS)))
+    return _NORM_KINDS[kind]
+
+
+def block_norm(x, weight=None, bias=None, scale=None, shift=None, kind="rms", eps=1e-6, quantize=False):
+    """The norm in front of a block: (norm(x) * weight + bias) * (1 + scale) + shift for x (M, C), in one pass.
+
+    kind "rms": v / sqrt(mean(v^2) + eps), "layer": (v - mean) / sqrt(var + eps), "none": v. weight, bias (C); scale, shift
+    (G, C) where G divides M: each row of them serves M / G consecutive rows of x, an image's positions for example. All float32
+    or x's type. Returns x's type, or with ``quantize`` an MxTensor for ``mx_gemm``."""
+    r = _native().block_norm(x, weight, bias, scale, shift, _norm_kind(kind), eps, quantize)
+    return MxTensor(*r, tuple(x.shape)) if quantize else r
+
+
+def block_norm_add(h, x, weight=None, bias=None, scale=None, shift=None, gate=None, residual_scale=1.0, kind="rms", eps=1e-6,
+                   following=None):
+    """The join behind a block: r = residual_scale * x + gate * block_norm(h, ...), h the block's output, x the stream it started
+    from, both (M, C) of one type; gate (G, C) as scale, or None. kind "none" joins h as it is.
+
+    following: the next block's norm, a dict of the keyword arguments of ``block_norm``; then (r, y) is returned, with
+    y = block_norm(r, **following) to the bit, from the same pass over the rows."""
+    if following is None:
+        return _native().block_norm_add(h, x, weight, bias, scale, shift, _norm_kind(kind), eps, gate, residual_scale, 0)
+    return _norm_add_following(h, x, (weight, bias, scale, shift, _norm_kind(kind), eps, gate, residual_scale), **following)
+
+
+def _norm_add_following(h, x, first, weight=None, bias=None, scale=None, shift=None, kind="rms", eps=1e-6, quantize=False):
+    r, y = _native().block_norm_add(h, x, *first, 2 if quantize else 1, weight, bias, scale, shift, _norm_kind(kind), eps)
+    return r, MxTensor(*y, tuple(x.shape)) if quantize else y
+
+
 class Context:
     """Stand-in for the reference's ``tracea.Context`` (src/interface/python.rs:367-462), Conv2d only.
     The reference builds an IR, generates CUDA text and compiles it here; this one forwards to the
