@@ -16,6 +16,9 @@ namespace tb200 {
 enum : int { kMxStoreTma = 0, kMxStoreRows = 1, kMxStoreMx = 2 };
 
 constexpr int kMxMaxStages = 8;
+// Warp 0 TMA, warp 1 MMA, warps 2..5 and 6..9 two epilogue groups, warp 10 TMA; pairs: warps 11 and 12 scales
+__host__ __device__ constexpr int mx_threads(bool pair) { return pair ? 416 : 352; }
+constexpr int kSecondProducer = 10, kScaleWarp = 11;
 
 struct MxGemmArgs {
   int M, N;
@@ -55,7 +58,7 @@ __host__ __device__ constexpr int mx_smem_bytes(int bn, int stages, bool pair, i
 __host__ __device__ constexpr int mx_scale_cols(int bn) { return 8 + 8 * mx_b_scale_tiles(bn); }
 
 template <typename OutT, int BN, bool kPair, int kStore>
-__global__ void __launch_bounds__(kNumThreads, 1)
+__global__ void __launch_bounds__(mx_threads(kPair), 1)
 mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
                      const __grid_constant__ CUtensorMap tmap_sa, const __grid_constant__ CUtensorMap tmap_sw,
                      const __grid_constant__ CUtensorMap tmap_out, const __grid_constant__ MxGemmArgs args) {
@@ -91,7 +94,8 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
   const uint32_t full_bar0 = bar_base, empty_bar0 = bar_base + 8u * kMxMaxStages;
   auto tfull_bar = [&](int b) { return bar_base + 8u * (2 * kMxMaxStages + b); };
   auto tempty_bar = [&](int b) { return bar_base + 8u * (2 * kMxMaxStages + 2 + b); };
-  constexpr uint32_t kNumBars = 2 * kMxMaxStages + 4;
+  const uint32_t scale_bar0 = bar_base + 8u * (2 * kMxMaxStages + 4);
+  constexpr uint32_t kNumBars = 3 * kMxMaxStages + 4;
   const uint32_t tmem_slot = bar_base + 8u * kNumBars;
   volatile uint32_t* tmem_slot_p = reinterpret_cast<volatile uint32_t*>(smem_gen + bar_off + 8u * kNumBars);
   volatile uint32_t* abort_p = tmem_slot_p + 1;
@@ -100,6 +104,7 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     for (int s = 0; s < num_stages; ++s) {
       mbar_init(full_bar0 + 8u * s, 1);
       mbar_init(empty_bar0 + 8u * s, 1);
+      mbar_init(scale_bar0 + 8u * s, 2);   // a commit per warp that copies scales
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(tfull_bar(b), 1);
@@ -144,8 +149,10 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
   const uint32_t full_leader0 = kPair ? __shfl_sync(0xffffffffu, mapa_cluster(full_bar0, 0u), 0) : full_bar0;
   const uint32_t ring_end = smem_base + ring_bytes;
 
-  if (warp == 0) {
-    // ------------------------------------------------------------ TMA producer (uniform control flow, one lane issues)
+  if (warp == 0 || warp == kSecondProducer) {
+    // ------------------------------------------------------------ TMA producers (uniform control flow, one lane issues)
+    // A warp needs ~140 cycles to issue a copy, whatever its size, and a stage has four: warp 0 brings A and its scales in, warp
+    // 10 W and its. Only warp 0 arms the stage's barrier; bytes may arrive on it before, its phase cannot end without that.
     const uint32_t issue = elect_one_lane();
     uint32_t stage_addr = smem_base, full_addr = full_bar0, empty_addr = empty_bar0, phase = 0;
     bool ok = true, stopped = false;
@@ -167,16 +174,20 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
           break;
         }
         const uint32_t full = full_leader0 + (full_addr - full_bar0);
-        if (leader) mbar_arrive_expect_tx_if(issue, full_addr, kPair ? 2u * kStageBytes : kStageBytes);
-        if constexpr (kPair) {
-          tma_load_2d_pair_if(issue, stage_addr, &tmap_a, full, it * kStageKBytes, a_row);
+        if (warp == 0) {
+          if (leader) mbar_arrive_expect_tx_if(issue, full_addr, kPair ? 2u * kStageBytes : kStageBytes);
+          if constexpr (kPair) {
+            tma_load_2d_pair_if(issue, stage_addr, &tmap_a, full, it * kStageKBytes, a_row);
+            tma_load_3d_pair_if(issue, stage_addr + kSaOff, &tmap_sa, full, 0, 2 * it, sa_tile);
+          } else {
+            tma_load_2d_if(issue, stage_addr, &tmap_a, full, it * kStageKBytes, a_row);
+            tma_load_3d_if(issue, stage_addr + kSaOff, &tmap_sa, full, 0, 2 * it, sa_tile);
+          }
+        } else if constexpr (kPair) {
           tma_load_2d_pair_if(issue, stage_addr + kABytes, &tmap_w, full, it * kStageKBytes, w_row);
-          tma_load_3d_pair_if(issue, stage_addr + kSaOff, &tmap_sa, full, 0, 2 * it, sa_tile);
           tma_load_3d_pair_if(issue, stage_addr + kSbOff, &tmap_sw, full, 0, 2 * it, sw_tile);
         } else {
-          tma_load_2d_if(issue, stage_addr, &tmap_a, full, it * kStageKBytes, a_row);
           tma_load_2d_if(issue, stage_addr + kABytes, &tmap_w, full, it * kStageKBytes, w_row);
-          tma_load_3d_if(issue, stage_addr + kSaOff, &tmap_sa, full, 0, 2 * it, sa_tile);
           tma_load_3d_if(issue, stage_addr + kSbOff, &tmap_sw, full, 0, 2 * it, sw_tile);
         }
         ++issued;
@@ -201,9 +212,8 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     // ------------------------------------------------------------ MMA issuer (uniform control flow, one lane issues)
     if (leader) {
       const uint32_t issue = elect_one_lane();
-      // operands: 128-byte swizzled rows, 8 rows to 1024 bytes; scales: 32 rows of 16 bytes, 8 rows to 128 bytes, not swizzled
+      // operands: 128-byte swizzled rows, 8 rows to 1024 bytes
       constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
-      constexpr uint32_t kScaleDescHi = (128u >> 4) | (1u << 14);
       const uint32_t idesc0 = args.idesc, idesc2 = args.idesc | (2u << 4) | (2u << 29);   // scale words' lower and upper halves
       const uint32_t base_units = smem_base >> 4;
       constexpr uint32_t kStageUnits = kStageBytes >> 4;
@@ -211,7 +221,24 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       int stage = 0, local = 0;
       uint32_t phase = 0;
       bool ok = true;
-      bool stage_ready = false;
+      bool ready = false;             // pairs: this stage's scales are known to be in place; else: the next stage's bytes are
+      bool scales_issued = false;     // not pairs: this stage's scales are on their way to tensor memory
+      const int my_steps = (worker < tiles ? (tiles - worker + num_workers - 1) / num_workers : 0) * k_iters;
+      int step = 0;
+      // not pairs: the copies of a stage's scales. They run in order with this warp's MMAs, so no wait lies between
+      auto copy_scales = [&](int s) {
+        constexpr uint32_t kScaleDescHi = (128u >> 4) | (1u << 14);   // 32 rows of 16 bytes, 8 rows to 128 bytes, not swizzled
+        const uint32_t src = base_units + static_cast<uint32_t>(s) * kStageUnits + (kSaOff >> 4);
+        const uint32_t dst = scale_cols0 + static_cast<uint32_t>(s) * kScaleCols;
+#pragma unroll
+        for (uint32_t k = 0; k < 2; ++k) {
+          tmem_cp_32x128b_if<kPair>(issue, dst + 4u * k, src + k * (kMxTileBytes >> 4), kScaleDescHi);
+#pragma unroll
+          for (uint32_t r = 0; r < kBTiles; ++r)
+            tmem_cp_32x128b_if<kPair>(issue, dst + 8u + 4u * (k * kBTiles + r), src + (2u + 2u * r + k) * (kMxTileBytes >> 4),
+                                      kScaleDescHi);
+        }
+      };
       for (int tile = worker; ok && tile < tiles; tile += num_workers, ++local) {
         const int buf = local & 1;
         if (!mbar_wait_bounded_uniform(tempty_bar(buf), ((local >> 1) & 1u) ^ 1u, abort_p, args.wait_limit)) {
@@ -224,36 +251,97 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
         tile_coords(tile, mt, nt);
         const uint32_t sw_shift = static_cast<uint32_t>(nt * BN % kMxTileRows) / 32u;   // the tile may start inside a scale tile
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(buf) * BN;
-        for (int it = 0; it < k_iters; ++it) {
-          if (!stage_ready && !mbar_wait_bounded_uniform(full_bar0 + 8u * stage, phase, abort_p, args.wait_limit)) {
-            if (issue) report_error_status(args.status, abort_p, kErrMmaWaitFull, static_cast<uint32_t>(it));
-            ok = false;
-            break;
-          }
-          tc_fence_after();
+        for (int it = 0; it < k_iters; ++it, ++step) {
           const uint32_t a = base_units + static_cast<uint32_t>(stage) * kStageUnits, b = a + (kABytes >> 4);
-          const uint32_t sa = a + (kSaOff >> 4), sb = a + (kSbOff >> 4);
           const uint32_t ta = scale_cols0 + static_cast<uint32_t>(stage) * kScaleCols, tb = ta + 8u;
-          // [tile of rows][k tile] in shared memory -> [k tile][tile of rows] in tensor memory
-#pragma unroll
-          for (uint32_t k = 0; k < 2; ++k) {
-            tmem_cp_32x128b_if<kPair>(issue, ta + 4u * k, sa + k * (kMxTileBytes >> 4), kScaleDescHi);
-#pragma unroll
-            for (uint32_t r = 0; r < kBTiles; ++r)
-              tmem_cp_32x128b_if<kPair>(issue, tb + 4u * (k * kBTiles + r), sb + (2u * r + k) * (kMxTileBytes >> 4), kScaleDescHi);
-          }
           const uint32_t empty = empty_bar0 + 8u * stage;
-          if (++stage == num_stages) { stage = 0; phase ^= 1u; }
-          const bool next = mx_mma_stage4_probe<kPair>(d_tmem, a, b, kDescHi, idesc0, idesc2, ta, ta + 4u, tb + sw_shift,
-                                                       tb + 4u * kBTiles + sw_shift, empty, full_bar0 + 8u * stage, phase,
-                                                       it > 0 ? 1u : 0u, issue);
-          stage_ready = __all_sync(0xffffffffu, next);
+          int next = stage + 1;
+          uint32_t next_phase = phase;
+          if (next == num_stages) { next = 0; next_phase ^= 1u; }
+          uint32_t probe_bar, probe_phase;
+          if constexpr (kPair) {
+            if (!ready && !mbar_wait_bounded_uniform(scale_bar0 + 8u * stage, phase, abort_p, args.wait_limit)) {
+              if (issue) report_error_status(args.status, abort_p, kErrMmaWaitFull, static_cast<uint32_t>(it));
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            probe_bar = scale_bar0 + 8u * next;
+            probe_phase = next_phase;
+          } else {
+            if (!scales_issued) {
+              if (!mbar_wait_bounded_uniform(full_bar0 + 8u * stage, phase, abort_p, args.wait_limit)) {
+                if (issue) report_error_status(args.status, abort_p, kErrMmaWaitFull, static_cast<uint32_t>(it));
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+              copy_scales(stage);
+            }
+            // the next stage's scales go ahead of this stage's MMAs where its bytes are known to have landed: copies right in
+            // front of the MMAs that read them hold the tensor pipe up
+            scales_issued = ready && step + 1 < my_steps;
+            if (scales_issued) {
+              tc_fence_after();
+              copy_scales(next);
+            }
+            int next2 = next + 1;
+            probe_phase = next_phase;
+            if (next2 == num_stages) { next2 = 0; probe_phase ^= 1u; }
+            probe_bar = full_bar0 + 8u * next2;
+          }
+          const bool landed = mx_mma_stage4_probe<kPair>(d_tmem, a, b, kDescHi, idesc0, idesc2, ta, ta + 4u, tb + sw_shift,
+                                                         tb + 4u * kBTiles + sw_shift, empty, probe_bar, probe_phase,
+                                                         it > 0 ? 1u : 0u, issue);
+          ready = __all_sync(0xffffffffu, landed);
+          stage = next;
+          phase = next_phase;
         }
         if (ok && issue) {
           if constexpr (kPair) mma_commit_pair(tfull_bar(buf));
           else mma_commit(tfull_bar(buf));
         }
         __syncwarp();
+      }
+    }
+  } else if (warp >= kScaleWarp) {
+    // ------------------------------------------------------------ scales: shared memory -> tensor memory (uniform, one lane issues)
+    // Warps of their own, each half of a stage's 256 columns: a copy takes ~50 cycles to issue, and with all of them in front of
+    // the MMAs in one warp a stage took 830 cycles against 520 without them. These wait for the stage's bytes, the MMA warp for
+    // the commits behind these copies. 8192^3: 279 us, 216 with one such warp, 213 with two.
+    if (leader) {
+      const uint32_t issue = elect_one_lane();
+      constexpr uint32_t kScaleDescHi = (128u >> 4) | (1u << 14);   // 32 rows of 16 bytes, 8 rows to 128 bytes, not swizzled
+      const uint32_t k = static_cast<uint32_t>(warp - kScaleWarp);
+      const uint32_t src0 = (smem_base + kSaOff + k * kMxTileBytes) >> 4, dst0 = tmem_base + 2u * BN;
+      uint32_t src = src0, dst = dst0;
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = worker; ok && tile < tiles; tile += num_workers) {
+        for (int it = 0; it < k_iters; ++it) {
+          if (!mbar_wait_bounded_uniform(full_bar0 + 8u * stage, phase, abort_p, args.wait_limit)) {
+            if (issue) report_error_status(args.status, abort_p, kErrMmaWaitFull, static_cast<uint32_t>(it));
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          // [tile of rows][k tile] in shared memory -> [k tile][tile of rows] in tensor memory
+          tmem_cp_32x128b_if<kPair>(issue, dst + 4u * k, src, kScaleDescHi);
+#pragma unroll
+          for (uint32_t r = 0; r < kBTiles; ++r)
+            tmem_cp_32x128b_if<kPair>(issue, dst + 8u + 4u * (k * kBTiles + r), src + (2u + 2u * r) * (kMxTileBytes >> 4),
+                                      kScaleDescHi);
+          tcgen05_commit_if<kPair>(issue, scale_bar0 + 8u * stage);
+          src += kStageBytes >> 4;
+          dst += kScaleCols;
+          if (++stage == num_stages) {
+            stage = 0;
+            phase ^= 1u;
+            src = src0;
+            dst = dst0;
+          }
+        }
       }
     }
   } else {

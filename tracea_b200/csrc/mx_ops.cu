@@ -291,7 +291,7 @@ void launch_mx_gemm(DeviceState& st, int dt, const Product& p, cudaStream_t stre
     }
   }
   const long long workers = std::min<long long>(m_tiles * n_tiles, kPair ? st.num_sms / 2 : st.num_sms);
-  launch(kern, grid_of(kPair ? 2 * workers : workers), tb200::kNumThreads, tb200::mx_smem_bytes(BN, stages, kPair, kDepth),
+  launch(kern, grid_of(kPair ? 2 * workers : workers), tb200::mx_threads(kPair), tb200::mx_smem_bytes(BN, stages, kPair, kDepth),
          kPair ? 2 : 1, kLaunchMxGemm, stream, ta, tw, tsa, tsw, to, g);
 }
 

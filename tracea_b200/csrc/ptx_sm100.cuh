@@ -628,6 +628,22 @@ __device__ __forceinline__ void tmem_cp_32x128b_if(uint32_t issue, uint32_t tadd
 #undef TB200_TMEM_CP
 }
 
+// Arrive on this CTA's `bar` once every tcgen05 operation the elected lane has issued so far is complete.
+template <bool kPair>
+__device__ __forceinline__ void tcgen05_commit_if(uint32_t issue, uint32_t bar) {
+#define TB200_COMMIT(GROUP)                                                                                       \
+  asm volatile(                                                                                                   \
+      "{\n"                                                                                                       \
+      ".reg .pred q;\n"                                                                                           \
+      "setp.ne.b32 q, %1, 0;\n"                                                                                   \
+      "@q tcgen05.commit.cta_group::" GROUP ".mbarrier::arrive::one.shared::cluster.b64 [%0];\n"                  \
+      "}\n" ::"r"(bar), "r"(issue)                                                                                \
+      : "memory")
+  if constexpr (kPair) TB200_COMMIT("2");
+  else TB200_COMMIT("1");
+#undef TB200_COMMIT
+}
+
 // One 128-byte k-step of kind::mxf4 as a single block, after mma_stage4_probe: four MMAs of 64 columns of K, the operands' rows
 // 32 bytes further on each (`a`, `b`: descriptor low words of the first), the scales of MMAs 0, 1 in columns sa0 / sb0 and of 2, 3
 // in sa1 / sb1, in the lower (idesc0) and the upper (idesc2) half of their words.
