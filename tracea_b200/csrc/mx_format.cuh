@@ -161,14 +161,14 @@ struct MxCopyArgs {
   long long row_stride, col_stride;   // of the matrix, in elements
   long long M;
   int K, blocks, k_tiles;
-  int vec;               // the matrix's rows can be read / written eight elements at a time
   int chunks;            // of 256 columns
 };
 
 constexpr int kMxCopyThreads = 256;
 
 // A warp takes 256 columns of four rows 32 apart, whose scales are 16 consecutive bytes a tile. One pass: bytes in and bytes out.
-template <typename T>
+// kVec: rows are read in 16-byte accesses, K a multiple of 8; the four rows' loads are in flight together.
+template <typename T, bool kVec>
 __global__ void __launch_bounds__(kMxCopyThreads)
 mx_quantize_kernel(const __grid_constant__ MxCopyArgs a) {
   ptx::griddep_launch_dependents();
@@ -181,28 +181,32 @@ mx_quantize_kernel(const __grid_constant__ MxCopyArgs a) {
   if (r0 - (r0 & 127) >= a.M) return;                    // warp-uniform
   const int col = chunk * 256 + lane * 8;
   const int count = min(8, a.K - col);
-  const T* src = static_cast<const T*>(a.src) + col * a.col_stride;
-  float v[4][8];
+  const T* src = static_cast<const T*>(a.src) + r0 * a.row_stride + col * a.col_stride;
+  uint4 raw[kVec ? 4 : 1][sizeof(T) / 2];
+  if constexpr (kVec) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const long long r = r0 + 32 * i;
-    if (a.vec && r < a.M && count == 8) load8<T>(src + r * a.row_stride, v[i]);
-    else load8_upto<T>(src + r * a.row_stride, a.col_stride, r < a.M ? count : 0, v[i]);
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int q = 0; q < static_cast<int>(sizeof(T) / 2); ++q)
+        raw[i][q] = r0 + 32 * i < a.M && count > 0 ? reinterpret_cast<const uint4*>(src + 32 * i * a.row_stride)[q]
+                                                   : make_uint4(0u, 0u, 0u, 0u);
   }
   uint32_t words[4];
+  uint8_t* dst = static_cast<uint8_t*>(a.dst) + r0 * (16LL * a.blocks) + (col >> 1);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const long long r = r0 + 32 * i;
-    const uint32_t codes = mx_quantize8(v[i], lane, words[i]);
-    if (r < a.M && (col >> 5) < a.blocks)
-      *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.dst) + r * (16LL * a.blocks) + (col >> 1)) = codes;
+    float v[8];
+    if constexpr (kVec) load8<T>(reinterpret_cast<const T*>(raw[i]), v);
+    else load8_upto<T>(src + 32 * i * a.row_stride, a.col_stride, r0 + 32 * i < a.M ? count : 0, v);
+    const uint32_t codes = mx_quantize8(v, lane, words[i]);
+    if (r0 + 32 * i < a.M && (col >> 5) < a.blocks) *reinterpret_cast<uint32_t*>(dst + 32 * i * (16LL * a.blocks)) = codes;
   }
   if ((lane & 15) == 0 && (col >> 7) < a.k_tiles)
     *reinterpret_cast<uint4*>(static_cast<uint8_t*>(a.scales) + mx_scale_word(r0, col >> 7, a.k_tiles)) =
         make_uint4(words[0], words[1], words[2], words[3]);
 }
 
-template <typename T>
+template <typename T, bool kVec>
 __global__ void __launch_bounds__(kMxCopyThreads)
 mx_dequantize_kernel(const __grid_constant__ MxCopyArgs a) {
   ptx::griddep_launch_dependents();
@@ -217,24 +221,22 @@ mx_dequantize_kernel(const __grid_constant__ MxCopyArgs a) {
   if (r0 >= a.M || count <= 0) return;
   const uint4 words = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.scales) + mx_scale_word(r0, col >> 7, a.k_tiles));
   const uint32_t word[4] = {words.x, words.y, words.z, words.w};
-  T* dst = static_cast<T*>(a.dst) + col * a.col_stride;
+  const uint8_t* src = static_cast<const uint8_t*>(a.src) + r0 * (16LL * a.blocks) + (col >> 1);
+  T* dst = static_cast<T*>(a.dst) + r0 * a.row_stride + col * a.col_stride;
   uint32_t codes[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const long long r = r0 + 32 * i;
-    codes[i] = r < a.M ? *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.src) + r * (16LL * a.blocks) + (col >> 1)) : 0u;
-  }
+  for (int i = 0; i < 4; ++i)
+    codes[i] = r0 + 32 * i < a.M ? *reinterpret_cast<const uint32_t*>(src + 32 * i * (16LL * a.blocks)) : 0u;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const long long r = r0 + 32 * i;
-    if (r >= a.M) break;
+    if (r0 + 32 * i >= a.M) break;
     const float s = mx_scale_value((word[i] >> (8 * ((col >> 5) & 3))) & 255u);
     float v[8];
     mx_unpack8(codes[i], v);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] *= s;
-    if (a.vec && count == 8) store8<T>(dst + r * a.row_stride, v);
-    else store8_upto<T>(dst + r * a.row_stride, a.col_stride, count, v);
+    if constexpr (kVec) store8<T>(dst + 32 * i * a.row_stride, v);
+    else store8_upto<T>(dst + 32 * i * a.row_stride, a.col_stride, count, v);
   }
 }
 

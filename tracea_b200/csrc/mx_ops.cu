@@ -137,7 +137,6 @@ tb200::MxCopyArgs copy_args(const Matrix& m, const Mx& q) {
   a.K = static_cast<int>(m.cols);
   a.blocks = static_cast<int>(q.blocks);
   a.k_tiles = static_cast<int>(q.k_tiles);
-  a.vec = rows_of_8(m) ? 1 : 0;
   a.chunks = static_cast<int>(ceil_div(m.cols, 256));
   return a;
 }
@@ -150,7 +149,9 @@ void quantize(const Matrix& x, const Mx& q, cudaStream_t stream) {
   a.src = x.ptr;
   a.dst = q.data;
   by_dtype(x.dtype, [&](auto tag) {
-    launch(tb200::mx_quantize_kernel<decltype(tag)>, copy_grid(a), tb200::kMxCopyThreads, 0, 1, kLaunchMxCopy, stream, a);
+    using T = decltype(tag);
+    launch(rows_of_8(x) && x.cols % 8 == 0 ? tb200::mx_quantize_kernel<T, true> : tb200::mx_quantize_kernel<T, false>, copy_grid(a),
+           tb200::kMxCopyThreads, 0, 1, kLaunchMxCopy, stream, a);
   });
 }
 
@@ -182,8 +183,9 @@ void mx_dequantize_checked(const TraceaMxMatrix& qv, const TraceaTensorView* out
   a.src = q.data;
   a.dst = out.ptr;
   by_dtype(out.dtype, [&](auto tag) {
-    launch(tb200::mx_dequantize_kernel<decltype(tag)>, copy_grid(a), tb200::kMxCopyThreads, 0, 1, kLaunchMxCopy,
-           static_cast<cudaStream_t>(stream), a);
+    using T = decltype(tag);
+    launch(rows_of_8(out) && out.cols % 8 == 0 ? tb200::mx_dequantize_kernel<T, true> : tb200::mx_dequantize_kernel<T, false>,
+           copy_grid(a), tb200::kMxCopyThreads, 0, 1, kLaunchMxCopy, static_cast<cudaStream_t>(stream), a);
   });
 }
 
@@ -454,31 +456,45 @@ tb200::NormStage load_stage(const TraceaNorm& n, int dev, long long C, TraceaDTy
   return s;
 }
 
+template <typename T, int kThreads, int kVecs, int kMode, bool kJoin, int kNext>
+void launch_norm_kernel(const tb200::BlockNormArgs& a, int num_sms, cudaStream_t stream) {
+  constexpr int kBlock = tb200::norm_block_threads(kThreads), kRows = kBlock / kThreads;
+  const long long blocks = std::min<long long>(ceil_div(a.M, kRows), static_cast<long long>(num_sms) * tb200::norm_blocks_per_sm(kThreads, kJoin));
+  launch(tb200::block_norm_kernel<T, kThreads, kVecs, kMode, kJoin, kNext>, static_cast<unsigned>(blocks), kBlock, 0, 1, kLaunchNorm,
+         stream, a);
+}
+
 template <typename T, int kThreads, int kVecs>
-void launch_norm_shape(const tb200::BlockNormArgs& a, bool join, int next, int num_sms, cudaStream_t stream) {
-  constexpr int kBlock = tb200::norm_block_threads(kThreads);
-  const long long rows = kBlock / kThreads;
-  const unsigned grid = static_cast<unsigned>(std::min<long long>(ceil_div(a.M, rows), static_cast<long long>(num_sms) * (2048 / kBlock)));
-  auto go = [&](auto kern) { launch(kern, grid, kBlock, 0, 1, kLaunchNorm, stream, a); };
+void launch_norm_shape(const tb200::BlockNormArgs& a, bool join, int next, bool vec, int num_sms, cudaStream_t stream) {
+  auto go = [&](auto joined, auto nexts) {
+    constexpr bool kJoin = decltype(joined)::value;
+    constexpr int kNext = decltype(nexts)::value;
+    constexpr int kOther = kNext == tb200::kNextMx ? tb200::kRowsSingle : tb200::kRowsSpread;
+    if (vec) launch_norm_kernel<T, kThreads, kVecs, tb200::kRowsVec, kJoin, kNext>(a, num_sms, stream);
+    else launch_norm_kernel<T, kThreads, kVecs, kOther, kJoin, kNext>(a, num_sms, stream);
+  };
+  using Rows = std::integral_constant<int, tb200::kNextRows>;
+  using Quantised = std::integral_constant<int, tb200::kNextMx>;
   if (!join) {
-    if (next == tb200::kNextRows) go(tb200::block_norm_kernel<T, kThreads, kVecs, false, tb200::kNextRows>);
-    else go(tb200::block_norm_kernel<T, kThreads, kVecs, false, tb200::kNextMx>);
+    if (next == tb200::kNextRows) go(std::false_type{}, Rows{});
+    else go(std::false_type{}, Quantised{});
   } else if (next == tb200::kNextNone) {
-    go(tb200::block_norm_kernel<T, kThreads, kVecs, true, tb200::kNextNone>);
+    go(std::true_type{}, std::integral_constant<int, tb200::kNextNone>{});
   } else if (next == tb200::kNextRows) {
-    go(tb200::block_norm_kernel<T, kThreads, kVecs, true, tb200::kNextRows>);
+    go(std::true_type{}, Rows{});
   } else {
-    go(tb200::block_norm_kernel<T, kThreads, kVecs, true, tb200::kNextMx>);
+    go(std::true_type{}, Quantised{});
   }
 }
 
 template <typename T>
-void launch_norm(const tb200::BlockNormArgs& a, bool join, int next, int num_sms, cudaStream_t stream) {
-  if (a.C <= 256) launch_norm_shape<T, 32, 1>(a, join, next, num_sms, stream);
-  else if (a.C <= 1024) launch_norm_shape<T, 32, 4>(a, join, next, num_sms, stream);
-  else if (a.C <= 2048) launch_norm_shape<T, 256, 1>(a, join, next, num_sms, stream);
-  else if (a.C <= 8192) launch_norm_shape<T, 256, 4>(a, join, next, num_sms, stream);
-  else launch_norm_shape<T, 512, 4>(a, join, next, num_sms, stream);
+void launch_norm(const tb200::BlockNormArgs& a, bool join, int next, bool vec, int num_sms, cudaStream_t stream) {
+  if (a.C <= 256) launch_norm_shape<T, 32, 1>(a, join, next, vec, num_sms, stream);
+  else if (a.C <= 1024) launch_norm_shape<T, 128, 1>(a, join, next, vec, num_sms, stream);
+  else if (a.C <= 2048) launch_norm_shape<T, 256, 1>(a, join, next, vec, num_sms, stream);
+  else if (a.C <= 4096) launch_norm_shape<T, 512, 1>(a, join, next, vec, num_sms, stream);
+  else if (a.C <= 8192) launch_norm_shape<T, 1024, 1>(a, join, next, vec, num_sms, stream);
+  else launch_norm_shape<T, 1024, 2>(a, join, next, vec, num_sms, stream);
 }
 
 // h == nullptr: the norm alone, of x. following == nullptr: the join alone.
@@ -545,11 +561,11 @@ void block_norm_checked(const TraceaTensorView* hv, const TraceaTensorView& xv, 
   a.M = M;
   a.C = static_cast<int>(C);
   a.rows_per_group = groups > 0 ? M / groups : 0;
-  a.vec = vec ? 1 : 0;
+  vec = vec && C % 8 == 0;
   DeviceGuard guard(dev);
   DeviceState& st = device_state(dev);
   by_dtype(x.dtype, [&](auto tag) {
-    launch_norm<decltype(tag)>(a, hv != nullptr, next, st.num_sms, static_cast<cudaStream_t>(stream));
+    launch_norm<decltype(tag)>(a, hv != nullptr, next, vec, st.num_sms, static_cast<cudaStream_t>(stream));
   });
 }
 
