@@ -8,9 +8,12 @@
 // Bound by memory: a row is read once into registers and everything is computed from there, in fp32. The second moment is taken
 // about the mean, in a pass of its own over the registers -- as mean(v^2) - mean^2 a row far from zero would lose it.
 //
-// A row belongs to a warp (up to 256 columns) or to a CTA whose threads hold eight columns each. The vectors per channel are as
-// many bytes as several rows: a CTA walks consecutive rows and keeps what they come to, v -> v * a + b, in registers until the
-// group of rows changes. It loads the next row before it works on this one.
+// A row belongs to a group of 32 to 512 threads with up to 32 columns each: what a thread does per row and not per column --
+// sums across threads, addresses, the loop -- is as many instructions as eight columns take (with eight a thread, 12544 x 1024
+// modulated took 16.0 us and was bound by issuing them). A CTA walks consecutive rows. The vectors per channel, as many bytes as
+// several rows, come to v -> v * a + b, which is kept in shared memory until the group of rows changes (up to 8192 columns).
+// Meanwhile rows are on their way: each thread copies its own columns to a ring in shared memory, several rows ahead, and needs
+// no barrier for them.
 #pragma once
 #include "mx_format.cuh"
 
@@ -24,7 +27,7 @@ struct NormVector {
   const void* ptr;
   long long group_stride;   // elements; 0 where there is one for all rows
   int f32;
-  int vec;                  // 16-byte loads of eight columns are aligned
+  int vec;                  // eight columns from a multiple of eight on are 16-byte aligned
 };
 struct NormStage {
   int kind;
@@ -39,7 +42,7 @@ struct BlockNormArgs {
   uint8_t* codes;           // the same in 4 bits
   uint8_t* scales;
   long long h_stride, x_stride, r_stride, y_stride;   // rows, in elements
-  long long M, rows_per_group;
+  int M, rows_per_group;
   int C, blocks, k_tiles;
   float residual_scale;
   NormVector gate;
@@ -52,28 +55,26 @@ enum : int { kRowsVec = 0, kRowsSingle = 1, kRowsSpread = 2 };
 
 template <typename T, int kMode, int kThreads>
 struct RowSlice {
-  uint4 raw[sizeof(T) / 2];           // kRowsVec: as loaded, so that the load can be far ahead of its use
-  float val[kMode == kRowsVec ? 1 : 8];
+  static constexpr int kBytes = 8 * sizeof(T);
   __device__ __forceinline__ static int col(int i, int t, int j) {
     return kMode == kRowsSpread ? (i * 8 + j) * kThreads + t : (i * kThreads + t) * 8 + j;
   }
-  __device__ __forceinline__ void load(const T* p, int i, int t, int C, bool live) {
-    if constexpr (kMode == kRowsVec) {
+  __device__ __forceinline__ static void load(const T* p, int i, int t, int C, float (&v)[8]) {
 #pragma unroll
-      for (int q = 0; q < static_cast<int>(sizeof(T) / 2); ++q)
-        raw[q] = live && col(i, t, 0) < C ? reinterpret_cast<const uint4*>(p + col(i, t, 0))[q] : make_uint4(0u, 0u, 0u, 0u);
-    } else {
+    for (int j = 0; j < 8; ++j) v[j] = col(i, t, j) < C ? OutTraits<T>::to_f(p[col(i, t, j)]) : 0.0f;
+  }
+  // kRowsVec: the same by way of shared memory; nothing is copied, and zeros are read, where there is no column or row.
+  __device__ __forceinline__ static void copy(uint32_t smem, const T* p, int i, int t, int C, bool live) {
+    if (live && col(i, t, 0) < C) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) val[j] = live && col(i, t, j) < C ? OutTraits<T>::to_f(p[col(i, t, j)]) : 0.0f;
+      for (int q = 0; q < kBytes / 16; ++q) ptx::cp_async_16(smem + 16 * q, reinterpret_cast<const uint4*>(p + col(i, t, 0)) + q);
     }
   }
-  __device__ __forceinline__ void get(float (&v)[8]) const {
-    if constexpr (kMode == kRowsVec) {
-      load8<T>(reinterpret_cast<const T*>(raw), v);
-    } else {
+  __device__ __forceinline__ static void copied(uint32_t smem, int i, int t, int C, float (&v)[8]) {
+    __align__(16) uint4 raw[kBytes / 16];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = val[j];
-    }
+    for (int q = 0; q < kBytes / 16; ++q) raw[q] = col(i, t, 0) < C ? ptx::ld_shared_v4(smem + 16 * q) : make_uint4(0u, 0u, 0u, 0u);
+    load8<T>(reinterpret_cast<const T*>(raw), v);
   }
   __device__ __forceinline__ static void store(T* p, int i, int t, int C, const float (&v)[8]) {
     if constexpr (kMode == kRowsVec) {
@@ -86,66 +87,54 @@ struct RowSlice {
   }
 };
 
-// Eight columns of a vector per channel (0 past C), or `missing` where there is none.
+// Eight columns of a vector per channel (undefined past C), or `missing` where there is none.
 template <typename T, int kMode, int kThreads>
-__device__ __forceinline__ void norm_vector8(const NormVector& p, float missing, long long group, int i, int t, int C, float (&v)[8]) {
-  if (p.ptr == nullptr) {
+__device__ __forceinline__ void norm_vector8(const NormVector& p, float missing, int group, int i, int t, int C, float (&v)[8]) {
+  using Slice = RowSlice<T, kMode, kThreads>;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = missing;
-    return;
-  }
+  for (int j = 0; j < 8; ++j) v[j] = missing;
+  if (p.ptr == nullptr) return;
   const long long at = group * p.group_stride;
-  using F = RowSlice<float, kMode, kThreads>;
-  if constexpr (kMode == kRowsVec) {
-    if (p.vec) {
-      if (p.f32) {
-        F s;
-        s.load(static_cast<const float*>(p.ptr) + at, i, t, C, true);
-        s.get(v);
-      } else {
-        RowSlice<T, kMode, kThreads> s;
-        s.load(static_cast<const T*>(p.ptr) + at, i, t, C, true);
-        s.get(v);
-      }
-      return;
+  if (kMode == kRowsVec && p.vec) {
+    if (Slice::col(i, t, 0) < C) {
+      if (p.f32) load8<float>(static_cast<const float*>(p.ptr) + at + Slice::col(i, t, 0), v);
+      else load8<T>(static_cast<const T*>(p.ptr) + at + Slice::col(i, t, 0), v);
     }
-  }
+  } else if (p.f32) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int c = F::col(i, t, j);
-    v[j] = c >= C ? 0.0f : (p.f32 ? static_cast<const float*>(p.ptr)[at + c] : OutTraits<T>::to_f(static_cast<const T*>(p.ptr)[at + c]));
+    for (int j = 0; j < 8; ++j)
+      if (Slice::col(i, t, j) < C) v[j] = static_cast<const float*>(p.ptr)[at + Slice::col(i, t, j)];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (Slice::col(i, t, j) < C) v[j] = OutTraits<T>::to_f(static_cast<const T*>(p.ptr)[at + Slice::col(i, t, j)]);
   }
 }
 
 // What a stage's vectors, and a join's gate, come to: v -> v * a + b.
 template <typename T, int kMode, int kThreads>
-__device__ __forceinline__ void affine8(const NormStage& s, const NormVector* gate, long long group, int i, int t, int C,
-                                        float (&a)[8], float (&b)[8]) {
-  float p[8];
-  norm_vector8<T, kMode, kThreads>(s.weight, 1.0f, group, i, t, C, a);
-  norm_vector8<T, kMode, kThreads>(s.bias, 0.0f, group, i, t, C, b);
-  if (s.scale.ptr != nullptr) {
-    norm_vector8<T, kMode, kThreads>(s.scale, 0.0f, group, i, t, C, p);
+__device__ __forceinline__ void norm_affine8(const NormStage& s, const NormVector* gate, int group, int i, int t, int C,
+                                             float (&a)[8], float (&b)[8]) {
+  float scale[8], shift[8], g[8];
+  norm_vector8<T, kMode, kThreads>(s.weight, 1.0f, 0, i, t, C, a);
+  norm_vector8<T, kMode, kThreads>(s.bias, 0.0f, 0, i, t, C, b);
+  norm_vector8<T, kMode, kThreads>(s.scale, 0.0f, group, i, t, C, scale);
+  norm_vector8<T, kMode, kThreads>(s.shift, 0.0f, group, i, t, C, shift);
+  if (gate != nullptr) norm_vector8<T, kMode, kThreads>(*gate, 1.0f, group, i, t, C, g);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      a[j] = fmaf(a[j], p[j], a[j]);
-      b[j] = fmaf(b[j], p[j], b[j]);
-    }
-  }
-  if (s.shift.ptr != nullptr) {
-    norm_vector8<T, kMode, kThreads>(s.shift, 0.0f, group, i, t, C, p);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) b[j] += p[j];
-  }
-  if (gate != nullptr && gate->ptr != nullptr) {
-    norm_vector8<T, kMode, kThreads>(*gate, 1.0f, group, i, t, C, p);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      a[j] *= p[j];
-      b[j] *= p[j];
+  for (int j = 0; j < 8; ++j) {
+    a[j] = fmaf(a[j], scale[j], a[j]);
+    b[j] = fmaf(b[j], scale[j], b[j]) + shift[j];
+    if (gate != nullptr) {
+      a[j] *= g[j];
+      b[j] *= g[j];
     }
   }
 }
+__device__ __forceinline__ bool has_shift(const NormStage& s) { return s.bias.ptr != nullptr || s.shift.ptr != nullptr; }
+
+// A CTA's rows are walked by groups of kThreads threads.
+__host__ __device__ constexpr int norm_block_threads(int row_threads) { return row_threads < 256 ? 256 : row_threads; }
 
 // The sum over the threads of a row, in every one of them, always in the same order. `slot` alternates between two buffers: the
 // barrier of one sum is behind every read of the sum before it.
@@ -154,22 +143,22 @@ __device__ __forceinline__ float row_sum(float v, float* smem, uint32_t& slot, i
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
   if constexpr (kThreads > 32) {
-    constexpr int kWarps = kThreads / 32;
-    float* s = smem + slot * 32;
+    constexpr int kWarps = kThreads / 32, kCtaWarps = norm_block_threads(kThreads) / 32;
+    float* s = smem + slot * 16;
     slot ^= 1u;
     if (lane == 0) s[warp] = v;
-    __syncthreads();
-    if constexpr (kWarps <= 8) {
-      float4 q[kWarps / 4];
-#pragma unroll
-      for (int i = 0; i < kWarps / 4; ++i) q[i] = reinterpret_cast<const float4*>(s)[i];
+    if constexpr (kWarps == kCtaWarps) __syncthreads();
+    else asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / kWarps), "n"(kThreads) : "memory");
+    s += warp / kWarps * kWarps;                 // the row's warps
+    if constexpr (kWarps == 2) {
+      v = s[0] + s[1];
+    } else {
       v = 0.0f;
 #pragma unroll
-      for (int i = 0; i < kWarps / 4; ++i) v += (q[i].x + q[i].y) + (q[i].z + q[i].w);
-    } else {
-      v = lane < kWarps ? s[lane] : 0.0f;
-#pragma unroll
-      for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+      for (int i = 0; i < kWarps / 4; ++i) {
+        const float4 q = reinterpret_cast<const float4*>(s)[i];
+        v += (q.x + q.y) + (q.z + q.w);
+      }
     }
   }
   return v;
@@ -177,126 +166,248 @@ __device__ __forceinline__ float row_sum(float v, float* smem, uint32_t& slot, i
 
 // v, the row with zeros past column C, becomes norm(v); columns past C are undefined.
 template <int kMode, int kThreads, int kVecs>
-__device__ __forceinline__ void norm_row(const NormStage& s, float (&v)[kVecs][8], int C, int t, float* smem, uint32_t& slot,
-                                         int lane, int warp) {
+__device__ __forceinline__ void norm_row(const NormStage& s, float (&v)[kVecs][8], int C, float inv_C, int t, float* smem,
+                                         uint32_t& slot, int lane, int warp) {
+  using Slice = RowSlice<float, kMode, kThreads>;
   if (s.kind == kNormNone) return;
-  float mean = 0.0f;
   if (s.kind == kNormLayer) {
-    float sum = 0.0f;
+    float a = 0.0f, b = 0.0f;
 #pragma unroll
     for (int i = 0; i < kVecs; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum += v[i][j];
-    mean = row_sum<kThreads>(sum, smem, slot, lane, warp) / static_cast<float>(C);
+      for (int j = 0; j < 8; j += 2) add2(a, b, v[i][j], v[i][j + 1]);
+    const float mean = row_sum<kThreads>(a + b, smem, slot, lane, warp) * inv_C;
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        add2(v[i][j], v[i][j + 1], -mean, -mean);
+        if constexpr (kMode != kRowsVec) {
+          if (Slice::col(i, t, j) >= C) v[i][j] = 0.0f;
+          if (Slice::col(i, t, j + 1) >= C) v[i][j + 1] = 0.0f;
+        } else if (Slice::col(i, t, 0) >= C) {
+          v[i][j] = v[i][j + 1] = 0.0f;
+        }
+      }
   }
-  float sq = 0.0f;
+  float a = 0.0f, b = 0.0f;
 #pragma unroll
   for (int i = 0; i < kVecs; ++i)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      v[i][j] -= mean;
-      if (RowSlice<float, kMode, kThreads>::col(i, t, j) < C) sq = fmaf(v[i][j], v[i][j], sq);
+    for (int j = 0; j < 8; j += 2) {
+      float x = v[i][j], y = v[i][j + 1];
+      fma2(x, y, x, y, a, b);
+      a = x;
+      b = y;
     }
-  const float inv = rsqrtf(row_sum<kThreads>(sq, smem, slot, lane, warp) / static_cast<float>(C) + s.eps);
+  const float inv = rsqrtf(fmaf(row_sum<kThreads>(a + b, smem, slot, lane, warp), inv_C, s.eps));
 #pragma unroll
   for (int i = 0; i < kVecs; ++i)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[i][j] *= inv;
+    for (int j = 0; j < 8; j += 2) mul2(v[i][j], v[i][j + 1], inv, inv);
 }
 
-__host__ __device__ constexpr int norm_block_threads(int row_threads) { return row_threads == 32 ? 256 : row_threads; }
-// CTAs an SM is to hold: 1024 threads of up to 64 registers, joins, which keep more, 768 of up to 80 (512 of 128 where a CTA is as many).
-__host__ __device__ constexpr int norm_blocks_per_sm(int row_threads, bool join) {
-  return row_threads == 1024 ? 1 : (join ? 768 : 1024) / norm_block_threads(row_threads);
+// The CTA's copy of a stage's a, then its b: slice (i, t)'s eight values as two halves of four, the first halves of all slices in
+// front, so that neighbouring threads' accesses are neighbours.
+template <int kSlices>
+__device__ __forceinline__ void norm_keep(float* kept, int slice, const float (&a)[8], const float (&b)[8]) {
+  float4* k = reinterpret_cast<float4*>(kept) + slice;
+  k[0] = make_float4(a[0], a[1], a[2], a[3]);
+  k[kSlices] = make_float4(a[4], a[5], a[6], a[7]);
+  k[2 * kSlices] = make_float4(b[0], b[1], b[2], b[3]);
+  k[3 * kSlices] = make_float4(b[4], b[5], b[6], b[7]);
+}
+
+// v -> v * a + b, from the CTA's copy (kKeep) or from the vectors.
+template <typename T, int kMode, int kThreads, int kVecs, bool kKeep>
+__device__ __forceinline__ void norm_apply8(const NormStage& s, const NormVector* gate, const float* kept, int group, bool shift,
+                                            int i, int t, int C, float (&v)[8]) {
+  constexpr int kSlices = kThreads * kVecs;
+  float a[8], b[8];
+  if constexpr (kKeep) {
+    const float4* k = reinterpret_cast<const float4*>(kept) + (i * kThreads + t);
+    *reinterpret_cast<float4*>(a) = k[0];
+    *reinterpret_cast<float4*>(a + 4) = k[kSlices];
+    if (shift) {
+      *reinterpret_cast<float4*>(b) = k[2 * kSlices];
+      *reinterpret_cast<float4*>(b + 4) = k[3 * kSlices];
+    }
+  } else {
+    norm_affine8<T, kMode, kThreads>(s, gate, group, i, t, C, a, b);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    if (shift) fma2(v[j], v[j + 1], a[j], a[j + 1], b[j], b[j + 1]);
+    else mul2(v[j], v[j + 1], a[j], a[j + 1]);
+  }
+}
+
+// The shape of a launch: shared memory is the CTA's copy of up to two stages' vectors, then (kRowsVec) the ring of rows.
+__host__ __device__ constexpr bool norm_keeps(int threads, int vecs) { return threads * vecs * 8 <= 8192; }
+__host__ __device__ constexpr int norm_kept_bytes(int threads, int vecs, bool join, int next) {
+  return norm_keeps(threads, vecs) ? threads * vecs * 8 * 2 * 4 * ((join ? 1 : 0) + (next != kNextNone ? 1 : 0)) : 0;
+}
+__host__ __device__ constexpr int norm_row_bytes(int threads, int vecs, bool join, int es) {
+  return norm_block_threads(threads) * vecs * 8 * es * (join ? 2 : 1);
+}
+// CTAs an SM is to hold: 64 registers a thread, 128 for joins and for more than sixteen columns.
+__host__ __device__ constexpr int norm_blocks_per_sm(int threads, int vecs, bool join) {
+  return (vecs <= 2 && !join ? 1024 : 512) / norm_block_threads(threads);
+}
+// Rows ahead: what the CTA's share of 190 KB of shared memory holds, four at most.
+__host__ __device__ constexpr int norm_depth(int threads, int vecs, bool join, int next, int es) {
+  const int n = (190 * 1024 / norm_blocks_per_sm(threads, vecs, join) - norm_kept_bytes(threads, vecs, join, next)) /
+                norm_row_bytes(threads, vecs, join, es);
+  return n > 4 ? 4 : (n < 1 ? 1 : n);
+}
+__host__ __device__ constexpr int norm_smem_bytes(int threads, int vecs, int mode, bool join, int next, int es) {
+  return norm_kept_bytes(threads, vecs, join, next) +
+         (mode == kRowsVec ? norm_depth(threads, vecs, join, next, es) * norm_row_bytes(threads, vecs, join, es) : 0);
 }
 
 template <typename T, int kThreads, int kVecs, int kMode, bool kJoin, int kNext>
-__global__ void __launch_bounds__(norm_block_threads(kThreads), norm_blocks_per_sm(kThreads, kJoin))
+__global__ void __launch_bounds__(norm_block_threads(kThreads), norm_blocks_per_sm(kThreads, kVecs, kJoin))
 block_norm_kernel(const __grid_constant__ BlockNormArgs a) {
   static_assert(!(kMode == kRowsSpread && kNext == kNextMx), "a block of the format is four neighbouring threads' columns");
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();
-  __shared__ __align__(16) float smem[64];
+  extern __shared__ __align__(16) uint8_t dynamic[];
+  __shared__ __align__(16) float sums[32];
   using Slice = RowSlice<T, kMode, kThreads>;
-  constexpr int kRows = norm_block_threads(kThreads) / kThreads;        // that a CTA has in hand at a time
-  constexpr bool kKeep = kVecs == 1 && kThreads < 1024;                 // the vectors per channel stay in registers
+  constexpr int kBlock = norm_block_threads(kThreads);
+  constexpr int kRows = kBlock / kThreads;                              // that a CTA has in hand at a time
+  constexpr bool kKeep = norm_keeps(kThreads, kVecs);
+  constexpr int kSlices = kThreads * kVecs;                             // of eight columns
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int t = kThreads == 32 ? lane : static_cast<int>(threadIdx.x);
-  const long long workers = static_cast<long long>(gridDim.x) * kRows;
-  const long long worker = static_cast<long long>(blockIdx.x) * kRows + (kRows > 1 ? warp : 0);
-  long long row = worker * a.M / workers;
-  const long long end = (worker + 1) * a.M / workers;
-  if (row >= end) return;                                               // the same for all threads of a row
+  const int t = static_cast<int>(threadIdx.x) % kThreads, sub = static_cast<int>(threadIdx.x) / kThreads;
   const int C = a.C;
+  const float inv_C = 1.0f / static_cast<float>(C);
+  const bool join_shift = kJoin && has_shift(a.join), norm_shift = has_shift(a.norm);
+  float* kept_join = reinterpret_cast<float*>(dynamic);
+  float* kept_norm = kept_join + (kJoin ? 16 * kSlices : 0);
   uint32_t slot = 0;
-  Slice hs[kJoin ? kVecs : 1], xs[kVecs];
-  auto load = [&](long long at) {
-    const bool live = at < end;
-    if constexpr (kJoin) {
-      const T* h = static_cast<const T*>(a.h) + at * a.h_stride;
-#pragma unroll
-      for (int i = 0; i < kVecs; ++i) hs[i].load(h, i, t, C, live);
-    }
-    const T* x = static_cast<const T*>(a.x) + at * a.x_stride;
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i) xs[i].load(x, i, t, C, live);
-  };
-  load(row);
-  float ja[8], jb[8], na[8], nb[8];
-  long long group = -1, group_end = -1;
-  for (; row < end; ++row) {
-    if (row >= group_end) {
-      group = a.rows_per_group > 0 ? row / a.rows_per_group : 0;
-      group_end = a.rows_per_group > 0 ? (group + 1) * a.rows_per_group : a.M;
-      if constexpr (kKeep) {
-        if constexpr (kJoin) affine8<T, kMode, kThreads>(a.join, &a.gate, group, 0, t, C, ja, jb);
-        if constexpr (kNext != kNextNone) affine8<T, kMode, kThreads>(a.norm, nullptr, group, 0, t, C, na, nb);
-      }
-    }
-    float v[kVecs][8];
-    float xv[kVecs][8];
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-      xs[i].get(kJoin ? xv[i] : v[i]);
-      if constexpr (kJoin) hs[i].get(v[i]);
-    }
-    load(row + 1);
-    if constexpr (kJoin) {
-      norm_row<kMode, kThreads, kVecs>(a.join, v, C, t, smem, slot, lane, warp);
-      T* r = static_cast<T*>(a.r) + row * a.r_stride;
+
+  // kRowsVec: ring slots [row][matrix][i][thread]
+  constexpr int kDepth = norm_depth(kThreads, kVecs, kJoin, kNext, sizeof(T));
+  constexpr uint32_t kRowBytes = norm_row_bytes(kThreads, kVecs, kJoin, sizeof(T));
+  constexpr uint32_t kSliceBytes = kRowBytes / (kVecs * (kJoin ? 2 : 1));
+  const uint32_t ring0 = ptx::smem_u32(dynamic) + norm_kept_bytes(kThreads, kVecs, kJoin, kNext) + threadIdx.x * Slice::kBytes;
+  uint32_t ring_at = ring0;
+
+  const int first = static_cast<int>(static_cast<long long>(blockIdx.x) * a.M / gridDim.x);
+  const int last = static_cast<int>((static_cast<long long>(blockIdx.x) + 1) * a.M / gridDim.x);
+  for (int seg = first; seg < last;) {                                  // rows of one group
+    const int group = a.rows_per_group > 0 ? seg / a.rows_per_group : 0;
+    const int seg_end = a.rows_per_group > 0 ? min(last, (group + 1) * a.rows_per_group) : last;
+    int row = seg + sub;
+    seg = seg_end;
+    const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+    const T* h = static_cast<const T*>(a.h) + (kJoin ? row * a.h_stride : 0);
+    const long long x_step = kRows * a.x_stride, h_step = kRows * a.h_stride;
+    int ahead = row;                                                    // the next row to be asked for, where x and h point
+    auto request = [&]() {                                              // into the slot that has been read last
 #pragma unroll
       for (int i = 0; i < kVecs; ++i) {
-        if constexpr (!kKeep) affine8<T, kMode, kThreads>(a.join, &a.gate, group, i, t, C, ja, jb);
+        Slice::copy(ring_at + i * kSliceBytes, x, i, t, C, ahead < seg_end);
+        if constexpr (kJoin) Slice::copy(ring_at + (kVecs + i) * kSliceBytes, h, i, t, C, ahead < seg_end);
+      }
+      ptx::cp_async_commit();
+      ring_at = ring_at == ring0 + (kDepth - 1) * kRowBytes ? ring0 : ring_at + kRowBytes;
+      x += x_step;
+      if constexpr (kJoin) h += h_step;
+      ahead += kRows;
+    };
+    if constexpr (kMode == kRowsVec) {
+#pragma unroll 1
+      for (int d = 0; d < kDepth; ++d) request();
+    }
+    if constexpr (kKeep) {
+      // with one row in hand a thread reads only what it has written
+      if constexpr (kRows > 1) __syncthreads();                         // the segment before has read its copy
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          v[i][j] = OutTraits<T>::to_f(OutTraits<T>::from_f(fmaf(a.residual_scale, xv[i][j], fmaf(v[i][j], ja[j], jb[j]))));
-          if (Slice::col(i, t, j) >= C) v[i][j] = 0.0f;
+      for (int n = 0; n < (kSlices + kBlock - 1) / kBlock; ++n) {
+        const int slice = n * kBlock + static_cast<int>(threadIdx.x);
+        if (kSlices % kBlock == 0 || slice < kSlices) {
+          float p[8], q[8];
+          if constexpr (kJoin) {
+            norm_affine8<T, kMode, kThreads>(a.join, &a.gate, group, slice / kThreads, slice % kThreads, C, p, q);
+            norm_keep<kSlices>(kept_join, slice, p, q);
+          }
+          if constexpr (kNext != kNextNone) {
+            norm_affine8<T, kMode, kThreads>(a.norm, nullptr, group, slice / kThreads, slice % kThreads, C, p, q);
+            norm_keep<kSlices>(kept_norm, slice, p, q);
+          }
         }
-        Slice::store(r, i, t, C, v[i]);
       }
+      if constexpr (kRows > 1) __syncthreads();
     }
-    if constexpr (kNext != kNextNone) {
-      norm_row<kMode, kThreads, kVecs>(a.norm, v, C, t, smem, slot, lane, warp);
+    T* r = static_cast<T*>(a.r) + row * a.r_stride;
+    T* y = static_cast<T*>(a.y) + row * a.y_stride;
+    for (; row < seg_end; row += kRows) {
+      float v[kVecs][8];
+      float xv[kVecs][8];
+      if constexpr (kMode == kRowsVec) ptx::cp_async_wait<kDepth - 1>();
 #pragma unroll
       for (int i = 0; i < kVecs; ++i) {
-        if constexpr (!kKeep) affine8<T, kMode, kThreads>(a.norm, nullptr, group, i, t, C, na, nb);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = fmaf(v[i][j], na[j], nb[j]);
-        if constexpr (kNext == kNextRows) {
-          Slice::store(static_cast<T*>(a.y) + row * a.y_stride, i, t, C, v[i]);
+        float(&xd)[8] = kJoin ? xv[i] : v[i];
+        if constexpr (kMode == kRowsVec) {
+          Slice::copied(ring_at + i * kSliceBytes, i, t, C, xd);
+          if constexpr (kJoin) Slice::copied(ring_at + (kVecs + i) * kSliceBytes, i, t, C, v[i]);
         } else {
-          const int col = Slice::col(i, t, 0);
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (col + j >= C) v[i][j] = 0.0f;
-          uint32_t word;
-          const uint32_t codes = mx_quantize8(v[i], lane, word);     // the whole warp: blocks are shared by lanes
-          if ((col >> 5) < a.blocks) *reinterpret_cast<uint32_t*>(a.codes + row * (16LL * a.blocks) + (col >> 1)) = codes;
-          if ((lane & 15) == 0 && (col >> 7) < a.k_tiles)
-            *reinterpret_cast<uint32_t*>(a.scales + mx_scale_word(row, col >> 7, a.k_tiles)) = word;
+          Slice::load(x, i, t, C, xd);
+          if constexpr (kJoin) Slice::load(h, i, t, C, v[i]);
         }
       }
+      if constexpr (kMode == kRowsVec) {
+        request();
+      } else {
+        x += x_step;
+        if constexpr (kJoin) h += h_step;
+      }
+      if constexpr (kJoin) {
+        norm_row<kMode, kThreads, kVecs>(a.join, v, C, inv_C, t, sums, slot, lane, warp);
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) {
+          norm_apply8<T, kMode, kThreads, kVecs, kKeep>(a.join, &a.gate, kept_join, group, join_shift, i, t, C, v[i]);
+#pragma unroll
+          for (int j = 0; j < 8; j += 2) {
+            float p = xv[i][j], q = xv[i][j + 1];
+            fma2(p, q, a.residual_scale, a.residual_scale, v[i][j], v[i][j + 1]);
+            v[i][j] = p;
+            v[i][j + 1] = q;
+          }
+          Slice::store(r, i, t, C, v[i]);
+          if constexpr (kNext != kNextNone) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              v[i][j] = Slice::col(i, t, kMode == kRowsVec ? 0 : j) < C ? OutTraits<T>::to_f(OutTraits<T>::from_f(v[i][j])) : 0.0f;
+          }
+        }
+        r += kRows * a.r_stride;
+      }
+      if constexpr (kNext != kNextNone) {
+        norm_row<kMode, kThreads, kVecs>(a.norm, v, C, inv_C, t, sums, slot, lane, warp);
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) {
+          norm_apply8<T, kMode, kThreads, kVecs, kKeep>(a.norm, nullptr, kept_norm, group, norm_shift, i, t, C, v[i]);
+          if constexpr (kNext == kNextRows) {
+            Slice::store(y, i, t, C, v[i]);
+          } else {
+            const int col = Slice::col(i, t, 0);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (col + (kMode == kRowsVec ? 0 : j) >= C) v[i][j] = 0.0f;
+            uint32_t byte;
+            const uint32_t codes = mx_quantize8(v[i], byte);            // the whole warp: blocks are shared by lanes
+            if ((col >> 5) < a.blocks) *reinterpret_cast<uint32_t*>(a.codes + row * (16LL * a.blocks) + (col >> 1)) = codes;
+            if ((lane & 3) == 0 && (col >> 7) < a.k_tiles)
+              a.scales[mx_scale_word(row, col >> 7, a.k_tiles) + ((col >> 5) & 3)] = static_cast<uint8_t>(byte);
+          }
+        }
+        y += kRows * a.y_stride;
+      }
     }
+    if constexpr (kMode == kRowsVec) ptx::cp_async_wait<0>();
   }
 }
 

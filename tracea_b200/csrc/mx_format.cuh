@@ -77,40 +77,73 @@ __device__ __forceinline__ void mx_unpack8(uint32_t w, float* v) {
   }
 }
 
-__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+// max(|a|, |b|, |c|), NaN if one of them is.
+__device__ __forceinline__ float max_abs3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float max_abs8(const float* v) {
+  return max_abs3(max_abs3(max_abs3(v[0], v[1], v[2]), v[3], v[4]), max_abs3(v[5], v[6], v[7]), 0.0f);
+}
+// Packed pairs: (a, b) * (c, d) [+ (e, f)].
+__device__ __forceinline__ void mul2(float& a, float& b, float c, float d) {
+  asm("{\n"
+      ".reg .b64 x, y;\n"
+      "mov.b64 x, {%0, %1};\n"
+      "mov.b64 y, {%2, %3};\n"
+      "mul.rn.f32x2 x, x, y;\n"
+      "mov.b64 {%0, %1}, x;\n"
+      "}\n"
+      : "+f"(a), "+f"(b)
+      : "f"(c), "f"(d));
+}
+__device__ __forceinline__ void fma2(float& a, float& b, float c, float d, float e, float f) {
+  asm("{\n"
+      ".reg .b64 x, y, z;\n"
+      "mov.b64 x, {%0, %1};\n"
+      "mov.b64 y, {%2, %3};\n"
+      "mov.b64 z, {%4, %5};\n"
+      "fma.rn.f32x2 x, x, y, z;\n"
+      "mov.b64 {%0, %1}, x;\n"
+      "}\n"
+      : "+f"(a), "+f"(b)
+      : "f"(c), "f"(d), "f"(e), "f"(f));
+}
 
 // Quantises eight consecutive columns a lane, a block to four neighbouring lanes, all 32 lanes taking part: returns the lane's
-// codes; `scales` is, in every lane of a group of 16, the word of that group's four blocks.
-__device__ __forceinline__ uint32_t mx_quantize8(const float (&v)[8], int lane, uint32_t& scales) {
-  uint32_t peak = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) peak = max(peak, abs_bits(v[j]));
-  peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, 1));
-  peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
-  const uint32_t byte = mx_scale_byte(peak);
+// codes, and the block's scale byte in each of its four lanes.
+__device__ __forceinline__ uint32_t mx_quantize8(const float (&v)[8], uint32_t& byte) {
+  float peak = max_abs8(v);
+  peak = max_abs3(peak, __shfl_xor_sync(0xffffffffu, peak, 1), 0.0f);
+  peak = max_abs3(peak, __shfl_xor_sync(0xffffffffu, peak, 2), 0.0f);
+  byte = mx_scale_byte(__float_as_uint(peak));
   const float inv = mx_inverse(byte);
   float s[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) s[j] = v[j] * inv;
-  scales = byte << (8 * ((lane >> 2) & 3));
-  scales |= __shfl_xor_sync(0xffffffffu, scales, 4);
-  scales |= __shfl_xor_sync(0xffffffffu, scales, 8);
+  for (int j = 0; j < 8; j += 2) {
+    s[j] = v[j];
+    s[j + 1] = v[j + 1];
+    mul2(s[j], s[j + 1], inv, inv);
+  }
   return byte == 255u ? 0u : mx_pack8(s);
 }
 
 // 32 consecutive columns in one thread -> 16 bytes of codes and the scale byte.
 __device__ __forceinline__ uint4 mx_quantize32(const float (&v)[32], uint32_t& byte) {
-  uint32_t peak = 0;
-#pragma unroll
-  for (int j = 0; j < 32; ++j) peak = max(peak, abs_bits(v[j]));
-  byte = mx_scale_byte(peak);
+  const float peak = max_abs3(max_abs3(max_abs8(v), max_abs8(v + 8), max_abs8(v + 16)), max_abs8(v + 24), 0.0f);
+  byte = mx_scale_byte(__float_as_uint(peak));
   const float inv = mx_inverse(byte);
   uint32_t w[4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     float s[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s[j] = v[8 * q + j] * inv;
+    for (int j = 0; j < 8; j += 2) {
+      s[j] = v[8 * q + j];
+      s[j + 1] = v[8 * q + j + 1];
+      mul2(s[j], s[j + 1], inv, inv);
+    }
     w[q] = byte == 255u ? 0u : mx_pack8(s);
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
@@ -198,7 +231,10 @@ mx_quantize_kernel(const __grid_constant__ MxCopyArgs a) {
     float v[8];
     if constexpr (kVec) load8<T>(reinterpret_cast<const T*>(raw[i]), v);
     else load8_upto<T>(src + 32 * i * a.row_stride, a.col_stride, r0 + 32 * i < a.M ? count : 0, v);
-    const uint32_t codes = mx_quantize8(v, lane, words[i]);
+    const uint32_t codes = mx_quantize8(v, words[i]);
+    words[i] <<= 8 * ((lane >> 2) & 3);                  // the word of four blocks, of 16 lanes
+    words[i] |= __shfl_xor_sync(0xffffffffu, words[i], 4);
+    words[i] |= __shfl_xor_sync(0xffffffffu, words[i], 8);
     if (r0 + 32 * i < a.M && (col >> 5) < a.blocks) *reinterpret_cast<uint32_t*>(dst + 32 * i * (16LL * a.blocks)) = codes;
   }
   if ((lane & 15) == 0 && (col >> 7) < a.k_tiles)
