@@ -16,7 +16,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libtracea_b200.so")
 SOURCES = [os.path.join(CSRC, f) for f in ("tracea_ffi.cu", "mx_ops.cu", "block_norm.cu")]
-HEADERS = [os.path.join(CSRC, f) for f in ("conv2d_sm100.cuh", "conv2d_small_sm100.cuh", "conv2d_window_sm100.cuh", "conv2d_rowband_sm100.cuh", "ptx_sm100.cuh", "layout_kernels.cuh", "library_state.cuh", "mx_host.cuh", "mx_format.cuh", "mx_gemm_sm100.cuh", "block_norm_sm100.cuh")] + [
+HEADERS = [os.path.join(CSRC, f) for f in ("conv2d_sm100.cuh", "conv2d_small_sm100.cuh", "conv2d_window_sm100.cuh", "conv2d_rowband_sm100.cuh", "ptx_sm100.cuh", "layout_kernels.cuh", "library_state.cuh", "mx_host.cuh", "mx_format.cuh", "mx_gemm_sm100.cuh", "mx_tokens_sm100.cuh", "block_norm_sm100.cuh")] + [
     os.path.join(HERE, "..", "include", "tracea_b200.h")]
 
 NVCC_FLAGS = [

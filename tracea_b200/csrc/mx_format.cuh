@@ -149,6 +149,24 @@ __device__ __forceinline__ uint4 mx_quantize32(const float (&v)[32], uint32_t& b
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// The activations of apply_act32 on one value.
+template <bool kFast>
+__device__ __forceinline__ float apply_act(float v, int act) {
+  if (act == kActRelu) return fmaxf(0.0f, v);
+  if (act == kActSilu) {
+    if constexpr (kFast) return __fdividef(v, 1.0f + __expf(-v));
+    else return v / (1.0f + expf(-v));
+  }
+  if (act == kActGelu) {
+    const float u = 0.79788456f * (v + 0.044715f * v * v * v);
+    float t;
+    if constexpr (kFast) asm("tanh.approx.f32 %0, %1;" : "=f"(t) : "f"(u));
+    else t = tanhf(u);
+    return 0.5f * v * (1.0f + t);
+  }
+  return v;
+}
+
 // Eight consecutive elements as fp32: `p` at the first one, 16 (32 for fp32) aligned bytes, or element by element.
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {

@@ -49,11 +49,15 @@ __host__ __device__ constexpr int mx_stage_bytes(int bn, bool pair) {
   return kBlockM * kStageKBytes + (pair ? bn / 2 : bn) * kStageKBytes + (1 + mx_b_scale_tiles(bn)) * 2 * kMxTileBytes;
 }
 constexpr int kMxBarrierBytes = 256;
+// Boxes of 32 rows x 128 bytes for each epilogue warp. Stages are worth more than a second box where a tile is large.
+__host__ __device__ constexpr int mx_staging_depth(int bn, int store) { return store == kMxStoreMx ? 0 : (bn == 256 ? 1 : 2); }
 __host__ __device__ constexpr int mx_smem_bytes(int bn, int stages, bool pair, int staging_depth) {
   return 1024 + stages * mx_stage_bytes(bn, pair) + kNumEpilogueWarps * (staging_depth * kStagingBoxBytes + bn * 4) + kMxBarrierBytes;
 }
 
-// TMEM columns: two accumulators, then the scales of every stage (8 columns of A's, 8 per tile of W's). A stage's columns are
+// Tiles of 256 columns leave no room in TMEM for a second accumulator beside the scales.
+__host__ __device__ constexpr int mx_accumulators(int bn) { return bn == 256 ? 1 : 2; }
+// TMEM columns: one or two accumulators, then the scales of every stage (8 columns of A's, 8 per tile of W's). A stage's columns are
 // rewritten when its shared memory is, which the stage's empty barrier orders behind the MMAs that read them.
 __host__ __device__ constexpr int mx_scale_cols(int bn) { return 8 + 8 * mx_b_scale_tiles(bn); }
 
@@ -71,9 +75,9 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
   constexpr uint32_t kStageBytes = mx_stage_bytes(BN, kPair);
   constexpr int kTileM = kPair ? 2 * kBlockM : kBlockM;
   constexpr uint32_t kScaleCols = mx_scale_cols(BN);
-  constexpr int kStagingDepth = kStore == kMxStoreTma ? 2 : (kStore == kMxStoreRows ? 1 : 0);
-  static_assert(BN % 64 == 0 && BN <= 192 && kStageBytes % 1024 == 0, "tile");
-  static_assert(2 * BN + kMxMaxStages * kScaleCols <= 512 || BN == 192, "TMEM columns (192: the host keeps to five stages)");
+  constexpr int kStagingDepth = mx_staging_depth(BN, kStore);
+  static_assert(BN % 64 == 0 && BN <= 256 && kStageBytes % 1024 == 0, "tile");
+  constexpr int kAcc = mx_accumulators(BN);            // the host keeps to as many stages as TMEM has columns of scales for
   constexpr uint32_t kTmemCols = 512;
   const uint32_t cta_rank = kPair ? __shfl_sync(0xffffffffu, cluster_ctarank(), 0) : 0u;
   const bool leader = cta_rank == 0u;
@@ -108,7 +112,7 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(tfull_bar(b), 1);
-      mbar_init(tempty_bar(b), kPair ? 8 : 4);   // the four warps of the group that drains it, in both CTAs of a pair
+      mbar_init(tempty_bar(b), (kPair ? 8 : 4) * (kAcc == 1 ? 2 : 1));   // the warps that drain it, in both CTAs of a pair
     }
     *abort_p = 0u;
     fence_mbar_init();
@@ -217,7 +221,7 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       const uint32_t idesc0 = args.idesc, idesc2 = args.idesc | (2u << 4) | (2u << 29);   // scale words' lower and upper halves
       const uint32_t base_units = smem_base >> 4;
       constexpr uint32_t kStageUnits = kStageBytes >> 4;
-      const uint32_t scale_cols0 = tmem_base + 2u * BN;
+      const uint32_t scale_cols0 = tmem_base + kAcc * BN;
       int stage = 0, local = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -240,8 +244,9 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
         }
       };
       for (int tile = worker; ok && tile < tiles; tile += num_workers, ++local) {
-        const int buf = local & 1;
-        if (!mbar_wait_bounded_uniform(tempty_bar(buf), ((local >> 1) & 1u) ^ 1u, abort_p, args.wait_limit)) {
+        const int buf = kAcc == 2 ? local & 1 : 0;
+        const uint32_t use = static_cast<uint32_t>(kAcc == 2 ? local >> 1 : local);
+        if (!mbar_wait_bounded_uniform(tempty_bar(buf), (use & 1u) ^ 1u, abort_p, args.wait_limit)) {
           if (issue) report_error_status(args.status, abort_p, kErrMmaWaitTmem, static_cast<uint32_t>(local));
           ok = false;
           break;
@@ -313,7 +318,7 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       const uint32_t issue = elect_one_lane();
       constexpr uint32_t kScaleDescHi = (128u >> 4) | (1u << 14);   // 32 rows of 16 bytes, 8 rows to 128 bytes, not swizzled
       const uint32_t k = static_cast<uint32_t>(warp - kScaleWarp);
-      const uint32_t src0 = (smem_base + kSaOff + k * kMxTileBytes) >> 4, dst0 = tmem_base + 2u * BN;
+      const uint32_t src0 = (smem_base + kSaOff + k * kMxTileBytes) >> 4, dst0 = tmem_base + kAcc * BN;
       uint32_t src = src0, dst = dst0;
       int stage = 0;
       uint32_t phase = 0;
@@ -345,8 +350,9 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       }
     }
   } else {
-    // ------------------------------------------------------------ epilogue: two groups of four warps, alternate tiles
-    // (the last tile is shared: each group takes every second group of columns), a row a lane
+    // ------------------------------------------------------------ epilogue: two groups of four warps, a row a lane
+    // With two accumulators they take alternate tiles, and of the last one -- nothing overlaps it -- each every second group of
+    // columns; with one accumulator they share every tile in that way.
     const int ew = warp - 2, egroup = ew >> 2, quarter = warp & 3;
     constexpr int kGroupCols = kStore == kMxStoreMx ? 64 : 128 / static_cast<int>(sizeof(OutT));
     constexpr int kGroups = BN / kGroupCols;
@@ -363,10 +369,11 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     int bias_tile = -1;
     bool ok = true;
     for (int local = 0; ok && local < my_tiles; ++local) {
-      const bool shared = local == my_tiles - 1 && kGroups > 1;
+      const bool shared = kAcc == 1 || (local == my_tiles - 1 && kGroups > 1);
       if ((local & 1) != egroup && !shared) continue;
       const int g_first = shared && (local & 1) != egroup ? 1 : 0, g_step = shared ? 2 : 1;
-      const int buf = local & 1;
+      const int buf = kAcc == 2 ? local & 1 : 0;
+      const uint32_t use = static_cast<uint32_t>(kAcc == 2 ? local >> 1 : local);
       int mt, nt;
       tile_coords(worker + local * num_workers, mt, nt);
       const int n_base = nt * BN;
@@ -387,7 +394,19 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
         __syncwarp();
         bias_tile = nt;
       }
-      const bool ready = mbar_wait_bounded(tfull_bar(buf), (local >> 1) & 1u, abort_p, 2 * args.wait_limit);
+      // the residual of the first groups of columns, one a box, while the accumulator is being computed
+      int res_ahead = g_first;                     // the first group whose residual is not in its box
+      if (kStore != kMxStoreMx && res != nullptr) {
+        if (kStore == kMxStoreTma && lane == 0) bulk_wait_group_read<0>();
+        __syncwarp();
+        for (int d = 0; d < kStagingDepth && res_ahead < kGroups && n_base + res_ahead * kGroupCols < args.N; ++d) {
+          const int n0 = n_base + res_ahead * kGroupCols;
+          load_rows<OutT>(args.res_vec, stg0 + (kStagingDepth == 2 ? box ^ (d & 1u) : 0u) * kStagingBoxBytes, res + n0,
+                          static_cast<long long>(m) * args.res_stride, row_ok, args.N - n0, lane);
+          res_ahead += g_step;
+        }
+      }
+      const bool ready = mbar_wait_bounded(tfull_bar(buf), use & 1u, abort_p, 2 * args.wait_limit);
       if (!__all_sync(0xffffffffu, ready)) {
         if (lane == 0) report_error_status(args.status, abort_p, kErrEpilogueWait, static_cast<uint32_t>(local));
         ok = false;
@@ -403,7 +422,7 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
 #pragma unroll
         for (int h = 0; h < kLdPerGroup; ++h) tmem_ld_32x32(taddr0 + g * kGroupCols + h * 32, v[h]);
         tmem_ld_wait();
-        if (g == kGroups - 1 && !shared) {
+        if (kAcc == 1 ? g + 2 >= kGroups : g == kGroups - 1 && !shared) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) {
@@ -414,11 +433,11 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
         if (!live) continue;
         const uint32_t stg = stg0 + box * kStagingBoxBytes;
         if constexpr (kStore == kMxStoreTma) {
-          if (lane == 0) bulk_wait_group_read<1>();   // this box's store, two groups ago, has been read out
+          if (lane == 0) bulk_wait_group_read<kStagingDepth - 1>();   // this box's last store has been read out
           __syncwarp();
         }
         if constexpr (kStore != kMxStoreMx) {
-          if (res != nullptr)
+          if (res != nullptr && g >= res_ahead)
             load_rows<OutT>(args.res_vec, stg, res + n0, static_cast<long long>(m) * args.res_stride, row_ok, args.N - n0, lane);
         }
         uint4 packed[8];
@@ -484,10 +503,11 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
               tma_store_2d(&tmap_out, stg, n0, m_row0);
               bulk_commit_group();
             }
-            box ^= 1u;
+            if constexpr (kStagingDepth == 2) box ^= 1u;
           } else {
             store_rows<OutT>(args.out_vec, stg, static_cast<OutT*>(args.out) + n0, static_cast<long long>(m) * args.out_stride,
                              row_ok, args.N - n0, lane);
+            if constexpr (kStagingDepth == 2) box ^= 1u;
           }
         }
       }

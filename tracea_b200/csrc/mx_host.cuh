@@ -86,9 +86,9 @@ inline unsigned grid_of(long long blocks) {
 // Every kernel here is a programmatic launch: it may come up beside the one in front of it, and waits for that before it touches
 // global memory.
 template <typename Kernel, typename... Args>
-void launch(Kernel kern, unsigned grid, int threads, int smem, int cluster, int kind, cudaStream_t stream, const Args&... args) {
+void launch(Kernel kern, dim3 grid, int threads, int smem, int cluster, int kind, cudaStream_t stream, const Args&... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
+  cfg.gridDim = grid;
   cfg.blockDim = dim3(static_cast<unsigned>(threads));
   cfg.dynamicSmemBytes = static_cast<size_t>(smem);
   cfg.stream = stream;

@@ -2,6 +2,7 @@
 // reference has no counterpart of any of them.
 #include "mx_host.cuh"
 #include "mx_gemm_sm100.cuh"
+#include "mx_tokens_sm100.cuh"
 
 namespace {
 
@@ -106,7 +107,7 @@ struct Product {
   bool to_mx = false;
 };
 
-std::atomic<bool> g_mx_attr_set[kMaxDevices][3][3][3];
+std::atomic<bool> g_mx_attr_set[kMaxDevices][3][4][3];
 
 template <typename OutT, int BN, bool kPair, int kStore>
 void launch_mx_gemm(DeviceState& st, int dt, const Product& p, cudaStream_t stream) {
@@ -131,10 +132,10 @@ void launch_mx_gemm(DeviceState& st, int dt, const Product& p, cudaStream_t stre
   g.num_n_tiles = static_cast<int>(n_tiles);
   g.panel_width = static_cast<int>(panel);
   g.panel_tiles = static_cast<int>(m_tiles * panel);
-  constexpr int kDepth = kStore == tb200::kMxStoreTma ? 2 : (kStore == tb200::kMxStoreRows ? 1 : 0);
+  constexpr int kDepth = tb200::mx_staging_depth(BN, kStore);
   const int room = 232448 - tb200::mx_smem_bytes(BN, 0, kPair, kDepth);
   int stages = std::min(room / tb200::mx_stage_bytes(BN, kPair), tb200::kMxMaxStages);
-  stages = std::min(stages, (512 - 2 * BN) / tb200::mx_scale_cols(BN));
+  stages = std::min(stages, (512 - tb200::mx_accumulators(BN) * BN) / tb200::mx_scale_cols(BN));
   g.num_stages = stages;
   g.idesc = tb200::ptx::make_mx_idesc(kTileM, BN);
   g.bias = p.bias;
@@ -178,14 +179,117 @@ void launch_mx_gemm(DeviceState& st, int dt, const Product& p, cudaStream_t stre
          kPair ? 2 : 1, kLaunchMxGemm, stream, ta, tw, tsa, tsw, to, g);
 }
 
+// ------------------------------------------------------------------ few rows
+struct TokensPlan {
+  int cols = 0, split = 1, steps = 0, stages = 0;   // cols == 0: not for this problem
+  bool fused = false;
+};
+
+// `in_place`: x is at hand in its storage type, its columns contiguous.
+TokensPlan plan_tokens(long long M, long long N, long long K, bool to_mx, bool in_place, int num_sms) {
+  TokensPlan p;
+  static const int knob_rows = env_int("TRACEA_B200_MX_TOKENS", tb200::kTokMaxRows);
+  static const int knob_fused = env_int("TRACEA_B200_MX_FUSED", 64);
+  const long long n_tiles = ceil_div(N, 128), k_iters = ceil_div(K, 256), m_tiles = ceil_div(M, tb200::kTokMaxRows);
+  if (knob_rows == 0 || m_tiles * n_tiles > num_sms) return p;
+  int split = 1;
+  while (split < (to_mx ? 4 : 8) && 2 * split <= k_iters && m_tiles * n_tiles * 2 * split <= num_sms) split *= 2;
+  if (!(M <= 32 || (M <= 64 && k_iters >= 8) || (split > 1 && k_iters >= 16))) return p;
+  p.cols = static_cast<int>(ceil_div(std::min<long long>(M, tb200::kTokMaxRows), 16) * 16);
+  p.split = split;
+  p.steps = static_cast<int>(ceil_div(k_iters, split));
+  p.fused = in_place && M <= 16 && M * p.steps <= knob_fused && p.steps <= tb200::kTokFusedSteps;
+  const int room = 232448 - 1024 - tb200::kTokBarrierBytes - (p.fused ? p.steps * static_cast<int>(tb200::tok_step_bytes(p.cols)) : 0);
+  const int stage = static_cast<int>(tb200::kTokWBytes + (p.fused ? 0u : tb200::tok_step_bytes(p.cols)));
+  p.stages = std::min({p.steps, tb200::kTokMaxStages, room / stage});
+  return p;
+}
+
+template <typename OutT, typename InT, bool kFused, bool kMxOut>
+void launch_tokens(DeviceState& st, const Product& p, const Matrix* x, const TokensPlan& plan, cudaStream_t stream) {
+  auto kern = tb200::mx_tokens_sm100_kernel<OutT, InT, kFused, kMxOut>;
+  static std::atomic<bool> done[kMaxDevices];
+  if (!done[st.dev].load(std::memory_order_relaxed)) {
+    TB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448));
+    done[st.dev].store(true, std::memory_order_relaxed);
+  }
+  tb200::MxTokensArgs g;
+  memset(&g, 0, sizeof(g));
+  g.M = static_cast<int>(p.a.rows);
+  g.N = static_cast<int>(p.w.rows);
+  g.K = static_cast<int>(p.a.cols);
+  g.cols = plan.cols;
+  g.k_iters = static_cast<int>(ceil_div(p.a.cols, 256));
+  g.split = plan.split;
+  g.num_stages = plan.stages;
+  g.idesc = tb200::ptx::make_mx_idesc(128, static_cast<uint32_t>(plan.cols));
+  CUtensorMap tw, tsw, ta, tsa;
+  encode_codes(&tw, p.w, 128);
+  encode_scales(&tsw, p.w, 1);
+  if constexpr (kFused) {
+    memset(&ta, 0, sizeof(ta));
+    memset(&tsa, 0, sizeof(tsa));
+    g.x = x->ptr;
+    g.x_stride = x->row_stride;
+    g.x_vec = rows_of_8(*x) ? 1 : 0;
+  } else {
+    encode_codes(&ta, p.a, plan.cols);
+    encode_scales(&tsa, p.a, 1);
+  }
+  if constexpr (kMxOut) {
+    g.out = p.out_mx.data;
+    g.out_scales = p.out_mx.scales;
+    g.out_blocks = static_cast<int>(p.out_mx.blocks);
+    g.out_k_tiles = static_cast<int>(p.out_mx.k_tiles);
+  } else {
+    g.out = p.out.ptr;
+    g.out_stride = p.out.row_stride;
+    g.out_vec = reinterpret_cast<uintptr_t>(p.out.ptr) % (4 * sizeof(OutT)) == 0 && p.out.row_stride % 4 == 0 ? 1 : 0;
+    if (p.epi.residual) {
+      g.residual = p.residual.ptr;
+      g.res_stride = p.residual.row_stride;
+    }
+  }
+  g.bias = p.bias;
+  g.bias_is_f32 = p.bias_is_f32 ? 1 : 0;
+  g.act = p.epi.act;
+  g.status = st.status;
+  const long long limit = g_test_wait_limit.load(std::memory_order_relaxed);
+  g.wait_limit = limit > 0 ? limit : tb200::kWaitLimitCycles;
+  g.test_producer_stop = g_test_producer_stop.load(std::memory_order_relaxed);
+  launch(kern, dim3(grid_of(ceil_div(p.w.rows, 128) * plan.split), grid_of(ceil_div(p.a.rows, tb200::kTokMaxRows))), tb200::kTokThreads,
+         tb200::tok_smem_bytes(plan.cols, plan.stages, kFused ? plan.steps : 0), plan.split, kLaunchMxTokens, stream, tw, tsw, ta, tsa, g);
+}
+
+void tokens_product(DeviceState& st, const Product& p, const Matrix* x, const TokensPlan& plan, cudaStream_t stream) {
+  if (p.to_mx) {
+    if (plan.fused)
+      by_dtype(x->dtype, [&](auto tag) { launch_tokens<__nv_bfloat16, decltype(tag), true, true>(st, p, x, plan, stream); });
+    else
+      launch_tokens<__nv_bfloat16, float, false, true>(st, p, x, plan, stream);
+    return;
+  }
+  by_dtype(p.out.dtype, [&](auto tag) {
+    using T = decltype(tag);
+    if (plan.fused) launch_tokens<T, T, true, false>(st, p, x, plan, stream);
+    else launch_tokens<T, float, false, false>(st, p, x, plan, stream);
+  });
+}
+
 void mx_product(DeviceState& st, const Product& p, cudaStream_t stream) {
+  const TokensPlan plan = plan_tokens(p.a.rows, p.w.rows, p.a.cols, p.to_mx, false, st.num_sms);
+  if (plan.cols != 0) {
+    tokens_product(st, p, nullptr, plan, stream);
+    return;
+  }
   const int force = env_int("TRACEA_B200_MX_BN", 0);
   const long long M = p.a.rows, N = p.w.rows;
   const int bn = force != 0 ? force : (M > 128 && ceil_div(M, 256) * ceil_div(N, 192) >= st.num_sms / 2 ? 192 : (N > 64 ? 128 : 64));
   auto tiled = [&](auto tag, int dt, auto store) {
     using T = decltype(tag);
     constexpr int kStore = decltype(store)::value;
-    if (bn == 192) launch_mx_gemm<T, 192, true, kStore>(st, dt, p, stream);
+    if (bn == 256) launch_mx_gemm<T, 256, true, kStore>(st, dt, p, stream);
+    else if (bn == 192) launch_mx_gemm<T, 192, true, kStore>(st, dt, p, stream);
     else if (bn == 128) launch_mx_gemm<T, 128, false, kStore>(st, dt, p, stream);
     else launch_mx_gemm<T, 64, false, kStore>(st, dt, p, stream);
   };
@@ -274,6 +378,12 @@ void mx_linear_checked(const TraceaTensorView& xv, const TraceaMxMatrix& wv, con
   p.a.cols = x.cols;
   p.a.blocks = ceil_div(x.cols, tb200::kMxBlock);
   p.a.k_tiles = ceil_div(x.cols, tb200::kMxTileCols);
+  const bool in_place = x.col_stride == 1 && (p.to_mx || x.dtype == p.out.dtype);
+  const TokensPlan plan = plan_tokens(x.rows, p.w.rows, x.cols, p.to_mx, in_place, st.num_sms);
+  if (plan.fused) {
+    tokens_product(st, p, &x, plan, stream);
+    return;
+  }
   const size_t data_bytes = static_cast<size_t>(x.rows * 16 * p.a.blocks + 255) / 256 * 256;
   Scratch scratch;
   scratch.alloc(st, data_bytes + static_cast<size_t>(ceil_div(x.rows, tb200::kMxTileRows) * p.a.k_tiles * tb200::kMxTileBytes), stream);
