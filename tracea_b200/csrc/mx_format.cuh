@@ -86,6 +86,12 @@ __device__ __forceinline__ float max_abs3(float a, float b, float c) {
 __device__ __forceinline__ float max_abs8(const float* v) {
   return max_abs3(max_abs3(max_abs3(v[0], v[1], v[2]), v[3], v[4]), max_abs3(v[5], v[6], v[7]), 0.0f);
 }
+// The smallest of three, NaN if one of them is.
+__device__ __forceinline__ float min_nan3(float a, float b, float c) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 // Packed pairs: (a, b) * (c, d) [+ (e, f)].
 __device__ __forceinline__ void mul2(float& a, float& b, float c, float d) {
   asm("{\n"

@@ -16,9 +16,11 @@ namespace tb200 {
 enum : int { kMxStoreTma = 0, kMxStoreRows = 1, kMxStoreMx = 2 };
 
 constexpr int kMxMaxStages = 8;
-// Warp 0 TMA, warp 1 MMA, warps 2..5 and 6..9 two epilogue groups, warp 10 TMA; pairs: warps 11 and 12 scales
-__host__ __device__ constexpr int mx_threads(bool pair) { return pair ? 416 : 352; }
-constexpr int kSecondProducer = 10, kScaleWarp = 11;
+// Warp 0 TMA, warp 1 MMA, then the epilogue's warps in groups of four, one more TMA, pairs: two for scales. Quantised output has
+// four groups, others, whose rows go through 64 registers at a time, two: what bounds an epilogue beside MMAs is the latency
+// of its chain of instructions (SiLU into 4 bits, 64 columns: 2050 cycles a warp at two warps a scheduler).
+__host__ __device__ constexpr int mx_epilogue_warps(int bn, int store) { return store == kMxStoreMx && bn > 64 ? 16 : 8; }
+__host__ __device__ constexpr int mx_threads(int bn, bool pair, int store) { return 32 * ((pair ? 5 : 3) + mx_epilogue_warps(bn, store)); }
 
 struct MxGemmArgs {
   int M, N;
@@ -51,8 +53,9 @@ __host__ __device__ constexpr int mx_stage_bytes(int bn, bool pair) {
 constexpr int kMxBarrierBytes = 256;
 // Boxes of 32 rows x 128 bytes for each epilogue warp. Stages are worth more than a second box where a tile is large.
 __host__ __device__ constexpr int mx_staging_depth(int bn, int store) { return store == kMxStoreMx ? 0 : (bn == 256 ? 1 : 2); }
-__host__ __device__ constexpr int mx_smem_bytes(int bn, int stages, bool pair, int staging_depth) {
-  return 1024 + stages * mx_stage_bytes(bn, pair) + kNumEpilogueWarps * (staging_depth * kStagingBoxBytes + bn * 4) + kMxBarrierBytes;
+__host__ __device__ constexpr int mx_smem_bytes(int bn, int stages, bool pair, int store) {
+  return 1024 + stages * mx_stage_bytes(bn, pair) + mx_epilogue_warps(bn, store) * (mx_staging_depth(bn, store) * kStagingBoxBytes + bn * 4) +
+         kMxBarrierBytes;
 }
 
 // Tiles of 256 columns leave no room in TMEM for a second accumulator beside the scales.
@@ -61,8 +64,46 @@ __host__ __device__ constexpr int mx_accumulators(int bn) { return bn == 256 ? 1
 // rewritten when its shared memory is, which the stage's empty barrier orders behind the MMAs that read them.
 __host__ __device__ constexpr int mx_scale_cols(int bn) { return 8 + 8 * mx_b_scale_tiles(bn); }
 
+// apply_act32 with fewer trips through the special-function unit, which bounds SiLU here: a tile of 192 columns of 1024 takes
+// 2200 cycles of MMAs and 128 x 192 exponentials and reciprocals, at 16 of these a cycle, 3100. Four values share a reciprocal,
+// 1 / a = (1 / abcd) bcd, which costs three roundings more, 2^-22 -- far below a 16- or 4-bit result's. The product of four stays
+// in range while each 1 + e^-x is below 2^31: a warp with a value below -20, or a NaN, takes the other way.
+template <bool kFast>
+__device__ __forceinline__ void mx_act32(float (&f)[32], int act) {
+  if (!kFast || act != kActSilu) {
+    apply_act32<kFast>(f, act);
+    return;
+  }
+  float low = f[0];
+#pragma unroll
+  for (int j = 1; j < 31; j += 2) low = min_nan3(low, f[j], f[j + 1]);
+  low = min_nan3(low, f[31], f[31]);
+  if (!__all_sync(0xffffffffu, low >= -20.0f)) {
+    apply_act32<kFast>(f, act);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 32; j += 4) {
+    float a[4] = {f[j], f[j + 1], f[j + 2], f[j + 3]};
+    mul2(a[0], a[1], -1.44269504f, -1.44269504f);
+    mul2(a[2], a[3], -1.44269504f, -1.44269504f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a[i]));
+    add2(a[0], a[1], 1.0f, 1.0f);
+    add2(a[2], a[3], 1.0f, 1.0f);
+    const float p = a[0] * a[1], q = a[2] * a[3];
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(p * q));
+    const float rp = r * q, rq = r * p;       // 1 / p, 1 / q
+    mul2(f[j], f[j + 1], a[1], a[0]);
+    mul2(f[j + 2], f[j + 3], a[3], a[2]);
+    mul2(f[j], f[j + 1], rp, rp);
+    mul2(f[j + 2], f[j + 3], rq, rq);
+  }
+}
+
 template <typename OutT, int BN, bool kPair, int kStore>
-__global__ void __launch_bounds__(mx_threads(kPair), 1)
+__global__ void __launch_bounds__(mx_threads(BN, kPair, kStore), 1)
 mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
                      const __grid_constant__ CUtensorMap tmap_sa, const __grid_constant__ CUtensorMap tmap_sw,
                      const __grid_constant__ CUtensorMap tmap_out, const __grid_constant__ MxGemmArgs args) {
@@ -77,6 +118,8 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
   constexpr uint32_t kScaleCols = mx_scale_cols(BN);
   constexpr int kStagingDepth = mx_staging_depth(BN, kStore);
   static_assert(BN % 64 == 0 && BN <= 256 && kStageBytes % 1024 == 0, "tile");
+  constexpr int kEpiWarps = mx_epilogue_warps(BN, kStore), kEpiGroups = kEpiWarps / 4;
+  constexpr int kSecondProducer = 2 + kEpiWarps, kScaleWarp = 3 + kEpiWarps;
   constexpr int kAcc = mx_accumulators(BN);            // the host keeps to as many stages as TMEM has columns of scales for
   constexpr uint32_t kTmemCols = 512;
   const uint32_t cta_rank = kPair ? __shfl_sync(0xffffffffu, cluster_ctarank(), 0) : 0u;
@@ -92,8 +135,8 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
   const int num_stages = args.num_stages;
   const uint32_t ring_bytes = static_cast<uint32_t>(num_stages) * kStageBytes;
   const uint32_t staging_base = smem_base + ring_bytes;
-  const uint32_t bias_off = ring_bytes + kNumEpilogueWarps * kStagingDepth * kStagingBoxBytes;
-  const uint32_t bar_off = bias_off + kNumEpilogueWarps * BN * 4;
+  const uint32_t bias_off = ring_bytes + kEpiWarps * kStagingDepth * kStagingBoxBytes;
+  const uint32_t bar_off = bias_off + kEpiWarps * BN * 4;
   const uint32_t bar_base = smem_base + bar_off;
   const uint32_t full_bar0 = bar_base, empty_bar0 = bar_base + 8u * kMxMaxStages;
   auto tfull_bar = [&](int b) { return bar_base + 8u * (2 * kMxMaxStages + b); };
@@ -112,7 +155,7 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(tfull_bar(b), 1);
-      mbar_init(tempty_bar(b), (kPair ? 8 : 4) * (kAcc == 1 ? 2 : 1));   // the warps that drain it, in both CTAs of a pair
+      mbar_init(tempty_bar(b), (kPair ? 8 : 4) * kEpiGroups / kAcc);   // the warps that drain it, in both CTAs of a pair
     }
     *abort_p = 0u;
     fence_mbar_init();
@@ -219,21 +262,20 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       // operands: 128-byte swizzled rows, 8 rows to 1024 bytes
       constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
       const uint32_t idesc0 = args.idesc, idesc2 = args.idesc | (2u << 4) | (2u << 29);   // scale words' lower and upper halves
-      const uint32_t base_units = smem_base >> 4;
       constexpr uint32_t kStageUnits = kStageBytes >> 4;
-      const uint32_t scale_cols0 = tmem_base + kAcc * BN;
-      int stage = 0, local = 0;
-      uint32_t phase = 0;
+      // The ring's state, moved by additions: this loop, not the tensor pipe, sets the pace of a stage (with a multiplication for
+      // every address 455 cycles, of which the MMAs of 256 x 192 take 384).
+      const uint32_t a_first = smem_base >> 4, ta_first = tmem_base + kAcc * BN;
+      const uint32_t a_end = a_first + static_cast<uint32_t>(num_stages) * kStageUnits;
+      uint32_t a = a_first, ta = ta_first, bar = 0, phase = 0;
+      int local = 0;
       bool ok = true;
       bool ready = false;             // pairs: this stage's scales are known to be in place; else: the next stage's bytes are
       bool scales_issued = false;     // not pairs: this stage's scales are on their way to tensor memory
-      const int my_steps = (worker < tiles ? (tiles - worker + num_workers - 1) / num_workers : 0) * k_iters;
-      int step = 0;
       // not pairs: the copies of a stage's scales. They run in order with this warp's MMAs, so no wait lies between
-      auto copy_scales = [&](int s) {
+      auto copy_scales = [&](uint32_t stage_a, uint32_t dst) {
         constexpr uint32_t kScaleDescHi = (128u >> 4) | (1u << 14);   // 32 rows of 16 bytes, 8 rows to 128 bytes, not swizzled
-        const uint32_t src = base_units + static_cast<uint32_t>(s) * kStageUnits + (kSaOff >> 4);
-        const uint32_t dst = scale_cols0 + static_cast<uint32_t>(s) * kScaleCols;
+        const uint32_t src = stage_a + (kSaOff >> 4);
 #pragma unroll
         for (uint32_t k = 0; k < 2; ++k) {
           tmem_cp_32x128b_if<kPair>(issue, dst + 4u * k, src + k * (kMxTileBytes >> 4), kScaleDescHi);
@@ -243,6 +285,7 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
                                       kScaleDescHi);
         }
       };
+      int steps_left = (worker < tiles ? (tiles - worker + num_workers - 1) / num_workers : 0) * k_iters;
       for (int tile = worker; ok && tile < tiles; tile += num_workers, ++local) {
         const int buf = kAcc == 2 ? local & 1 : 0;
         const uint32_t use = static_cast<uint32_t>(kAcc == 2 ? local >> 1 : local);
@@ -252,55 +295,54 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
           break;
         }
         tc_fence_after();
-        int mt, nt;
-        tile_coords(tile, mt, nt);
-        const uint32_t sw_shift = static_cast<uint32_t>(nt * BN % kMxTileRows) / 32u;   // the tile may start inside a scale tile
+        uint32_t sw_shift = 0;        // the tile may start inside a tile of scales
+        if constexpr (BN % kMxTileRows != 0) {
+          int mt, nt;
+          tile_coords(tile, mt, nt);
+          sw_shift = static_cast<uint32_t>(nt * BN % kMxTileRows) / 32u;
+        }
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(buf) * BN;
-        for (int it = 0; it < k_iters; ++it, ++step) {
-          const uint32_t a = base_units + static_cast<uint32_t>(stage) * kStageUnits, b = a + (kABytes >> 4);
-          const uint32_t ta = scale_cols0 + static_cast<uint32_t>(stage) * kScaleCols, tb = ta + 8u;
-          const uint32_t empty = empty_bar0 + 8u * stage;
-          int next = stage + 1;
-          uint32_t next_phase = phase;
-          if (next == num_stages) { next = 0; next_phase ^= 1u; }
-          uint32_t probe_bar, probe_phase;
+        for (int it = 0; it < k_iters; ++it) {
+          uint32_t next_a = a + kStageUnits, next_ta = ta + kScaleCols, next_bar = bar + 8u, next_phase = phase;
+          if (next_a == a_end) { next_a = a_first; next_ta = ta_first; next_bar = 0; next_phase ^= 1u; }
+          uint32_t probe_bar = scale_bar0 + next_bar, probe_phase = next_phase;
           if constexpr (kPair) {
-            if (!ready && !mbar_wait_bounded_uniform(scale_bar0 + 8u * stage, phase, abort_p, args.wait_limit)) {
+            if (!ready && !mbar_wait_bounded_uniform(scale_bar0 + bar, phase, abort_p, args.wait_limit)) {
               if (issue) report_error_status(args.status, abort_p, kErrMmaWaitFull, static_cast<uint32_t>(it));
               ok = false;
               break;
             }
             tc_fence_after();
-            probe_bar = scale_bar0 + 8u * next;
-            probe_phase = next_phase;
           } else {
             if (!scales_issued) {
-              if (!mbar_wait_bounded_uniform(full_bar0 + 8u * stage, phase, abort_p, args.wait_limit)) {
+              if (!mbar_wait_bounded_uniform(full_bar0 + bar, phase, abort_p, args.wait_limit)) {
                 if (issue) report_error_status(args.status, abort_p, kErrMmaWaitFull, static_cast<uint32_t>(it));
                 ok = false;
                 break;
               }
               tc_fence_after();
-              copy_scales(stage);
+              copy_scales(a, ta);
             }
             // the next stage's scales go ahead of this stage's MMAs where its bytes are known to have landed: copies right in
             // front of the MMAs that read them hold the tensor pipe up
-            scales_issued = ready && step + 1 < my_steps;
+            scales_issued = ready && --steps_left > 0;
             if (scales_issued) {
               tc_fence_after();
-              copy_scales(next);
+              copy_scales(next_a, next_ta);
             }
-            int next2 = next + 1;
-            probe_phase = next_phase;
-            if (next2 == num_stages) { next2 = 0; probe_phase ^= 1u; }
-            probe_bar = full_bar0 + 8u * next2;
+            probe_bar = full_bar0 + next_bar + 8u;
+            if (next_a + kStageUnits == a_end) { probe_bar = full_bar0; probe_phase ^= 1u; }
           }
-          const bool landed = mx_mma_stage4_probe<kPair>(d_tmem, a, b, kDescHi, idesc0, idesc2, ta, ta + 4u, tb + sw_shift,
-                                                         tb + 4u * kBTiles + sw_shift, empty, probe_bar, probe_phase,
-                                                         it > 0 ? 1u : 0u, issue);
+          const uint32_t b = a + (kABytes >> 4), tb = ta + 8u + sw_shift;
+          bool landed;
+          if (it == 0)
+            landed = mx_mma_stage4_probe<kPair, false>(d_tmem, a, b, kDescHi, idesc0, idesc2, ta, ta + 4u, tb, tb + 4u * kBTiles,
+                                                       empty_bar0 + bar, probe_bar, probe_phase, issue);
+          else
+            landed = mx_mma_stage4_probe<kPair, true>(d_tmem, a, b, kDescHi, idesc0, idesc2, ta, ta + 4u, tb, tb + 4u * kBTiles,
+                                                      empty_bar0 + bar, probe_bar, probe_phase, issue);
+          a = next_a; ta = next_ta; bar = next_bar; phase = next_phase;
           ready = __all_sync(0xffffffffu, landed);
-          stage = next;
-          phase = next_phase;
         }
         if (ok && issue) {
           if constexpr (kPair) mma_commit_pair(tfull_bar(buf));
@@ -350,11 +392,12 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       }
     }
   } else {
-    // ------------------------------------------------------------ epilogue: two groups of four warps, a row a lane
-    // With two accumulators they take alternate tiles, and of the last one -- nothing overlaps it -- each every second group of
-    // columns; with one accumulator they share every tile in that way.
+    // ------------------------------------------------------------ epilogue: groups of four warps, a row a lane
+    // With two accumulators, half of the groups take every second tile, and all of them the last one, which nothing overlaps; with
+    // one accumulator all take every tile. Groups that share a tile take alternate groups of columns.
     const int ew = warp - 2, egroup = ew >> 2, quarter = warp & 3;
-    constexpr int kGroupCols = kStore == kMxStoreMx ? 64 : 128 / static_cast<int>(sizeof(OutT));
+    constexpr int kShare = kEpiGroups / kAcc;
+    constexpr int kGroupCols = kStore == kMxStoreMx ? 32 : 128 / static_cast<int>(sizeof(OutT));
     constexpr int kGroups = BN / kGroupCols;
     constexpr int kLdPerGroup = kGroupCols / 32;
     constexpr int kVec = 16 / sizeof(OutT);
@@ -369,9 +412,9 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     int bias_tile = -1;
     bool ok = true;
     for (int local = 0; ok && local < my_tiles; ++local) {
-      const bool shared = kAcc == 1 || (local == my_tiles - 1 && kGroups > 1);
-      if ((local & 1) != egroup && !shared) continue;
-      const int g_first = shared && (local & 1) != egroup ? 1 : 0, g_step = shared ? 2 : 1;
+      const bool last = kAcc == 2 && local == my_tiles - 1;
+      if (kAcc == 2 && !last && (local & 1) != egroup / kShare) continue;
+      const int g_first = last ? egroup : egroup % kShare, g_step = last ? kEpiGroups : kShare;
       const int buf = kAcc == 2 ? local & 1 : 0;
       const uint32_t use = static_cast<uint32_t>(kAcc == 2 ? local >> 1 : local);
       int mt, nt;
@@ -422,11 +465,11 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
 #pragma unroll
         for (int h = 0; h < kLdPerGroup; ++h) tmem_ld_32x32(taddr0 + g * kGroupCols + h * 32, v[h]);
         tmem_ld_wait();
-        if (kAcc == 1 ? g + 2 >= kGroups : g == kGroups - 1 && !shared) {
+        if (!last && g + kShare >= kGroups) {        // (nobody waits for the buffer of the last tile)
           tc_fence_before();
           __syncwarp();
           if (lane == 0) {
-            if constexpr (kPair) mbar_arrive_cluster(mapa_cluster(tempty_bar(buf), 0u));
+            if constexpr (kPair) mbar_arrive_cluster_relaxed(mapa_cluster(tempty_bar(buf), 0u));
             else mbar_arrive(tempty_bar(buf));
           }
         }
@@ -454,7 +497,7 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
             add2(f[j4 * 4 + 2], f[j4 * 4 + 3], b4.z, b4.w);
           }
           if constexpr (kStore == kMxStoreMx) {
-            apply_act32<true>(f, args.act);
+            mx_act32<true>(f, args.act);
             // columns past N: their scales are whatever lies behind the last row of W, and may not reach the block's
             if (n0 + h * 32 + 32 > args.N) {
 #pragma unroll
@@ -463,7 +506,7 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
             }
             uint32_t byte;
             packed[h] = mx_quantize32(f, byte);
-            scale_bytes |= byte << (8 * h);
+            scale_bytes = byte;
           } else {
             if (res != nullptr) {
 #pragma unroll
@@ -475,22 +518,21 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
             if (args.act == kActRelu) {
               finish32<OutT, true>(f, nullptr, false, packed + h * kChunksPerLd);
             } else {
-              apply_act32<sizeof(OutT) == 2>(f, args.act);
+              mx_act32<sizeof(OutT) == 2>(f, args.act);
               finish32<OutT, false>(f, nullptr, false, packed + h * kChunksPerLd);
             }
           }
         }
         if constexpr (kStore == kMxStoreMx) {
-          // two blocks of this lane's row: up to 32 bytes of codes and half a word of scales
+          // a block of this lane's row; behind the last one, the rest of its word of scales is 0
           const int blk = n0 / kMxBlock;
           if (row_ok) {
-            uint8_t* codes = static_cast<uint8_t*>(args.out) + static_cast<long long>(m) * (16LL * args.out_blocks) + 16LL * blk;
-            reinterpret_cast<uint4*>(codes)[0] = packed[0];
-            if (blk + 1 < args.out_blocks) reinterpret_cast<uint4*>(codes)[1] = packed[1];
-            uint8_t* sw = args.out_scales + mx_scale_word(m, blk >> 2, args.out_k_tiles) + (blk & 3);
-            // the last word is written whole: blocks past N are 0
-            if ((blk & 3) == 0 && blk + 2 >= args.out_blocks) *reinterpret_cast<uint32_t*>(sw) = scale_bytes;
-            else *reinterpret_cast<uint16_t*>(sw) = static_cast<uint16_t>(scale_bytes);
+            *reinterpret_cast<uint4*>(static_cast<uint8_t*>(args.out) + static_cast<long long>(m) * (16LL * args.out_blocks) + 16LL * blk) =
+                packed[0];
+            uint8_t* sw = args.out_scales + mx_scale_word(m, blk >> 2, args.out_k_tiles);
+            sw[blk & 3] = static_cast<uint8_t>(scale_bytes);
+            if (blk + 1 == args.out_blocks)
+              for (int b = (blk & 3) + 1; b < 4; ++b) sw[b] = 0;
           }
         } else {
 #pragma unroll

@@ -132,8 +132,7 @@ void launch_mx_gemm(DeviceState& st, int dt, const Product& p, cudaStream_t stre
   g.num_n_tiles = static_cast<int>(n_tiles);
   g.panel_width = static_cast<int>(panel);
   g.panel_tiles = static_cast<int>(m_tiles * panel);
-  constexpr int kDepth = tb200::mx_staging_depth(BN, kStore);
-  const int room = 232448 - tb200::mx_smem_bytes(BN, 0, kPair, kDepth);
+  const int room = 232448 - tb200::mx_smem_bytes(BN, 0, kPair, kStore);
   int stages = std::min(room / tb200::mx_stage_bytes(BN, kPair), tb200::kMxMaxStages);
   stages = std::min(stages, (512 - tb200::mx_accumulators(BN) * BN) / tb200::mx_scale_cols(BN));
   g.num_stages = stages;
@@ -175,7 +174,7 @@ void launch_mx_gemm(DeviceState& st, int dt, const Product& p, cudaStream_t stre
     }
   }
   const long long workers = std::min<long long>(m_tiles * n_tiles, kPair ? st.num_sms / 2 : st.num_sms);
-  launch(kern, grid_of(kPair ? 2 * workers : workers), tb200::mx_threads(kPair), tb200::mx_smem_bytes(BN, stages, kPair, kDepth),
+  launch(kern, grid_of(kPair ? 2 * workers : workers), tb200::mx_threads(BN, kPair, kStore), tb200::mx_smem_bytes(BN, stages, kPair, kStore),
          kPair ? 2 : 1, kLaunchMxGemm, stream, ta, tw, tsa, tsw, to, g);
 }
 
@@ -276,15 +275,45 @@ void tokens_product(DeviceState& st, const Product& p, const Matrix* x, const To
   });
 }
 
+// Columns of a tile: 64 or 128 in a CTA, 192 or 256 in a pair of CTAs (256 rows). By the time of the busiest CTA or pair, in
+// us: what a launch takes once, and per wave of tiles either its k-steps (an SM has 16 KB of A and half or all of the columns' rows
+// of W to bring in a step) and what lies between two tiles, or its epilogue, whichever is longer. 192 columns have two accumulators,
+// 256 one, which pays for its wider steps only over a long K. Measured / this formula, columns 64, 128, 192, 256:
+//   8192 x 8192 x 8192         480 249 210 201 / 448 263 212 206     12544 x 4096 x 1024    64  34  31 43 / 60 33 31 40
+//   4096 x 4096 x 4096          68  32  29  33 / 60  37  32  35      the same, SiLU           -  41  46 59 / 60 41 48 60
+//   2048 x 2048 x 2048        12.6 7.3 9.2 9.1 / 11 7.9 10 8.7       1024 x 1024 x 2048   4.8 5.3 6.7  - / 4.8 5.4 7.0 8.6
+int pick_mx_tile(long long M, long long N, long long K, int act, int num_sms) {
+  static const int forced = env_int("TRACEA_B200_MX_BN", 0);
+  if (forced != 0) return forced;
+  struct Form {
+    int bn;
+    double once, step, between, epilogue, epilogue_act;
+  };
+  static const Form forms[4] = {{64, 2.6, 0.24, 0.2, 0.75, 0.9}, {128, 2.9, 0.28, 0.25, 1.15, 1.75},
+                                {192, 4.0, 0.33, 0.4, 1.8, 2.9}, {256, 4.0, 0.41, 1.3, 3.3, 5.1}};
+  const double steps = static_cast<double>(ceil_div(K, 256));
+  int best = 0;
+  double best_time = 0.0;
+  for (const Form& f : forms) {
+    const bool pair = f.bn >= 192;
+    const long long waves = ceil_div(ceil_div(M, pair ? 256 : 128) * ceil_div(N, f.bn), pair ? num_sms / 2 : num_sms);
+    const double epilogue = act == tb200::kActSilu || act == tb200::kActGelu ? f.epilogue_act : f.epilogue;
+    const double time = f.once + static_cast<double>(waves) * std::max(steps * f.step + f.between, epilogue);
+    if (best == 0 || time < best_time) {
+      best = f.bn;
+      best_time = time;
+    }
+  }
+  return best;
+}
+
 void mx_product(DeviceState& st, const Product& p, cudaStream_t stream) {
   const TokensPlan plan = plan_tokens(p.a.rows, p.w.rows, p.a.cols, p.to_mx, false, st.num_sms);
   if (plan.cols != 0) {
     tokens_product(st, p, nullptr, plan, stream);
     return;
   }
-  const int force = env_int("TRACEA_B200_MX_BN", 0);
-  const long long M = p.a.rows, N = p.w.rows;
-  const int bn = force != 0 ? force : (M > 128 && ceil_div(M, 256) * ceil_div(N, 192) >= st.num_sms / 2 ? 192 : (N > 64 ? 128 : 64));
+  const int bn = pick_mx_tile(p.a.rows, p.w.rows, p.a.cols, p.epi.act, st.num_sms);
   auto tiled = [&](auto tag, int dt, auto store) {
     using T = decltype(tag);
     constexpr int kStore = decltype(store)::value;
