@@ -136,6 +136,14 @@ __device__ __forceinline__ bool has_shift(const NormStage& s) { return s.bias.pt
 // A CTA's rows are walked by groups of kThreads threads.
 __host__ __device__ constexpr int norm_block_threads(int row_threads) { return row_threads < 256 ? 256 : row_threads; }
 
+// A barrier of the threads of a row.
+template <int kThreads>
+__device__ __forceinline__ void row_barrier(int warp) {
+  if constexpr (kThreads == 32) __syncwarp();
+  else if constexpr (kThreads == norm_block_threads(kThreads)) __syncthreads();
+  else asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / (kThreads / 32)), "n"(kThreads) : "memory");
+}
+
 // The sum over the threads of a row, in every one of them, always in the same order. `slot` alternates between two buffers: the
 // barrier of one sum is behind every read of the sum before it.
 template <int kThreads>
@@ -143,12 +151,11 @@ __device__ __forceinline__ float row_sum(float v, float* smem, uint32_t& slot, i
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
   if constexpr (kThreads > 32) {
-    constexpr int kWarps = kThreads / 32, kCtaWarps = norm_block_threads(kThreads) / 32;
+    constexpr int kWarps = kThreads / 32;
     float* s = smem + slot * 16;
     slot ^= 1u;
     if (lane == 0) s[warp] = v;
-    if constexpr (kWarps == kCtaWarps) __syncthreads();
-    else asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / kWarps), "n"(kThreads) : "memory");
+    row_barrier<kThreads>(warp);
     s += warp / kWarps * kWarps;                 // the row's warps
     if constexpr (kWarps == 2) {
       v = s[0] + s[1];
@@ -176,7 +183,8 @@ __device__ __forceinline__ void norm_row(const NormStage& s, float (&v)[kVecs][8
     for (int i = 0; i < kVecs; ++i)
 #pragma unroll
       for (int j = 0; j < 8; j += 2) add2(a, b, v[i][j], v[i][j + 1]);
-    const float mean = row_sum<kThreads>(a + b, smem, slot, lane, warp) * inv_C;
+    // divided, not multiplied by 1 / C: the mean of a constant row is its constant then, where the sums are exact
+    const float mean = row_sum<kThreads>(a + b, smem, slot, lane, warp) / static_cast<float>(C);
 #pragma unroll
     for (int i = 0; i < kVecs; ++i)
 #pragma unroll
@@ -260,9 +268,13 @@ __host__ __device__ constexpr int norm_depth(int threads, int vecs, bool join, i
                 norm_row_bytes(threads, vecs, join, es);
   return n > 4 ? 4 : (n < 1 ? 1 : n);
 }
+// kRowsSingle, joins: the join is done with the columns spread, as where its rows are not quantised, so that it gives the same bits
+// whatever follows it; its result changes hands through shared memory, a row of fp32 for every row in hand.
+__host__ __device__ constexpr int norm_join_mode(int mode) { return mode == kRowsSingle ? kRowsSpread : mode; }
 __host__ __device__ constexpr int norm_smem_bytes(int threads, int vecs, int mode, bool join, int next, int es) {
   return norm_kept_bytes(threads, vecs, join, next) +
-         (mode == kRowsVec ? norm_depth(threads, vecs, join, next, es) * norm_row_bytes(threads, vecs, join, es) : 0);
+         (mode == kRowsVec ? norm_depth(threads, vecs, join, next, es) * norm_row_bytes(threads, vecs, join, es)
+                           : (mode == kRowsSingle && join ? norm_block_threads(threads) * vecs * 8 * 4 : 0));
 }
 
 template <typename T, int kThreads, int kVecs, int kMode, bool kJoin, int kNext>
@@ -274,6 +286,8 @@ block_norm_kernel(const __grid_constant__ BlockNormArgs a) {
   extern __shared__ __align__(16) uint8_t dynamic[];
   __shared__ __align__(16) float sums[32];
   using Slice = RowSlice<T, kMode, kThreads>;
+  constexpr int kJoinMode = norm_join_mode(kMode);
+  using JoinSlice = RowSlice<T, kJoin ? kJoinMode : kMode, kThreads>;
   constexpr int kBlock = norm_block_threads(kThreads);
   constexpr int kRows = kBlock / kThreads;                              // that a CTA has in hand at a time
   constexpr bool kKeep = norm_keeps(kThreads, kVecs);
@@ -330,7 +344,7 @@ block_norm_kernel(const __grid_constant__ BlockNormArgs a) {
         if (kSlices % kBlock == 0 || slice < kSlices) {
           float p[8], q[8];
           if constexpr (kJoin) {
-            norm_affine8<T, kMode, kThreads>(a.join, &a.gate, group, slice / kThreads, slice % kThreads, C, p, q);
+            norm_affine8<T, kJoinMode, kThreads>(a.join, &a.gate, group, slice / kThreads, slice % kThreads, C, p, q);
             norm_keep<kSlices>(kept_join, slice, p, q);
           }
           if constexpr (kNext != kNextNone) {
@@ -354,8 +368,8 @@ block_norm_kernel(const __grid_constant__ BlockNormArgs a) {
           Slice::copied(ring_at + i * kSliceBytes, i, t, C, xd);
           if constexpr (kJoin) Slice::copied(ring_at + (kVecs + i) * kSliceBytes, i, t, C, v[i]);
         } else {
-          Slice::load(x, i, t, C, xd);
-          if constexpr (kJoin) Slice::load(h, i, t, C, v[i]);
+          JoinSlice::load(x, i, t, C, xd);
+          if constexpr (kJoin) JoinSlice::load(h, i, t, C, v[i]);
         }
       }
       if constexpr (kMode == kRowsVec) {
@@ -365,10 +379,10 @@ block_norm_kernel(const __grid_constant__ BlockNormArgs a) {
         if constexpr (kJoin) h += h_step;
       }
       if constexpr (kJoin) {
-        norm_row<kMode, kThreads, kVecs>(a.join, v, C, inv_C, t, sums, slot, lane, warp);
+        norm_row<kJoinMode, kThreads, kVecs>(a.join, v, C, inv_C, t, sums, slot, lane, warp);
 #pragma unroll
         for (int i = 0; i < kVecs; ++i) {
-          norm_apply8<T, kMode, kThreads, kVecs, kKeep>(a.join, &a.gate, kept_join, group, join_shift, i, t, C, v[i]);
+          norm_apply8<T, kJoinMode, kThreads, kVecs, kKeep>(a.join, &a.gate, kept_join, group, join_shift, i, t, C, v[i]);
 #pragma unroll
           for (int j = 0; j < 8; j += 2) {
             float p = xv[i][j], q = xv[i][j + 1];
@@ -376,14 +390,27 @@ block_norm_kernel(const __grid_constant__ BlockNormArgs a) {
             v[i][j] = p;
             v[i][j + 1] = q;
           }
-          Slice::store(r, i, t, C, v[i]);
+          JoinSlice::store(r, i, t, C, v[i]);
           if constexpr (kNext != kNextNone) {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-              v[i][j] = Slice::col(i, t, kMode == kRowsVec ? 0 : j) < C ? OutTraits<T>::to_f(OutTraits<T>::from_f(v[i][j])) : 0.0f;
+              v[i][j] = JoinSlice::col(i, t, kMode == kRowsVec ? 0 : j) < C ? OutTraits<T>::to_f(OutTraits<T>::from_f(v[i][j])) : 0.0f;
           }
         }
         r += kRows * a.r_stride;
+        if constexpr (kJoinMode != kMode) {
+          float* exchange = reinterpret_cast<float*>(dynamic + norm_kept_bytes(kThreads, kVecs, kJoin, kNext)) + sub * kSlices * 8;
+#pragma unroll
+          for (int i = 0; i < kVecs; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) exchange[JoinSlice::col(i, t, j)] = v[i][j];
+          row_barrier<kThreads>(warp);
+#pragma unroll
+          for (int i = 0; i < kVecs; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] = exchange[Slice::col(i, t, j)];
+          row_barrier<kThreads>(warp);                                  // before the next row is written there
+        }
       }
       if constexpr (kNext != kNextNone) {
         norm_row<kMode, kThreads, kVecs>(a.norm, v, C, inv_C, t, sums, slot, lane, warp);

@@ -61,7 +61,7 @@ inline Mx load_mx(const TraceaMxMatrix& v, const char* name, int dev) {
   Mx m;
   m.data = static_cast<uint8_t*>(v.data);
   m.scales = static_cast<uint8_t*>(v.scales);
-  if (v.rows > 0x7fffffffULL || v.cols == 0 || v.cols > 0x7fffff00ULL)
+  if (v.rows > 0x7fffff00ULL || v.cols == 0 || v.cols > 0x7fffff00ULL)
     TB_FAIL(TRACEA_INVALID_PARAMS, "%s: %llu x %llu is out of range", name, (unsigned long long)v.rows, (unsigned long long)v.cols);
   m.rows = static_cast<long long>(v.rows);
   m.cols = static_cast<long long>(v.cols);

@@ -184,13 +184,17 @@ struct TokensPlan {
   bool fused = false;
 };
 
-// `in_place`: x is at hand in its storage type, its columns contiguous.
+// `in_place`: x is at hand in its storage type, its columns contiguous. The form of few rows, and quantising inside it, where they are
+// the faster ones (us, rows / this form / the general one):
+//   4096 x 4096   1 4.8 7.6   32 5.5 7.4   64 6.6 7.1  128 7.3 7.2        1000 x 2048    1 3.6 4.9   32 4.3 5.0  64 5.0 5.0  128 6.7 5.2
+//   4096 x 1024   1 3.6 4.2   32 4.0 4.2   64 4.6 4.1  128 6.2 4.2        256 x 16384    1 4.2 18   128 7.3 18
+// Quantising inside costs each CTA rows x steps passes of eight warps, a launch and a round trip ~2.2 us.
 TokensPlan plan_tokens(long long M, long long N, long long K, bool to_mx, bool in_place, int num_sms) {
   TokensPlan p;
   static const int knob_rows = env_int("TRACEA_B200_MX_TOKENS", tb200::kTokMaxRows);
   static const int knob_fused = env_int("TRACEA_B200_MX_FUSED", 64);
   const long long n_tiles = ceil_div(N, 128), k_iters = ceil_div(K, 256), m_tiles = ceil_div(M, tb200::kTokMaxRows);
-  if (knob_rows == 0 || m_tiles * n_tiles > num_sms) return p;
+  if (knob_rows == 0 || (M > 64 && m_tiles * n_tiles > num_sms)) return p;
   int split = 1;
   while (split < (to_mx ? 4 : 8) && 2 * split <= k_iters && m_tiles * n_tiles * 2 * split <= num_sms) split *= 2;
   if (!(M <= 32 || (M <= 64 && k_iters >= 8) || (split > 1 && k_iters >= 16))) return p;
@@ -198,9 +202,11 @@ TokensPlan plan_tokens(long long M, long long N, long long K, bool to_mx, bool i
   p.split = split;
   p.steps = static_cast<int>(ceil_div(k_iters, split));
   p.fused = in_place && M <= 16 && M * p.steps <= knob_fused && p.steps <= tb200::kTokFusedSteps;
-  const int room = 232448 - 1024 - tb200::kTokBarrierBytes - (p.fused ? p.steps * static_cast<int>(tb200::tok_step_bytes(p.cols)) : 0);
+  // more CTAs than SMs: two to an SM
+  const int share = m_tiles * n_tiles * split > num_sms ? 232448 / 2 - 1024 : 232448;
+  const int room = share - 1024 - tb200::kTokBarrierBytes - (p.fused ? p.steps * static_cast<int>(tb200::tok_step_bytes(p.cols)) : 0);
   const int stage = static_cast<int>(tb200::kTokWBytes + (p.fused ? 0u : tb200::tok_step_bytes(p.cols)));
-  p.stages = std::min({p.steps, tb200::kTokMaxStages, room / stage});
+  p.stages = std::max(1, std::min({p.steps, tb200::kTokMaxStages, room / stage}));
   return p;
 }
 

@@ -1,5 +1,6 @@
 """torch.nn front end of the conv path: the reference's `TraceaConv2d` / `patch_conv2d`
-(tracea-python/python/tracea/__init__.py:19-56), forward only.
+(tracea-python/python/tracea/__init__.py:19-56), forward only; and of the 4-bit products, `MxLinear` and `MxFeedForward`, which
+the reference does not have.
 
 Differences from the reference's module, all deliberate:
   * dilation > 1 is computed here (the reference falls back to PyTorch for it);
@@ -43,6 +44,71 @@ class TraceaConv2d(torch.nn.Conv2d):
         bias = self.bias.detach() if self.bias is not None else None
         return ops.conv2d_nchw(x, self._kernel_weight(), bias, None, self.stride, self.padding, self.dilation, 1,
                                "bias" if bias is not None else None)
+
+
+class MxLinear(torch.nn.Linear):
+    """Drop-in for torch.nn.Linear on CUDA tensors whose weight and input are multiplied in the 4-bit microscaled format
+    (``ops.mx_gemm``): the weight is quantised once per version, the input, of any leading shape and fp32, fp16 or bf16, in every
+    call. The output has the input's type; ``epilogue`` is an activation of ``ops.gemm``. Forward only, as TraceaConv2d."""
+
+    def __init__(self, in_features, out_features, bias=True, epilogue=None, device=None, dtype=None):
+        super().__init__(in_features, out_features, bias, device, dtype)
+        if epilogue not in (None, "relu", "silu"):
+            raise NotImplementedError("MxLinear: epilogue=%r is not supported" % (epilogue,))
+        self.epilogue = epilogue
+
+    def _kernel_weight(self):
+        w = self.weight.detach()
+        if w.is_inference():                      # no version to go by
+            return ops.mx_quantize(w)
+        # The cached entry holds the weight it was made from, so that another one cannot lie at its address.
+        cached = getattr(self, "_tracea_quantized", None)
+        if (cached is None or cached[1] != w._version or cached[0].data_ptr() != w.data_ptr() or cached[0].dtype != w.dtype
+                or cached[0].device != w.device or cached[0].shape != w.shape or cached[0].stride() != w.stride()):
+            cached = (w, w._version, ops.mx_quantize(w))
+            self._tracea_quantized = cached
+        return cached[2]
+
+    def requantize(self):
+        """Forget the quantised weight. Needed after a change that torch does not count, one through ``weight.data``."""
+        self._tracea_quantized = None
+
+    def product(self, rows, dtype=None, quantize=False):
+        """The layer on (M, in_features) rows, a tensor or an MxTensor; see ``ops.mx_gemm`` for dtype and quantize."""
+        bias = None if self.bias is None else self.bias.detach()
+        if bias is not None and bias.dtype != torch.float32:
+            bias = bias.float()
+        parts = [p for p in ("bias" if bias is not None else None, self.epilogue) if p]
+        return ops.mx_gemm(rows, self._kernel_weight(), bias, "+".join(parts) or None, None, dtype, quantize)
+
+    def forward(self, x):
+        y = self.product(x.detach().reshape(-1, self.in_features))
+        return y.view(*x.shape[:-1], self.out_features)
+
+
+class MxFeedForward(torch.nn.Module):
+    """A feed-forward block with a norm in front and one behind it, in four launches:
+
+        r = residual_scale * x + gate * (norm(down(silu(up(norm(x) * (1 + scale) + shift)))))
+
+    Both products read 4-bit operands; the norm in front and the first product write theirs in that format. x: (..., C), its
+    leading dimension the samples when gate, scale or shift, (samples, C), are given. Forward only."""
+
+    def __init__(self, dim, hidden, norm="rms", eps=1e-6, residual_scale=1.0, bias=True, device=None, dtype=None):
+        super().__init__()
+        self.norm, self.eps, self.residual_scale = norm, eps, residual_scale
+        self.pre_weight = torch.nn.Parameter(torch.ones(dim, device=device))
+        self.post_weight = torch.nn.Parameter(torch.ones(dim, device=device))
+        self.up = MxLinear(dim, hidden, bias, "silu", device, dtype)
+        self.down = MxLinear(hidden, dim, bias, None, device, dtype)
+
+    def forward(self, x, gate=None, scale=None, shift=None):
+        rows = x.detach().reshape(-1, x.shape[-1])
+        q = ops.block_norm(rows, self.pre_weight.detach(), None, scale, shift, self.norm, self.eps, quantize=True)
+        h = self.down.product(self.up.product(q, quantize=True), dtype=x.dtype)
+        r = ops.block_norm_add(h, rows, self.post_weight.detach(), gate=gate, residual_scale=self.residual_scale, kind=self.norm,
+                               eps=self.eps)
+        return r.view(x.shape)
 
 
 def patch_conv2d():
