@@ -63,18 +63,22 @@ struct RowSlice {
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = col(i, t, j) < C ? OutTraits<T>::to_f(p[col(i, t, j)]) : 0.0f;
   }
-  // kRowsVec: the same by way of shared memory; nothing is copied, and zeros are read, where there is no column or row.
+  // kRowsVec: the same by way of shared memory. Columns past C are never copied: their places hold zeros from the start.
   __device__ __forceinline__ static void copy(uint32_t smem, const T* p, int i, int t, int C, bool live) {
     if (live && col(i, t, 0) < C) {
 #pragma unroll
       for (int q = 0; q < kBytes / 16; ++q) ptx::cp_async_16(smem + 16 * q, reinterpret_cast<const uint4*>(p + col(i, t, 0)) + q);
     }
   }
-  __device__ __forceinline__ static void copied(uint32_t smem, int i, int t, int C, float (&v)[8]) {
+  __device__ __forceinline__ static void copied(uint32_t smem, float (&v)[8]) {
     __align__(16) uint4 raw[kBytes / 16];
 #pragma unroll
-    for (int q = 0; q < kBytes / 16; ++q) raw[q] = col(i, t, 0) < C ? ptx::ld_shared_v4(smem + 16 * q) : make_uint4(0u, 0u, 0u, 0u);
+    for (int q = 0; q < kBytes / 16; ++q) raw[q] = ptx::ld_shared_v4(smem + 16 * q);
     load8<T>(reinterpret_cast<const T*>(raw), v);
+  }
+  __device__ __forceinline__ static void zero(uint32_t smem) {
+#pragma unroll
+    for (int q = 0; q < kBytes / 16; ++q) ptx::st_shared_v4(smem + 16 * q, make_uint4(0u, 0u, 0u, 0u));
   }
   __device__ __forceinline__ static void store(T* p, int i, int t, int C, const float (&v)[8]) {
     if constexpr (kMode == kRowsVec) {
@@ -133,29 +137,33 @@ __device__ __forceinline__ void norm_affine8(const NormStage& s, const NormVecto
 }
 __device__ __forceinline__ bool has_shift(const NormStage& s) { return s.bias.ptr != nullptr || s.shift.ptr != nullptr; }
 
-// A CTA's rows are walked by groups of kThreads threads.
-__host__ __device__ constexpr int norm_block_threads(int row_threads) { return row_threads < 256 ? 256 : row_threads; }
+// A CTA's rows are walked by groups of kThreads threads. A join's CTA is as large as an SM holds where rows are short: with 256
+// threads each, copies of the vectors took shared memory that rows on their way can use (65536 x 256 bf16 and next norm 24.5 ->
+// 20.9 us; of 4096 columns it would cost, 91 -> 100).
+__host__ __device__ constexpr int norm_block_threads(int row_threads, bool join) {
+  return join && row_threads <= 64 ? 768 : (row_threads < 256 ? 256 : row_threads);
+}
 
 // A barrier of the threads of a row.
-template <int kThreads>
+template <int kThreads, int kBlock>
 __device__ __forceinline__ void row_barrier(int warp) {
   if constexpr (kThreads == 32) __syncwarp();
-  else if constexpr (kThreads == norm_block_threads(kThreads)) __syncthreads();
+  else if constexpr (kThreads == kBlock) __syncthreads();
   else asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / (kThreads / 32)), "n"(kThreads) : "memory");
 }
 
 // The sum over the threads of a row, in every one of them, always in the same order. `slot` alternates between two buffers: the
 // barrier of one sum is behind every read of the sum before it.
-template <int kThreads>
+template <int kThreads, int kBlock>
 __device__ __forceinline__ float row_sum(float v, float* smem, uint32_t& slot, int lane, int warp) {
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
   if constexpr (kThreads > 32) {
     constexpr int kWarps = kThreads / 32;
-    float* s = smem + slot * 16;
+    float* s = smem + slot * 32;
     slot ^= 1u;
     if (lane == 0) s[warp] = v;
-    row_barrier<kThreads>(warp);
+    row_barrier<kThreads, kBlock>(warp);
     s += warp / kWarps * kWarps;                 // the row's warps
     if constexpr (kWarps == 2) {
       v = s[0] + s[1];
@@ -171,8 +179,8 @@ __device__ __forceinline__ float row_sum(float v, float* smem, uint32_t& slot, i
   return v;
 }
 
-// v, the row with zeros past column C, becomes norm(v); columns past C are undefined.
-template <int kMode, int kThreads, int kVecs>
+// v, the row with zeros past column C, becomes norm(v), zeros where they were.
+template <int kMode, int kThreads, int kVecs, int kBlock>
 __device__ __forceinline__ void norm_row(const NormStage& s, float (&v)[kVecs][8], int C, float inv_C, int t, float* smem,
                                          uint32_t& slot, int lane, int warp) {
   using Slice = RowSlice<float, kMode, kThreads>;
@@ -184,18 +192,14 @@ __device__ __forceinline__ void norm_row(const NormStage& s, float (&v)[kVecs][8
 #pragma unroll
       for (int j = 0; j < 8; j += 2) add2(a, b, v[i][j], v[i][j + 1]);
     // divided, not multiplied by 1 / C: the mean of a constant row is its constant then, where the sums are exact
-    const float mean = row_sum<kThreads>(a + b, smem, slot, lane, warp) / static_cast<float>(C);
+    const float mean = row_sum<kThreads, kBlock>(a + b, smem, slot, lane, warp) / static_cast<float>(C);
 #pragma unroll
     for (int i = 0; i < kVecs; ++i)
 #pragma unroll
       for (int j = 0; j < 8; j += 2) {
-        add2(v[i][j], v[i][j + 1], -mean, -mean);
-        if constexpr (kMode != kRowsVec) {
-          if (Slice::col(i, t, j) >= C) v[i][j] = 0.0f;
-          if (Slice::col(i, t, j + 1) >= C) v[i][j + 1] = 0.0f;
-        } else if (Slice::col(i, t, 0) >= C) {
-          v[i][j] = v[i][j + 1] = 0.0f;
-        }
+        const float m0 = Slice::col(i, t, kMode == kRowsVec ? 0 : j) < C ? mean : 0.0f;
+        const float m1 = Slice::col(i, t, kMode == kRowsVec ? 0 : j + 1) < C ? mean : 0.0f;
+        add2(v[i][j], v[i][j + 1], -m0, -m1);
       }
   }
   float a = 0.0f, b = 0.0f;
@@ -208,7 +212,7 @@ __device__ __forceinline__ void norm_row(const NormStage& s, float (&v)[kVecs][8
       a = x;
       b = y;
     }
-  const float inv = rsqrtf(fmaf(row_sum<kThreads>(a + b, smem, slot, lane, warp), inv_C, s.eps));
+  const float inv = rsqrtf(fmaf(row_sum<kThreads, kBlock>(a + b, smem, slot, lane, warp), inv_C, s.eps));
 #pragma unroll
   for (int i = 0; i < kVecs; ++i)
 #pragma unroll
@@ -256,11 +260,11 @@ __host__ __device__ constexpr int norm_kept_bytes(int threads, int vecs, bool jo
   return norm_keeps(threads, vecs) ? threads * vecs * 8 * 2 * 4 * ((join ? 1 : 0) + (next != kNextNone ? 1 : 0)) : 0;
 }
 __host__ __device__ constexpr int norm_row_bytes(int threads, int vecs, bool join, int es) {
-  return norm_block_threads(threads) * vecs * 8 * es * (join ? 2 : 1);
+  return norm_block_threads(threads, join) * vecs * 8 * es * (join ? 2 : 1);
 }
-// CTAs an SM is to hold: 64 registers a thread, 128 for joins and for more than sixteen columns.
+// CTAs an SM is to hold: 1024 threads of 64 registers; joins 768 of 80 or 512 of 128, which more than sixteen columns have too.
 __host__ __device__ constexpr int norm_blocks_per_sm(int threads, int vecs, bool join) {
-  return (vecs <= 2 && !join ? 1024 : 512) / norm_block_threads(threads);
+  return join && threads <= 64 ? 1 : (vecs <= 2 && !join ? 1024 : 512) / norm_block_threads(threads, join);
 }
 // Rows ahead: what the CTA's share of 190 KB of shared memory holds, four at most.
 __host__ __device__ constexpr int norm_depth(int threads, int vecs, bool join, int next, int es) {
@@ -274,21 +278,21 @@ __host__ __device__ constexpr int norm_join_mode(int mode) { return mode == kRow
 __host__ __device__ constexpr int norm_smem_bytes(int threads, int vecs, int mode, bool join, int next, int es) {
   return norm_kept_bytes(threads, vecs, join, next) +
          (mode == kRowsVec ? norm_depth(threads, vecs, join, next, es) * norm_row_bytes(threads, vecs, join, es)
-                           : (mode == kRowsSingle && join ? norm_block_threads(threads) * vecs * 8 * 4 : 0));
+                           : (mode == kRowsSingle && join ? norm_block_threads(threads, join) * vecs * 8 * 4 : 0));
 }
 
 template <typename T, int kThreads, int kVecs, int kMode, bool kJoin, int kNext>
-__global__ void __launch_bounds__(norm_block_threads(kThreads), norm_blocks_per_sm(kThreads, kVecs, kJoin))
+__global__ void __launch_bounds__(norm_block_threads(kThreads, kJoin), norm_blocks_per_sm(kThreads, kVecs, kJoin))
 block_norm_kernel(const __grid_constant__ BlockNormArgs a) {
   static_assert(!(kMode == kRowsSpread && kNext == kNextMx), "a block of the format is four neighbouring threads' columns");
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();
   extern __shared__ __align__(16) uint8_t dynamic[];
-  __shared__ __align__(16) float sums[32];
+  __shared__ __align__(16) float sums[64];
   using Slice = RowSlice<T, kMode, kThreads>;
   constexpr int kJoinMode = norm_join_mode(kMode);
   using JoinSlice = RowSlice<T, kJoin ? kJoinMode : kMode, kThreads>;
-  constexpr int kBlock = norm_block_threads(kThreads);
+  constexpr int kBlock = norm_block_threads(kThreads, kJoin);
   constexpr int kRows = kBlock / kThreads;                              // that a CTA has in hand at a time
   constexpr bool kKeep = norm_keeps(kThreads, kVecs);
   constexpr int kSlices = kThreads * kVecs;                             // of eight columns
@@ -308,6 +312,13 @@ block_norm_kernel(const __grid_constant__ BlockNormArgs a) {
   const uint32_t ring0 = ptx::smem_u32(dynamic) + norm_kept_bytes(kThreads, kVecs, kJoin, kNext) + threadIdx.x * Slice::kBytes;
   uint32_t ring_at = ring0;
 
+  if constexpr (kMode == kRowsVec) {
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i)
+      if (Slice::col(i, t, 0) >= C)
+#pragma unroll 1
+        for (uint32_t at = ring0 + i * kSliceBytes; at < ring0 + kDepth * kRowBytes; at += kVecs * kSliceBytes) Slice::zero(at);
+  }
   const int first = static_cast<int>(static_cast<long long>(blockIdx.x) * a.M / gridDim.x);
   const int last = static_cast<int>((static_cast<long long>(blockIdx.x) + 1) * a.M / gridDim.x);
   for (int seg = first; seg < last;) {                                  // rows of one group
@@ -365,8 +376,8 @@ block_norm_kernel(const __grid_constant__ BlockNormArgs a) {
       for (int i = 0; i < kVecs; ++i) {
         float(&xd)[8] = kJoin ? xv[i] : v[i];
         if constexpr (kMode == kRowsVec) {
-          Slice::copied(ring_at + i * kSliceBytes, i, t, C, xd);
-          if constexpr (kJoin) Slice::copied(ring_at + (kVecs + i) * kSliceBytes, i, t, C, v[i]);
+          Slice::copied(ring_at + i * kSliceBytes, xd);
+          if constexpr (kJoin) Slice::copied(ring_at + (kVecs + i) * kSliceBytes, v[i]);
         } else {
           JoinSlice::load(x, i, t, C, xd);
           if constexpr (kJoin) JoinSlice::load(h, i, t, C, v[i]);
@@ -379,7 +390,7 @@ block_norm_kernel(const __grid_constant__ BlockNormArgs a) {
         if constexpr (kJoin) h += h_step;
       }
       if constexpr (kJoin) {
-        norm_row<kJoinMode, kThreads, kVecs>(a.join, v, C, inv_C, t, sums, slot, lane, warp);
+        norm_row<kJoinMode, kThreads, kVecs, kBlock>(a.join, v, C, inv_C, t, sums, slot, lane, warp);
 #pragma unroll
         for (int i = 0; i < kVecs; ++i) {
           norm_apply8<T, kJoinMode, kThreads, kVecs, kKeep>(a.join, &a.gate, kept_join, group, join_shift, i, t, C, v[i]);
@@ -390,11 +401,23 @@ block_norm_kernel(const __grid_constant__ BlockNormArgs a) {
             v[i][j] = p;
             v[i][j + 1] = q;
           }
-          JoinSlice::store(r, i, t, C, v[i]);
-          if constexpr (kNext != kNextNone) {
+          if constexpr (kMode == kRowsVec && sizeof(T) == 2) {         // rounded once, stored and read back from that
+            uint4 w;
+            w.x = pack2<T, false>(v[i][0], v[i][1]);
+            w.y = pack2<T, false>(v[i][2], v[i][3]);
+            w.z = pack2<T, false>(v[i][4], v[i][5]);
+            w.w = pack2<T, false>(v[i][6], v[i][7]);
+            if (JoinSlice::col(i, t, 0) < C) *reinterpret_cast<uint4*>(r + JoinSlice::col(i, t, 0)) = w;
+            load8<T>(reinterpret_cast<const T*>(&w), v[i]);
+          } else {
+            JoinSlice::store(r, i, t, C, v[i]);
+          }
+          if constexpr (kNext != kNextNone && !(kMode == kRowsVec && sizeof(T) == 2)) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              v[i][j] = JoinSlice::col(i, t, kMode == kRowsVec ? 0 : j) < C ? OutTraits<T>::to_f(OutTraits<T>::from_f(v[i][j])) : 0.0f;
+            for (int j = 0; j < 8; ++j) {
+              v[i][j] = OutTraits<T>::to_f(OutTraits<T>::from_f(v[i][j]));
+              if (kMode != kRowsVec && JoinSlice::col(i, t, j) >= C) v[i][j] = 0.0f;    // kRowsVec: it is, a being 1 and b 0 there
+            }
           }
         }
         r += kRows * a.r_stride;
@@ -404,16 +427,16 @@ block_norm_kernel(const __grid_constant__ BlockNormArgs a) {
           for (int i = 0; i < kVecs; ++i)
 #pragma unroll
             for (int j = 0; j < 8; ++j) exchange[JoinSlice::col(i, t, j)] = v[i][j];
-          row_barrier<kThreads>(warp);
+          row_barrier<kThreads, kBlock>(warp);
 #pragma unroll
           for (int i = 0; i < kVecs; ++i)
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[i][j] = exchange[Slice::col(i, t, j)];
-          row_barrier<kThreads>(warp);                                  // before the next row is written there
+          row_barrier<kThreads, kBlock>(warp);                                  // before the next row is written there
         }
       }
       if constexpr (kNext != kNextNone) {
-        norm_row<kMode, kThreads, kVecs>(a.norm, v, C, inv_C, t, sums, slot, lane, warp);
+        norm_row<kMode, kThreads, kVecs, kBlock>(a.norm, v, C, inv_C, t, sums, slot, lane, warp);
 #pragma unroll
         for (int i = 0; i < kVecs; ++i) {
           norm_apply8<T, kMode, kThreads, kVecs, kKeep>(a.norm, nullptr, kept_norm, group, norm_shift, i, t, C, v[i]);
@@ -423,7 +446,7 @@ block_norm_kernel(const __grid_constant__ BlockNormArgs a) {
             const int col = Slice::col(i, t, 0);
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-              if (col + (kMode == kRowsVec ? 0 : j) >= C) v[i][j] = 0.0f;
+              if (kMode != kRowsVec && col + j >= C) v[i][j] = 0.0f;
             uint32_t byte;
             const uint32_t codes = mx_quantize8(v[i], byte);            // the whole warp: blocks are shared by lanes
             if ((col >> 5) < a.blocks) *reinterpret_cast<uint32_t*>(a.codes + row * (16LL * a.blocks) + (col >> 1)) = codes;
