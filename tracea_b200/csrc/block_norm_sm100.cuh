@@ -139,9 +139,9 @@ __device__ __forceinline__ bool has_shift(const NormStage& s) { return s.bias.pt
 
 // A CTA's rows are walked by groups of kThreads threads. A join's CTA is as large as an SM holds where rows are short: with 256
 // threads each, copies of the vectors took shared memory that rows on their way can use (65536 x 256 bf16 and next norm 24.5 ->
-// 20.9 us; of 4096 columns it would cost, 91 -> 100).
+// 20.9 us; of 1001 columns, 333 rows, it would cost, 3.7 -> 4.8, of 4096, 91 -> 100).
 __host__ __device__ constexpr int norm_block_threads(int row_threads, bool join) {
-  return join && row_threads <= 64 ? 768 : (row_threads < 256 ? 256 : row_threads);
+  return join && row_threads == 32 ? 768 : (row_threads < 256 ? 256 : row_threads);
 }
 
 // A barrier of the threads of a row.
@@ -264,7 +264,7 @@ __host__ __device__ constexpr int norm_row_bytes(int threads, int vecs, bool joi
 }
 // CTAs an SM is to hold: 1024 threads of 64 registers; joins 768 of 80 or 512 of 128, which more than sixteen columns have too.
 __host__ __device__ constexpr int norm_blocks_per_sm(int threads, int vecs, bool join) {
-  return join && threads <= 64 ? 1 : (vecs <= 2 && !join ? 1024 : 512) / norm_block_threads(threads, join);
+  return join && threads == 32 ? 1 : (vecs <= 2 && !join ? 1024 : 512) / norm_block_threads(threads, join);
 }
 // Rows ahead: what the CTA's share of 190 KB of shared memory holds, four at most.
 __host__ __device__ constexpr int norm_depth(int threads, int vecs, bool join, int next, int es) {
