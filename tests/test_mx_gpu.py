@@ -255,6 +255,36 @@ def test_every_tile_width_is_right_for_every_size(columns):
     assert r.returncode == 0 and "forms ok" in r.stdout, r.stdout[-2000:] + r.stderr[-2000:]
 
 
+@pytest.mark.parametrize("m, n, k", [(1, 70, 100), (5, 1000, 2048), (40, 33, 64), (300, 161, 300), (700, 1001, 513), (2500, 2500, 256)])
+def test_scales_of_rows_past_the_end_reach_no_bit(m, n, k):
+    """0, NaN and random bytes there: the same results, where neighbouring columns share a reciprocal above all."""
+    a, _ = matrix(m, k, 20)
+    w, _ = matrix(n, k, 21, 0.3)
+    bias = torch.randn(n, generator=torch.Generator().manual_seed(1)).cuda()
+    gen = torch.Generator(device="cuda").manual_seed(2)
+
+    def refilled(q, fill):
+        rows = torch.arange(q.scales.shape[0] * 128, device="cuda").view(-1, 4, 32).permute(0, 2, 1)     # row of (tile, lane, word)
+        past = (rows >= q.shape[0])[:, None, :, :, None].expand(-1, q.scales.shape[1], -1, -1, 4).reshape(q.scales.shape)
+        s = q.scales.clone()
+        other = torch.randint(0, 256, s.shape, generator=gen, device="cuda", dtype=torch.uint8) if fill is None else torch.full_like(s, fill)
+        s[past] = other[past]
+        return ops.MxTensor(q.data, s, q.shape)
+
+    for e in ("bias+silu", "bias", "gelu"):
+        b = bias if "bias" in e else None
+        for out in (torch.bfloat16, torch.float32):
+            first = ops.mx_gemm(a, w, b, e, dtype=out)
+            assert not first.isnan().any()
+            for fill in (0, None, 130):
+                assert torch.equal(ops.mx_gemm(refilled(a, fill), refilled(w, fill), b, e, dtype=out), first)
+        q = ops.mx_gemm(a, w, b, e, quantize=True)
+        for fill in (0, None):
+            q2 = ops.mx_gemm(refilled(a, fill), refilled(w, fill), b, e, quantize=True)
+            assert torch.equal(q2.data, q.data) and torch.equal(q2.dequantize(torch.float32), q.dequantize(torch.float32))
+    status_ok()
+
+
 def test_a_nan_block_reaches_its_row_and_nothing_else():
     for m, n, k in ((3, 200, 300), (300, 200, 300)):
         a, av = matrix(m, k, 6)

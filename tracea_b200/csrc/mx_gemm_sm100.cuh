@@ -67,7 +67,8 @@ __host__ __device__ constexpr int mx_scale_cols(int bn) { return 8 + 8 * mx_b_sc
 // apply_act32 with fewer trips through the special-function unit, which bounds SiLU here: a tile of 192 columns of 1024 takes
 // 2200 cycles of MMAs and 128 x 192 exponentials and reciprocals, at 16 of these a cycle, 3100. Four values share a reciprocal,
 // 1 / a = (1 / abcd) bcd, which costs three roundings more, 2^-22 -- far below a 16- or 4-bit result's. The product of four stays
-// in range while each 1 + e^-x is below 2^31: a warp with a value below -20, or a NaN, takes the other way.
+// in range while each 1 + e^-x is below 2^31: 32 columns of a row with a value below -20, or a NaN, take the other way. (Each lane
+// for itself: rows past M, whose scales are anyone's, must not choose for the others.)
 template <bool kFast>
 __device__ __forceinline__ void mx_act32(float (&f)[32], int act) {
   if (!kFast || act != kActSilu) {
@@ -78,7 +79,7 @@ __device__ __forceinline__ void mx_act32(float (&f)[32], int act) {
 #pragma unroll
   for (int j = 1; j < 31; j += 2) low = min_nan3(low, f[j], f[j + 1]);
   low = min_nan3(low, f[31], f[31]);
-  if (!__all_sync(0xffffffffu, low >= -20.0f)) {
+  if (!(low >= -20.0f)) {
     apply_act32<kFast>(f, act);
     return;
   }
@@ -496,14 +497,14 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
             add2(f[j4 * 4 + 0], f[j4 * 4 + 1], b4.x, b4.y);
             add2(f[j4 * 4 + 2], f[j4 * 4 + 3], b4.z, b4.w);
           }
+          // columns past N: their scales are whatever lies behind the last row of W, and may not reach their neighbours' results
+          if (n0 + h * 32 + 32 > args.N) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (n0 + h * 32 + j >= args.N) f[j] = 0.0f;
+          }
           if constexpr (kStore == kMxStoreMx) {
             mx_act32<true>(f, args.act);
-            // columns past N: their scales are whatever lies behind the last row of W, and may not reach the block's
-            if (n0 + h * 32 + 32 > args.N) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (n0 + h * 32 + j >= args.N) f[j] = 0.0f;
-            }
             uint32_t byte;
             packed[h] = mx_quantize32(f, byte);
             scale_bytes = byte;
