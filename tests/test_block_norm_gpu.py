@@ -163,6 +163,33 @@ def test_strided_rows_and_in_place(c, dtype):
     assert_rows(xr, *mxref.norm(d(before), "rms", EPS, d(w)))
 
 
+@pytest.mark.parametrize("c", [40, 333, 1024, 2051, 5000])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("quantize", [False, True])
+def test_result_over_the_blocks_output(c, dtype, quantize):
+    """r over h, with a norm behind it, more rows than the grid has CTAs; and an x that is one row for all."""
+    m = 700
+    h, x = rows(m, c, dtype, 10), rows(1, c, dtype, 11).expand(m, c)
+    s = stage(vectors(c, 7, torch.float32, 3), ("scale", "shift"))
+    want_r, want_y = ops.block_norm_add(h, x, **s, kind="layer", following={"kind": "rms", "quantize": quantize})
+    y64, err = mxref.norm(d(h), "layer", EPS, scale=d(s["scale"]), shift=d(s["shift"]))
+    assert_rows(want_r, d(x) + y64, err + 8 * 2.0 ** -24 * (2 * np.abs(y64) + 4 + np.abs(d(x))))
+    as_view = lambda t: ffi.View(t.data_ptr(), t.shape, t.stride(), ops._DTYPES[t.dtype], 0)
+    over, y = h.clone(), torch.empty_like(h)
+    vh, vx, vs, vt, vy = (as_view(t) for t in (over, x, s["scale"], s["shift"], y))
+    n = ffi.Norm(ffi.NORM_LAYER, EPS, None, None, ctypes.pointer(vs.c), ctypes.pointer(vt.c))
+    f = ffi.Norm(ffi.NORM_RMS, EPS)
+    q = ops.mx_quantize(h)
+    mq = ffi.MxMatrix(q.data.data_ptr(), q.scales.data_ptr(), m, c, 0)
+    st = ffi.load().tracea_block_norm_add(vh.c, vx.c, ctypes.byref(n), None, 1.0, ctypes.byref(vh.c), ctypes.byref(f),
+                                          None if quantize else ctypes.byref(vy.c), ctypes.byref(mq) if quantize else None,
+                                          torch.cuda.current_stream().cuda_stream)
+    assert st == ffi.SUCCESS, ffi.last_error()
+    torch.cuda.synchronize()
+    assert torch.equal(over, want_r)
+    assert torch.equal(q.data, want_y.data) if quantize else torch.equal(y, want_y)
+
+
 def test_quantized_rows_leave_the_scales_of_rows_behind_them():
     x = rows(130, 300, "bf16", 8)
     lib = ffi.load()

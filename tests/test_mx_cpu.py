@@ -134,6 +134,14 @@ def test_gemm_refuses(lib, a, w, bias, res, c, cq, kind, status, text):
     refused(status, text, lib.tracea_mx_linear(x.c, w, opt(bias), opt(res), opt(c), q, p))
 
 
+@pytest.mark.parametrize("dtype", [ffi.DTYPE_FLOAT32, ffi.DTYPE_BFLOAT16])
+def test_a_bias_between_elements_is_refused(lib, dtype):
+    bias = ffi.View(P + 1, (16,), (1,), dtype, 0)
+    p = ffi.GemmParams(ffi.EPILOGUE_BIAS_ADD, None)
+    refused(ffi.INVALID_PARAMS, "bias is not aligned", lib.tracea_mx_gemm(A, W, opt(bias), None, opt(C), None, p))
+    refused(ffi.INVALID_PARAMS, "bias is not aligned", lib.tracea_mx_linear(view((8, 64)).c, W, opt(bias), None, opt(C), None, p))
+
+
 X = view((6, 40))
 V = view((40,), dtype=ffi.DTYPE_FLOAT32)
 

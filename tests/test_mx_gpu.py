@@ -10,6 +10,7 @@ import ctypes
 import os
 import subprocess
 import sys
+import threading
 
 import numpy as np
 import pytest
@@ -339,6 +340,99 @@ def test_strided_outputs_and_residuals(m, n, k, out):
         assert torch.equal(c, kept)
 
 
+# more CTAs than SMs; several groups of rows, the last one of a single row; and both with the input quantised inside
+@pytest.mark.parametrize("m, n, k", [(1, 20011, 300), (7, 19300, 64), (33, 25000, 100), (64, 19999, 2050), (129, 300, 4100), (200, 130, 8192),
+                                     (450, 300, 4097), (385, 40, 10000)])
+def test_few_rows_beyond_one_wave_and_beyond_one_group(m, n, k):
+    w, wv = matrix(n, k, 2, k ** -0.5)
+    x = torch.randn(m, k, generator=torch.Generator().manual_seed(m)).bfloat16()
+    av = torch.from_numpy(mxref.values(x.double().numpy())).cuda()
+    bias = torch.randn(n, generator=torch.Generator().manual_seed(n)).cuda()
+    res = torch.randn(m, n, generator=torch.Generator().manual_seed(k)).bfloat16().cuda()
+    lib = ffi.load()
+    for a in (x.cuda(), ops.mx_quantize(x.cuda())):
+        before = lib.tracea_b200_launch_count_of(ffi.KERNEL_MX_TOKENS)
+        assert_close(ops.mx_gemm(a, w, bias, "bias+residual", res), *reference(av, wv, "bias+residual", bias, res, torch.bfloat16))
+        assert_quantized(ops.mx_gemm(a, w, bias, "bias+silu", quantize=True), *reference(av, wv, "bias+silu", bias, None, torch.bfloat16))
+        few = m <= 32 or k > 7 * 256                  # more rows than 32 take that form over a longer K only
+        assert lib.tracea_b200_launch_count_of(ffi.KERNEL_MX_TOKENS) == before + (2 if few else 0)
+    status_ok()
+
+
+@pytest.mark.parametrize("m, k", [(1, 64), (5, 4096), (300, 64), (1000, 513)])
+def test_one_column_and_a_matrix_times_itself(m, k):
+    a, av = matrix(m, k, 8)
+    assert_close(ops.mx_gemm(a, a, dtype=torch.float32), *reference(av, av, None, None, None, torch.float32))
+    w, wv = matrix(1, k, 9)
+    for pitch, dtype in ((1, torch.bfloat16), (8, torch.bfloat16), (3, torch.float32), (4, torch.float32)):
+        whole = torch.full((m, pitch), 7.0, dtype=dtype, device="cuda")
+        c = whole[:, :1]
+        mats = [ffi.MxMatrix(q.data.data_ptr(), q.scales.data_ptr(), *q.shape, 0) for q in (a, w)]
+        v = ffi.View(c.data_ptr(), c.shape, (pitch, 1), ops._DTYPES[dtype], 0)
+        p = ffi.GemmParams(0, torch.cuda.current_stream().cuda_stream)
+        assert ffi.load().tracea_mx_gemm(*mats, None, None, ctypes.byref(v.c), None, p) == ffi.SUCCESS
+        torch.cuda.synchronize()
+        assert_close(c, *reference(av, wv, None, None, None, dtype))
+        assert (whole[:, 1:] == 7).all()
+    status_ok()
+
+
+def test_no_rows():
+    w, _ = matrix(40, 64, 1)
+    x = torch.empty(0, 64, device="cuda")
+    q = ops.mx_quantize(x)
+    assert q.data.shape == (0, 32) and q.scales.shape == (0, 1, 512) and q.dequantize().shape == (0, 64)
+    for a in (x, q):
+        assert ops.mx_gemm(a, w).shape == (0, 40) and ops.mx_gemm(a, w, quantize=True).shape == (0, 40)
+    assert ops.block_norm(x).shape == (0, 64) and ops.block_norm(x, quantize=True).shape == (0, 64)
+    r, y = ops.block_norm_add(x, x, following={"quantize": True})
+    assert r.shape == (0, 64) and y.shape == (0, 64)
+    assert nn.MxLinear(64, 40, device="cuda")(x.view(2, 0, 64)).shape == (2, 0, 40)
+    assert nn.MxFeedForward(64, 40, device="cuda")(x.view(2, 0, 64)).shape == (2, 0, 64)
+    with pytest.raises(ffi.TraceaError, match="no rows"):
+        ops.mx_gemm(ops.mx_quantize(torch.ones(3, 64, device="cuda")), q)
+
+
+def test_two_threads_at_once():
+    a, _ = matrix(500, 1024, 1)
+    w, _ = matrix(600, 1024, 2, 0.03)
+    x = torch.randn(5, 1024, device="cuda").bfloat16()
+    wanted = [ops.mx_gemm(a, w), ops.mx_gemm(x, w), ops.block_norm(x, kind="layer")]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def worker():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(100):
+                got = [ops.mx_gemm(a, w), ops.mx_gemm(x, w), ops.block_norm(x, kind="layer")]
+                torch.cuda.current_stream().synchronize()
+                wrong.extend(1 for g, t in zip(got, wanted) if not torch.equal(g, t))
+
+    threads = [threading.Thread(target=worker) for _ in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    status_ok()
+
+
+def test_another_device_than_the_current_one():
+    if torch.cuda.device_count() < 2:
+        pytest.skip("needs two GPUs")
+    with torch.cuda.device(1):
+        x, wt = torch.randn(5, 256).cuda(), torch.randn(200, 256).cuda()
+    with torch.cuda.device(0):
+        w = ops.mx_quantize(wt)
+        got = [ops.mx_gemm(x, w), ops.mx_gemm(x, w, quantize=True).dequantize(), ops.block_norm_add(x, x)]
+        torch.cuda.synchronize(1)
+    with torch.cuda.device(1):
+        want = [ops.mx_gemm(x, w), ops.mx_gemm(x, w, quantize=True).dequantize(), ops.block_norm_add(x, x)]
+    assert all(torch.equal(g, t) for g, t in zip(got, want))
+    with pytest.raises(ffi.TraceaError, match="is on device"):
+        ops.mx_gemm(x.to("cuda:0"), w)
+
+
 def test_the_same_call_gives_the_same_bits():
     for m, n, k in ((1, 4096, 4096), (48, 256, 16384), (700, 900, 1000), (2100, 2100, 2100)):
         a, _ = matrix(m, k, 10)
@@ -465,6 +559,64 @@ def test_linear_module():
         assert_close(lin(x).view(10, 130), *reference(xv, wv(), "bias+silu", lin.bias.detach(), None, torch.float32))
     half = nn.MxLinear(64, 32, bias=False, device="cuda", dtype=torch.float16)
     assert half(torch.randn(3, 64, device="cuda").half()).dtype == torch.float16
+
+
+def test_linear_module_on_other_streams_and_in_graphs():
+    lin = nn.MxLinear(512, 256, device="cuda", epilogue="silu")
+    x = torch.randn(3, 512, device="cuda")
+
+    def change():
+        lin.weight.data.copy_(torch.randn(256, 512, device="cuda"))
+        lin.requantize()
+
+    result = lambda: ops.mx_gemm(x, ops.mx_quantize(lin.weight.detach()), lin.bias.detach(), "bias+silu")
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):                                # the first stream is late with the quantised weight
+        change()
+        torch.cuda.synchronize()
+        got = []
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                if i == 0:
+                    torch.cuda._sleep(20000000)
+                got.append(lin(x))
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], result()) and torch.equal(got[1], result())
+    # quantised in the graph: nothing to read before a replay, and each replay reads the weight as it is
+    change()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = lin(x)
+    assert torch.equal(lin(x), result())
+    for _ in range(2):
+        change()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, result())
+    # quantised before: the graph keeps to that weight after the layer has dropped it
+    lin(x)
+    h = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(h):
+        y = lin(x)
+    old = result()
+    change()
+    for _ in range(50):
+        lin.weight.data.add_(0.0)
+        lin.requantize()
+        assert torch.equal(lin(x), result())
+    junk = [torch.full((256, 256), 119, dtype=torch.uint8, device="cuda") for _ in range(50)]
+    h.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, old) and len(junk) == 50
+    with torch.inference_mode():
+        assert torch.equal(lin(x), result())
+    lin.half()                                        # a 16-bit bias is added as it is, or, into a quantised output, as fp32
+    x = x.half()
+    assert torch.equal(lin(x), result())
+    q = lin.product(x, quantize=True)
+    want = ops.mx_gemm(x, ops.mx_quantize(lin.weight.detach()), lin.bias.detach().float(), "bias+silu", quantize=True)
+    assert torch.equal(q.data, want.data)
+    status_ok()
 
 
 @pytest.mark.parametrize("samples, positions, c, hidden, dtype", [(1, 1, 64, 96, "bf16"), (3, 49, 200, 333, "f16"), (4, 196, 512, 1024, "bf16")])

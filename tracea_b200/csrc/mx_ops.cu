@@ -332,7 +332,8 @@ void mx_product(DeviceState& st, const Product& p, cudaStream_t stream) {
     tiled(__nv_bfloat16{}, 0, std::integral_constant<int, tb200::kMxStoreMx>{});
     return;
   }
-  const bool tma = aligned16(p.out.ptr) && p.out.row_stride * p.out.es % 16 == 0;
+  // (a store that ends inside 16 bytes would write all of them, past a row's end where its stride leaves room)
+  const bool tma = aligned16(p.out.ptr) && p.out.row_stride * p.out.es % 16 == 0 && p.out.cols * p.out.es % 16 == 0;
   by_dtype(p.out.dtype, [&](auto tag) {
     const int dt = p.out.dtype == TRACEA_DTYPE_BFLOAT16 ? 0 : (p.out.dtype == TRACEA_DTYPE_FLOAT16 ? 1 : 2);
     if (tma) tiled(tag, dt, std::integral_constant<int, tb200::kMxStoreTma>{});
@@ -379,6 +380,8 @@ Product check_product(int dev, long long M, long long K, const TraceaMxMatrix& w
     p.bias_is_f32 = biasv->dtype == TRACEA_DTYPE_FLOAT32;
     if (!p.bias_is_f32 && (p.to_mx || biasv->dtype != dtype))
       TB_FAIL(TRACEA_INVALID_PARAMS, "bias must be float32 or have the dtype of c");
+    if ((reinterpret_cast<uintptr_t>(biasv->ptr) & (elem_size(biasv->dtype) - 1)) != 0)
+      TB_FAIL(TRACEA_INVALID_PARAMS, "bias is not aligned to its elements");
     p.bias = biasv->ptr;
   }
   return p;

@@ -49,7 +49,11 @@ class TraceaConv2d(torch.nn.Conv2d):
 class MxLinear(torch.nn.Linear):
     """Drop-in for torch.nn.Linear on CUDA tensors whose weight and input are multiplied in the 4-bit microscaled format
     (``ops.mx_gemm``): the weight is quantised once per version, the input, of any leading shape and fp32, fp16 or bf16, in every
-    call. The output has the input's type; ``epilogue`` is an activation of ``ops.gemm``. Forward only, as TraceaConv2d."""
+    call. The output has the input's type; ``epilogue`` is an activation of ``ops.gemm``. Forward only, as TraceaConv2d.
+
+    A new version waits once for the device: other streams may read the quantised weight from then on. A CUDA graph that is
+    captured with a quantised weight at hand keeps to that one, whatever becomes of the layer's; captured right after
+    ``requantize()`` it quantises the weight in every replay."""
 
     def __init__(self, in_features, out_features, bias=True, epilogue=None, device=None, dtype=None):
         super().__init__(in_features, out_features, bias, device, dtype)
@@ -65,18 +69,28 @@ class MxLinear(torch.nn.Linear):
         cached = getattr(self, "_tracea_quantized", None)
         if (cached is None or cached[1] != w._version or cached[0].data_ptr() != w.data_ptr() or cached[0].dtype != w.dtype
                 or cached[0].device != w.device or cached[0].shape != w.shape or cached[0].stride() != w.stride()):
-            cached = (w, w._version, ops.mx_quantize(w))
-            self._tracea_quantized = cached
+            q = ops.mx_quantize(w)
+            if torch.cuda.is_current_stream_capturing():
+                return q                          # the graph's: nothing is in it before a replay
+            torch.cuda.synchronize(w.device)      # it is complete for every stream, and nothing reads the old one any more
+            self._tracea_quantized = (w, w._version, q)
+            return q
+        if torch.cuda.is_current_stream_capturing():
+            self.__dict__.setdefault("_tracea_captured", {})[id(cached)] = cached     # graphs read it as long as the layer lives
         return cached[2]
 
     def requantize(self):
         """Forget the quantised weight. Needed after a change that torch does not count, one through ``weight.data``."""
+        cached = getattr(self, "_tracea_quantized", None)
+        if cached is not None and not torch.cuda.is_current_stream_capturing():
+            torch.cuda.synchronize(cached[0].device)
         self._tracea_quantized = None
 
     def product(self, rows, dtype=None, quantize=False):
         """The layer on (M, in_features) rows, a tensor or an MxTensor; see ``ops.mx_gemm`` for dtype and quantize."""
         bias = None if self.bias is None else self.bias.detach()
-        if bias is not None and bias.dtype != torch.float32:
+        out = dtype or (torch.bfloat16 if isinstance(rows, ops.MxTensor) else rows.dtype)
+        if bias is not None and bias.dtype != torch.float32 and (quantize or bias.dtype != out):
             bias = bias.float()
         parts = [p for p in ("bias" if bias is not None else None, self.epilogue) if p]
         return ops.mx_gemm(rows, self._kernel_weight(), bias, "+".join(parts) or None, None, dtype, quantize)
@@ -87,7 +101,7 @@ class MxLinear(torch.nn.Linear):
 
 
 class MxFeedForward(torch.nn.Module):
-    """A feed-forward block with a norm in front and one behind it, in four launches:
+    """A feed-forward block with a norm in front and one behind it, in four launches (five where ``up`` has a 16-bit bias):
 
         r = residual_scale * x + gate * (norm(down(silu(up(norm(x) * (1 + scale) + shift)))))
 
