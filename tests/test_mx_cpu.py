@@ -142,6 +142,17 @@ def test_a_bias_between_elements_is_refused(lib, dtype):
     refused(ffi.INVALID_PARAMS, "bias is not aligned", lib.tracea_mx_linear(view((8, 64)).c, W, opt(bias), None, opt(C), None, p))
 
 
+def test_more_rows_than_can_be_numbered_are_refused(lib):
+    x = view(((1 << 31) - 1, 64), device=0)
+    y = view(((1 << 31) - 1, 16), device=0)
+    p = ffi.GemmParams(0, None)
+    refused(ffi.UNSUPPORTED_CONFIG, "rows, at most", lib.tracea_mx_linear(x.c, W, None, None, opt(y), None, p))
+    n = norm()
+    refused(ffi.UNSUPPORTED_CONFIG, "rows, at most", lib.tracea_block_norm(x.c, ctypes.byref(n), opt(x), None, None))
+    refused(ffi.UNSUPPORTED_CONFIG, "rows, at most",
+            lib.tracea_block_norm_add(x.c, x.c, ctypes.byref(n), None, 1.0, opt(x), None, None, None, None))
+
+
 X = view((6, 40))
 V = view((40,), dtype=ffi.DTYPE_FLOAT32)
 

@@ -117,6 +117,7 @@ void block_norm_checked(const TraceaTensorView* hv, const TraceaTensorView& xv, 
   const int dev = xv.device_id;
   if (dev < 0) TB_FAIL(TRACEA_INVALID_PARAMS, "%s takes device tensors (device_id >= 0)", entry);
   const Matrix x = load_matrix(xv, "x", dev);
+  check_rows(x, "x");
   const long long M = x.rows, C = x.cols;
   if (C == 0) TB_FAIL(TRACEA_INVALID_PARAMS, "x has no columns");
   if (C > kNormMaxColumns) TB_FAIL(TRACEA_UNSUPPORTED_CONFIG, "%lld columns: at most %lld", C, kNormMaxColumns);

@@ -52,6 +52,11 @@ inline int row_vec(const void* ptr, long long row_stride, long long cols, int es
   return es;
 }
 
+// Row numbers, and those of rows a CTA looks ahead to, are 32-bit.
+inline void check_rows(const Matrix& m, const char* name) {
+  if (m.rows > 0x7fffff00LL) TB_FAIL(TRACEA_UNSUPPORTED_CONFIG, "%s: %lld rows, at most %lld", name, m.rows, 0x7fffff00LL);
+}
+
 struct Mx {
   uint8_t *data, *scales;
   long long rows, cols, blocks, k_tiles;

@@ -406,6 +406,7 @@ void mx_linear_checked(const TraceaTensorView& xv, const TraceaMxMatrix& wv, con
   const int dev = xv.device_id;
   if (dev < 0) TB_FAIL(TRACEA_INVALID_PARAMS, "tracea_mx_linear takes device tensors (device_id >= 0)");
   const Matrix x = load_matrix(xv, "x", dev);
+  check_rows(x, "x");
   Product p = check_product(dev, x.rows, x.cols, wv, bias, res, c, c_mx, gp);
   if (x.rows == 0) return;
   DeviceGuard guard(dev);
