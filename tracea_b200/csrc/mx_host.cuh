@@ -44,10 +44,11 @@ inline void check_output(const Matrix& m, const char* name) {
 inline bool rows_of_8(const Matrix& m) {
   return m.col_stride == 1 && aligned16(m.ptr) && m.row_stride * m.es % 16 == 0;
 }
-// Bytes a lane may move at once along rows: 16, 4, or one element.
+// Bytes a lane may move at once along rows: 16, 8, 4, or one element.
 inline int row_vec(const void* ptr, long long row_stride, long long cols, int es) {
   const uintptr_t a = reinterpret_cast<uintptr_t>(ptr);
   if (a % 16 == 0 && row_stride * es % 16 == 0 && cols * es % 16 == 0) return 16;
+  if (a % 8 == 0 && row_stride * es % 8 == 0 && cols * es % 8 == 0) return 8;
   if (a % 4 == 0 && row_stride * es % 4 == 0 && cols * es % 4 == 0) return 4;
   return es;
 }
