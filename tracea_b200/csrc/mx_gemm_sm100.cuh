@@ -330,6 +330,7 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       const uint32_t a_end = a_first + static_cast<uint32_t>(num_stages) * kStageUnits;
       uint32_t a = a_first, ta = ta_first, bar = 0, phase = 0;
       int local = 0;
+      uint32_t sw_shifts = 0;
       bool ok = true;
       bool ready = false;             // pairs: this stage's scales are known to be in place; else: the next stage's bytes are
       bool scales_issued = false;     // not pairs: this stage's scales are on their way to tensor memory
@@ -358,9 +359,12 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
         tc_fence_after();
         uint32_t sw_shift = 0;        // the tile may start inside a tile of scales
         if constexpr (BN % kMxTileRows != 0) {
-          int mt, nt;
-          tile_coords(tile, mt, nt);
-          sw_shift = static_cast<uint32_t>(nt * BN % kMxTileRows) / 32u;
+          if ((local & 31) == 0) {    // a lane each for the next 32 tiles: the divisions would hold every tile up
+            int mt, nt;
+            tile_coords(min(tile + lane * num_workers, tiles - 1), mt, nt);
+            sw_shifts = static_cast<uint32_t>(nt * BN % kMxTileRows) / 32u;
+          }
+          sw_shift = __shfl_sync(0xffffffffu, sw_shifts, local & 31);
         }
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(buf) * BN;
         for (int it = 0; it < k_iters; ++it) {
@@ -395,13 +399,8 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
             if (next_a + kStageUnits == a_end) { probe_bar = full_bar0; probe_phase ^= 1u; }
           }
           const uint32_t b = a + (kABytes >> 4), tb = ta + 8u + sw_shift;
-          bool landed;
-          if (it == 0)
-            landed = mx_mma_stage4_probe<kPair, false>(d_tmem, a, b, kDescHi, idesc0, idesc2, ta, ta + 4u, tb, tb + 4u * kBTiles,
-                                                       empty_bar0 + bar, probe_bar, probe_phase, issue);
-          else
-            landed = mx_mma_stage4_probe<kPair, true>(d_tmem, a, b, kDescHi, idesc0, idesc2, ta, ta + 4u, tb, tb + 4u * kBTiles,
-                                                      empty_bar0 + bar, probe_bar, probe_phase, issue);
+          const bool landed = mx_mma_stage4_probe<kPair>(d_tmem, a, b, kDescHi, idesc0, idesc2, ta, ta + 4u, tb, tb + 4u * kBTiles,
+                                                         empty_bar0 + bar, probe_bar, probe_phase, it != 0 ? 1u : 0u, issue);
           a = next_a; ta = next_ta; bar = next_bar; phase = next_phase;
           ready = __all_sync(0xffffffffu, landed);
         }

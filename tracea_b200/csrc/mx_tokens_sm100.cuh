@@ -183,12 +183,8 @@ mx_tokens_sm100_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_
         tmem_cp_32x128b_if<false>(issue, tw + 4u * k, sw + k * (kMxTileBytes >> 4), kScaleDescHi);
         tmem_cp_32x128b_if<false>(issue, tt + 4u * k, st + k * (kMxTileBytes >> 4), kScaleDescHi);
       }
-      if (it == 0)
-        mx_mma_stage4_probe<false, false>(tmem_base, w, tok, kDescHi, idesc0, idesc2, tw, tw + 4u, tt, tt + 4u, empty_bar(stage),
-                                          full_bar(stage), phase, issue);
-      else
-        mx_mma_stage4_probe<false, true>(tmem_base, w, tok, kDescHi, idesc0, idesc2, tw, tw + 4u, tt, tt + 4u, empty_bar(stage),
-                                         full_bar(stage), phase, issue);
+      mx_mma_stage4_probe<false>(tmem_base, w, tok, kDescHi, idesc0, idesc2, tw, tw + 4u, tt, tt + 4u, empty_bar(stage),
+                                 full_bar(stage), phase, it != 0 ? 1u : 0u, issue);
       if (++stage == num_stages) { stage = 0; phase ^= 1u; }
     }
     if (ok && issue) mma_commit(tfull_bar);

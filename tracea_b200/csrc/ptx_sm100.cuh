@@ -691,11 +691,11 @@ __device__ __forceinline__ void tcgen05_commit_if(uint32_t issue, uint32_t bar) 
 // One 128-byte k-step of kind::mxf4 as a single block, after mma_stage4_probe: four MMAs of 64 columns of K, the operands' rows
 // 32 bytes further on each (`a`, `b`: descriptor low words of the first), the scales of MMAs 0, 1 in columns sa0 / sb0 and of 2, 3
 // in sa1 / sb1, in the lower (idesc0) and the upper (idesc2) half of their words.
-template <bool kPair, bool kFirstAccumulates>
+template <bool kPair>
 __device__ __forceinline__ bool mx_mma_stage4_probe(uint32_t tmem_d, uint32_t a, uint32_t b, uint32_t desc_hi, uint32_t idesc0,
                                                     uint32_t idesc2, uint32_t sa0, uint32_t sa1, uint32_t sb0, uint32_t sb1,
                                                     uint32_t empty_bar, uint32_t next_full_bar, uint32_t next_parity,
-                                                    uint32_t issue) {
+                                                    uint32_t first_accumulates, uint32_t issue) {
   uint32_t ready;
 #define TB200_MX_STAGE(GROUP, COMMIT)                                                                            \
   asm volatile(                                                                                                  \
@@ -732,7 +732,7 @@ __device__ __forceinline__ bool mx_mma_stage4_probe(uint32_t tmem_d, uint32_t a,
       "}\n"                                                                                                      \
       : "=r"(ready)                                                                                              \
       : "r"(tmem_d), "r"(a), "r"(b), "r"(desc_hi), "r"(idesc0), "r"(idesc2), "r"(sa0), "r"(sa1), "r"(sb0),       \
-        "r"(sb1), "r"(empty_bar), "r"(next_full_bar), "r"(next_parity), "n"(kFirstAccumulates ? 1 : 0), "r"(issue) \
+        "r"(sb1), "r"(empty_bar), "r"(next_full_bar), "r"(next_parity), "r"(first_accumulates), "r"(issue) \
       : "memory")
   if constexpr (kPair) {
     TB200_MX_STAGE("2", ".mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%11], msk;\n");
