@@ -95,6 +95,13 @@ def test_join(m, c, dtype):
     status_ok()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("m, c", [(600, 1024), (1001, 520), (1500, 1000), (640, 1001)])
+def test_rows_of_a_warp(m, c, dtype):
+    test_norm(m, c, dtype)
+    test_join(m, c, dtype)
+
+
 @pytest.mark.parametrize("dtype, far", [("f32", 1e4), ("f32", -1e6), ("bf16", 300.0)])
 def test_rows_far_from_zero_keep_their_spread(dtype, far):
     x = rows(40, 1000, dtype, 4, far)

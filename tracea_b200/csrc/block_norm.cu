@@ -61,7 +61,7 @@ tb200::NormStage load_stage(const TraceaNorm& n, int dev, long long C, TraceaDTy
 
 template <typename T, int kThreads, int kVecs, int kMode, bool kJoin, int kNext>
 void launch_norm_kernel(const tb200::BlockNormArgs& a, int dev, int num_sms, cudaStream_t stream) {
-  constexpr int kBlock = tb200::norm_block_threads(kThreads, kJoin);
+  constexpr int kBlock = tb200::norm_block_threads(kThreads, kVecs, kJoin);
   const long long blocks =
       std::min<long long>(a.M, static_cast<long long>(num_sms) * tb200::norm_blocks_per_sm(kThreads, kVecs, kJoin));
   constexpr int kSmem = tb200::norm_smem_bytes(kThreads, kVecs, kMode, kJoin, kNext, sizeof(T));
@@ -76,14 +76,14 @@ void launch_norm_kernel(const tb200::BlockNormArgs& a, int dev, int num_sms, cud
   launch(kern, static_cast<unsigned>(blocks), kBlock, kSmem, 1, kLaunchNorm, stream, a);
 }
 
-template <typename T, int kThreads, int kVecs>
+template <typename T, int kThreads, int kVecs, bool kVecOnly = false>
 void launch_norm_shape(const tb200::BlockNormArgs& a, bool join, int next, bool vec, int dev, int num_sms, cudaStream_t stream) {
   auto go = [&](auto joined, auto nexts) {
     constexpr bool kJoin = decltype(joined)::value;
     constexpr int kNext = decltype(nexts)::value;
     constexpr int kOther = kNext == tb200::kNextMx ? tb200::kRowsSingle : tb200::kRowsSpread;
-    if (vec) launch_norm_kernel<T, kThreads, kVecs, tb200::kRowsVec, kJoin, kNext>(a, dev, num_sms, stream);
-    else launch_norm_kernel<T, kThreads, kVecs, kOther, kJoin, kNext>(a, dev, num_sms, stream);
+    if (kVecOnly || vec) launch_norm_kernel<T, kThreads, kVecs, tb200::kRowsVec, kJoin, kNext>(a, dev, num_sms, stream);
+    else if constexpr (!kVecOnly) launch_norm_kernel<T, kThreads, kVecs, kOther, kJoin, kNext>(a, dev, num_sms, stream);
   };
   using Rows = std::integral_constant<int, tb200::kNextRows>;
   using Quantised = std::integral_constant<int, tb200::kNextMx>;
@@ -101,8 +101,16 @@ void launch_norm_shape(const tb200::BlockNormArgs& a, bool join, int next, bool 
 
 template <typename T>
 void launch_norm(const tb200::BlockNormArgs& a, bool join, int next, bool vec, int dev, int num_sms, cudaStream_t stream) {
+  // A warp to a row of up to 1024 columns, or two. One costs fewer instructions, two have more rows' loads under way. Layer norm,
+  // the same quantised, its join, with the next norm, with that quantised, us, two warps / one, 1024 columns of bf16:
+  //     148 rows  2.8 2.9   3.0 3.3   2.8 2.9   3.4 3.5   3.7 4.0        20000 rows  17 16   21 19   20 20   31 29    34 28
+  //   12544 rows   13 11    14 12     14 12     21 17     23 20          80000 rows  58 61   68 58   86 81  116 117  117 88
+  // 704 of fp32, 12544 rows: 17 15, 17 16, 20 18, 29 26, 29 26; 80000: 81 79, 75 70, 108 122, 151 165, 152 122. Rows that are not
+  // 16-byte aligned lose as often as they win. The choice may depend on the rows alone: the same row has the same bits in all forms.
+  const bool warp_rows = vec && a.M >= 4 * num_sms && static_cast<long long>(a.M) * a.C * static_cast<long long>(sizeof(T)) <= (40LL << 20);
   if (a.C <= 256) launch_norm_shape<T, 32, 1>(a, join, next, vec, dev, num_sms, stream);
   else if (a.C <= 512) launch_norm_shape<T, 32, 2>(a, join, next, vec, dev, num_sms, stream);
+  else if (a.C <= 1024 && warp_rows) launch_norm_shape<T, 32, 4, true>(a, join, next, vec, dev, num_sms, stream);
   else if (a.C <= 1024) launch_norm_shape<T, 64, 2>(a, join, next, vec, dev, num_sms, stream);
   else if (a.C <= 2048) launch_norm_shape<T, 128, 2>(a, join, next, vec, dev, num_sms, stream);
   else if (a.C <= 4096) launch_norm_shape<T, 256, 2>(a, join, next, vec, dev, num_sms, stream);

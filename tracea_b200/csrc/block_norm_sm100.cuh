@@ -140,8 +140,8 @@ __device__ __forceinline__ bool has_shift(const NormStage& s) { return s.bias.pt
 // A CTA's rows are walked by groups of kThreads threads. A join's CTA is as large as an SM holds where rows are short: with 256
 // threads each, copies of the vectors took shared memory that rows on their way can use (65536 x 256 bf16 and next norm 24.5 ->
 // 20.9 us; of 1001 columns, 333 rows, it would cost, 3.7 -> 4.8, of 4096, 91 -> 100).
-__host__ __device__ constexpr int norm_block_threads(int row_threads, bool join) {
-  return join && row_threads == 32 ? 768 : (row_threads < 256 ? 256 : row_threads);
+__host__ __device__ constexpr int norm_block_threads(int row_threads, int vecs, bool join) {
+  return join && row_threads == 32 && vecs <= 2 ? 768 : (row_threads < 256 ? 256 : row_threads);
 }
 
 // A barrier of the threads of a row.
@@ -260,11 +260,11 @@ __host__ __device__ constexpr int norm_kept_bytes(int threads, int vecs, bool jo
   return norm_keeps(threads, vecs) ? threads * vecs * 8 * 2 * 4 * ((join ? 1 : 0) + (next != kNextNone ? 1 : 0)) : 0;
 }
 __host__ __device__ constexpr int norm_row_bytes(int threads, int vecs, bool join, int es) {
-  return norm_block_threads(threads, join) * vecs * 8 * es * (join ? 2 : 1);
+  return norm_block_threads(threads, vecs, join) * vecs * 8 * es * (join ? 2 : 1);
 }
 // CTAs an SM is to hold: 1024 threads of 64 registers; joins 768 of 80 or 512 of 128, which more than sixteen columns have too.
 __host__ __device__ constexpr int norm_blocks_per_sm(int threads, int vecs, bool join) {
-  return join && threads == 32 ? 1 : (vecs <= 2 && !join ? 1024 : 512) / norm_block_threads(threads, join);
+  return join && threads == 32 && vecs <= 2 ? 1 : (vecs <= 2 && !join ? 1024 : 512) / norm_block_threads(threads, vecs, join);
 }
 // Rows ahead: what the CTA's share of 190 KB of shared memory holds, four at most.
 __host__ __device__ constexpr int norm_depth(int threads, int vecs, bool join, int next, int es) {
@@ -278,11 +278,11 @@ __host__ __device__ constexpr int norm_join_mode(int mode) { return mode == kRow
 __host__ __device__ constexpr int norm_smem_bytes(int threads, int vecs, int mode, bool join, int next, int es) {
   return norm_kept_bytes(threads, vecs, join, next) +
          (mode == kRowsVec ? norm_depth(threads, vecs, join, next, es) * norm_row_bytes(threads, vecs, join, es)
-                           : (mode == kRowsSingle && join ? norm_block_threads(threads, join) * vecs * 8 * 4 : 0));
+                           : (mode == kRowsSingle && join ? norm_block_threads(threads, vecs, join) * vecs * 8 * 4 : 0));
 }
 
 template <typename T, int kThreads, int kVecs, int kMode, bool kJoin, int kNext>
-__global__ void __launch_bounds__(norm_block_threads(kThreads, kJoin), norm_blocks_per_sm(kThreads, kVecs, kJoin))
+__global__ void __launch_bounds__(norm_block_threads(kThreads, kVecs, kJoin), norm_blocks_per_sm(kThreads, kVecs, kJoin))
 block_norm_kernel(const __grid_constant__ BlockNormArgs a) {
   static_assert(!(kMode == kRowsSpread && kNext == kNextMx), "a block of the format is four neighbouring threads' columns");
   ptx::griddep_launch_dependents();
@@ -292,7 +292,7 @@ block_norm_kernel(const __grid_constant__ BlockNormArgs a) {
   using Slice = RowSlice<T, kMode, kThreads>;
   constexpr int kJoinMode = norm_join_mode(kMode);
   using JoinSlice = RowSlice<T, kJoin ? kJoinMode : kMode, kThreads>;
-  constexpr int kBlock = norm_block_threads(kThreads, kJoin);
+  constexpr int kBlock = norm_block_threads(kThreads, kVecs, kJoin);
   constexpr int kRows = kBlock / kThreads;                              // that a CTA has in hand at a time
   constexpr bool kKeep = norm_keeps(kThreads, kVecs);
   constexpr int kSlices = kThreads * kVecs;                             // of eight columns
