@@ -63,7 +63,7 @@ template <typename T, int kThreads, int kVecs, int kMode, bool kJoin, int kNext>
 void launch_norm_kernel(const tb200::BlockNormArgs& a, int dev, int num_sms, cudaStream_t stream) {
   constexpr int kBlock = tb200::norm_block_threads(kThreads, kVecs, kJoin);
   const long long blocks =
-      std::min<long long>(a.M, static_cast<long long>(num_sms) * tb200::norm_blocks_per_sm(kThreads, kVecs, kJoin));
+      std::min<long long>(a.M, static_cast<long long>(num_sms) * tb200::norm_blocks_per_sm(kThreads, kVecs, kJoin, sizeof(T)));
   constexpr int kSmem = tb200::norm_smem_bytes(kThreads, kVecs, kMode, kJoin, kNext, sizeof(T));
   auto kern = tb200::block_norm_kernel<T, kThreads, kVecs, kMode, kJoin, kNext>;
   if constexpr (kSmem > 47 * 1024) {
