@@ -92,14 +92,14 @@ __device__ __forceinline__ void mx_act32(float (&f)[32], int act) {
     for (int i = 0; i < 4; ++i) asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a[i]));
     add2(a[0], a[1], 1.0f, 1.0f);
     add2(a[2], a[3], 1.0f, 1.0f);
-    const float p = a[0] * a[1], q = a[2] * a[3];
-    float r;
+    float p = a[0], q = a[1], r;
+    mul2(p, q, a[2], a[3]);
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(p * q));
-    const float rp = r * q, rq = r * p;       // 1 / p, 1 / q
-    mul2(f[j], f[j + 1], a[1], a[0]);
-    mul2(f[j + 2], f[j + 3], a[3], a[2]);
-    mul2(f[j], f[j + 1], rp, rp);
-    mul2(f[j + 2], f[j + 3], rq, rq);
+    const float rp = r * q, rq = r * p;       // 1 / (a[0] a[2]), 1 / (a[1] a[3])
+    mul2(f[j], f[j + 1], a[2], a[3]);
+    mul2(f[j + 2], f[j + 3], a[0], a[1]);
+    mul2(f[j], f[j + 1], rp, rq);
+    mul2(f[j + 2], f[j + 3], rp, rq);
   }
 }
 
@@ -469,16 +469,35 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     const OutT* res = static_cast<const OutT*>(args.residual);
     const int my_tiles = worker < tiles ? (tiles - worker + num_workers - 1) / num_workers : 0;
     uint32_t box = 0;
-    int bias_tile = -1;
+    // The bias of the tile after this one is on its way to registers while this one is waited for and finished (12544 x 4096 x 1024
+    // bf16 30.4 us; 34.7 where each was loaded as its tile began). Tiles of 256 columns, for long K, have no registers for that.
+    int bias_tile = -1, ahead_tile = -1;
+    float ahead[BN / 32];
+    auto load_bias = [&](int nt) {
+      ahead_tile = nt;
+#pragma unroll
+      for (int j = 0; j < BN / 32; ++j) {
+        const int n = nt * BN + j * 32 + lane;
+        ahead[j] = 0.0f;
+        if (args.bias != nullptr && n < args.N)
+          ahead[j] = args.bias_is_f32 ? ld_global_f32(static_cast<const float*>(args.bias) + n)
+                                      : OutTraits<OutT>::to_f(static_cast<const OutT*>(args.bias)[n]);
+      }
+    };
+    auto next_tile = [&](int local) {
+      ++local;
+      if (kAcc == 2 && local < my_tiles - 1 && (local & 1) != egroup / kShare) ++local;
+      return local;
+    };
     bool ok = true;
-    for (int local = 0; ok && local < my_tiles; ++local) {
+    int local = next_tile(-1), mt = 0, nt = 0, local_next, mt_next = 0, nt_next = 0;
+    if (local < my_tiles) tile_coords(worker + local * num_workers, mt, nt);
+    for (; ok && local < my_tiles; local = local_next, mt = mt_next, nt = nt_next) {
       const bool last = kAcc == 2 && local == my_tiles - 1;
-      if (kAcc == 2 && !last && (local & 1) != egroup / kShare) continue;
+      local_next = next_tile(local);
       const int g_first = last ? egroup : egroup % kShare, g_step = last ? kEpiGroups : kShare;
       const int buf = kAcc == 2 ? local & 1 : 0;
       const uint32_t use = static_cast<uint32_t>(kAcc == 2 ? local >> 1 : local);
-      int mt, nt;
-      tile_coords(worker + local * num_workers, mt, nt);
       const int n_base = nt * BN;
       const int m_row0 = mt * kTileM + static_cast<int>(cta_rank) * kBlockM + quarter * 32;
       const int m = m_row0 + lane;
@@ -495,19 +514,17 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
           res_ahead += g_step;
         }
       }
-      if (nt != bias_tile) {
+      if (bias_tile < 0 || (args.bias != nullptr && nt != bias_tile)) {
+        if (nt != ahead_tile) load_bias(nt);
         __syncwarp();
 #pragma unroll
-        for (int j = 0; j < BN / 32; ++j) {
-          const int n = n_base + j * 32 + lane;
-          float b = 0.0f;
-          if (args.bias != nullptr && n < args.N)
-            b = args.bias_is_f32 ? ld_global_f32(static_cast<const float*>(args.bias) + n)
-                                 : OutTraits<OutT>::to_f(static_cast<const OutT*>(args.bias)[n]);
-          bias_w[j * 32 + lane] = b;
-        }
+        for (int j = 0; j < BN / 32; ++j) bias_w[j * 32 + lane] = ahead[j];
         __syncwarp();
         bias_tile = nt;
+      }
+      if (local_next < my_tiles) {
+        tile_coords(worker + local_next * num_workers, mt_next, nt_next);
+        if (BN < 256 && args.bias != nullptr && nt_next != bias_tile) load_bias(nt_next);
       }
       const bool ready = mbar_wait_bounded(tfull_bar(buf), use & 1u, abort_p, 2 * args.wait_limit);
       if (!__all_sync(0xffffffffu, ready)) {
