@@ -285,8 +285,8 @@ void tokens_product(DeviceState& st, const Product& p, const Matrix* x, const To
 // us: what a launch takes once, and per wave of tiles either its k-steps (an SM has 16 KB of A and half or all of the columns' rows
 // of W to bring in a step) and what lies between two tiles, or its epilogue, whichever is longer. 192 columns have two accumulators,
 // 256 one, which pays for its wider steps only over a long K. Measured / this formula, columns 64, 128, 192, 256:
-//   8192 x 8192 x 8192         480 249 210 201 / 448 263 212 206     12544 x 4096 x 1024    64  34  31 43 / 60 33 31 40
-//   4096 x 4096 x 4096          68  32  29  33 / 60  37  32  35      the same, SiLU           -  41  46 59 / 60 41 48 60
+//   8192 x 8192 x 8192         352 251 204 192 / 444 261 212 206     12544 x 4096 x 1024    49  38  31 34 / 53 33 31 36
+//   4096 x 4096 x 4096          49  32  30  32 / 59  36  32  35      the same, SiLU          53  41  41 47 / 53 41 42 47
 //   2048 x 2048 x 2048        12.6 7.3 9.2 9.1 / 11 7.9 10 8.7       1024 x 1024 x 2048   4.8 5.3 6.7  - / 4.8 5.4 7.0 8.6
 int pick_mx_tile(long long M, long long N, long long K, int act, int num_sms) {
   static const int forced = env_int("TRACEA_B200_MX_BN", 0);
@@ -296,7 +296,7 @@ int pick_mx_tile(long long M, long long N, long long K, int act, int num_sms) {
     double once, step, between, epilogue, epilogue_act;
   };
   static const Form forms[4] = {{64, 2.6, 0.24, 0.2, 0.75, 0.9}, {128, 2.9, 0.28, 0.25, 1.15, 1.75},
-                                {192, 4.0, 0.33, 0.4, 1.8, 2.9}, {256, 4.0, 0.41, 1.3, 3.3, 5.1}};
+                                {192, 4.0, 0.33, 0.4, 1.8, 2.5}, {256, 4.0, 0.41, 1.3, 2.7, 3.9}};
   const double steps = static_cast<double>(ceil_div(K, 256));
   int best = 0;
   double best_time = 0.0;
