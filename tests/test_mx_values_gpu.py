@@ -1,0 +1,55 @@
+"""Values at which an epilogue of the 4-bit products can go wrong on a B200: NaN behind a ReLU, results far apart that share
+arithmetic, and activations where their formula cancels.
+
+Most of these put exact values in front of an activation: codes of zero as input, and the values as an fp32 bias."""
+import pytest
+import torch
+
+from test_mx_gpu import DT, matrix, status_ok
+from tracea_b200 import ops
+
+pytestmark = pytest.mark.gpu
+
+
+def zeros(m, k):
+    return ops.mx_quantize(torch.zeros(m, k, device="cuda"))
+
+
+# rows of both forms of the product, and a K at which 40 rows take the one for few
+@pytest.mark.parametrize("m, k", [(1, 300), (40, 300), (40, 2048), (300, 300), (700, 513)])
+@pytest.mark.parametrize("out", ["f32", "f16", "bf16", "mx"])
+def test_relu_keeps_nan(m, k, out):
+    n = 200
+    _, av = matrix(m, k, 1)
+    w, wv = matrix(n, k, 2)
+    bias = torch.randn(n, generator=torch.Generator().manual_seed(3)).cuda()
+
+    def product(a, b, epilogue, residual=None):
+        args = (a, b, bias if "bias" in epilogue else None, epilogue, residual)
+        return ops.mx_gemm(*args, quantize=True).dequantize(torch.float32) if out == "mx" else ops.mx_gemm(*args, dtype=DT[out])
+
+    x = av.float()
+    clean = ops.mx_quantize(x)
+    x[m // 2, 40] = float("nan")
+    y = wv.float()
+    y[5, 0] = float("inf")
+    rest = torch.arange(m, device="cuda") != m // 2
+    for e in ("relu", "bias+relu"):
+        want = product(clean, w, e)
+        assert (want >= 0).all() and (want == 0).any()
+        inputs = [ops.mx_quantize(x)] + ([x.to(DT[out])] if out != "mx" else [x])
+        got = product(inputs[0], w, e)
+        assert got[m // 2].isnan().all() and torch.equal(got[rest], want[rest])
+        assert product(inputs[1], w, e)[m // 2].isnan().all()
+        got = product(clean, ops.mx_quantize(y), e)
+        assert got[:, 5].isnan().all()
+        others = torch.arange(n, device="cuda") != 5 if out != "mx" else torch.arange(n, device="cuda") >= 32   # a block is NaN as a whole
+        assert torch.equal(got[:, others], want[:, others])
+    if out != "mx":
+        r = torch.randn(m, n, generator=torch.Generator().manual_seed(4)).to(DT[out]).cuda()
+        want = product(clean, w, "bias+residual+relu", r)
+        r[0, 7] = float("nan")
+        got = product(clean, w, "bias+residual+relu", r)
+        assert got[0, 7].isnan() and got.isnan().sum() == 1
+        assert torch.equal(got.nan_to_num(nan=0.0), torch.where(got.isnan(), 0.0, want))
+    status_ok()

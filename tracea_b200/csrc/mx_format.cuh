@@ -155,10 +155,17 @@ __device__ __forceinline__ uint4 mx_quantize32(const float (&v)[32], uint32_t& b
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// The activations of apply_act32 on one value.
+// ReLU that keeps a NaN, so that a NaN block reaches the output whatever the epilogue (fmaxf would return the other operand).
+__device__ __forceinline__ float relu_nan(float v) {
+  float d;
+  asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(d) : "f"(v));
+  return d;
+}
+
+// The activations of apply_act32 on one value; ReLU keeps NaN.
 template <bool kFast>
 __device__ __forceinline__ float apply_act(float v, int act) {
-  if (act == kActRelu) return fmaxf(0.0f, v);
+  if (act == kActRelu) return relu_nan(v);
   if (act == kActSilu) {
     if constexpr (kFast) return __fdividef(v, 1.0f + __expf(-v));
     else return v / (1.0f + expf(-v));

@@ -71,6 +71,11 @@ __host__ __device__ constexpr int mx_scale_cols(int bn) { return 8 + 8 * mx_b_sc
 // for itself: rows past M, whose scales are anyone's, must not choose for the others.)
 template <bool kFast>
 __device__ __forceinline__ void mx_act32(float (&f)[32], int act) {
+  if (act == kActRelu) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) f[j] = relu_nan(f[j]);
+    return;
+  }
   if (!kFast || act != kActSilu) {
     apply_act32<kFast>(f, act);
     return;
@@ -597,7 +602,7 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
                 add16<OutT>(f + c * kVec, ld_shared_v4(stg + lane_row_off + ((cc ^ lane_xor) << 4)));
               }
             }
-            if (args.act == kActRelu) {
+            if (sizeof(OutT) == 2 && args.act == kActRelu) {        // in the rounding, which keeps NaN
               finish32<OutT, true>(f, nullptr, false, packed + h * kChunksPerLd);
             } else {
               mx_act32<sizeof(OutT) == 2>(f, args.act);
