@@ -451,6 +451,7 @@ block_norm_kernel(const __grid_constant__ BlockNormArgs a) {
             uint32_t byte;
             const uint32_t codes = mx_quantize8(v[i], byte);            // the whole warp: blocks are shared by lanes
             if ((col >> 5) < a.blocks) *reinterpret_cast<uint32_t*>(a.codes + row * (16LL * a.blocks) + (col >> 1)) = codes;
+            else if (kMode == kRowsVec) byte = 0u;                      // past the last block: 0 times the row's factor, which may be NaN
             if ((lane & 3) == 0 && (col >> 7) < a.k_tiles)
               a.scales[mx_scale_word(row, col >> 7, a.k_tiles) + ((col >> 5) & 3)] = static_cast<uint8_t>(byte);
           }
