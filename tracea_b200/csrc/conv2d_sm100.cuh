@@ -214,6 +214,21 @@ __host__ __device__ constexpr int conv_smem_bytes(int bn, int stages, bool pair,
          kNumEpilogueWarps * staging_depth * kStagingBoxBytes + bias_bytes + kBarrierBytes;
 }
 
+// Tensor memory and clusters. A CTA that allocates columns which another CTA on its SM holds waits until they are handed back, and
+// CTAs of a cluster wait for one another. So two clusters on different streams, each with a CTA that holds columns and one that
+// waits for the other's, would wait without end: nothing bounds an allocation or a cluster barrier. CTAs of clusters whose columns
+// exceed an SM's 512 must therefore not fit one SM. Their shared memory sees to that: 228 KB an SM, of which a CTA takes 1 KB besides
+// its own. A CTA of a pair has 512 columns and at least this much; one of the 4-bit product for few rows, 256 columns, has at least
+// kTokMinSmem. (CTAs that are in no cluster hand theirs back whatever others do.)
+constexpr int kSmSmemBytes = 228 * 1024, kCtaReservedSmem = 1024;
+constexpr int kPairMinSmem = 150 * 1024;
+static_assert(2 * (kPairMinSmem + kCtaReservedSmem) > kSmSmemBytes, "two pairs on an SM");
+// What a launch of the general kernel asks for.
+__host__ __device__ constexpr int conv_launch_smem_bytes(int bn, int stages, bool pair, bool rows2, int staging_depth, int bias_bytes) {
+  const int n = conv_smem_bytes(bn, stages, pair, rows2, staging_depth, bias_bytes);
+  return pair && n < kPairMinSmem ? kPairMinSmem : n;
+}
+
 // (a, b) += (c, d) as one packed fp32x2 add.
 __device__ __forceinline__ void add2(float& a, float& b, float c, float d) {
   asm("{\n"

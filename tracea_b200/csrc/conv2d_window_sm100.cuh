@@ -60,7 +60,8 @@ struct WindowKernelArgs {
 };
 
 __host__ __device__ constexpr uint32_t window_smem_bytes(uint32_t w_bytes, uint32_t slot_bytes) {
-  return w_bytes + 2u * slot_bytes + 8u * kWinStageBytes + kWinBN * 4u + 256u + 1024u;
+  const uint32_t n = w_bytes + 2u * slot_bytes + 8u * kWinStageBytes + kWinBN * 4u + 256u + 1024u;
+  return n > kPairMinSmem ? n : kPairMinSmem;    // a pair's CTA: see there
 }
 
 namespace ptx {

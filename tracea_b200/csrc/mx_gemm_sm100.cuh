@@ -63,6 +63,12 @@ __host__ __device__ constexpr int mx_accumulators(int bn) { return bn == 256 ? 1
 // TMEM columns: one or two accumulators, then the scales of every stage (8 columns of A's, 8 per tile of W's). A stage's columns are
 // rewritten when its shared memory is, which the stage's empty barrier orders behind the MMAs that read them.
 __host__ __device__ constexpr int mx_scale_cols(int bn) { return 8 + 8 * mx_b_scale_tiles(bn); }
+// Pipeline stages: what shared memory holds and tensor memory has columns of scales for.
+__host__ __device__ constexpr int mx_num_stages(int bn, bool pair, int store) {
+  const int in_smem = (232448 - mx_smem_bytes(bn, 0, pair, store)) / mx_stage_bytes(bn, pair);
+  const int in_tmem = (512 - mx_accumulators(bn) * bn) / mx_scale_cols(bn), n = in_smem < in_tmem ? in_smem : in_tmem;
+  return n < kMxMaxStages ? n : kMxMaxStages;
+}
 
 // apply_act32 with fewer trips through the special-function unit, which bounds SiLU here: a tile of 192 columns of 1024 takes
 // 2200 cycles of MMAs and 128 x 192 exponentials and reciprocals, at 16 of these a cycle, 3100. Four values share a reciprocal,

@@ -132,9 +132,8 @@ void launch_mx_gemm(DeviceState& st, int dt, const Product& p, cudaStream_t stre
   g.num_n_tiles = static_cast<int>(n_tiles);
   g.panel_width = static_cast<int>(panel);
   g.panel_tiles = static_cast<int>(m_tiles * panel);
-  const int room = 232448 - tb200::mx_smem_bytes(BN, 0, kPair, kStore);
-  int stages = std::min(room / tb200::mx_stage_bytes(BN, kPair), tb200::kMxMaxStages);
-  stages = std::min(stages, (512 - tb200::mx_accumulators(BN) * BN) / tb200::mx_scale_cols(BN));
+  constexpr int stages = tb200::mx_num_stages(BN, kPair, kStore), smem = tb200::mx_smem_bytes(BN, stages, kPair, kStore);
+  static_assert(!kPair || smem >= tb200::kPairMinSmem, "see there");
   g.num_stages = stages;
   g.idesc = tb200::ptx::make_mx_idesc(kTileM, BN);
   g.bias = p.bias;
@@ -174,8 +173,8 @@ void launch_mx_gemm(DeviceState& st, int dt, const Product& p, cudaStream_t stre
     }
   }
   const long long workers = std::min<long long>(m_tiles * n_tiles, kPair ? st.num_sms / 2 : st.num_sms);
-  launch(kern, grid_of(kPair ? 2 * workers : workers), tb200::mx_threads(BN, kPair, kStore), tb200::mx_smem_bytes(BN, stages, kPair, kStore),
-         kPair ? 2 : 1, kLaunchMxGemm, stream, ta, tw, tsa, tsw, to, g);
+  launch(kern, grid_of(kPair ? 2 * workers : workers), tb200::mx_threads(BN, kPair, kStore), smem, kPair ? 2 : 1,
+         kLaunchMxGemm, stream, ta, tw, tsa, tsw, to, g);
 }
 
 // ------------------------------------------------------------------ few rows

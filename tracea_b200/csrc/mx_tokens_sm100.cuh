@@ -55,10 +55,11 @@ __host__ __device__ constexpr uint32_t tok_front_bytes(int cols, int stages, int
   const uint32_t sums = static_cast<uint32_t>(cols) * 512u;
   return ring > sums ? ring : sums;
 }
-// At least kTokMinSmem: two of these CTAs share an SM's 512 columns of tensor memory, a third, or one of a pair of the general
-// kernels (which have all 512), must not come up beside them. Its allocation would wait for theirs while CTAs of its own cluster
-// wait for it at a cluster barrier -- and so round in a ring, when launches on other streams stand so on several SMs.
+// At least kTokMinSmem: two of these CTAs share an SM's 512 columns of tensor memory; a third, or one of a pair of any other kernel,
+// must not come up beside them (see kPairMinSmem).
 constexpr int kTokMinSmem = 80 * 1024;
+static_assert(3 * (kTokMinSmem + kCtaReservedSmem) > kSmSmemBytes && kTokMinSmem + kPairMinSmem + 2 * kCtaReservedSmem > kSmSmemBytes,
+              "clusters with more than an SM's tensor memory");
 __host__ __device__ constexpr int tok_smem_bytes(int cols, int stages, int fused_steps) {
   const int n = 1024 + static_cast<int>(tok_front_bytes(cols, stages, fused_steps)) + kTokBarrierBytes;
   return n > kTokMinSmem ? n : kTokMinSmem;

@@ -1357,7 +1357,7 @@ void conv2d_core(DeviceState& st, StaticArena* arena, const View4& x_in, const V
     }
     const int forced_stages = knobs().force_stages;
     if (forced_stages >= 2 && forced_stages <= stages) stages = forced_stages;
-    const int smem = tb200::conv_smem_bytes(bn, stages, pair_v, rows2_v, depth, bias_bytes);
+    const int smem = tb200::conv_launch_smem_bytes(bn, stages, pair_v, rows2_v, depth, bias_bytes);
 
     CUtensorMap tmap_w;
     encode_w(&tmap_w, pair_v ? bn / 2 : bn);
