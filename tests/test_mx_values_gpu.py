@@ -5,7 +5,7 @@ Most of these put exact values in front of an activation: codes of zero as input
 import pytest
 import torch
 
-from test_mx_gpu import DT, matrix, status_ok
+from test_mx_gpu import DT, assert_close, assert_quantized, matrix, status_ok
 from tracea_b200 import ops
 
 pytestmark = pytest.mark.gpu
@@ -52,4 +52,28 @@ def test_relu_keeps_nan(m, k, out):
         got = product(clean, w, "bias+residual+relu", r)
         assert got[0, 7].isnan() and got.isnan().sum() == 1
         assert torch.equal(got.nan_to_num(nan=0.0), torch.where(got.isnan(), 0.0, want))
+    status_ok()
+
+
+@pytest.mark.parametrize("m", [1, 300])
+@pytest.mark.parametrize("out", ["f32", "f16", "bf16", "mx"])
+def test_silu_of_values_far_apart(m, out):
+    """Neighbours of 32 columns share reciprocals: none of them may carry another's size into a result. -19.9 and the like are the
+    lowest that do; next to them values up to the type's largest, in every place of four."""
+    large = {"f16": [6e4, 3e3, 65504.0, 1.0], "mx": [1e30, 1e20, 3e38, 2e38]}.get(out, [1e30, 1e20, 3e38, 1.0])
+    low = [-19.9, -19.0, -12.0, -1.0]
+    v = torch.tensor([low[(i // 32 + i) % 4] for i in range(512)])
+    for i in range(64):
+        v[8 * i + i % 8] = large[i // 8 % 4]
+    v[256::16] = large[0]
+    bias = v.cuda()
+    a, w = zeros(m, 64), zeros(512, 64)
+    y = (bias.double() * torch.sigmoid(bias.double())).expand(m, 512)
+    err = (2.0 ** -20 if out == "f32" else 2.0 ** -16) * y.abs() + 1e-37          # as in test_mx_gpu.py
+    if out == "mx":
+        assert_quantized(ops.mx_gemm(a, w, bias, "bias+silu", quantize=True), y, err)
+    else:
+        got = ops.mx_gemm(a, w, bias, "bias+silu", dtype=DT[out])
+        assert got.isfinite().all()
+        assert_close(got, y, err)
     status_ok()

@@ -107,10 +107,11 @@ __device__ __forceinline__ void mx_act32(float (&f)[32], int act) {
     mul2(p, q, a[2], a[3]);
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(p * q));
     const float rp = r * q, rq = r * p;       // 1 / (a[0] a[2]), 1 / (a[1] a[3])
+    // the reciprocals, at most 1, before the values: a value times a neighbour's denominator may pass fp32's range
+    mul2(a[0], a[1], rp, rq);
+    mul2(a[2], a[3], rp, rq);
     mul2(f[j], f[j + 1], a[2], a[3]);
     mul2(f[j + 2], f[j + 3], a[0], a[1]);
-    mul2(f[j], f[j + 1], rp, rq);
-    mul2(f[j + 2], f[j + 3], rp, rq);
   }
 }
 
