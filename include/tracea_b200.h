@@ -264,8 +264,9 @@ TraceaStatus tracea_mx_dequantize(TraceaMxMatrix q, TraceaTensorView *out, void 
 /* c = epilogue(a w^T), a [M,K], w [N,K] (a Linear layer's weight as it lies), accumulated in fp32. Exactly one of c and c_mx is
  * given: c [M,N] in FLOAT32, FLOAT16 or BFLOAT16 with contiguous columns and any row stride, rounded once; or c_mx, quantised from
  * the fp32 results. Epilogue kinds, bias (fp32, or the dtype of c) and residual ([M,N], the dtype of c; not with c_mx) as
- * tracea_gemm; a NaN stays one behind every activation, ReLU too. The output may not overlap the inputs, except that c may be the residual. M = 0 is a no-op. At most 2^31 - 256 rows,
- * as in the entries below. */
+ * tracea_gemm; a NaN stays one behind every activation, ReLU too. SiLU and GELU of 16- and 4-bit outputs are good to 2^-14 of the
+ * result before its rounding; FLOAT32 ones use library functions, GELU as x / 2 (1 + tanh), good to 2^-22 |x|. The output may not
+ * overlap the inputs, except that c may be the residual. M = 0 is a no-op. At most 2^31 - 256 rows, as in the entries below. */
 TraceaStatus tracea_mx_gemm(TraceaMxMatrix a, TraceaMxMatrix w, const TraceaTensorView *bias, const TraceaTensorView *residual,
                             TraceaTensorView *c, TraceaMxMatrix *c_mx, TraceaGemmParams params);
 

@@ -5,6 +5,7 @@ Most of these put exact values in front of an activation: codes of zero as input
 import pytest
 import torch
 
+import mxref
 from test_mx_gpu import DT, assert_close, assert_quantized, matrix, status_ok
 from tracea_b200 import ops
 
@@ -76,4 +77,37 @@ def test_silu_of_values_far_apart(m, out):
         got = ops.mx_gemm(a, w, bias, "bias+silu", dtype=DT[out])
         assert got.isfinite().all()
         assert_close(got, y, err)
+    status_ok()
+
+
+def columns(values):
+    """(a row of ones, w, x): a w^T is x, close to `values`, exactly: each as four elements of the format in blocks of their own."""
+    left, w = values.double().numpy().copy(), torch.zeros(len(values), 128, dtype=torch.float64)
+    for b in range(4):
+        w[:, 32 * b] = torch.from_numpy(mxref.values(left[:, None])[:, 0])
+        left -= w[:, 32 * b].numpy()
+    a = torch.zeros(1, 128)
+    a[:, ::32] = 1.0
+    return a.cuda(), ops.mx_quantize(w.float().cuda()), w.sum(1).cuda()
+
+
+@pytest.mark.parametrize("m", [1, 300])
+@pytest.mark.parametrize("out", ["f16", "bf16", "mx"])
+def test_gelu_is_good_to_the_outputs_rounding_where_it_cancels(m, out):
+    """x / (1 + e^z), z = -2 sqrt(2 / pi) (x + 0.044715 x^3). In fp32 z is off by at most five half steps, 5 2^-24 |z|, by which e^z is
+    off relative to itself; the exponential (2^-22), the sum, the quotient (2^-22) and the product add less than 2^-20. The output's
+    rounding, half a step, is assert_close's."""
+    a, w, x = columns(torch.linspace(-14, 14, 4096))
+    a = ops.mx_quantize(a.expand(m, 128))
+    z = -2 * (2 / torch.pi) ** 0.5 * (x + 0.044715 * x ** 3)
+    y = (x / (1 + torch.exp(z))).expand(m, -1)
+    err = (z.abs() * 2.0 ** -21 + 2.0 ** -20) * y.abs() + 1e-37
+    if out == "mx":
+        assert_quantized(ops.mx_gemm(a, w, None, "gelu", quantize=True), y, err)
+    else:
+        assert_close(ops.mx_gemm(a, w, None, "gelu", dtype=DT[out]), y, err)
+    a, w, x = columns(torch.tensor([2.0 ** 70, -2.0 ** 70, 1.5 * 2.0 ** 127, -1.5 * 2.0 ** 127, 0.0, 32.0, -32.0, 1.5 * 2.0 ** 126] * 8))
+    if out == "bf16":
+        got = ops.mx_gemm(ops.mx_quantize(a.expand(m, 128)), w, None, "gelu", dtype=torch.bfloat16)
+        assert torch.equal(got, x.clamp(min=0).bfloat16().expand(m, -1))
     status_ok()

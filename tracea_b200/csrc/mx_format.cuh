@@ -162,7 +162,11 @@ __device__ __forceinline__ float relu_nan(float v) {
   return d;
 }
 
-// The activations of apply_act32 on one value; ReLU keeps NaN.
+// GELU of 16- and 4-bit outputs. (1 + tanh u) / 2 = 1 / (1 + e^-2u), which unlike the left side does not cancel for negative values:
+// with tanh.approx (2^-11) results at -3 were off by a fifth. The exponent, in powers of two, is v (kGeluA + kGeluB v^2).
+constexpr float kGeluA = -2.3022082f, kGeluB = -0.10294324f;      // -2 sqrt(2 / pi) log2(e), the same times 0.044715
+
+// The activations of apply_act32 on one value, but for ReLU, which keeps NaN, and GELU.
 template <bool kFast>
 __device__ __forceinline__ float apply_act(float v, int act) {
   if (act == kActRelu) return relu_nan(v);
@@ -171,11 +175,14 @@ __device__ __forceinline__ float apply_act(float v, int act) {
     else return v / (1.0f + expf(-v));
   }
   if (act == kActGelu) {
-    const float u = 0.79788456f * (v + 0.044715f * v * v * v);
-    float t;
-    if constexpr (kFast) asm("tanh.approx.f32 %0, %1;" : "=f"(t) : "f"(u));
-    else t = tanhf(u);
-    return 0.5f * v * (1.0f + t);
+    if constexpr (kFast) {
+      float t = v * fmaf(kGeluB, v * v, kGeluA);
+      asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(t));
+      return __fdividef(v, 1.0f + t);
+    } else {
+      const float u = 0.79788456f * (v + 0.044715f * v * v * v);
+      return 0.5f * v * (1.0f + tanhf(u));
+    }
   }
   return v;
 }

@@ -82,6 +82,22 @@ __device__ __forceinline__ void mx_act32(float (&f)[32], int act) {
     for (int j = 0; j < 32; ++j) f[j] = relu_nan(f[j]);
     return;
   }
+  if (kFast && act == kActGelu) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+      float a = f[j], b = f[j + 1];
+      mul2(a, b, f[j], f[j + 1]);
+      fma2(a, b, kGeluB, kGeluB, kGeluA, kGeluA);
+      mul2(a, b, f[j], f[j + 1]);
+      asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a));
+      asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(b));
+      add2(a, b, 1.0f, 1.0f);
+      asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(a));
+      asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(b));
+      mul2(f[j], f[j + 1], a, b);
+    }
+    return;
+  }
   if (!kFast || act != kActSilu) {
     apply_act32<kFast>(f, act);
     return;
