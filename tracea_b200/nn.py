@@ -79,6 +79,10 @@ class MxLinear(torch.nn.Linear):
             self.__dict__.setdefault("_tracea_captured", {})[id(cached)] = cached     # graphs read it as long as the layer lives
         return cached[2]
 
+    def __getstate__(self):
+        """Copies and pickles go without the quantised weight: their parameter counts its versions anew."""
+        return {k: v for k, v in super().__getstate__().items() if k not in ("_tracea_quantized", "_tracea_captured")}
+
     def requantize(self):
         """Forget the quantised weight. Needed after a change that torch does not count, one through ``weight.data``."""
         cached = getattr(self, "_tracea_quantized", None)
