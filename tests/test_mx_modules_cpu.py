@@ -50,3 +50,19 @@ def test_a_copy_of_the_layer_takes_nothing_of_what_the_layer_keeps(quantized, ho
     for layer in (lin, other):                            # and both keep theirs
         layer._kernel_weight()
     assert len(quantized) == before
+
+
+@pytest.mark.parametrize("make", [lambda p: torch.optim.Adam(p, fused=True), lambda p: torch.optim.AdamW(p, lr=0.1, fused=True),
+                                  lambda p: torch.optim.SGD(p, lr=0.1, fused=True), lambda p: torch.optim.SGD(p, lr=0.1)])
+def test_a_step_of_any_optimizer_is_seen(quantized, make):
+    """Fused ones write the weight without counting a version of it."""
+    lin = nn.MxLinear(8, 4)
+    optimizer = make(lin.parameters())
+    for _ in range(3):
+        lin.weight.grad = torch.ones_like(lin.weight)
+        lin._kernel_weight()
+        optimizer.step()
+        assert torch.equal(lin._kernel_weight(), lin.weight)
+    before = len(quantized)
+    lin._kernel_weight()
+    assert len(quantized) == before

@@ -10,7 +10,10 @@ Differences from the reference's module, all deliberate:
   * OIHW-contiguous weights are packed into the kernel's [K][R][S][C] layout once per weight version
     (`ops.prepack_conv2d_weight`) and then read in place on every call.
 """
+import weakref
+
 import torch
+from torch.optim.optimizer import register_optimizer_step_post_hook
 
 from . import ops
 
@@ -46,6 +49,26 @@ class TraceaConv2d(torch.nn.Conv2d):
                                "bias" if bias is not None else None)
 
 
+# Layers that keep a quantised weight. Some optimizers, torch's fused ones among them, write a weight without counting a version of it,
+# so the layers that a step has changed are told.
+_quantized_layers = weakref.WeakSet()
+_step_hook = None
+
+
+def _after_step(optimizer, args, kwargs):
+    written = {id(p) for group in optimizer.param_groups for p in group["params"] if p.grad is not None}
+    for layer in list(_quantized_layers):
+        if id(layer.weight) in written:
+            layer.requantize()
+
+
+def _watch(layer):
+    global _step_hook
+    if _step_hook is None:
+        _step_hook = register_optimizer_step_post_hook(_after_step)
+    _quantized_layers.add(layer)
+
+
 class MxLinear(torch.nn.Linear):
     """Drop-in for torch.nn.Linear on CUDA tensors whose weight and input are multiplied in the 4-bit microscaled format
     (``ops.mx_gemm``): the weight is quantised once per version, the input, of any leading shape and fp32, fp16 or bf16, in every
@@ -53,7 +76,7 @@ class MxLinear(torch.nn.Linear):
 
     A new version waits once for the device: other streams may read the quantised weight from then on. A CUDA graph that is
     captured with a quantised weight at hand keeps to that one, whatever becomes of the layer's; captured right after
-    ``requantize()`` it quantises the weight in every replay."""
+    ``requantize()``, or after a step of an optimizer, it quantises the weight in every replay."""
 
     def __init__(self, in_features, out_features, bias=True, epilogue=None, device=None, dtype=None):
         super().__init__(in_features, out_features, bias, device, dtype)
@@ -74,6 +97,7 @@ class MxLinear(torch.nn.Linear):
                 return q                          # the graph's: nothing is in it before a replay
             torch.cuda.synchronize(w.device)      # it is complete for every stream, and nothing reads the old one any more
             self._tracea_quantized = (w, w._version, q)
+            _watch(self)
             return q
         if torch.cuda.is_current_stream_capturing():
             self.__dict__.setdefault("_tracea_captured", {})[id(cached)] = cached     # graphs read it as long as the layer lives
@@ -84,7 +108,8 @@ class MxLinear(torch.nn.Linear):
         return {k: v for k, v in super().__getstate__().items() if k not in ("_tracea_quantized", "_tracea_captured")}
 
     def requantize(self):
-        """Forget the quantised weight. Needed after a change that torch does not count, one through ``weight.data``."""
+        """Forget the quantised weight. Needed after a change that torch does not count: one through ``weight.data``, or by the replay
+        of a graph. (Steps of a torch.optim.Optimizer are noticed, those that torch does not count too.)"""
         cached = getattr(self, "_tracea_quantized", None)
         if cached is not None and not torch.cuda.is_current_stream_capturing():
             torch.cuda.synchronize(cached[0].device)
