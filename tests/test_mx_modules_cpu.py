@@ -1,6 +1,7 @@
 """What nn.MxLinear keeps between calls, without a GPU: the conversion is replaced by one that counts and copies."""
 import copy
 import io
+import types
 
 import pytest
 import torch
@@ -18,7 +19,9 @@ def quantized(monkeypatch):
         return w.detach().clone()
 
     monkeypatch.setattr(nn.ops, "mx_quantize", quantize)
-    monkeypatch.setattr(torch.cuda, "synchronize", lambda *a: None)
+    stream = types.SimpleNamespace(synchronize=lambda: None)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: stream)
+    monkeypatch.setattr(nn, "_stream_handle", lambda index: 0)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     return made
 

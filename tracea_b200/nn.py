@@ -49,6 +49,11 @@ class TraceaConv2d(torch.nn.Conv2d):
                                "bias" if bias is not None else None)
 
 
+def _stream_handle(device_index):
+    """The current stream's handle. torch.cuda.current_stream takes 2 us, a fifth of a layer's call."""
+    return torch._C._cuda_getCurrentRawStream(device_index)
+
+
 # Layers that keep a quantised weight. Some optimizers, torch's fused ones among them, write a weight without counting a version of it,
 # so the layers that a step has changed are told.
 _quantized_layers = weakref.WeakSet()
@@ -74,9 +79,11 @@ class MxLinear(torch.nn.Linear):
     (``ops.mx_gemm``): the weight is quantised once per version, the input, of any leading shape and fp32, fp16 or bf16, in every
     call. The output has the input's type; ``epilogue`` is an activation of ``ops.gemm``. Forward only, as TraceaConv2d.
 
-    A new version waits once for the device: other streams may read the quantised weight from then on. A CUDA graph that is
-    captured with a quantised weight at hand keeps to that one, whatever becomes of the layer's; captured right after
-    ``requantize()``, or after a step of an optimizer, it quantises the weight in every replay."""
+    A new version waits once for the current stream: other streams may read the quantised weight from then on. (Like any call
+    that may allocate, it ends a capture that another thread has open in torch's "global" mode; "thread_local" ones go on.) A CUDA
+    graph that is captured with a quantised weight at hand keeps to that one, whatever becomes of the layer's, and the layer holds it
+    as long as it lives; captured right after ``requantize()``, or after a step of an optimizer, it quantises the weight in every
+    replay. A weight made in inference mode has no versions and is quantised in every call."""
 
     def __init__(self, in_features, out_features, bias=True, epilogue=None, device=None, dtype=None):
         super().__init__(in_features, out_features, bias, device, dtype)
@@ -89,18 +96,21 @@ class MxLinear(torch.nn.Linear):
         if w.is_inference():                      # no version to go by
             return ops.mx_quantize(w)
         # The cached entry holds the weight it was made from, so that another one cannot lie at its address.
-        cached = getattr(self, "_tracea_quantized", None)
-        if (cached is None or cached[1] != w._version or cached[0].data_ptr() != w.data_ptr() or cached[0].dtype != w.dtype
+        cached, version = getattr(self, "_tracea_quantized", None), w._version
+        if (cached is None or cached[1] != version or cached[0].data_ptr() != w.data_ptr() or cached[0].dtype != w.dtype
                 or cached[0].device != w.device or cached[0].shape != w.shape or cached[0].stride() != w.stride()):
             q = ops.mx_quantize(w)
             if torch.cuda.is_current_stream_capturing():
                 return q                          # the graph's: nothing is in it before a replay
-            torch.cuda.synchronize(w.device)      # it is complete for every stream, and nothing reads the old one any more
-            self._tracea_quantized = (w, w._version, q)
+            torch.cuda.current_stream(w.device).synchronize()    # complete for every stream (no capture lets the device be waited for)
+            self._tracea_quantized = (w, version, q, w.device.index, _stream_handle(w.device.index))
             _watch(self)
             return q
         if torch.cuda.is_current_stream_capturing():
             self.__dict__.setdefault("_tracea_captured", {})[id(cached)] = cached     # graphs read it as long as the layer lives
+        elif _stream_handle(cached[3]) != cached[4]:
+            # once it is dropped, its memory, one allocation, waits for what this stream reads
+            cached[2].data.record_stream(torch.cuda.current_stream(w.device))
         return cached[2]
 
     def __getstate__(self):
@@ -110,9 +120,6 @@ class MxLinear(torch.nn.Linear):
     def requantize(self):
         """Forget the quantised weight. Needed after a change that torch does not count: one through ``weight.data``, or by the replay
         of a graph. (Steps of a torch.optim.Optimizer are noticed, those that torch does not count too.)"""
-        cached = getattr(self, "_tracea_quantized", None)
-        if cached is not None and not torch.cuda.is_current_stream_capturing():
-            torch.cuda.synchronize(cached[0].device)
         self._tracea_quantized = None
 
     def product(self, rows, dtype=None, quantize=False):
