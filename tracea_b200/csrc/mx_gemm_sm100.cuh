@@ -287,8 +287,8 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
 
   if (warp == 0 || warp == kSecondProducer) {
     // ------------------------------------------------------------ TMA producers (uniform control flow, one lane issues)
-    // A warp needs ~140 cycles to issue a copy, whatever its size, and a stage has four: warp 0 brings A and its scales in, warp
-    // 10 W and its. Only warp 0 arms the stage's barrier; bytes may arrive on it before, its phase cannot end without that.
+    // A warp needs ~140 cycles to issue a copy, whatever its size, and a stage has four: warp 0 brings A and its scales in, the other
+    // one W and its. Only warp 0 arms the stage's barrier; bytes may arrive on it before, its phase cannot end without that.
     const uint32_t issue = elect_one_lane();
     uint32_t stage_addr = smem_base, full_addr = full_bar0, empty_addr = empty_bar0, phase = 0;
     bool ok = true, stopped = false;
@@ -375,7 +375,6 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
                                       kScaleDescHi);
         }
       };
-      int steps_left = (worker < tiles ? (tiles - worker + num_workers - 1) / num_workers : 0) * k_iters;
       for (int tile = worker; ok && tile < tiles; tile += num_workers, ++local) {
         const int buf = kAcc == 2 ? local & 1 : 0;
         const uint32_t use = static_cast<uint32_t>(kAcc == 2 ? local >> 1 : local);
@@ -417,8 +416,9 @@ mx_gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
               copy_scales(a, ta);
             }
             // the next stage's scales go ahead of this stage's MMAs where its bytes are known to have landed: copies right in
-            // front of the MMAs that read them hold the tensor pipe up
-            scales_issued = ready && --steps_left > 0;
+            // front of the MMAs that read them hold the tensor pipe up. (Behind the last step there is no such stage: nobody
+            // loads it, so the phase that the probe asks for does not end.)
+            scales_issued = ready;
             if (scales_issued) {
               tc_fence_after();
               copy_scales(next_a, next_ta);
