@@ -300,6 +300,8 @@ TraceaStatus tracea_block_norm(TraceaTensorView x, const TraceaNorm *norm, Trace
 
 /* r = residual_scale * x + gate * norm(h): joins a block's output h to the stream x it started from. h, x, r: [M,C], one dtype;
  * gate: [G,C] as scale above, or NULL. With `following`, y (or y_mx) = following(r), of r as it is stored, in the same pass.
+ * The bits are those of two calls where h, x, r and y either all have 16-byte aligned rows (and C % 8 = 0) or would not in the second
+ * call either; else the sums are taken in another order.
  * r may be x or h itself; otherwise outputs overlap nothing. */
 TraceaStatus tracea_block_norm_add(TraceaTensorView h, TraceaTensorView x, const TraceaNorm *norm, const TraceaTensorView *gate,
                                    float residual_scale, TraceaTensorView *r, const TraceaNorm *following, TraceaTensorView *y,

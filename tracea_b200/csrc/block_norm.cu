@@ -106,7 +106,9 @@ void launch_norm(const tb200::BlockNormArgs& a, bool join, int next, bool vec, i
   //     148 rows  2.8 2.9   3.0 3.3   2.8 2.9   3.4 3.5   3.7 4.0        20000 rows  17 16   21 19   20 20   31 29    34 28
   //   12544 rows   13 11    14 12     14 12     21 17     23 20          80000 rows  58 61   68 58   86 81  116 117  117 88
   // 704 of fp32, 12544 rows: 17 15, 17 16, 20 18, 29 26, 29 26; 80000: 81 79, 75 70, 108 122, 151 165, 152 122. Rows that are not
-  // 16-byte aligned lose as often as they win. The choice may depend on the rows alone: the same row has the same bits in all forms.
+  // 16-byte aligned lose as often as they win. The choice may depend on the rows alone, not on what the call does with them:
+  // aligned alike, the same rows have the same bits in all of a call's forms. (The bound on bytes is the fp32 rows'; 16-bit ones past it
+  // would gain in three forms and lose up to 5 % in two.)
   const bool warp_rows = vec && a.M >= 4 * num_sms && static_cast<long long>(a.M) * a.C * static_cast<long long>(sizeof(T)) <= (40LL << 20);
   if (a.C <= 256) launch_norm_shape<T, 32, 1>(a, join, next, vec, dev, num_sms, stream);
   else if (a.C <= 512) launch_norm_shape<T, 32, 2>(a, join, next, vec, dev, num_sms, stream);

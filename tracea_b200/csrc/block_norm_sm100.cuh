@@ -3,7 +3,8 @@
 //   norm:  y = stage(r), in the storage type or in the 4-bit format of mx_format.cuh
 // where stage(v) = (norm(v) * weight + bias) * (1 + scale) + shift, and norm(v) = v / sqrt(mean(v^2) + eps) (rms),
 // (v - mean) / sqrt(mean((v - mean)^2) + eps) (layer) or v (none). A call does either or both; the norm behind a join reads r as it
-// is stored, so that both in one call give the bits of two calls.
+// is stored, so that both in one call give the bits of two calls where all their rows allow the same accesses (16 bytes or not). A
+// row that is summed in the other form's order differs by fp32's rounding.
 //
 // Bound by memory: a row is read once into registers and everything is computed from there, in fp32. The second moment is taken
 // about the mean, in a pass of its own over the registers -- as mean(v^2) - mean^2 a row far from zero would lose it.

@@ -318,7 +318,8 @@ def block_norm_add(h, x, weight=None, bias=None, scale=None, shift=None, gate=No
     from, both (M, C) of one type; gate (G, C) as scale, or None. kind "none" joins h as it is.
 
     following: the next block's norm, a dict of the keyword arguments of ``block_norm``; then (r, y) is returned, with
-    y = block_norm(r, **following) to the bit, from the same pass over the rows."""
+    y = block_norm(r, **following), from the same pass over the rows. The same bits where the rows of h and x are 16-byte aligned,
+    as r's are where C is a multiple of 8 (or C is not one); else the sums of y's norm are taken in another order."""
     if following is None:
         return _native().block_norm_add(h, x, weight, bias, scale, shift, _norm_kind(kind), eps, gate, residual_scale, 0)
     return _norm_add_following(h, x, (weight, bias, scale, shift, _norm_kind(kind), eps, gate, residual_scale), **following)
