@@ -88,7 +88,7 @@ def test_a_replaced_weight_is_not_overwritten_while_another_stream_reads_it():
         with torch.no_grad():
             lin.weight.mul_(2.0)
         new = lin(x)
-        size = lin._tracea_quantized[2].data.untyped_storage().nbytes()
+        size = ops.mx_quantize(lin.weight.detach()).data.untyped_storage().nbytes()
         lin.requantize()
         junk = [torch.full((size,), 119, dtype=torch.uint8, device="cuda") for _ in range(20)]
         torch.cuda.synchronize()
