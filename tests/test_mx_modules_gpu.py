@@ -95,3 +95,9 @@ def test_a_replaced_weight_is_not_overwritten_while_another_stream_reads_it():
         assert torch.equal(got, want) and torch.equal(new, result(lin, x)) and len(junk) == 20
         lin(x), torch.cuda.synchronize()
     status_ok()
+
+
+def test_feed_forward_of_no_samples():
+    ff = nn.MxFeedForward(64, 96, device="cuda")
+    none = torch.empty(0, 64, device="cuda")
+    assert ff(torch.empty(0, 7, 64, device="cuda"), gate=none, scale=none, shift=none).shape == (0, 7, 64)

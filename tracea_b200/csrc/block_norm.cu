@@ -12,7 +12,8 @@ tb200::NormVector load_vector(const TraceaTensorView* v, const char* name, int d
                               long long M, long long& groups) {
   tb200::NormVector o = {nullptr, 0, 0, 0};
   if (v == nullptr) return o;
-  if (v->ptr == nullptr || v->device_id != dev) TB_FAIL(TRACEA_INVALID_PARAMS, "%s must be on device %d", name, dev);
+  const bool none = grouped && M == 0;                              // no samples, and so maybe no groups
+  if ((v->ptr == nullptr && !none) || v->device_id != dev) TB_FAIL(TRACEA_INVALID_PARAMS, "%s must be on device %d", name, dev);
   if (v->shape == nullptr || v->rank != (grouped ? 2u : 1u))
     TB_FAIL(TRACEA_INVALID_PARAMS, "%s must have shape [%s%lld]", name, grouped ? "groups, " : "", C);
   const int d = grouped ? 1 : 0;
@@ -24,6 +25,7 @@ tb200::NormVector load_vector(const TraceaTensorView* v, const char* name, int d
   const int es = elem_size(v->dtype);
   if ((reinterpret_cast<uintptr_t>(v->ptr) & (es - 1)) != 0) TB_FAIL(TRACEA_INVALID_PARAMS, "%s is not aligned to its elements", name);
   if (grouped) {
+    if (none) return o;
     const unsigned long long n = v->shape[0];
     if (n == 0 || n > 0x7fffffffULL || M % static_cast<long long>(n) != 0)
       TB_FAIL(TRACEA_INVALID_PARAMS, "%s has %llu groups, which do not divide the %lld rows", name, n, M);
