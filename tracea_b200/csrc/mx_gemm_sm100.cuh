@@ -70,7 +70,7 @@ __host__ __device__ constexpr int mx_num_stages(int bn, bool pair, int store) {
   return n < kMxMaxStages ? n : kMxMaxStages;
 }
 
-// apply_act32 with fewer trips through the special-function unit, which bounds SiLU here: a tile of 192 columns of 1024 takes
+// apply_act32, but for ReLU, which keeps NaN, and GELU (see kGeluA), with fewer trips through the special-function unit for SiLU: a tile of 192 columns of 1024 takes
 // 2200 cycles of MMAs and 128 x 192 exponentials and reciprocals, at 16 of these a cycle, 3100. Four values share a reciprocal,
 // 1 / a = (1 / abcd) bcd, which costs three roundings more, 2^-22 -- far below a 16- or 4-bit result's. The product of four stays
 // in range while each 1 + e^-x is below 2^31: 32 columns of a row with a value below -20, or a NaN, take the other way. (Each lane

@@ -283,7 +283,8 @@ void tokens_product(DeviceState& st, const Product& p, const Matrix* x, const To
 // Columns of a tile: 64 or 128 in a CTA, 192 or 256 in a pair of CTAs (256 rows). By the time of the busiest CTA or pair, in
 // us: what a launch takes once, and per wave of tiles either its k-steps (an SM has 16 KB of A and half or all of the columns' rows
 // of W to bring in a step) and what lies between two tiles, or its epilogue, whichever is longer. 192 columns have two accumulators,
-// 256 one, which pays for its wider steps only over a long K. Measured / this formula, columns 64, 128, 192, 256:
+// 256 one, which pays for its wider steps only over a long K. Measured / this formula, columns 64, 128, 192, 256, bf16 outputs (fp32 and
+// 4-bit ones take the same choice):
 //   8192 x 8192 x 8192         352 251 204 192 / 444 261 212 206     12544 x 4096 x 1024    49  38  31 34 / 53 33 31 36
 //   4096 x 4096 x 4096          49  32  30  32 / 59  36  32  35      the same, SiLU          53  41  41 47 / 53 41 42 47
 //   2048 x 2048 x 2048        12.6 7.3 9.2 9.1 / 11 7.9 10 8.7       1024 x 1024 x 2048   4.8 5.3 6.7  - / 4.8 5.4 7.0 8.6
