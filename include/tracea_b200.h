@@ -307,6 +307,80 @@ TraceaStatus tracea_block_norm_add(TraceaTensorView h, TraceaTensorView x, const
                                    float residual_scale, TraceaTensorView *r, const TraceaNorm *following, TraceaTensorView *y,
                                    TraceaMxMatrix *y_mx, void *stream);
 
+/* ---- rows of heads and the cache of keys and values. No counterpart in the reference. --------------------------------------- */
+
+/* x: [tokens, heads, D] with contiguous columns (a slice of a projection's rows, say); y: the same of x's dtype, may be x itself;
+ * weight: [D], FLOAT32 or x's dtype, contiguous, or NULL. */
+typedef struct {
+  TraceaTensorView x;
+  const TraceaTensorView *weight;
+  TraceaTensorView *y;
+} TraceaHeads;
+
+/* Pair i of a head's first 2 * pairs columns -- columns 2i and 2i + 1 if interleaved, else i and i + pairs -- is turned by
+ * position * frequencies[i] radians: (a cos - b sin, b cos + a sin). `frequencies` is device memory. The angle is computed in 64 bits. */
+typedef struct {
+  const double *frequencies;
+  uint32_t pairs;
+  int32_t interleaved;
+} TraceaRotation;
+
+/* y = rotate(norm(x) * weight) for queries and keys (either may be NULL) of the same tokens and D, even and at most 256: norm per head
+ * (TRACEA_NORM_NONE or TRACEA_NORM_RMS), in fp32, rounded once. positions: [tokens], INT32, needed with a rotation (NULL: none). */
+TraceaStatus tracea_head_norm_rotate(const TraceaHeads *q, const TraceaHeads *k, TraceaNormKind kind, float eps,
+                                     const TraceaRotation *rotation, const TraceaTensorView *positions, void *stream);
+
+/* Keys and values in 8 bits, in pages of P = page_size tokens (16, 32, 64 or 128) of `heads` heads of D = head_dim columns (a multiple
+ * of 16 up to 128), dense device memory:
+ *   k, v                 [pages][heads][P][D] elements of e4m3 (sign, four exponent bits, three mantissa bits; no infinities), 16-byte
+ *                        aligned
+ *   k_scales, v_scales   [pages][heads] bytes b, 87 <= b <= 167: the block's elements stand for 2^(b - 127) times themselves */
+typedef struct {
+  void *k;
+  void *v;
+  uint8_t *k_scales;
+  uint8_t *v_scales;
+  uint64_t pages;
+  uint32_t heads;
+  uint32_t page_size;
+  uint32_t head_dim;
+  int32_t device_id;
+} TraceaKvCache;
+
+/* What the rows of a call belong to, INT32 device memory that is read on the device: sequence s has lengths[s] tokens, this call's
+ * included, token j in row j % P of page pages[s][j / P]; rows starts[s] .. starts[s + 1] - 1 of the call are its last ones. starts
+ * ([sequences + 1], not decreasing, from 0 to the rows) may be NULL: row s is the last token of sequence s. An entry of `pages` outside
+ * the cache is a page that is not there, and so is what the table is too short for: nothing is written to it and nothing of it is
+ * attended to. Sequences share pages only where no call writes to them. */
+typedef struct {
+  TraceaTensorView pages;   /* [sequences, width] */
+  TraceaTensorView lengths; /* [sequences] */
+  const TraceaTensorView *starts;
+} TraceaSequences;
+
+/* Puts k (norm, k_weight and rotation by the token's position j as above) and v, both [rows, heads, D], into the cache. A block that
+ * gets tokens gets the scale that reaches its largest value, the smallest 2^e with |values| <= 448 * 2^e, -40 <= e <= 40 -- or keeps the
+ * one it has, if that is larger and the block holds older tokens; where theirs grows, they are rounded to it. Elements are rounded to
+ * nearest, ties to even, and saturate. A token whose key or value in a head is not finite becomes a NaN key and a zero value there, and
+ * counts for no scale. Rows of a page behind the sequence's last token are left as they are. q, if given ([rows, a multiple of heads, D]),
+ * is normalised and rotated into q->y in the same launch, and so are the rows whose page is not there. */
+TraceaStatus tracea_kv_append(TraceaKvCache cache, TraceaSequences sequences, TraceaTensorView k, TraceaTensorView v,
+                              const TraceaTensorView *k_weight, const TraceaHeads *q, TraceaNormKind kind, float eps,
+                              const TraceaRotation *rotation, void *stream);
+
+/* out = softmax(scale * q k^T) v over the tokens of the cache that each row sees: those of its sequence, if `causal` up to its own
+ * position, if window > 0 none more than window - 1 positions in front of its own. q and out: [rows, H, D],
+ * FLOAT16 or BFLOAT16, H a multiple of the cache's heads, which H / heads consecutive ones share. A row that sees nothing becomes 0;
+ * one that sees a NaN key, NaN (values of the cache hold none). Scores, maxima, sums and the result are held in fp32; the weights of the values are rounded to 11 bits. */
+typedef struct {
+  float scale;
+  int32_t causal;
+  uint32_t window;
+  void *stream;
+} TraceaKvAttentionParams;
+TraceaStatus tracea_kv_attention(TraceaTensorView q, TraceaKvCache cache, TraceaSequences sequences, TraceaTensorView *out,
+                                 TraceaKvAttentionParams params);
+
 /* Thread-local last error text: tracea-ffi/src/lib.rs:87-109. Returns bytes copied (without the
  * terminating NUL), -1 when buf is NULL or len is 0. */
 int32_t tracea_get_last_error(uint8_t *buf, size_t len);
@@ -354,7 +428,8 @@ uint64_t tracea_b200_launch_count(void);
  * over K, 2 the resident-filter kernel (stride-1 small filters over 64-channel activations), 3 layout adapters,
  * 4 the row-band kernel (few-channel 16-bit images such as the RGB stem), 5 the small-tile kernel (problems of up to one
  * wave of 64-row tiles); and 6, those of 0, 1 and 5 that read a copied input by whole filter rows instead of tap by tap; 7
- * conversions to and from the 4-bit format, 8 its matrix product, 9 the form of that for few rows, 10 norms.
+ * conversions to and from the 4-bit format, 8 its matrix product, 9 the form of that for few rows, 10 norms; 11 norms and rotations
+ * of heads and appending to a cache, 12 attention over a cache for few rows a sequence, 13 for many.
  * Lets tests and benchmarks see which path a call took. 0 for any other `kind`. No counterpart in the reference. */
 uint64_t tracea_b200_launch_count_of(int32_t kind);
 

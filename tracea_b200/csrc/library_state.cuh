@@ -98,9 +98,11 @@ inline std::atomic<int> g_test_producer_stop{-1};
 inline std::atomic<unsigned long long> g_kernel_launches{0};   // every kernel this library has launched (conv + layout adapters)
 // the same, by kind: 0 general implicit-GEMM kernel, 1 its K-split instantiations, 2 resident-filter kernel, 3 layout adapters,
 // 4 row-band kernel, 5 small-tile kernel; and 6, those of 0, 1 and 5 whose k-chunks run over whole filter rows; 7 conversions to
-// and from the 4-bit format, 8 its matrix product, 9 the form of that for few rows, 10 norms
-constexpr int kLaunchKinds = 11;
-constexpr int kLaunchMxCopy = 7, kLaunchMxGemm = 8, kLaunchMxTokens = 9, kLaunchNorm = 10;
+// and from the 4-bit format, 8 its matrix product, 9 the form of that for few rows, 10 norms; 11 norms and rotations of heads and
+// appending to a cache, 12 attention over a cache for few rows a sequence, 13 for many
+constexpr int kLaunchKinds = 14;
+constexpr int kLaunchMxCopy = 7, kLaunchMxGemm = 8, kLaunchMxTokens = 9, kLaunchNorm = 10, kLaunchHeads = 11, kLaunchKvTokens = 12,
+              kLaunchKvRows = 13;
 inline std::atomic<unsigned long long> g_launches_by_kind[kLaunchKinds];
 inline EncodeTiledFn g_encode_tiled = nullptr;
 inline EncodeIm2colFn g_encode_im2col = nullptr;

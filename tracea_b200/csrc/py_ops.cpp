@@ -448,6 +448,186 @@ PyObject* py_block_norm_add(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// ------------------------------------------------------------------ rows of heads and the cache of keys and values
+float float_arg(PyObject* o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred() != nullptr) throw PyError{};
+  return static_cast<float>(v);
+}
+
+void heads_rank(const at::Tensor& t, const char* name) {
+  if (t.dim() != 3) {
+    PyErr_Format(PyExc_ValueError, "%s must have three dimensions: (tokens, heads, columns)", name);
+    throw PyError{};
+  }
+}
+
+// Rows of heads, their weight and, where asked for, a new tensor for the result.
+struct HeadsArg {
+  View x, w, y;
+  at::Tensor out;
+  TraceaHeads h;
+  HeadsArg(const at::Tensor& t, PyObject* weight, const char* name, const char* weight_name) {
+    heads_rank(t, name);
+    out = at::empty({t.size(0), t.size(1), t.size(2)}, t.options());
+    fill(x, t);
+    fill(y, out);
+    h.x = x.v;
+    h.y = &y.v;
+    h.weight = opt(optional_tensor(weight, weight_name), w);
+  }
+};
+
+// The rotation of `frequencies` (None: none), which have to lie where `like` does.
+struct RotationArg {
+  TraceaRotation r;
+  bool given;
+  RotationArg(PyObject* frequencies, bool interleaved, const at::Tensor& like) : given(frequencies != Py_None) {
+    if (!given) return;
+    const at::Tensor& f = tensor_arg(frequencies, "frequencies");
+    if (f.scalar_type() != at::kDouble || f.dim() != 1 || !f.is_contiguous() || f.device() != like.device() || f.size(0) > 0x7fffffff) {
+      PyErr_SetString(PyExc_ValueError, "frequencies must be a contiguous float64 vector on the device of the rows");
+      throw PyError{};
+    }
+    r.frequencies = f.data_ptr<double>();
+    r.pairs = static_cast<uint32_t>(f.size(0));
+    r.interleaved = interleaved ? 1 : 0;
+  }
+  const TraceaRotation* get() const { return given ? &r : nullptr; }
+};
+
+// head_norm_rotate(q or None, k or None, positions, frequencies, interleaved, q_weight, k_weight, kind, eps) -> (q, k)
+PyObject* py_head_norm_rotate(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!arg_count(n, 9, "head_norm_rotate")) return nullptr;
+  return guarded([&]() -> PyObject* {
+    const at::Tensor *q = optional_tensor(a[0], "q"), *k = optional_tensor(a[1], "k"), *pos = optional_tensor(a[2], "positions");
+    if (q == nullptr && k == nullptr) {
+      PyErr_SetString(PyExc_ValueError, "neither q nor k is given");
+      throw PyError{};
+    }
+    const at::Tensor& first = q != nullptr ? *q : *k;
+    c10::optional<HeadsArg> hq, hk;
+    if (q != nullptr) hq.emplace(*q, a[5], "q", "q_weight");
+    if (k != nullptr) hk.emplace(*k, a[6], "k", "k_weight");
+    const RotationArg rot(a[3], PyObject_IsTrue(a[4]), first);
+    View vp;
+    const TraceaTensorView* pp = opt(pos, vp);
+    const auto kind = static_cast<TraceaNormKind>(int_arg(a[7]));
+    const float eps = float_arg(a[8]);
+    void* stream = stream_of(first);
+    const TraceaStatus st = without_gil([&] {
+      return tracea_head_norm_rotate(hq ? &hq->h : nullptr, hk ? &hk->h : nullptr, kind, eps, rot.get(), pp, stream);
+    });
+    if (st != TRACEA_SUCCESS) raise_status(st, "tracea_head_norm_rotate");
+    PyObject* first_out = q != nullptr ? THPVariable_Wrap(hq->out) : Py_NewRef(Py_None);
+    PyObject* second = first_out == nullptr ? nullptr : k != nullptr ? THPVariable_Wrap(hk->out) : Py_NewRef(Py_None);
+    PyObject* pair = second != nullptr ? PyTuple_Pack(2, first_out, second) : nullptr;
+    Py_XDECREF(first_out);
+    Py_XDECREF(second);
+    return pair;
+  });
+}
+
+// The cache of four tensors: k, v (pages, heads, P, D), of one-byte elements, and the scales (pages, heads), uint8.
+TraceaKvCache cache_arg(PyObject* const* a) {
+  const at::Tensor &k = tensor_arg(a[0], "cache.k"), &v = tensor_arg(a[1], "cache.v"), &ks = tensor_arg(a[2], "cache.k_scales"),
+                   &vs = tensor_arg(a[3], "cache.v_scales");
+  auto bad = [](const at::Tensor& t) { return t.scalar_type() != at::kFloat8_e4m3fn || !t.is_contiguous(); };
+  if (bad(k) || bad(v) || k.dim() != 4 || v.sizes() != k.sizes() || ks.scalar_type() != at::kByte || vs.scalar_type() != at::kByte ||
+      !ks.is_contiguous() || !vs.is_contiguous() || ks.dim() != 2 || ks.size(0) != k.size(0) || ks.size(1) != k.size(1) ||
+      vs.sizes() != ks.sizes() || v.device() != k.device() || ks.device() != k.device() || vs.device() != k.device()) {
+    PyErr_SetString(PyExc_ValueError, "a cache is contiguous tensors on one device: k and v float8_e4m3fn (pages, heads, page size, columns), "
+                                      "k_scales and v_scales uint8 (pages, heads)");
+    throw PyError{};
+  }
+  for (int d = 1; d < 4; ++d) {
+    if (k.size(d) > 0x7fffffff) {
+      PyErr_SetString(PyExc_ValueError, "cache: out of range");
+      throw PyError{};
+    }
+  }
+  TraceaKvCache c;
+  c.k = k.data_ptr();
+  c.v = v.data_ptr();
+  c.k_scales = ks.data_ptr<uint8_t>();
+  c.v_scales = vs.data_ptr<uint8_t>();
+  c.pages = static_cast<uint64_t>(k.size(0));
+  c.heads = static_cast<uint32_t>(k.size(1));
+  c.page_size = static_cast<uint32_t>(k.size(2));
+  c.head_dim = static_cast<uint32_t>(k.size(3));
+  c.device_id = cuda_index(k);
+  return c;
+}
+
+struct SequencesArg {
+  View pages, lengths, starts;
+  TraceaSequences s;
+  SequencesArg(PyObject* const* a) {
+    fill(pages, tensor_arg(a[0], "pages"));
+    fill(lengths, tensor_arg(a[1], "lengths"));
+    s.pages = pages.v;
+    s.lengths = lengths.v;
+    s.starts = opt(optional_tensor(a[2], "starts"), starts);
+  }
+};
+
+// kv_append(k cache, v cache, k scales, v scales, pages, lengths, starts, k, v, k_weight, q or None, q_weight, frequencies, interleaved,
+// kind, eps) -> q or None
+PyObject* py_kv_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!arg_count(n, 16, "kv_append")) return nullptr;
+  return guarded([&]() -> PyObject* {
+    const TraceaKvCache cache = cache_arg(a);
+    const SequencesArg seqs(a + 4);
+    const at::Tensor &k = tensor_arg(a[7], "k"), &v = tensor_arg(a[8], "v");
+    const at::Tensor* q = optional_tensor(a[10], "q");
+    heads_rank(k, "k");
+    heads_rank(v, "v");
+    View vk, vv, vw;
+    fill(vk, k);
+    fill(vv, v);
+    const TraceaTensorView* pw = opt(optional_tensor(a[9], "k_weight"), vw);
+    c10::optional<HeadsArg> hq;
+    if (q != nullptr) hq.emplace(*q, a[11], "q", "q_weight");
+    const RotationArg rot(a[12], PyObject_IsTrue(a[13]), k);
+    const auto kind = static_cast<TraceaNormKind>(int_arg(a[14]));
+    const float eps = float_arg(a[15]);
+    void* stream = stream_of(k);
+    const TraceaStatus st = without_gil([&] {
+      return tracea_kv_append(cache, seqs.s, vk.v, vv.v, pw, hq ? &hq->h : nullptr, kind, eps, rot.get(), stream);
+    });
+    if (st != TRACEA_SUCCESS) raise_status(st, "tracea_kv_append");
+    return q != nullptr ? THPVariable_Wrap(hq->out) : Py_NewRef(Py_None);
+  });
+}
+
+// kv_attention(q, k cache, v cache, k scales, v scales, pages, lengths, starts, scale, causal, window) -> out
+PyObject* py_kv_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!arg_count(n, 11, "kv_attention")) return nullptr;
+  return guarded([&]() -> PyObject* {
+    const at::Tensor& q = tensor_arg(a[0], "q");
+    heads_rank(q, "q");
+    const TraceaKvCache cache = cache_arg(a + 1);
+    const SequencesArg seqs(a + 5);
+    TraceaKvAttentionParams p;
+    p.scale = float_arg(a[8]);
+    p.causal = PyObject_IsTrue(a[9]) ? 1 : 0;
+    const long window = int_arg(a[10]);
+    if (window < 0 || window > 0x7fffffffL) {
+      PyErr_SetString(PyExc_ValueError, "window must be 0 (none) or a number of tokens");
+      throw PyError{};
+    }
+    p.window = static_cast<uint32_t>(window);
+    p.stream = stream_of(q);
+    at::Tensor out = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
+    View vq, vo;
+    fill(vq, q);
+    fill(vo, out);
+    const TraceaStatus st = without_gil([&] { return tracea_kv_attention(vq.v, cache, seqs.s, &vo.v, p); });
+    if (st != TRACEA_SUCCESS) raise_status(st, "tracea_kv_attention");
+    return THPVariable_Wrap(out);
+  });
+}
+
 PyMethodDef kMethods[] = {
     {"conv2d", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_conv2d)), METH_FASTCALL, nullptr},
     {"gemm", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_gemm)), METH_FASTCALL, nullptr},
@@ -457,6 +637,9 @@ PyMethodDef kMethods[] = {
     {"mx_gemm", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_mx_gemm)), METH_FASTCALL, nullptr},
     {"block_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_block_norm)), METH_FASTCALL, nullptr},
     {"block_norm_add", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_block_norm_add)), METH_FASTCALL, nullptr},
+    {"head_norm_rotate", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_head_norm_rotate)), METH_FASTCALL, nullptr},
+    {"kv_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_kv_append)), METH_FASTCALL, nullptr},
+    {"kv_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_kv_attention)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_ops_native", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

@@ -29,7 +29,8 @@ EXPORTED_SYMBOLS = (
     "tracea_gemm", "tracea_conv_transpose2d", "tracea_conv2d_prepack_bytes", "tracea_conv2d_prepack",
     "tracea_gemm_prepack_b_bytes", "tracea_gemm_prepack_b",
     "tracea_mx_data_bytes", "tracea_mx_scale_bytes", "tracea_mx_quantize", "tracea_mx_dequantize", "tracea_mx_gemm",
-    "tracea_mx_linear", "tracea_block_norm", "tracea_block_norm_add",
+    "tracea_mx_linear", "tracea_block_norm", "tracea_block_norm_add", "tracea_head_norm_rotate", "tracea_kv_append",
+    "tracea_kv_attention",
 )
 
 
@@ -94,6 +95,28 @@ class Norm(ctypes.Structure):
     _fields_ = [("kind", ctypes.c_int), ("eps", ctypes.c_float), ("weight", ctypes.POINTER(TensorView)),
                 ("bias", ctypes.POINTER(TensorView)), ("scale", ctypes.POINTER(TensorView)),
                 ("shift", ctypes.POINTER(TensorView))]
+
+
+class Heads(ctypes.Structure):
+    _fields_ = [("x", TensorView), ("weight", ctypes.POINTER(TensorView)), ("y", ctypes.POINTER(TensorView))]
+
+
+class Rotation(ctypes.Structure):
+    _fields_ = [("frequencies", ctypes.c_void_p), ("pairs", ctypes.c_uint32), ("interleaved", ctypes.c_int32)]
+
+
+class KvCache(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scales", ctypes.c_void_p), ("v_scales", ctypes.c_void_p),
+                ("pages", ctypes.c_uint64), ("heads", ctypes.c_uint32), ("page_size", ctypes.c_uint32),
+                ("head_dim", ctypes.c_uint32), ("device_id", ctypes.c_int32)]
+
+
+class Sequences(ctypes.Structure):
+    _fields_ = [("pages", TensorView), ("lengths", TensorView), ("starts", ctypes.POINTER(TensorView))]
+
+
+class KvAttentionParams(ctypes.Structure):
+    _fields_ = [("scale", ctypes.c_float), ("causal", ctypes.c_int32), ("window", ctypes.c_uint32), ("stream", ctypes.c_void_p)]
 
 
 class TraceaError(RuntimeError):
@@ -174,8 +197,13 @@ def load():
     lib.tracea_mx_linear.argtypes = [TensorView, MxMatrix, pv, pv, pv, pm, GemmParams]
     lib.tracea_block_norm.argtypes = [TensorView, pn, pv, pm, ctypes.c_void_p]
     lib.tracea_block_norm_add.argtypes = [TensorView, TensorView, pn, pv, ctypes.c_float, pv, pn, pv, pm, ctypes.c_void_p]
+    ph, pr = ctypes.POINTER(Heads), ctypes.POINTER(Rotation)
+    lib.tracea_head_norm_rotate.argtypes = [ph, ph, ctypes.c_int, ctypes.c_float, pr, pv, ctypes.c_void_p]
+    lib.tracea_kv_append.argtypes = [KvCache, Sequences, TensorView, TensorView, pv, ph, ctypes.c_int, ctypes.c_float, pr,
+                                     ctypes.c_void_p]
+    lib.tracea_kv_attention.argtypes = [TensorView, KvCache, Sequences, pv, KvAttentionParams]
     for name in ("tracea_mx_quantize", "tracea_mx_dequantize", "tracea_mx_gemm", "tracea_mx_linear", "tracea_block_norm",
-                 "tracea_block_norm_add"):
+                 "tracea_block_norm_add", "tracea_head_norm_rotate", "tracea_kv_append", "tracea_kv_attention"):
         getattr(lib, name).restype = ctypes.c_int
     _lib = lib
     return lib

@@ -330,6 +330,89 @@ def _norm_add_following(h, x, first, weight=None, bias=None, scale=None, shift=N
     return r, MxTensor(*y, tuple(x.shape)) if quantize else y
 
 
+def rotary_frequencies(columns, base=10000.0, device=None):
+    """The usual angles per position of a rotation of ``columns`` columns, base^(-2i / columns) for pair i: float64, (columns / 2)."""
+    if columns % 2 != 0:
+        raise ValueError("a rotation takes an even number of columns")
+    return torch.pow(float(base), -torch.arange(0, columns, 2, dtype=torch.float64, device=device) / columns)
+
+
+def head_norm_rotate(q, k, positions=None, frequencies=None, interleaved=False, q_weight=None, k_weight=None, kind="rms", eps=1e-6):
+    """Queries and keys between their projections and attention: each head's columns normalised, times a weight, and rotated by the
+    token's position, in one pass. Returns new (q, k).
+
+    q (T, H, D) and k (T, H', D), either may be None; their columns are contiguous, other strides any (slices of one projection, say);
+    float32, float16 or bfloat16, D even and at most 256. kind "rms" or "none"; weights (D), float32 or the rows' type. positions (T),
+    int32, and frequencies, float64 radians per position (``rotary_frequencies``): pair i of the first 2 * len(frequencies) columns,
+    columns 2i and 2i + 1 if ``interleaved`` and i and i + len(frequencies) if not, is turned by positions * frequencies[i], an angle
+    that is computed in 64 bits."""
+    return _native().head_norm_rotate(q, k, positions, frequencies, interleaved, q_weight, k_weight, _norm_kind(kind), eps)
+
+
+class KvCache:
+    """Keys and values in 8 bits, in pages (TraceaKvCache of include/tracea_b200.h): ``k`` and ``v``, float8_e4m3fn of shape (pages,
+    heads, page_size, head_dim), and ``k_scales``, ``v_scales``, uint8 of shape (pages, heads): a page's and head's elements stand for
+    2^(byte - 127) times themselves. ``kv_append`` fills it, ``kv_attention`` reads it; a sequence's pages are the caller's to hand out."""
+
+    __slots__ = ("k", "v", "k_scales", "v_scales")
+
+    def __init__(self, k, v, k_scales, v_scales):
+        self.k, self.v, self.k_scales, self.v_scales = k, v, k_scales, v_scales
+
+    @classmethod
+    def empty(cls, pages, heads, head_dim, page_size=64, device="cuda"):
+        """A cache of ``pages`` pages of ``page_size`` (16, 32, 64 or 128) tokens, ``head_dim`` a multiple of 16 up to 128. All zeros."""
+        if page_size not in (16, 32, 64, 128):
+            raise ValueError("page_size must be 16, 32, 64 or 128")
+        if head_dim % 16 != 0 or not 16 <= head_dim <= 128:
+            raise ValueError("head_dim must be a multiple of 16 up to 128")
+        k, v = (torch.zeros((pages, heads, page_size, head_dim), dtype=torch.uint8, device=device) for _ in "kv")
+        ks, vs = (torch.full((pages, heads), 87, dtype=torch.uint8, device=device) for _ in "kv")
+        return cls(k.view(torch.float8_e4m3fn), v.view(torch.float8_e4m3fn), ks, vs)
+
+    @property
+    def device(self):
+        return self.k.device
+
+    @property
+    def page_size(self):
+        return self.k.shape[2]
+
+    def __repr__(self):
+        return "KvCache(%d pages of %d tokens, %d heads of %d, device=%s)" % (self.k.shape[0], self.k.shape[2], self.k.shape[1],
+                                                                             self.k.shape[3], self.k.device)
+
+
+def kv_append(cache, k, v, pages, lengths, starts=None, frequencies=None, interleaved=False, k_weight=None, q=None, q_weight=None,
+              kind="none", eps=1e-6):
+    """Puts new tokens' keys and values into ``cache``, the keys normalised and rotated on the way as ``head_norm_rotate`` does, by the
+    tokens' positions in their sequences. With ``q``, the queries of the same tokens, (T, H, D) with H a multiple of the cache's heads,
+    returns them normalised and rotated, from the same launch.
+
+    k, v (T, heads, D): the last tokens of the sequences. int32 tensors, read on the device: ``lengths`` (B), each sequence's tokens, the
+    new ones included; ``pages`` (B, width), its pages: token j lies in row j % page_size of page pages[s, j // page_size], and is dropped
+    where that is no page of the cache; ``starts`` (B + 1): rows starts[s] .. starts[s + 1] - 1 belong to sequence s -- None: row s is
+    the one new token of sequence s.
+
+    A block, the tokens of a page and head, has one scale: the smallest power of two 2^e of which 448 reach its largest value,
+    -40 <= e <= 40. It grows when a larger value is appended, and the block's older tokens are then rounded anew; a page's first token
+    starts it afresh. A token with a key or value in a head that is not finite is kept there as a NaN key and a zero value."""
+    return _native().kv_append(cache.k, cache.v, cache.k_scales, cache.v_scales, pages, lengths, starts, k, v, k_weight, q, q_weight,
+                               frequencies, interleaved, _norm_kind(kind), eps)
+
+
+def kv_attention(q, cache, pages, lengths, starts=None, scale=None, causal=True, window=0):
+    """Attention of queries (T, H, D), float16 or bfloat16, to the tokens of their sequences in ``cache``; ``pages``, ``lengths`` and
+    ``starts`` as in ``kv_append``, after which it is called. H a multiple of the cache's heads: H / heads consecutive heads of q share
+    one of the cache. scale: 1 / sqrt(D) unless given.
+
+    Rows see their sequence up to their own position (``causal``) or all of it, and with ``window`` no tokens more than window - 1
+    positions in front of their own. A row that sees no token gives 0."""
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    return _native().kv_attention(q, cache.k, cache.v, cache.k_scales, cache.v_scales, pages, lengths, starts, scale, causal, window)
+
+
 class Context:
     """Stand-in for the reference's ``tracea.Context`` (src/interface/python.rs:367-462), Conv2d only.
     The reference builds an IR, generates CUDA text and compiles it here; this one forwards to the
