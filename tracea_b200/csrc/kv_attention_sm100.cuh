@@ -1,0 +1,57 @@
+// What the kernels of attention over the cache share.
+//
+// One maximum serves the softmax and the values' scales: with s the score in powers of two and m >= s + ev for all tokens so far, up to
+// a slack, the weights 2^(s + ev - m) need no scaling of v^ and fit halves, whatever the pages' scales are; the softmax's denominator
+// is the sum of 2^(s + ev - m) 2^-ev. Since |ev| <= 40, neither can leave the range of fp32. The slack: m moves only when a score
+// passes it by 2^kSlack, so the sums are rescaled a few times a sequence and not every step.
+#pragma once
+#include "heads_sm100.cuh"
+
+namespace tb200 {
+
+constexpr float kSlack = 8.0f;   // weights up to 2^8 in halves, which reach 2^16
+
+struct KvAttentionArgs {
+  CacheRef cache;
+  SequencesRef seqs;
+  const void* q;
+  void* out;
+  long long q_token, q_head, out_token, out_head;
+  int q_vec;                     // q's heads can be read eight columns at a time
+  int out_vec;                   // columns of out that can be written at a time: 8, 4 or 1
+  int group;                     // heads of q to a head of keys
+  int causal, window;
+  int fewest, most;              // sequences with fewer or more rows (times group) are another kernel's
+  int row_tiles;
+  float scale_log2;              // |scale| * log2(e)
+  float sign;                    // of the scale
+  uint32_t* status;
+  long long wait_limit;          // cycles any single wait may take before its role gives up
+  int test_producer_stop;
+};
+
+__device__ __forceinline__ float exp2_ftz(float x) {
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x));
+  return x;
+}
+__device__ __forceinline__ uint32_t pack_halves(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ void mma_16x8x16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The power of two that brings a row whose largest absolute value is `peak` into [1, 2); 1 for a row of zeros or one that is not finite.
+// `back` is its inverse. (Both within the normal range: peak 2^-127 and smaller, or 2^127 and larger, are not brought all the way.)
+__device__ __forceinline__ float row_scale(float peak, float& back) {
+  int e = static_cast<int>(__float_as_uint(peak) >> 23) - 127;
+  if (peak == 0.0f || e == 128) e = 0;
+  e = min(max(e, -126), 126);
+  back = power_of_two(e);
+  return power_of_two(-e);
+}
+
+}  // namespace tb200

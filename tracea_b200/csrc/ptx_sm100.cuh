@@ -174,6 +174,16 @@ __device__ __forceinline__ bool mbar_wait_bounded_uniform(uint32_t bar, uint32_t
   }
 }
 
+// More, or fewer, registers a thread for a warpgroup: out of what the block was launched with.
+template <int kRegs>
+__device__ __forceinline__ void regs_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+template <int kRegs>
+__device__ __forceinline__ void regs_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+
 // One lane of a converged warp, as a 0 / 1 word (elect.sync).
 __device__ __forceinline__ uint32_t elect_one_lane() {
   uint32_t pred;
@@ -661,6 +671,22 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
                : "memory");
 }
 
+// One MMA of 16 columns of K whose A is in tensor memory, two halves to a column (whole-warp code, see mma_stage4_probe).
+__device__ __forceinline__ void mma_tmem_a_if(uint32_t issue, uint32_t tmem_d, uint32_t tmem_a, uint32_t b, uint32_t desc_hi,
+                                              uint32_t idesc, uint32_t accumulates) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p, q;\n"
+      ".reg .b64 db;\n"
+      "setp.ne.b32 p, %5, 0;\n"
+      "setp.ne.b32 q, %6, 0;\n"
+      "mov.b64 db, {%2, %3};\n"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n"
+      "}\n" ::"r"(tmem_d),
+      "r"(tmem_a), "r"(b), "r"(desc_hi), "r"(idesc), "r"(accumulates), "r"(issue)
+      : "memory");
+}
+
 // ------------------------------------------------------------------ block-scaled MMA (4-bit operands, a scale per 32 of K)
 // 32 rows of 16 bytes in shared memory -> 32 lanes x 4 columns of tensor memory, repeated for the four lane quarters (kPair: in
 // both CTAs, each from its own shared memory). Whole-warp code, predicated on `issue`; runs in order with the issuing thread's
@@ -797,6 +823,16 @@ __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r
         "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
         "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
         "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+// The same of 16 columns.
+__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      :
+      : "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() {
