@@ -378,14 +378,20 @@ __device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi) {
   return r;
 }
 __device__ __forceinline__ uint32_t e4m3_four(float a, float b, float c, float d) { return e4m3_pair(a, b) | (e4m3_pair(c, d) << 16); }
-// The halves' values of two elements.
-__device__ __forceinline__ uint32_t halves_of_e4m3(uint32_t pair) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(pair)));
-  return r;
+// Four elements as halves, two to a word.
+__device__ __forceinline__ void halves_of_e4m3(uint32_t four, uint32_t& lo, uint32_t& hi) {
+  asm("{\n"
+      ".reg .b16 l, h;\n"
+      "mov.b32 {l, h}, %2;\n"
+      "cvt.rn.f16x2.e4m3x2 %0, l;\n"
+      "cvt.rn.f16x2.e4m3x2 %1, h;\n"
+      "}\n"
+      : "=r"(lo), "=r"(hi)
+      : "r"(four));
 }
 __device__ __forceinline__ uint32_t e4m3_rescaled(uint32_t four, float factor) {
-  const uint32_t lo = halves_of_e4m3(four & 0xffffu), hi = halves_of_e4m3(four >> 16);
+  uint32_t lo, hi;
+  halves_of_e4m3(four, lo, hi);
   const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&lo)), y = __half22float2(*reinterpret_cast<const __half2*>(&hi));
   return e4m3_four(x.x * factor, x.y * factor, y.x * factor, y.y * factor);
 }

@@ -7,19 +7,47 @@ namespace {
 
 using namespace tb200_host;
 
-template <typename T, int kD>
-void launch_tokens(const tb200::KvAttentionArgs& a, int splits, int dev, cudaStream_t stream) {
+// Sequences of up to so many tokens are split over a cluster's CTAs, if that fills no more than the machine; one launch.
+constexpr long long kSharedTokens = 4096;
+
+template <typename Kernel>
+void allow_smem(Kernel kern, std::atomic<bool> (&done)[kMaxDevices], int dev, int bytes) {
+  if (done[dev].load(std::memory_order_relaxed)) return;
+  TB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  done[dev].store(true, std::memory_order_relaxed);
+}
+
+template <typename T, int kD, bool kExact>
+void launch_tokens(tb200::KvTokensArgs& c, DeviceState& st, int dev, cudaStream_t stream) {
   constexpr int kSmem = tb200::kv_token_smem_bytes<kD>();
-  auto kern = tb200::kv_tokens_kernel<T, kD>;
-  static std::atomic<bool> done[kMaxDevices];
-  if (!done[dev].load(std::memory_order_relaxed)) {
-    TB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
-    done[dev].store(true, std::memory_order_relaxed);
+  static std::atomic<bool> done[2][kMaxDevices];
+  const tb200::KvAttentionArgs& a = c.a;
+  const long long heads = static_cast<long long>(a.cache.heads) * a.row_tiles, pairs = heads * a.seqs.count;
+  const int slots = tb200::kKvTokenCtas * st.num_sms;
+  // The tokens that a sequence may have, as far as the host knows.
+  long long most = static_cast<long long>(a.seqs.table_width) << a.cache.page_shift;
+  if (a.window > 0) most = std::min<long long>(most, a.window + 16LL * tb200::kKvTokenTiles);
+  if (pairs * 8 <= slots && most <= kSharedTokens && heads <= 65535) {
+    auto kern = tb200::kv_tokens_kernel<T, kD, kExact, tb200::kShared>;
+    allow_smem(kern, done[0], dev, kSmem);
+    c.splits = 8;
+    while (c.splits > 1 && c.splits * 16 * tb200::kKvTokenWarps >= 2 * most) c.splits /= 2;     // a step for every other warp at least
+    launch(kern, dim3(grid_of(static_cast<long long>(a.seqs.count) * c.splits), static_cast<unsigned>(heads)), tb200::kKvTokenThreads, kSmem,
+           c.splits, kLaunchKvTokens, stream, c);
+    return;
   }
-  const long long heads = static_cast<long long>(a.cache.heads) * a.row_tiles;
-  if (heads > 65535) TB_FAIL(TRACEA_UNSUPPORTED_CONFIG, "%d heads of keys with %d tiles of rows", a.cache.heads, a.row_tiles);
-  const dim3 grid(grid_of(static_cast<long long>(a.seqs.count) * splits), static_cast<unsigned>(heads));
-  launch(kern, grid, tb200::kKvTokenThreads, kSmem, splits, kLaunchKvTokens, stream, a);
+  auto kern = tb200::kv_tokens_kernel<T, kD, kExact, tb200::kFlat>;
+  allow_smem(kern, done[1], dev, kSmem);
+  c.ctas = slots;
+  const size_t rows = 2 * static_cast<size_t>(slots) * tb200::kKvTokenRows;
+  Scratch scratch;
+  scratch.alloc(st, rows * (kD * sizeof(float) + sizeof(float2)) + slots * sizeof(int4), stream);
+  c.sums = static_cast<float*>(scratch.ptr);
+  c.tops = reinterpret_cast<float2*>(c.sums + rows * kD);
+  c.cuts = reinterpret_cast<int4*>(c.tops + rows);
+  launch(kern, static_cast<unsigned>(slots), tb200::kKvTokenThreads, kSmem, 1, kLaunchKvTokens, stream, c);
+  const int join_rows = a.seqs.starts == nullptr ? std::min(a.group, tb200::kKvTokenRows) : tb200::kKvTokenRows;
+  launch(tb200::kv_join_kernel<T, kD>, dim3(static_cast<unsigned>(slots), static_cast<unsigned>(join_rows)), 32 * tb200::kKvJoinWarps, 0, 1, kLaunchKvTokens, stream, c);
 }
 
 template <typename T, int kD>
@@ -102,11 +130,13 @@ void kv_attention_checked(const TraceaTensorView& qv, const TraceaKvCache& cache
       a.fewest = 1;
       a.most = only_few ? 0x7fffffff : kFew;
       a.row_tiles = static_cast<int>(ceil_div(a.seqs.starts == nullptr ? a.group : std::min<long long>(all_rows, kFew), tb200::kKvTokenRows));
-      const long long pairs = static_cast<long long>(a.seqs.count) * a.cache.heads * a.row_tiles;
-      int splits = 1;
-      while (splits < 8 && pairs * splits < st.num_sms) splits *= 2;
-      if (a.cache.D <= 64) launch_tokens<T, 64>(a, splits, dev, stream);
-      else launch_tokens<T, 128>(a, splits, dev, stream);
+      tb200::KvTokensArgs c;
+      memset(&c, 0, sizeof(c));
+      c.a = a;
+      if (a.cache.D == 64) launch_tokens<T, 64, true>(c, st, dev, stream);
+      else if (a.cache.D < 64) launch_tokens<T, 64, false>(c, st, dev, stream);
+      else if (a.cache.D == 128) launch_tokens<T, 128, true>(c, st, dev, stream);
+      else launch_tokens<T, 128, false>(c, st, dev, stream);
     }
   });
 }

@@ -44,6 +44,29 @@ __device__ __forceinline__ void mma_16x8x16(float (&c)[4], const uint32_t (&a)[4
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// By what sums with the maximum m and the denominator l are taken in where the maximum of all is `top`: 0 for a part that has seen
+// nothing, but for one that has seen nothing but NaN.
+__device__ __forceinline__ float part_factor(float m, float l, float top) {
+  return m == -INFINITY ? (l != l ? 1.0f : 0.0f) : exp2_ftz(m - top);
+}
+__device__ __forceinline__ void add_scaled(float4& sum, const float4& v, float f) {
+  sum.x += f * v.x;
+  sum.y += f * v.y;
+  sum.z += f * v.z;
+  sum.w += f * v.w;
+}
+// Four columns times `inv`; `vec` of them can be written at a time.
+template <typename T>
+__device__ __forceinline__ void store_4(T* p, const float4& v, float inv, int vec) {
+  if (vec >= 4) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T, false>(v.x * inv, v.y * inv), pack2<T, false>(v.z * inv, v.w * inv));
+  } else {
+    p[0] = static_cast<T>(v.x * inv);
+    p[1] = static_cast<T>(v.y * inv);
+    p[2] = static_cast<T>(v.z * inv);
+    p[3] = static_cast<T>(v.w * inv);
+  }
+}
 // The power of two that brings a row whose largest absolute value is `peak` into [1, 2); 1 for a row of zeros or one that is not finite.
 // `back` is its inverse. (Both within the normal range: peak 2^-127 and smaller, or 2^127 and larger, are not brought all the way.)
 __device__ __forceinline__ float row_scale(float peak, float& back) {

@@ -327,10 +327,13 @@ __global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid
         const int row = kRowsOfLoad * i + my_row;
         const uint32_t line = dst + my_block * kBlock + row * 128;
         const uint4 x = raw[i];
-        st_shared_v4(line + ((my_unit ^ (row & 7)) * 16),
-                     make_uint4(halves_of_e4m3(x.x & 0xffffu), halves_of_e4m3(x.x >> 16), halves_of_e4m3(x.y & 0xffffu), halves_of_e4m3(x.y >> 16)));
-        st_shared_v4(line + (((my_unit + 1) ^ (row & 7)) * 16),
-                     make_uint4(halves_of_e4m3(x.z & 0xffffu), halves_of_e4m3(x.z >> 16), halves_of_e4m3(x.w & 0xffffu), halves_of_e4m3(x.w >> 16)));
+        uint4 first, second;
+        halves_of_e4m3(x.x, first.x, first.y);
+        halves_of_e4m3(x.y, first.z, first.w);
+        halves_of_e4m3(x.z, second.x, second.y);
+        halves_of_e4m3(x.w, second.z, second.w);
+        st_shared_v4(line + ((my_unit ^ (row & 7)) * 16), first);
+        st_shared_v4(line + (((my_unit + 1) ^ (row & 7)) * 16), second);
       }
     };
     ids = load_ids(0);
