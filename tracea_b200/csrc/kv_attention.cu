@@ -17,18 +17,18 @@ void allow_smem(Kernel kern, std::atomic<bool> (&done)[kMaxDevices], int dev, in
   done[dev].store(true, std::memory_order_relaxed);
 }
 
-template <typename T, int kD, bool kExact>
+template <typename T, int kRows, int kD, bool kExact>
 void launch_tokens(tb200::KvTokensArgs& c, DeviceState& st, int dev, cudaStream_t stream) {
-  constexpr int kSmem = tb200::kv_token_smem_bytes<kD>();
+  constexpr int kSmem = tb200::kv_token_smem_bytes(kRows, kD);
   static std::atomic<bool> done[2][kMaxDevices];
   const tb200::KvAttentionArgs& a = c.a;
   const long long heads = static_cast<long long>(a.cache.heads) * a.row_tiles, pairs = heads * a.seqs.count;
-  const int slots = tb200::kKvTokenCtas * st.num_sms;
+  const int slots = tb200::kv_token_ctas(kRows) * st.num_sms;
   // The tokens that a sequence may have, as far as the host knows.
   long long most = static_cast<long long>(a.seqs.table_width) << a.cache.page_shift;
   if (a.window > 0) most = std::min<long long>(most, a.window + 16LL * tb200::kKvTokenTiles);
   if (pairs * 8 <= slots && most <= kSharedTokens && heads <= 65535) {
-    auto kern = tb200::kv_tokens_kernel<T, kD, kExact, tb200::kShared>;
+    auto kern = tb200::kv_tokens_kernel<T, kRows, kD, kExact, tb200::kShared>;
     allow_smem(kern, done[0], dev, kSmem);
     c.splits = 8;
     while (c.splits > 1 && c.splits * 16 * tb200::kKvTokenWarps >= 2 * most) c.splits /= 2;     // a step for every other warp at least
@@ -36,17 +36,17 @@ void launch_tokens(tb200::KvTokensArgs& c, DeviceState& st, int dev, cudaStream_
            c.splits, kLaunchKvTokens, stream, c);
     return;
   }
-  auto kern = tb200::kv_tokens_kernel<T, kD, kExact, tb200::kFlat>;
+  auto kern = tb200::kv_tokens_kernel<T, kRows, kD, kExact, tb200::kFlat>;
   allow_smem(kern, done[1], dev, kSmem);
   c.ctas = slots;
-  const size_t rows = 2 * static_cast<size_t>(slots) * tb200::kKvTokenRows;
+  const size_t rows = 2 * static_cast<size_t>(slots) * kRows;
   Scratch scratch;
   scratch.alloc(st, rows * (kD * sizeof(float) + sizeof(float2)) + slots * sizeof(int4), stream);
   c.sums = static_cast<float*>(scratch.ptr);
   c.tops = reinterpret_cast<float2*>(c.sums + rows * kD);
   c.cuts = reinterpret_cast<int4*>(c.tops + rows);
   launch(kern, static_cast<unsigned>(slots), tb200::kKvTokenThreads, kSmem, 1, kLaunchKvTokens, stream, c);
-  const int join_rows = a.seqs.starts == nullptr ? std::min(a.group, tb200::kKvTokenRows) : tb200::kKvTokenRows;
+  const int join_rows = a.seqs.starts == nullptr ? std::min(a.group, kRows) : kRows;
   launch(tb200::kv_join_kernel<T, kD>, dim3(static_cast<unsigned>(slots), static_cast<unsigned>(join_rows)), 32 * tb200::kKvJoinWarps, 0, 1, kLaunchKvTokens, stream, c);
 }
 
@@ -129,14 +129,21 @@ void kv_attention_checked(const TraceaTensorView& qv, const TraceaKvCache& cache
     if (!only_many) {
       a.fewest = 1;
       a.most = only_few ? 0x7fffffff : kFew;
-      a.row_tiles = static_cast<int>(ceil_div(a.seqs.starts == nullptr ? a.group : std::min<long long>(all_rows, kFew), tb200::kKvTokenRows));
+      const long long most_rows = a.seqs.starts == nullptr ? a.group : std::min<long long>(all_rows, kFew);
+      a.tile_rows = most_rows <= 8 ? 8 : tb200::kKvTokenRows;
+      a.row_tiles = static_cast<int>(ceil_div(most_rows, a.tile_rows));
       tb200::KvTokensArgs c;
       memset(&c, 0, sizeof(c));
       c.a = a;
-      if (a.cache.D == 64) launch_tokens<T, 64, true>(c, st, dev, stream);
-      else if (a.cache.D < 64) launch_tokens<T, 64, false>(c, st, dev, stream);
-      else if (a.cache.D == 128) launch_tokens<T, 128, true>(c, st, dev, stream);
-      else launch_tokens<T, 128, false>(c, st, dev, stream);
+      auto go = [&](auto rows) {
+        constexpr int kRows = decltype(rows)::value;
+        if (a.cache.D == 64) launch_tokens<T, kRows, 64, true>(c, st, dev, stream);
+        else if (a.cache.D < 64) launch_tokens<T, kRows, 64, false>(c, st, dev, stream);
+        else if (a.cache.D == 128) launch_tokens<T, kRows, 128, true>(c, st, dev, stream);
+        else launch_tokens<T, kRows, 128, false>(c, st, dev, stream);
+      };
+      if (a.tile_rows == 8) go(std::integral_constant<int, 8>{});
+      else go(std::integral_constant<int, tb200::kKvTokenRows>{});
     }
   });
 }

@@ -22,7 +22,7 @@ struct KvAttentionArgs {
   int group;                     // heads of q to a head of keys
   int causal, window;
   int fewest, most;              // sequences with fewer or more rows (times group) are another kernel's
-  int row_tiles;
+  int tile_rows, row_tiles;      // few rows: of a tile, and tiles of a sequence at most
   float scale_log2;              // |scale| * log2(e)
   float sign;                    // of the scale
   uint32_t* status;
@@ -37,6 +37,12 @@ __device__ __forceinline__ float exp2_ftz(float x) {
 __device__ __forceinline__ uint32_t pack_halves(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// An 8 x 8 matrix of halves, row lane / 4 and columns 2 (lane % 4) and the next in each lane, transposed.
+__device__ __forceinline__ uint32_t transposed_8x8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
 __device__ __forceinline__ void mma_16x8x16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {

@@ -2,11 +2,12 @@
 //
 //   out = softmax(scale q K^T) V,   K = 2^ek k^, V = 2^ev v^ with a power of two per page and head, k^ and v^ in e4m3
 //
-// Bound by reading the cache once. The heads of q that share a head of keys (times the tokens of the sequence) are the 16 rows of the
-// matrix instructions, so the cache is read once for all of them; elements of e4m3 are halves exactly, and so are those of q, times a
+// Bound by reading the cache once. The heads of q that share a head of keys (times the tokens of the sequence) are columns of the
+// matrix instructions, 8 or 16 of them, and the cache's tokens (for the scores) and columns (for the results) their rows, so that few
+// heads take few instructions and the cache is read once for all of them; elements of e4m3 are halves exactly, and so are those of q, times a
 // power of two per row, to 11 bits of the row's largest. A warp takes 16 tokens at a time and keeps its own copies under way, 512
 // consecutive bytes each: copies by the lanes of what each multiplies, 64 bytes of eight rows, stop at 4.9 TB/s where these reach 6.7. In
-// shared memory the 16-byte columns of a row are exchanged so that no two lanes meet on a bank (see below). Three CTAs of four warps share an SM, so that one's first loads, each of which waits for the one in front of it -- the
+// shared memory the 16-byte columns of a row are exchanged so that no two lanes meet on a bank (see below). Several CTAs of four warps share an SM, so that one's first loads, each of which waits for the one in front of it -- the
 // lengths, the places of the pages, the pages -- and its sums' meeting lie beside the others' work.
 //
 // The work is split along the cache in one of two ways:
@@ -21,29 +22,28 @@ namespace tb200 {
 
 constexpr int kKvTokenWarps = 4;
 constexpr int kKvTokenThreads = 32 * kKvTokenWarps;
-constexpr int kKvTokenCtas = 3;                // of an SM
-constexpr int kKvTokenStages = 4;              // steps of 16 tokens that a warp has under way
-constexpr int kKvTokenRows = 16;
+constexpr int kKvTokenRows = 16;               // of a tile, or 8
 constexpr int kKvTokenTiles = 4;               // sequences of up to 64 rows a head of keys come here
 constexpr int kKvMetaPages = 256;              // pages whose places and scales are in shared memory at a time
 constexpr int kKvFlatSteps = 8;                // a CTA's piece of the line is no shorter than two steps a warp
-constexpr int kKvFlatCost = 12;                // steps that take as long as a piece's beginning and end; less where pieces are short
+constexpr int kKvFlatCost = 12;                // steps that take as long as a piece's beginning and end
 
 struct KvTokensArgs {
   KvAttentionArgs a;
   int splits;                    // kShared: CTAs of a cluster
   int ctas;                      // kFlat
-  float* sums;                   // kFlat: two slots a CTA of [16][kD] unscaled results,
-  float2* tops;                  // and [16] of {maximum, denominator};
+  float* sums;                   // kFlat: two slots a CTA of [kRows][kD] unscaled results,
+  float2* tops;                  // and [kRows] of {maximum, denominator};
   int4* cuts;                    // of each CTA, the pair that begins in it and ends in another: {sequence or -1, pair, slot, last CTA}
 };
 
-// kD: D rounded up to 64 or 128; columns past D are zeros that nothing is read for.
-template <int kD>
-__host__ __device__ constexpr int kv_token_step_bytes() { return 16 * kD * 2; }
-template <int kD>
-__host__ __device__ constexpr int kv_token_smem_bytes() {
-  return kKvTokenWarps * kKvTokenStages * kv_token_step_bytes<kD>() + kKvMetaPages * 8;
+// kRows: rows of a tile, 8 or 16. kD: D rounded up to 64 or 128; columns past D are zeros that nothing is read for.
+// CTAs of an SM, and steps of 16 tokens that a warp has under way, one of them in work.
+__host__ __device__ constexpr int kv_token_ctas(int rows) { return rows == 8 ? 4 : 3; }
+__host__ __device__ constexpr int kv_token_stages(int rows) { return rows == 8 ? 3 : 4; }
+__host__ __device__ constexpr int kv_token_step_bytes(int d) { return 16 * d * 2; }
+__host__ __device__ constexpr int kv_token_smem_bytes(int rows, int d) {
+  return kKvTokenWarps * kv_token_stages(rows) * kv_token_step_bytes(d) + kKvMetaPages * 8;
 }
 
 // What a sequence's rows see of it, in steps of 16 tokens; at least one step, so that rows that see nothing are written too.
@@ -68,7 +68,7 @@ __device__ __forceinline__ TokenSpan token_span(const KvAttentionArgs& a, int se
   s.see_hi = min(s.length, a.seqs.table_width << a.cache.page_shift);
   s.step_lo = s.see_lo >> 4;
   s.steps = max(1, ((s.see_hi + 15) >> 4) - s.step_lo);
-  s.tiles = (s.rows + kKvTokenRows - 1) / kKvTokenRows;
+  s.tiles = (s.rows + a.tile_rows - 1) / a.tile_rows;
   return s;
 }
 // kFlat's line: the sequences' steps, for each in turn those of every head and tile (a pair), each pair with `cost` places in front for
@@ -119,25 +119,27 @@ __device__ __forceinline__ int token_sequence(const KvAttentionArgs& a, long lon
 enum { kShared = 0, kFlat = 1 };
 
 // kExact: D == kD.
-template <typename T, int kD, bool kExact, int kSplit>
-__global__ void __launch_bounds__(kKvTokenThreads, kKvTokenCtas) kv_tokens_kernel(const __grid_constant__ KvTokensArgs call) {
+template <typename T, int kRows, int kD, bool kExact, int kSplit>
+__global__ void __launch_bounds__(kKvTokenThreads, kv_token_ctas(kRows)) kv_tokens_kernel(const __grid_constant__ KvTokensArgs call) {
   using namespace ptx;
   constexpr int kSegments = kD / 64;             // of 64 columns: 16 a lane of a quad
   constexpr int kValueBytes = kD / 8;            // of a token that a lane takes
-  constexpr int kTilesV = kD / 8;                // 8-column tiles of the result
-  constexpr int kStep = kv_token_step_bytes<kD>();
+  constexpr int kTilesV = kD / 16;               // 16-column tiles of the result
+  constexpr int kN = kRows / 8;                  // 8-row tiles of q
+  constexpr int kStages = kv_token_stages(kRows);
+  constexpr int kStep = kv_token_step_bytes(kD);
   const KvAttentionArgs& args = call.a;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float row_factor[kKvTokenWarps][kKvTokenRows], row_m[kKvTokenWarps][kKvTokenRows], row_l[kKvTokenWarps][kKvTokenRows];
-  __shared__ float cta_m[kKvTokenRows], cta_l[kKvTokenRows];
-  int* const meta_page = reinterpret_cast<int*>(smem + kKvTokenWarps * kKvTokenStages * kStep);
+  __shared__ float row_factor[kKvTokenWarps][kRows], row_m[kKvTokenWarps][kRows], row_l[kKvTokenWarps][kRows];
+  __shared__ float cta_m[kRows], cta_l[kRows];
+  int* const meta_page = reinterpret_cast<int*>(smem + kKvTokenWarps * kStages * kStep);
   uint32_t* const meta_scale = reinterpret_cast<uint32_t*>(meta_page + kKvMetaPages);
   griddep_launch_dependents();
   griddep_wait();
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int D = kExact ? kD : args.cache.D, shift = args.cache.page_shift, page_steps = shift - 4;     // log2 of a page's steps
-  const uint32_t ring = smem_u32(smem) + warp * (kKvTokenStages * kStep);
+  const uint32_t ring = smem_u32(smem) + warp * (kStages * kStep);
   const long long page_bytes = (static_cast<long long>(args.cache.heads) << shift) * D;
   const uint32_t splits = kSplit == kShared ? cluster_ctas() : 1u, rank = kSplit == kShared ? cluster_ctarank() : 0u;
 
@@ -158,13 +160,13 @@ __global__ void __launch_bounds__(kKvTokenThreads, kKvTokenCtas) kv_tokens_kerne
 
   long long from = 0, to = 1, before = 0;        // kFlat: this CTA's piece of the line, and where its sequence begins
   long long piece0 = 0, quota = 1;
-  int seq = static_cast<int>(blockIdx.x / splits), cost = 0;
+  int seq = static_cast<int>(blockIdx.x / splits);
+  constexpr int cost = kKvFlatCost;
   bool used = false;                             // shared memory is, by a pair in front
   if constexpr (kSplit == kFlat) {
     long long steps, pairs;
     token_totals(args, steps, pairs);
-    cost = static_cast<int>(min(static_cast<long long>(kKvFlatCost), steps / (4 * call.ctas)));
-    quota = max((steps + pairs * cost + call.ctas - 1) / call.ctas, static_cast<long long>(kKvFlatSteps));
+    quota = max((steps + pairs * cost + call.ctas - 1) / call.ctas, static_cast<long long>(cost + kKvFlatSteps));
     piece0 = from = quota * blockIdx.x;
     to = min(steps + pairs * cost, from + quota);
     if (threadIdx.x == 0) call.cuts[blockIdx.x] = make_int4(-1, 0, 0, 0);
@@ -204,7 +206,7 @@ __global__ void __launch_bounds__(kKvTokenThreads, kKvTokenCtas) kv_tokens_kerne
       my_hi = static_cast<int>(static_cast<long long>(span.steps) * (rank + 1) / splits);
     }
     const bool whole = my_lo == 0 && my_hi == span.steps;
-    const int first_row = tile * kKvTokenRows, rows = min(kKvTokenRows, span.rows - first_row);
+    const int first_row = tile * kRows, rows = min(kRows, span.rows - first_row);
     const int begin = span.length - span.rows / args.group;        // position of the sequence's first row
     const int pos_lo = begin + first_row / args.group, pos_hi = begin + (first_row + rows - 1) / args.group;
     const int see_lo = span.see_lo, see_hi = span.see_hi;
@@ -212,15 +214,20 @@ __global__ void __launch_bounds__(kKvTokenThreads, kKvTokenCtas) kv_tokens_kerne
     const uint8_t* const k_head = args.cache.k + (static_cast<long long>(head) << shift) * D;
     const uint8_t* const v_head = args.cache.v + (static_cast<long long>(head) << shift) * D;
 
-    float factor[2];
-    int pos[2];
-    uint32_t qa[kSegments][4][4];
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-    float o[kTilesV][4];
+    // Of each 8 rows of q this lane has row g as an operand, and rows 2t and 2t + 1 of scores, weights and results.
+    float factor[kN][2];
+    int pos[kN][2];
+    uint32_t qb[kN][kSegments][4][2];
+    float m[kN][2], l[kN][2], o[kN][kTilesV][4];
 #pragma unroll
-    for (int j = 0; j < kTilesV; ++j)
+    for (int n = 0; n < kN; ++n) {
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[j][i] = 0.0f;
+      for (int j = 0; j < kTilesV; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[n][j][i] = 0.0f;
+    }
 
     for (int part = lo; part < hi;) {
       // the places of this part's pages, then, while the first copies are under way, their scales
@@ -229,7 +236,7 @@ __global__ void __launch_bounds__(kKvTokenThreads, kKvTokenCtas) kv_tokens_kerne
       const int pages = ((part_end - 1) >> page_steps) - page0 + 1;
       if (part != lo || used) __syncthreads();
       if (!kExact && part == lo) {               // the columns past D, which no copy writes
-        for (int i = threadIdx.x; i < kKvTokenWarps * kKvTokenStages * kStep / 16; i += kKvTokenThreads)
+        for (int i = threadIdx.x; i < kKvTokenWarps * kStages * kStep / 16; i += kKvTokenThreads)
           st_shared_v4(smem_u32(smem) + 16 * i, make_uint4(0u, 0u, 0u, 0u));
       }
       for (int i = threadIdx.x; i < pages; i += kKvTokenThreads) {
@@ -266,7 +273,7 @@ __global__ void __launch_bounds__(kKvTokenThreads, kKvTokenCtas) kv_tokens_kerne
       };
       const int first = part + warp;
 #pragma unroll
-      for (int s = 0; s < kKvTokenStages - 1; ++s) {
+      for (int s = 0; s < kStages - 1; ++s) {
         if (first + s * kKvTokenWarps < part_end) fetch(first + s * kKvTokenWarps, s);
         cp_async_commit();
       }
@@ -276,12 +283,11 @@ __global__ void __launch_bounds__(kKvTokenThreads, kKvTokenCtas) kv_tokens_kerne
         meta_scale[i] = id >= 0 ? args.cache.k_scales[block] | (static_cast<uint32_t>(args.cache.v_scales[block]) << 8) : 0x7f7fu;
       }
       if (part == lo) {
-        // rows of q as the first operand: rows g and g + 8, the columns that the second operand's lane has (see below)
+        // q as the second operand, the columns that the first operand's lane has (see below)
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int r = g + 8 * half, all = first_row + r;
-          const bool live = r < rows;
-          pos[half] = begin + all / args.group;
+        for (int n = 0; n < kN; ++n) {
+          const int all = first_row + 8 * n + g;
+          const bool live = 8 * n + g < rows;
           const T* p = static_cast<const T*>(args.q) + (span.row0 + (live ? all / args.group : 0)) * args.q_token +
                        (head * args.group + (live ? all % args.group : 0)) * args.q_head;
           float v[kSegments][16];
@@ -307,13 +313,18 @@ __global__ void __launch_bounds__(kKvTokenThreads, kKvTokenCtas) kv_tokens_kerne
           peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
           float back;
           const float up = args.sign * row_scale(peak, back);
-          factor[half] = back * args.scale_log2;
+          back *= args.scale_log2;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            factor[n][j] = __shfl_sync(0xffffffffu, back, 4 * (2 * t + j));
+            pos[n][j] = begin + (first_row + 8 * n + 2 * t + j) / args.group;
+          }
 #pragma unroll
           for (int i = 0; i < kSegments; ++i)
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
-              qa[i][s][half] = pack_halves(v[i][4 * s] * up, v[i][4 * s + 1] * up);
-              qa[i][s][half + 2] = pack_halves(v[i][4 * s + 2] * up, v[i][4 * s + 3] * up);
+              qb[n][i][s][0] = pack_halves(v[i][4 * s] * up, v[i][4 * s + 1] * up);
+              qb[n][i][s][1] = pack_halves(v[i][4 * s + 2] * up, v[i][4 * s + 3] * up);
             }
         }
       }
@@ -323,140 +334,142 @@ __global__ void __launch_bounds__(kKvTokenThreads, kKvTokenCtas) kv_tokens_kerne
       for (int step = first; step < part_end; step += kKvTokenWarps) {
         {
           __syncwarp();                          // every lane has read what is overwritten
-          const int ahead = step + (kKvTokenStages - 1) * kKvTokenWarps;
-          if (ahead < part_end) fetch(ahead, (stage + kKvTokenStages - 1) % kKvTokenStages);
+          const int ahead = step + (kStages - 1) * kKvTokenWarps;
+          if (ahead < part_end) fetch(ahead, (stage + kStages - 1) % kStages);
           cp_async_commit();
         }
-        cp_async_wait<kKvTokenStages - 1>();
+        cp_async_wait<kStages - 1>();
         __syncwarp();                            // every lane's copies are there
         const int at_page = (step >> page_steps) - page0;
         const uint32_t scales = meta_scale[at_page];
         const float k_scale = power_of_two(static_cast<int>(scales & 0xffu) - 127), ev = static_cast<float>(static_cast<int>(scales >> 8) - 127);
-        const uint32_t src = ring + stage * kStep;
+        const uint8_t* const src = smem + warp * (kStages * kStep) + stage * kStep;
         // scores: the order of the columns in the sums is free, so long as both operands have the same. A lane's 16 bytes of a
-        // segment are four instructions' worth.
-        float s[2][4];
+        // segment, of rows g and g + 8, are four instructions' worth.
+        float s[kN][4];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int n = 0; n < kN; ++n)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) s[i][j] = 0.0f;
+          for (int j = 0; j < 4; ++j) s[n][j] = 0.0f;
 #pragma unroll
-          for (int seg = 0; seg < kSegments; ++seg) {
-            const uint4 w = ld_shared_v4(src + i * 8 * kD + (k_at ^ (64 * seg)));
-            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+        for (int seg = 0; seg < kSegments; ++seg) {
+          const uint4 x = *reinterpret_cast<const uint4*>(src + (k_at ^ (64 * seg))), y = *reinterpret_cast<const uint4*>(src + 8 * kD + (k_at ^ (64 * seg)));
+          const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              uint32_t b0, b1;
-              halves_of_e4m3(words[j], b0, b1);
-              mma_16x8x16(s[i], qa[seg][j], b0, b1);
-            }
+          for (int j = 0; j < 4; ++j) {
+            uint32_t a[4];
+            halves_of_e4m3(xs[j], a[0], a[2]);
+            halves_of_e4m3(ys[j], a[1], a[3]);
+#pragma unroll
+            for (int n = 0; n < kN; ++n) mma_16x8x16(s[n], a, qb[n][seg][j][0], qb[n][seg][j][1]);
           }
         }
-        // s[i][2 half + j]: row g + 8 half, token 8i + 2t + j of the step
+        // s[n][2 half + j]: token g + 8 half of the step, row 8n + 2t + j
         const int at = step << 4;
-        float peak[2] = {-INFINITY, -INFINITY};
-        const float c[2] = {factor[0] * k_scale, factor[1] * k_scale};
         const bool page_there = meta_page[at_page] >= 0;
         if (!page_there || at + 16 > see_hi || (args.causal && at + 15 > pos_lo) || (args.window > 0 && at <= pos_hi - args.window)) {
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
+          for (int n = 0; n < kN; ++n)
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
-#pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                const int token = at + 8 * i + 2 * t + j;
-                const bool seen = page_there && token < see_hi && (!args.causal || token <= pos[half]) &&
-                                  (args.window == 0 || token > pos[half] - args.window);
-                s[i][2 * half + j] = seen ? s[i][2 * half + j] * c[half] + ev : -INFINITY;
-              }
+            for (int i = 0; i < 4; ++i) {
+              const int token = at + g + 8 * (i >> 1), p = pos[n][i & 1];
+              const bool seen = page_there && token < see_hi && (!args.causal || token <= p) && (args.window == 0 || token > p - args.window);
+              s[n][i] = seen ? s[n][i] * (factor[n][i & 1] * k_scale) + ev : -INFINITY;
+            }
         } else {
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
+          for (int n = 0; n < kN; ++n)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[i][j] = s[i][j] * c[j >> 1] + ev;
+            for (int i = 0; i < 4; ++i) s[n][i] = s[n][i] * (factor[n][i & 1] * k_scale) + ev;
         }
+        bool grown = false;
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
-          peak[half] = fmaxf(fmaxf(s[0][2 * half], s[0][2 * half + 1]), fmaxf(s[1][2 * half], s[1][2 * half + 1]));
-        if (__any_sync(0xffffffffu, peak[0] > m[0] + kSlack || peak[1] > m[1] + kSlack)) {
+        for (int n = 0; n < kN; ++n)
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            float p = fmaxf(peak[half], m[half]);
-            p = fmaxf(p, __shfl_xor_sync(0xffffffffu, p, 1));
-            p = fmaxf(p, __shfl_xor_sync(0xffffffffu, p, 2));
-            const float shrink = p == m[half] ? 1.0f : exp2_ftz(m[half] - p);
-            m[half] = p;
-            l[half] *= shrink;
+          for (int j = 0; j < 2; ++j) grown = grown || fmaxf(s[n][j], s[n][2 + j]) > m[n][j] + kSlack;
+        if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
-            for (int j = 0; j < kTilesV; ++j) {
-              o[j][2 * half] *= shrink;
-              o[j][2 * half + 1] *= shrink;
+          for (int n = 0; n < kN; ++n)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float p = fmaxf(fmaxf(s[n][j], s[n][2 + j]), m[n][j]);
+#pragma unroll
+              for (int x = 4; x < 32; x <<= 1) p = fmaxf(p, __shfl_xor_sync(0xffffffffu, p, x));
+              const float shrink = p == m[n][j] ? 1.0f : exp2_ftz(m[n][j] - p);
+              m[n][j] = p;
+              l[n][j] *= shrink;
+#pragma unroll
+              for (int v = 0; v < kTilesV; ++v) {
+                o[n][v][j] *= shrink;
+                o[n][v][2 + j] *= shrink;
+              }
             }
-          }
         }
-        const float base[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};   // a row that has seen nothing
-        float sum[2] = {0.0f, 0.0f};
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            s[i][j] = exp2_ftz(s[i][j] - base[j >> 1]);
-            sum[j >> 1] += s[i][j];
-          }
         const float unscale = power_of_two(127 - static_cast<int>(scales >> 8));
-        l[0] += sum[0] * unscale;
-        l[1] += sum[1] * unscale;
-        const uint32_t pa[4] = {pack_halves(s[0][0], s[0][1]), pack_halves(s[0][2], s[0][3]), pack_halves(s[1][0], s[1][1]),
-                                pack_halves(s[1][2], s[1][3])};
-        // values: two tokens' elements of a column make a word of the second operand
+        uint32_t pb[kN][2];
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float base = m[n][j] == -INFINITY ? 0.0f : m[n][j];      // a row that has seen nothing
+            s[n][j] = exp2_ftz(s[n][j] - base);
+            s[n][2 + j] = exp2_ftz(s[n][2 + j] - base);
+            l[n][j] += (s[n][j] + s[n][2 + j]) * unscale;
+          }
+          // from two rows of a token to two tokens of a row
+          pb[n][0] = transposed_8x8(pack_halves(s[n][0], s[n][1]));
+          pb[n][1] = transposed_8x8(pack_halves(s[n][2], s[n][3]));
+        }
+        // values: two tokens' elements of a column make a word of the first operand
         uint32_t w[4][kValueBytes / 4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           if constexpr (kValueBytes == 16) {
-            const uint4 x = ld_shared_v4(src + (i >> 1) * 1024 + (i & 1) * 128 + (v_at ^ (64 * (i & 1))));
+            const uint4 x = *reinterpret_cast<const uint4*>(src + (i >> 1) * 1024 + (i & 1) * 128 + (v_at ^ (64 * (i & 1))));
             w[i][0] = x.x;
             w[i][1] = x.y;
             w[i][2] = x.z;
             w[i][3] = x.w;
           } else {
-            const uint2 x = ld_shared_v2(src + (i >> 1) * 512 + (v_at ^ (64 * (i & 1))));
+            const uint2 x = *reinterpret_cast<const uint2*>(src + (i >> 1) * 512 + (v_at ^ (64 * (i & 1))));
             w[i][0] = x.x;
             w[i][1] = x.y;
           }
         }
 #pragma unroll
-        for (int q = 0; q < kValueBytes / 4; ++q) {
-          uint32_t b0, b1, c0, c1;
-          halves_of_e4m3(__byte_perm(w[0][q], w[1][q], 0x5140), b0, b1);
-          halves_of_e4m3(__byte_perm(w[2][q], w[3][q], 0x5140), c0, c1);
-          mma_16x8x16(o[4 * q], pa, b0, c0);
-          mma_16x8x16(o[4 * q + 1], pa, b1, c1);
-          halves_of_e4m3(__byte_perm(w[0][q], w[1][q], 0x7362), b0, b1);
-          halves_of_e4m3(__byte_perm(w[2][q], w[3][q], 0x7362), c0, c1);
-          mma_16x8x16(o[4 * q + 2], pa, b0, c0);
-          mma_16x8x16(o[4 * q + 3], pa, b1, c1);
-        }
-        stage = (stage + 1) % kKvTokenStages;
+        for (int q = 0; q < kValueBytes / 4; ++q)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {          // columns 4q + 2h and the next of the lane's
+            const uint32_t mix = h == 0 ? 0x5140 : 0x7362;
+            uint32_t a[4];
+            halves_of_e4m3(__byte_perm(w[0][q], w[1][q], mix), a[0], a[1]);
+            halves_of_e4m3(__byte_perm(w[2][q], w[3][q], mix), a[2], a[3]);
+#pragma unroll
+            for (int n = 0; n < kN; ++n) mma_16x8x16(o[n][2 * q + h], a, pb[n][0], pb[n][1]);
+          }
+        stage = (stage + 1) % kStages;
       }
       cp_async_wait_all();
       part = part_end;
     }
 
-    // The sums of the warps, always in the same order. o[j][2 half + i]: row g + 8 half, column kValueBytes (2t + i) + j.
+    // The sums of the warps, always in the same order. o[n][v][2i + j]: row 8n + 2t + j, column kValueBytes g + 2v + i.
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
-      l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
-      if (t == 0) {
-        row_m[warp][g + 8 * half] = m[half];
-        row_l[warp][g + 8 * half] = l[half];
+    for (int n = 0; n < kN; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], x);
+        if (g == 0) {
+          row_m[warp][8 * n + 2 * t + j] = m[n][j];
+          row_l[warp][8 * n + 2 * t + j] = l[n][j];
+        }
       }
-    }
     __syncthreads();
     constexpr int kRowFloats = kD + 4;                      // of a row of partial sums: keeps 8 rows off each other's banks
     float* const part = reinterpret_cast<float*>(smem);
-    static_assert(kKvTokenWarps * kKvTokenRows * kRowFloats * 4 <= kv_token_smem_bytes<kD>(), "the partial sums lie over the ring");
-    if (threadIdx.x < kKvTokenRows) {
+    static_assert(kKvTokenWarps * kRows * kRowFloats * 4 <= kv_token_smem_bytes(kRows, kD), "the partial sums lie over the ring");
+    if (threadIdx.x < kRows) {
       float top = -INFINITY, total = 0.0f;
 #pragma unroll
       for (int w = 0; w < kKvTokenWarps; ++w) top = fmaxf(top, row_m[w][threadIdx.x]);
@@ -470,15 +483,18 @@ __global__ void __launch_bounds__(kKvTokenThreads, kKvTokenCtas) kv_tokens_kerne
       cta_l[threadIdx.x] = total;
     }
 #pragma unroll
-    for (int j = 0; j < kTilesV; ++j)
+    for (int n = 0; n < kN; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        part[(warp * kKvTokenRows + g + 8 * (i >> 1)) * kRowFloats + kValueBytes * (2 * t + (i & 1)) + j] = o[j][i];
+      for (int v = 0; v < kTilesV; ++v)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          *reinterpret_cast<float2*>(part + (warp * kRows + 8 * n + 2 * t + j) * kRowFloats + kValueBytes * g + 2 * v) =
+              make_float2(o[n][v][j], o[n][v][2 + j]);
     __syncthreads();
     auto sum_of_warps = [&](int r, int d) {
       float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-      for (int w = 0; w < kKvTokenWarps; ++w) add_scaled(sum, *reinterpret_cast<const float4*>(part + (w * kKvTokenRows + r) * kRowFloats + d), row_factor[w][r]);
+      for (int w = 0; w < kKvTokenWarps; ++w) add_scaled(sum, *reinterpret_cast<const float4*>(part + (w * kRows + r) * kRowFloats + d), row_factor[w][r]);
       return sum;
     };
     auto write = [&](int r, int d, const float4& sum, float total) {
@@ -495,10 +511,10 @@ __global__ void __launch_bounds__(kKvTokenThreads, kKvTokenCtas) kv_tokens_kerne
         if (d >= D) continue;
         const float4 sum = sum_of_warps(r, d);
         if (whole) write(r, d, sum, cta_l[r]);
-        else *reinterpret_cast<float4*>(call.sums + (static_cast<long long>(slot) * kKvTokenRows + r) * kD + d) = sum;
+        else *reinterpret_cast<float4*>(call.sums + (static_cast<long long>(slot) * kRows + r) * kD + d) = sum;
       }
       if (!whole && static_cast<int>(threadIdx.x) < rows)
-        call.tops[static_cast<long long>(slot) * kKvTokenRows + threadIdx.x] = make_float2(cta_m[threadIdx.x], cta_l[threadIdx.x]);
+        call.tops[static_cast<long long>(slot) * kRows + threadIdx.x] = make_float2(cta_m[threadIdx.x], cta_l[threadIdx.x]);
     } else {
       for (int i = threadIdx.x; i < items; i += kKvTokenThreads) {
         const int r = i / (kD / 4), d = 4 * (i % (kD / 4));
@@ -546,9 +562,9 @@ __global__ void __launch_bounds__(32 * kKvJoinWarps) kv_join_kernel(const __grid
   const int4 cut = call.cuts[c0];                           // {sequence, pair, slot, last CTA}
   if (cut.x < 0) return;
   const TokenSpan span = token_span(args, cut.x);
-  const int head = cut.y / span.tiles, all = cut.y % span.tiles * kKvTokenRows + row;
+  const int head = cut.y / span.tiles, all = cut.y % span.tiles * args.tile_rows + row;
   if (all >= span.rows) return;
-  auto slot = [&](int c) { return (2 * static_cast<long long>(c) + (c == c0 ? cut.z : 0)) * kKvTokenRows + row; };
+  auto slot = [&](int c) { return (2 * static_cast<long long>(c) + (c == c0 ? cut.z : 0)) * args.tile_rows + row; };
   float top = -INFINITY;
   for (int c = c0 + lane; c <= cut.w; c += 32) top = fmaxf(top, call.tops[slot(c)].x);
 #pragma unroll
