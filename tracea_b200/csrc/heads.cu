@@ -5,6 +5,25 @@ namespace {
 
 using namespace tb200_host;
 
+// f(lanes of a row, or 0: a warp, column by column; whether a rotation's pairs are neighbours).
+template <typename F>
+void by_head_lanes(int lanes, bool neighbours, F&& f) {
+  auto with = [&](auto row_lanes) {
+    if constexpr (decltype(row_lanes)::value > 0) {      // the scalar form goes by its columns alone
+      if (neighbours) return f(row_lanes, std::true_type{});
+    }
+    f(row_lanes, std::false_type{});
+  };
+  switch (lanes) {
+    case 1: with(std::integral_constant<int, 1>{}); break;
+    case 2: with(std::integral_constant<int, 2>{}); break;
+    case 4: with(std::integral_constant<int, 4>{}); break;
+    case 8: with(std::integral_constant<int, 8>{}); break;
+    case 16: with(std::integral_constant<int, 16>{}); break;
+    default: with(std::integral_constant<int, 0>{});
+  }
+}
+
 // Whether a rotation and the columns suit lanes of 16 columns (see HeadLane).
 bool lanes_of_16(long long cols, const tb200::Rotation& rot) { return cols % 16 == 0 && rot.pairs % 8 == 0; }
 
@@ -48,26 +67,27 @@ void head_rotate_checked(const TraceaHeads* q, const TraceaHeads* k, TraceaNormK
   a.tokens = static_cast<int>(first.tokens);
   a.D = static_cast<int>(first.cols);
   vec = vec && lanes_of_16(first.cols, a.rot);
-  a.lanes = vec ? head_lanes(first.cols) : 32;
-  const long long passes = ceil_div(heads, 32 / a.lanes);
+  const int lanes = vec ? head_lanes(first.cols) : 32;
+  const long long passes = ceil_div(a.rows[0].heads, 32 / lanes) + ceil_div(a.rows[1].heads, 32 / lanes);
+  if (passes > 0xffff) TB_FAIL(TRACEA_UNSUPPORTED_CONFIG, "%lld heads", heads);
   a.passes = static_cast<int>(passes);
   DeviceGuard guard(dev);
   DeviceState& st = device_state(dev);
   // Warps that share a token compute its angles each for itself, so no more of them than give the machine its 32 an SM.
   const long long wanted = ceil_div(32LL * st.num_sms, first.tokens);
-  a.splits = static_cast<int>(std::max(1LL, std::min(passes, wanted)));
-  const unsigned grid = grid_of(ceil_div(first.tokens * a.splits, tb200::kHeadThreads / 32));
+  const dim3 grid(grid_of(ceil_div(first.tokens, tb200::kHeadThreads / 32)), static_cast<unsigned>(std::max(1LL, std::min(passes, wanted))));
   by_dtype(first.dtype, [&](auto tag) {
-    using T = decltype(tag);
-    const auto kern = vec ? tb200::head_rotate_kernel<T, true> : tb200::head_rotate_kernel<T, false>;
-    launch(kern, grid, tb200::kHeadThreads, 0, 1, kLaunchHeads, static_cast<cudaStream_t>(stream), a);
+    by_head_lanes(vec ? lanes : 0, a.rot.interleaved != 0, [&](auto row_lanes, auto neighbours) {
+      launch(tb200::head_rotate_kernel<decltype(tag), decltype(row_lanes)::value, decltype(neighbours)::value>, grid, tb200::kHeadThreads, 0, 1,
+             kLaunchHeads, static_cast<cudaStream_t>(stream), a);
+    });
   });
 }
 
-template <typename T, bool kVec, int kRows>
+template <typename T, int kLanes, bool kNeighbours, int kRows>
 void launch_append(const tb200::KvAppendArgs& a, dim3 grid, int dev, cudaStream_t stream) {
   const int smem = a.turn_rows * a.rot.pairs * static_cast<int>(sizeof(float2));
-  auto kern = tb200::kv_append_kernel<T, kVec, kRows>;
+  auto kern = tb200::kv_append_kernel<T, kLanes, kNeighbours, kRows>;
   constexpr int kMost = tb200::kCacheMaxPage * (tb200::kCacheMaxColumns / 2) * static_cast<int>(sizeof(float2));
   static std::atomic<bool> done[kMaxDevices];
   if (smem > 40 * 1024 && !done[dev].load(std::memory_order_relaxed)) {
@@ -114,7 +134,7 @@ void kv_append_checked(const TraceaKvCache& cache, const TraceaSequences& seqs, 
   a.rot = load_rotation(rotation, k.cols);
   if (k.tokens == 0 || a.seqs.count == 0) return;
   vec = vec && lanes_of_16(k.cols, a.rot);
-  a.lanes = vec ? head_lanes(k.cols) : 32;
+  const int lanes = vec ? head_lanes(k.cols) : 32;
   const int size = 1 << a.cache.page_shift;
   a.turn_rows = a.seqs.starts != nullptr ? size : 1;
   DeviceGuard guard(dev);
@@ -126,18 +146,23 @@ void kv_append_checked(const TraceaKvCache& cache, const TraceaSequences& seqs, 
   while (a.heads_per_cta > 1 && pages * ceil_div(a.cache.heads, a.heads_per_cta) < 4LL * st.num_sms) a.heads_per_cta = (a.heads_per_cta + 1) / 2;
   const dim3 grid(grid_of(pages), static_cast<unsigned>(ceil_div(a.cache.heads, a.heads_per_cta)));
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int rows = a.seqs.starts == nullptr ? 1 : std::max(1, size * a.lanes / tb200::kHeadThreads);
+  const int rows = a.seqs.starts == nullptr ? 1 : std::max(1, size * lanes / tb200::kHeadThreads);
   by_dtype(k.dtype, [&](auto tag) {
-    using T = decltype(tag);
-    if (vec) {
-      if (rows <= 1) launch_append<T, true, 1>(a, grid, dev, s);
-      else if (rows == 2) launch_append<T, true, 2>(a, grid, dev, s);
-      else launch_append<T, true, 4>(a, grid, dev, s);
-    } else if (rows <= 4) {
-      launch_append<T, false, 4>(a, grid, dev, s);
-    } else {
-      launch_append<T, false, 16>(a, grid, dev, s);
-    }
+    by_head_lanes(vec ? lanes : 0, a.rot.interleaved != 0, [&](auto row_lanes, auto neighbours) {
+      using T = decltype(tag);
+      constexpr int kLanes = decltype(row_lanes)::value;
+      constexpr bool kNeighbours = decltype(neighbours)::value;
+      if constexpr (kLanes == 0) {
+        if (rows <= 4) launch_append<T, 0, false, 4>(a, grid, dev, s);
+        else launch_append<T, 0, false, 16>(a, grid, dev, s);
+      } else if constexpr (kLanes <= 8) {
+        if (rows <= 1) launch_append<T, kLanes, kNeighbours, 1>(a, grid, dev, s);
+        else if constexpr (kLanes >= 4) {
+          if (rows == 2) launch_append<T, kLanes, kNeighbours, 2>(a, grid, dev, s);
+          else if constexpr (kLanes == 8) launch_append<T, kLanes, kNeighbours, 4>(a, grid, dev, s);
+        }
+      }
+    });
   });
 }
 

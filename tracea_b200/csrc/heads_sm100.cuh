@@ -47,38 +47,62 @@ __device__ __forceinline__ float2 rotation_of(int position, double frequency) {
 }
 
 // ------------------------------------------------------------------ a lane's columns of a row
-// kVec: 16 columns, lane c of the row in two runs of 8: 8c and 8c + pairs, which a rotation of halves pairs, for the rotated columns
-// of that kind; 16c and 16c + 8 for others. Rows are 16-byte aligned, D and the rotated columns multiples of 16.
-// Else: kPairs pairs of columns, pair number lane + 32 i, of any row of an even number of columns, which a warp holds.
-template <bool kVec, int kScalarPairs>
+// A lane holds kPairs pairs (x, y) of columns, which a rotation turns into (x cos - y sin, y cos + x sin).
+// kLanes > 0: so many lanes hold a row, 8 pairs each, 16 columns in two runs of 8: 8c and 8c + pairs for lane c, which a rotation of
+// halves pairs, for the rotated columns of that kind; 16c and 16c + 8 for others. Rows are 16-byte aligned, D and the rotated columns
+// multiples of 16.
+// kLanes = 0: a warp holds a row of any even number of columns, a lane the pairs number lane + 32 i.
+__host__ __device__ constexpr int head_row_lanes(int lanes) { return lanes > 0 ? lanes : 32; }
+template <int kLanes, int kScalarPairs>
 struct HeadLane {
+  static constexpr bool kVec = kLanes > 0;
   static constexpr int kPairs = kVec ? 8 : kScalarPairs;
-  int first[kVec ? 1 : kPairs], second[kVec ? 1 : kPairs];   // columns; -1: none
+  int first[kVec ? 1 : kPairs], second[kVec ? 1 : kPairs];   // columns; 0, 0 where there are none
   int angle;                                                 // number of the first pair's angle
-  bool live, turned, neighbours;
+  int live;                                                  // pairs that there are
+  bool turned;
 
   __device__ __forceinline__ HeadLane(int lane, int D, const Rotation& rot) {
-    neighbours = rot.interleaved != 0;
     if constexpr (kVec) {
-      live = 16 * lane < D;
+      live = 16 * lane < D ? kPairs : 0;
       turned = 16 * lane < 2 * rot.pairs;
       angle = 8 * lane;
-      const bool halves = turned && !neighbours;
-      first[0] = halves ? 8 * lane : 16 * lane;
-      second[0] = halves ? 8 * lane + rot.pairs : 16 * lane + 8;
+      const bool halves = turned && rot.interleaved == 0;
+      first[0] = live == 0 ? 0 : halves ? 8 * lane : 16 * lane;
+      second[0] = live == 0 ? 0 : halves ? 8 * lane + rot.pairs : 16 * lane + 8;
     } else {
-      live = turned = true;
+      turned = true;
       angle = lane;
+      live = 0;
 #pragma unroll
       for (int i = 0; i < kPairs; ++i) {
         const int p = lane + 32 * i;
-        const bool halves = p < rot.pairs && !neighbours;
-        first[i] = 2 * p < D ? (halves ? p : 2 * p) : -1;
-        second[i] = halves ? p + rot.pairs : 2 * p + 1;
+        const bool halves = p < rot.pairs && rot.interleaved == 0;
+        if (2 * p < D) live = i + 1;
+        first[i] = 2 * p >= D ? 0 : halves ? p : 2 * p;
+        second[i] = 2 * p >= D ? 0 : halves ? p + rot.pairs : 2 * p + 1;
       }
     }
   }
 };
+
+// Between the order of the runs in memory and that of pairs of neighbours.
+__device__ __forceinline__ void runs_to_pairs(float (&x)[8], float (&y)[8]) {
+  const float a[8] = {x[0], x[2], x[4], x[6], y[0], y[2], y[4], y[6]}, b[8] = {x[1], x[3], x[5], x[7], y[1], y[3], y[5], y[7]};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    x[i] = a[i];
+    y[i] = b[i];
+  }
+}
+__device__ __forceinline__ void pairs_to_runs(float (&x)[8], float (&y)[8]) {
+  const float a[8] = {x[0], y[0], x[1], y[1], x[2], y[2], x[3], y[3]}, b[8] = {x[4], y[4], x[5], y[5], x[6], y[6], x[7], y[7]};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    x[i] = a[i];
+    y[i] = b[i];
+  }
+}
 
 template <typename T>
 struct Vec8 {   // eight consecutive elements as they are loaded
@@ -91,139 +115,176 @@ __device__ __forceinline__ void fetch8(const T* p, Vec8<T>& v) {
 }
 template <typename T>
 __device__ __forceinline__ void widen8(const Vec8<T>& v, float (&o)[8]) {
-  const T* e = reinterpret_cast<const T*>(&v);
+  if constexpr (sizeof(T) == 4) {
+    const float* e = reinterpret_cast<const float*>(&v);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) o[i] = static_cast<float>(e[i]);
+    for (int i = 0; i < 8; ++i) o[i] = e[i];
+  } else {
+    unpack2<T>(v.w[0].x, o[0], o[1]);
+    unpack2<T>(v.w[0].y, o[2], o[3]);
+    unpack2<T>(v.w[0].z, o[4], o[5]);
+    unpack2<T>(v.w[0].w, o[6], o[7]);
+  }
 }
-// A lane's columns of a row as they lie in memory.
-template <typename T, bool kVec, int kScalarPairs>
+
+// A lane's columns of a row as they lie in memory. Lanes without columns, and those whose row is not one, load some other of the same
+// tensor: a branch around a load costs more.
+template <typename T, int kLanes, int kScalarPairs>
 struct HeadRaw {
-  using Lane = HeadLane<kVec, kScalarPairs>;
+  using Lane = HeadLane<kLanes, kScalarPairs>;
+  static constexpr int kPairs = Lane::kPairs;
   Vec8<T> va, vb;
   T sa[kScalarPairs], sb[kScalarPairs];
 
-  __device__ __forceinline__ void load(const T* row, const Lane& l, bool live) {
-    if constexpr (kVec) {
-      if (live && l.live) {
-        fetch8(row + l.first[0], va);
-        fetch8(row + l.second[0], vb);
-      } else {
-        memset(&va, 0, sizeof(va));
-        memset(&vb, 0, sizeof(vb));
-      }
+  __device__ __forceinline__ void load(const T* row, const Lane& l) {
+    if constexpr (Lane::kVec) {
+      fetch8(row + l.first[0], va);
+      fetch8(row + l.second[0], vb);
     } else {
 #pragma unroll
-      for (int i = 0; i < Lane::kPairs; ++i) {
-        const bool here = live && l.first[i] >= 0;
-        sa[i] = here ? row[l.first[i]] : static_cast<T>(0.0f);
-        sb[i] = here ? row[l.second[i]] : static_cast<T>(0.0f);
+      for (int i = 0; i < kPairs; ++i) {
+        sa[i] = row[l.first[i]];
+        sb[i] = row[l.second[i]];
       }
     }
   }
-  __device__ __forceinline__ void values(float (&a)[Lane::kPairs], float (&b)[Lane::kPairs]) const {
-    if constexpr (kVec) {
-      widen8(va, a);
-      widen8(vb, b);
+  template <bool kNeighbours>
+  __device__ __forceinline__ void values(const Lane& l, float (&x)[kPairs], float (&y)[kPairs]) const {
+    if constexpr (Lane::kVec) {
+      widen8(va, x);
+      widen8(vb, y);
+      if constexpr (kNeighbours) runs_to_pairs(x, y);
     } else {
 #pragma unroll
-      for (int i = 0; i < Lane::kPairs; ++i) {
-        a[i] = static_cast<float>(sa[i]);
-        b[i] = static_cast<float>(sb[i]);
+      for (int i = 0; i < kPairs; ++i) {
+        x[i] = i < l.live ? static_cast<float>(sa[i]) : 0.0f;
+        y[i] = i < l.live ? static_cast<float>(sb[i]) : 0.0f;
       }
     }
   }
 };
 
-// The norm of a row (a mean over D columns; `lanes` lanes, a power of two, hold it) times `weight`, fp32 in shared memory, or nullptr.
-template <bool kVec, int kScalarPairs>
-__device__ __forceinline__ void head_norm(const HeadLane<kVec, kScalarPairs>& l, float (&a)[HeadLane<kVec, kScalarPairs>::kPairs],
-                                          float (&b)[HeadLane<kVec, kScalarPairs>::kPairs], int lanes, float inv_columns, float eps,
-                                          const float* weight) {
-  constexpr int kPairs = HeadLane<kVec, kScalarPairs>::kPairs;
-  float sum = 0.0f;
-#pragma unroll
-  for (int i = 0; i < kPairs; ++i) sum += a[i] * a[i] + b[i] * b[i];
-  for (int o = lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  const float inv = 1.0f / sqrtf(sum * inv_columns + eps);
-#pragma unroll
-  for (int i = 0; i < kPairs; ++i) {
-    a[i] *= inv;
-    b[i] *= inv;
-  }
-  if (weight == nullptr) return;
-  if constexpr (kVec) {
-    if (l.live) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        a[i] *= weight[l.first[0] + i];
-        b[i] *= weight[l.second[0] + i];
-      }
+template <bool kNeighbours, typename T, int kLanes, int kScalarPairs>
+__device__ __forceinline__ void head_store(T* row, const HeadLane<kLanes, kScalarPairs>& l, float (&x)[HeadLane<kLanes, kScalarPairs>::kPairs],
+                                           float (&y)[HeadLane<kLanes, kScalarPairs>::kPairs]) {
+  if constexpr (kLanes > 0) {
+    if constexpr (kNeighbours) pairs_to_runs(x, y);
+    if (l.live > 0) {
+      store8(row + l.first[0], x);
+      store8(row + l.second[0], y);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < kPairs; ++i) {
-      if (l.first[i] >= 0) {
-        a[i] *= weight[l.first[i]];
-        b[i] *= weight[l.second[i]];
+    for (int i = 0; i < kScalarPairs; ++i) {
+      if (i < l.live) {
+        row[l.first[i]] = static_cast<T>(x[i]);
+        row[l.second[i]] = static_cast<T>(y[i]);
       }
     }
   }
 }
 
-__device__ __forceinline__ void turn_pair(float& a, float& b, float2 cs) {
-  const float x = a * cs.x - b * cs.y;
-  b = b * cs.x + a * cs.y;
-  a = x;
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t pack_f32x2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
 }
-// `turns`: the token's cosines and sines, of pair 0 on, in shared memory.
-template <bool kVec, int kScalarPairs>
-__device__ __forceinline__ void head_turn(const HeadLane<kVec, kScalarPairs>& l, float (&a)[HeadLane<kVec, kScalarPairs>::kPairs],
-                                          float (&b)[HeadLane<kVec, kScalarPairs>::kPairs], const float2* turns, int pairs) {
-  if constexpr (kVec) {
-    if (!l.turned) return;
-    float2 cs[8];
+__device__ __forceinline__ void unpack_f32x2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// 1 / sqrt(mean + eps) of a row, to 2 units in the last place.
+template <int kLanes, int kScalarPairs>
+__device__ __forceinline__ float head_norm(const HeadLane<kLanes, kScalarPairs>& l, const float (&x)[HeadLane<kLanes, kScalarPairs>::kPairs],
+                                           const float (&y)[HeadLane<kLanes, kScalarPairs>::kPairs], float inv_columns, float eps) {
+  constexpr int kPairs = HeadLane<kLanes, kScalarPairs>::kPairs;
+  uint64_t both = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float4 v = *reinterpret_cast<const float4*>(turns + l.angle + 2 * i);
-      cs[2 * i] = make_float2(v.x, v.y);
-      cs[2 * i + 1] = make_float2(v.z, v.w);
+  for (int i = 0; i < kPairs; ++i) {
+    const uint64_t v = pack_f32x2(x[i], y[i]);
+    both = fma_f32x2(v, v, both);
+  }
+  float sum, other;
+  unpack_f32x2(both, sum, other);
+  sum = l.live > 0 ? sum + other : 0.0f;
+#pragma unroll
+  for (int o = head_row_lanes(kLanes) / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return rsqrtf(sum * inv_columns + eps);
+}
+
+// A lane's weights, 1 where there are none; `weight`: fp32 in shared memory, or nullptr.
+template <bool kNeighbours, int kLanes, int kScalarPairs>
+__device__ __forceinline__ void head_weights(const HeadLane<kLanes, kScalarPairs>& l, const float* weight,
+                                             float (&wx)[HeadLane<kLanes, kScalarPairs>::kPairs], float (&wy)[HeadLane<kLanes, kScalarPairs>::kPairs]) {
+  if (weight == nullptr) {
+#pragma unroll
+    for (int i = 0; i < HeadLane<kLanes, kScalarPairs>::kPairs; ++i) wx[i] = wy[i] = 1.0f;
+  } else if constexpr (kLanes > 0) {
+    load8(weight + l.first[0], wx);
+    load8(weight + l.second[0], wy);
+    if constexpr (kNeighbours) runs_to_pairs(wx, wy);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kScalarPairs; ++i) {
+      wx[i] = weight[l.first[i]];
+      wy[i] = weight[l.second[i]];
     }
-    if (!l.neighbours) {
+  }
+}
+// A lane's cosines and sines; `turns`: a token's, from pair 0 on, in shared memory.
+template <int kLanes, int kScalarPairs>
+__device__ __forceinline__ void head_turns(const HeadLane<kLanes, kScalarPairs>& l, const float2* turns, int pairs,
+                                           float2 (&cs)[HeadLane<kLanes, kScalarPairs>::kPairs]) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) turn_pair(a[i], b[i], cs[i]);
-    } else {
+  for (int i = 0; i < HeadLane<kLanes, kScalarPairs>::kPairs; ++i) cs[i] = make_float2(1.0f, 0.0f);
+  if constexpr (kLanes > 0) {
+    if (l.turned) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        turn_pair(a[2 * i], a[2 * i + 1], cs[i]);
-        turn_pair(b[2 * i], b[2 * i + 1], cs[4 + i]);
+        const float4 v = *reinterpret_cast<const float4*>(turns + l.angle + 2 * i);
+        cs[2 * i] = make_float2(v.x, v.y);
+        cs[2 * i + 1] = make_float2(v.z, v.w);
       }
     }
   } else {
 #pragma unroll
     for (int i = 0; i < kScalarPairs; ++i)
-      if (l.angle + 32 * i < pairs) turn_pair(a[i], b[i], turns[l.angle + 32 * i]);
+      if (l.angle + 32 * i < pairs) cs[i] = turns[l.angle + 32 * i];
   }
 }
-
-template <typename T, bool kVec, int kScalarPairs>
-__device__ __forceinline__ void head_store(T* row, const HeadLane<kVec, kScalarPairs>& l,
-                                           const float (&a)[HeadLane<kVec, kScalarPairs>::kPairs],
-                                           const float (&b)[HeadLane<kVec, kScalarPairs>::kPairs]) {
-  if constexpr (kVec) {
-    if (l.live) {
-      store8(row + l.first[0], a);
-      store8(row + l.second[0], b);
-    }
-  } else {
+// Weights and rotation together, for rows of one token: (x, y) -> factor (x xx + y xy, y yy + x yx), two pairs at a time.
+template <int kPairs>
+struct HeadTurn {
+  uint64_t xx[kPairs / 2], xy[kPairs / 2], yy[kPairs / 2], yx[kPairs / 2];
+  __device__ __forceinline__ HeadTurn(const float (&wx)[kPairs], const float (&wy)[kPairs], const float2 (&cs)[kPairs]) {
 #pragma unroll
-    for (int i = 0; i < kScalarPairs; ++i) {
-      if (l.first[i] >= 0) {
-        row[l.first[i]] = static_cast<T>(a[i]);
-        row[l.second[i]] = static_cast<T>(b[i]);
-      }
+    for (int i = 0; i < kPairs / 2; ++i) {
+      const int a = 2 * i, b = 2 * i + 1;
+      xx[i] = pack_f32x2(wx[a] * cs[a].x, wx[b] * cs[b].x);
+      xy[i] = pack_f32x2(-wy[a] * cs[a].y, -wy[b] * cs[b].y);
+      yy[i] = pack_f32x2(wy[a] * cs[a].x, wy[b] * cs[b].x);
+      yx[i] = pack_f32x2(wx[a] * cs[a].y, wx[b] * cs[b].y);
     }
   }
-}
+  __device__ __forceinline__ void apply(float (&x)[kPairs], float (&y)[kPairs], float factor) const {
+    const uint64_t f = pack_f32x2(factor, factor);
+#pragma unroll
+    for (int i = 0; i < kPairs / 2; ++i) {
+      const uint64_t u = mul_f32x2(pack_f32x2(x[2 * i], x[2 * i + 1]), f), v = mul_f32x2(pack_f32x2(y[2 * i], y[2 * i + 1]), f);
+      unpack_f32x2(fma_f32x2(v, xy[i], mul_f32x2(u, xx[i])), x[2 * i], x[2 * i + 1]);
+      unpack_f32x2(fma_f32x2(u, yx[i], mul_f32x2(v, yy[i])), y[2 * i], y[2 * i + 1]);
+    }
+  }
+};
 
 // ------------------------------------------------------------------ norm and rotation of rows of heads
 struct HeadRows {
@@ -240,8 +301,7 @@ struct HeadRotateArgs {
   Rotation rot;
   const int* positions;
   int tokens, D, norm;
-  int lanes;                   // lanes of a row
-  int splits, passes;          // warps of a token; passes of a warp over 32 / lanes heads that a token takes in all
+  int passes;                  // of a warp, over as many heads as it holds, that a token takes in all; blockIdx.y shares them out
   float eps;
 };
 
@@ -252,19 +312,18 @@ __device__ __forceinline__ void weights_to_shared(float* dst, const void* weight
     dst[i] = is_f32 ? static_cast<const float*>(weight)[i] : static_cast<float>(static_cast<const T*>(weight)[i]);
 }
 
-// A warp takes a token's heads 32 / lanes at a time, or, where the tokens alone would not fill the machine, a share of them. Two
-// passes' loads are under way at once.
-template <typename T, bool kVec>
-__global__ void __launch_bounds__(kHeadThreads) head_rotate_kernel(const __grid_constant__ HeadRotateArgs args) {
-  using Lane = HeadLane<kVec, 4>;
-  constexpr int kPairs = Lane::kPairs, kAhead = 2;
-  __shared__ float weights[2][kHeadMaxColumns];
+// A warp takes as many of a token's heads as it holds at a time, queries and then keys, or, where the tokens alone would not fill the
+// machine, a share of them. The weights and the token's rotation stay in registers over them; kAhead passes' loads are under way at once.
+template <typename T, int kLanes, bool kNeighbours>
+__global__ void __launch_bounds__(kHeadThreads, 3) head_rotate_kernel(const __grid_constant__ HeadRotateArgs args) {
+  using Lane = HeadLane<kLanes, 4>;
+  constexpr int kPairs = Lane::kPairs, kRowLanes = head_row_lanes(kLanes), kHeads = 32 / kRowLanes, kAhead = 2;
+  __shared__ __align__(16) float weights[2][kHeadMaxColumns];
   __shared__ __align__(16) float2 turns[kHeadThreads / 32][kHeadMaxColumns / 2];
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long id = static_cast<long long>(blockIdx.x) * (kHeadThreads / 32) + warp;
-  const int token = static_cast<int>(id / args.splits), split = static_cast<int>(id % args.splits);
+  const long long token = static_cast<long long>(blockIdx.x) * (kHeadThreads / 32) + warp;
   for (int r = 0; r < 2; ++r) weights_to_shared<T>(weights[r], args.rows[r].weight, args.rows[r].weight_f32, args.D);
   if (token < args.tokens && args.rot.pairs > 0) {
     const int position = args.positions[token];
@@ -272,33 +331,46 @@ __global__ void __launch_bounds__(kHeadThreads) head_rotate_kernel(const __grid_
   }
   __syncthreads();
   if (token >= args.tokens) return;
-  const int lanes = kVec ? args.lanes : 32, group = lane / lanes, per_pass = 32 / lanes;
-  const Lane l(lane % lanes, args.D, args.rot);
-  const int heads = args.rows[0].heads + args.rows[1].heads;
-  const int begin = static_cast<int>(static_cast<long long>(args.passes) * split / args.splits);
-  const int end = static_cast<int>(static_cast<long long>(args.passes) * (split + 1) / args.splits);
+  const int group = lane / kRowLanes;
+  const Lane l(lane % kRowLanes, args.D, args.rot);
   const float inv_columns = 1.0f / static_cast<float>(args.D);
-  for (int pass = begin; pass < end; pass += kAhead) {
-    HeadRaw<T, kVec, 4> raw[kAhead];
-    int head[kAhead], which[kAhead];
+  float2 cs[kPairs];
+  head_turns(l, turns[warp], args.rot.pairs, cs);
+  const int split_begin = args.passes * static_cast<int>(blockIdx.y) / static_cast<int>(gridDim.y);
+  const int split_end = args.passes * static_cast<int>(blockIdx.y + 1) / static_cast<int>(gridDim.y);
+  int before = 0;
+#pragma unroll 1
+  for (int which = 0; which < 2; ++which) {
+    const HeadRows& rows = args.rows[which];
+    const int passes = (rows.heads + kHeads - 1) / kHeads;
+    const int begin = max(0, split_begin - before), end = min(passes, split_end - before);
+    before += passes;
+    if (begin >= end) continue;
+    float wx[kPairs], wy[kPairs];
+    head_weights<kNeighbours>(l, args.norm && rows.weight != nullptr ? weights[which] : nullptr, wx, wy);
+    const HeadTurn<kPairs> turn(wx, wy, cs);
+    const int heads = rows.heads;
+    const long long x_step = kHeads * rows.x_head, y_step = kHeads * rows.y_head;
+    const T* src = static_cast<const T*>(rows.x) + token * rows.x_token + (begin * kHeads + group) * rows.x_head;
+    T* dst = static_cast<T*>(rows.y) + token * rows.y_token + (begin * kHeads + group) * rows.y_head;
+    const T* const some = static_cast<const T*>(rows.x) + token * rows.x_token;
+    for (int pass = begin; pass < end; pass += kAhead) {
+      HeadRaw<T, kLanes, 4> raw[kAhead];
+      bool here[kAhead];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      head[u] = (pass + u) * per_pass + group;
-      const bool live = pass + u < end && head[u] < heads;
-      which[u] = head[u] >= args.rows[0].heads ? 1 : 0;
-      if (which[u]) head[u] -= args.rows[0].heads;
-      if (!live) head[u] = -1;
-      const HeadRows& rows = args.rows[which[u]];
-      raw[u].load(static_cast<const T*>(rows.x) + token * rows.x_token + (live ? head[u] : 0) * rows.x_head, l, live);
-    }
+      for (int u = 0; u < kAhead; ++u) {
+        here[u] = pass + u < end && (pass + u) * kHeads + group < heads;
+        raw[u].load(here[u] ? src + u * x_step : some, l);
+      }
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      float a[kPairs], b[kPairs];
-      raw[u].values(a, b);
-      const HeadRows& rows = args.rows[which[u]];
-      if (args.norm) head_norm(l, a, b, lanes, inv_columns, args.eps, rows.weight != nullptr ? weights[which[u]] : nullptr);
-      head_turn(l, a, b, turns[warp], args.rot.pairs);
-      if (head[u] >= 0) head_store(static_cast<T*>(rows.y) + token * rows.y_token + head[u] * rows.y_head, l, a, b);
+      for (int u = 0; u < kAhead; ++u) {
+        float x[kPairs], y[kPairs];
+        raw[u].template values<kNeighbours>(l, x, y);
+        turn.apply(x, y, args.norm ? head_norm(l, x, y, inv_columns, args.eps) : 1.0f);
+        if (here[u]) head_store<kNeighbours>(dst + u * y_step, l, x, y);
+      }
+      src += kAhead * x_step;
+      dst += kAhead * y_step;
     }
   }
 }
@@ -377,7 +449,15 @@ __device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi) {
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
 }
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 __device__ __forceinline__ uint32_t e4m3_four(float a, float b, float c, float d) { return e4m3_pair(a, b) | (e4m3_pair(c, d) << 16); }
+__device__ __forceinline__ uint2 e4m3_eight(const float (&v)[8]) {
+  return make_uint2(e4m3_four(v[0], v[1], v[2], v[3]), e4m3_four(v[4], v[5], v[6], v[7]));
+}
 // Four elements as halves, two to a word.
 __device__ __forceinline__ void halves_of_e4m3(uint32_t four, uint32_t& lo, uint32_t& hi) {
   asm("{\n"
@@ -404,7 +484,7 @@ struct KvAppendArgs {
   const void* v;
   long long v_token, v_head;
   Rotation rot;
-  int norm, lanes;
+  int norm;
   int group;                   // heads of q to one of k
   int heads_per_cta;           // of k
   int turn_rows;               // rows of angles in shared memory
@@ -414,13 +494,14 @@ struct KvAppendArgs {
 // A CTA takes the new tokens of one page of a sequence, and some heads: for each the keys and values, whose scales need all of the
 // block's rows and so stay in registers until they are known, and the queries' heads that go with it. A block belongs to one CTA:
 // nothing is shared, nothing atomic. kRows: rows of a block that a lane holds.
-template <typename T, bool kVec, int kRows>
-__global__ void __launch_bounds__(kHeadThreads) kv_append_kernel(const __grid_constant__ KvAppendArgs args) {
+template <typename T, int kLanes, bool kNeighbours, int kRows>
+__global__ void __launch_bounds__(kHeadThreads, kLanes > 0 && kRows <= 2 ? 2 : 1) kv_append_kernel(const __grid_constant__ KvAppendArgs args) {
   constexpr int kScalarPairs = kCacheMaxColumns / 64;
-  using Lane = HeadLane<kVec, kScalarPairs>;
-  constexpr int kPairs = Lane::kPairs, kWarps = kHeadThreads / 32;
+  using Lane = HeadLane<kLanes, kScalarPairs>;
+  using Raw = HeadRaw<T, kLanes, kScalarPairs>;
+  constexpr int kPairs = Lane::kPairs, kWarps = kHeadThreads / 32, kRowLanes = head_row_lanes(kLanes), kRowsAtOnce = kHeadThreads / kRowLanes;
   extern __shared__ __align__(16) float2 turns[];          // [turn_rows][pairs]
-  __shared__ float weights[2][kCacheMaxColumns];
+  __shared__ __align__(16) float weights[2][kCacheMaxColumns];
   __shared__ float peaks[2][2][kWarps];                    // two heads in turn: one barrier a head
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();
@@ -448,53 +529,66 @@ __global__ void __launch_bounds__(kHeadThreads) kv_append_kernel(const __grid_co
   }
   __syncthreads();
 
-  const int lanes = kVec ? args.lanes : 32, rows_at_once = kHeadThreads / lanes;
-  const int my_row = static_cast<int>(threadIdx.x) / lanes, my_lane = static_cast<int>(threadIdx.x) % lanes;
+  const int my_row = static_cast<int>(threadIdx.x) / kRowLanes, my_lane = static_cast<int>(threadIdx.x) % kRowLanes;
   const Lane l(my_lane, D, args.rot);
   const Lane plain(my_lane, D, Rotation{nullptr, 0, 0});   // values are not rotated: their columns in order
   const float inv_columns = 1.0f / static_cast<float>(D);
   const int head0 = static_cast<int>(blockIdx.y) * args.heads_per_cta, head1 = min(args.cache.heads, head0 + args.heads_per_cta);
 
   if (page >= 0) {
+    Raw rk[kRows], rv[kRows];
+    const T *k_row[kRows], *v_row[kRows];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const int r = my_row + i * kRowsAtOnce;
+      const long long row = row0 + (r < count ? r : 0);
+      k_row[i] = static_cast<const T*>(args.k.x) + row * args.k.x_token + head0 * args.k.x_head;
+      v_row[i] = static_cast<const T*>(args.v) + row * args.v_token + head0 * args.v_head;
+      rk[i].load(k_row[i], l);
+      rv[i].load(v_row[i], plain);
+    }
     for (int head = head0; head < head1; ++head) {
       const long long block = page * args.cache.heads + head;
       uint8_t* ck = args.cache.k + (block << shift) * D;
       uint8_t* cv = args.cache.v + (block << shift) * D;
       const int old_k = static_cast<int>(args.cache.k_scales[block]) - 127, old_v = static_cast<int>(args.cache.v_scales[block]) - 127;
-      HeadRaw<T, kVec, kScalarPairs> rk[kRows], rv[kRows];
-#pragma unroll
-      for (int i = 0; i < kRows; ++i) {
-        const int r = my_row + i * rows_at_once;
-        const long long row = row0 + r;
-        rk[i].load(static_cast<const T*>(args.k.x) + row * args.k.x_token + head * args.k.x_head, l, r < count);
-        rv[i].load(static_cast<const T*>(args.v) + row * args.v_token + head * args.v_head, plain, r < count);
-      }
-      float ka[kRows][kPairs], kb[kRows][kPairs];
+      float kx[kRows][kPairs], ky[kRows][kPairs];
       float peak_k = 0.0f, peak_v = 0.0f;
       uint32_t bad = 0u;
 #pragma unroll
       for (int i = 0; i < kRows; ++i) {
-        rk[i].values(ka[i], kb[i]);
-        if (args.norm) head_norm(l, ka[i], kb[i], lanes, inv_columns, args.eps, args.k.weight != nullptr ? weights[1] : nullptr);
-        if (my_row + i * rows_at_once < count) head_turn(l, ka[i], kb[i], turns + (my_row + i * rows_at_once) * pairs, pairs);
-        float va[kPairs], vb[kPairs];
-        rv[i].values(va, vb);
-        float mk = 0.0f, mv = 0.0f;
-        bool finite = true;
+        const int r = my_row + i * kRowsAtOnce;
+        rk[i].template values<kNeighbours>(l, kx[i], ky[i]);
+        float wx[kPairs], wy[kPairs];
+        head_weights<kNeighbours>(l, args.norm && args.k.weight != nullptr ? weights[1] : nullptr, wx, wy);
+        const float factor = args.norm ? head_norm(l, kx[i], ky[i], inv_columns, args.eps) : 1.0f;
+        float2 cs[kPairs];
+        head_turns(l, turns + (r < count ? r : 0) * pairs, pairs, cs);
+        float mk = 0.0f, mv = 0.0f;                        // NaN if there is one among them
 #pragma unroll
         for (int j = 0; j < kPairs; ++j) {
-          mk = fmaxf(mk, fmaxf(fabsf(ka[i][j]), fabsf(kb[i][j])));
-          mv = fmaxf(mv, fmaxf(fabsf(va[j]), fabsf(vb[j])));
-          finite = finite && isfinite(ka[i][j]) && isfinite(kb[i][j]) && isfinite(va[j]) && isfinite(vb[j]);
+          const float x = kx[i][j] * (factor * wx[j]), y = ky[i][j] * (factor * wy[j]);
+          kx[i][j] = x * cs[j].x - y * cs[j].y;
+          ky[i][j] = y * cs[j].x + x * cs[j].y;
+          mk = max_nan(mk, max_nan(fabsf(kx[i][j]), fabsf(ky[i][j])));
         }
+        float vx[kPairs], vy[kPairs];
+        rv[i].template values<false>(plain, vx, vy);
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) mv = max_nan(mv, max_nan(fabsf(vx[j]), fabsf(vy[j])));
+        if (l.live == 0 || r >= count) mk = mv = 0.0f;
         // a token that is not finite counts for no scale: a vote of its lanes
-        const uint32_t votes = __ballot_sync(0xffffffffu, !finite);
-        const uint32_t mine = lanes == 32 ? votes : (votes >> ((threadIdx.x & 31) / lanes * lanes)) & ((1u << lanes) - 1u);
+        const uint32_t votes = __ballot_sync(0xffffffffu, !(mk < INFINITY && mv < INFINITY));
+        const uint32_t mine = kRowLanes == 32 ? votes : (votes >> ((threadIdx.x & 31) / kRowLanes * kRowLanes)) & ((1u << (kRowLanes % 32)) - 1u);
         if (mine != 0u) bad |= 1u << i;
         else {
           peak_k = fmaxf(peak_k, mk);
           peak_v = fmaxf(peak_v, mv);
         }
+      }
+      if (head + 1 < head1) {
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) rk[i].load(k_row[i] += args.k.x_head, l);
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
@@ -520,41 +614,49 @@ __global__ void __launch_bounds__(kHeadThreads) kv_append_kernel(const __grid_co
       const float sk = power_of_two(-ek), sv = power_of_two(-ev);
 #pragma unroll
       for (int i = 0; i < kRows; ++i) {
-        const int r = my_row + i * rows_at_once;
+        const int r = my_row + i * kRowsAtOnce;
         if (r >= count) continue;
-        const bool drop = (bad >> i) & 1u;
-        float va[kPairs], vb[kPairs];
-        rv[i].values(va, vb);
+        float vx[kPairs], vy[kPairs];
+        rv[i].template values<false>(plain, vx, vy);
 #pragma unroll
         for (int j = 0; j < kPairs; ++j) {
-          ka[i][j] = drop ? __int_as_float(0x7fffffff) : ka[i][j] * sk;
-          kb[i][j] = drop ? __int_as_float(0x7fffffff) : kb[i][j] * sk;
-          va[j] = drop ? 0.0f : va[j] * sv;
-          vb[j] = drop ? 0.0f : vb[j] * sv;
+          kx[i][j] *= sk;
+          ky[i][j] *= sk;
+          vx[j] *= sv;
+          vy[j] *= sv;
+        }
+        if ((bad >> i) & 1u) {
+#pragma unroll
+          for (int j = 0; j < kPairs; ++j) {
+            kx[i][j] = ky[i][j] = __int_as_float(0x7fffffff);
+            vx[j] = vy[j] = 0.0f;
+          }
         }
         uint8_t *dk = ck + static_cast<long long>(first + r) * D, *dv = cv + static_cast<long long>(first + r) * D;
-        if constexpr (kVec) {
-          if (l.live) {
-            *reinterpret_cast<uint2*>(dk + l.first[0]) =
-                make_uint2(e4m3_four(ka[i][0], ka[i][1], ka[i][2], ka[i][3]), e4m3_four(ka[i][4], ka[i][5], ka[i][6], ka[i][7]));
-            *reinterpret_cast<uint2*>(dk + l.second[0]) =
-                make_uint2(e4m3_four(kb[i][0], kb[i][1], kb[i][2], kb[i][3]), e4m3_four(kb[i][4], kb[i][5], kb[i][6], kb[i][7]));
-            *reinterpret_cast<uint4*>(dv + plain.first[0]) =
-                make_uint4(e4m3_four(va[0], va[1], va[2], va[3]), e4m3_four(va[4], va[5], va[6], va[7]),
-                           e4m3_four(vb[0], vb[1], vb[2], vb[3]), e4m3_four(vb[4], vb[5], vb[6], vb[7]));
+        if constexpr (kLanes > 0) {
+          if constexpr (kNeighbours) pairs_to_runs(kx[i], ky[i]);
+          if (l.live > 0) {
+            *reinterpret_cast<uint2*>(dk + l.first[0]) = e4m3_eight(kx[i]);
+            *reinterpret_cast<uint2*>(dk + l.second[0]) = e4m3_eight(ky[i]);
+            const uint2 lo = e4m3_eight(vx), hi = e4m3_eight(vy);
+            *reinterpret_cast<uint4*>(dv + plain.first[0]) = make_uint4(lo.x, lo.y, hi.x, hi.y);
           }
         } else {
 #pragma unroll
           for (int j = 0; j < kPairs; ++j) {
-            if (l.first[j] >= 0) {
-              const uint32_t ek2 = e4m3_pair(ka[i][j], kb[i][j]), ev2 = e4m3_pair(va[j], vb[j]);
-              dk[l.first[j]] = static_cast<uint8_t>(ek2);
-              dk[l.second[j]] = static_cast<uint8_t>(ek2 >> 8);
-              dv[plain.first[j]] = static_cast<uint8_t>(ev2);
-              dv[plain.second[j]] = static_cast<uint8_t>(ev2 >> 8);
+            if (j < l.live) {
+              const uint32_t k2 = e4m3_pair(kx[i][j], ky[i][j]), v2 = e4m3_pair(vx[j], vy[j]);
+              dk[l.first[j]] = static_cast<uint8_t>(k2);
+              dk[l.second[j]] = static_cast<uint8_t>(k2 >> 8);
+              dv[plain.first[j]] = static_cast<uint8_t>(v2);
+              dv[plain.second[j]] = static_cast<uint8_t>(v2 >> 8);
             }
           }
         }
+      }
+      if (head + 1 < head1) {
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) rv[i].load(v_row[i] += args.v_head, plain);
       }
       if (first > 0) {                                     // the page's older tokens, where the scale has grown
         const int vecs = first * D / 16;
@@ -577,29 +679,36 @@ __global__ void __launch_bounds__(kHeadThreads) kv_append_kernel(const __grid_co
   }
 
   if (args.q.x == nullptr) return;
-  // the queries that go with these heads
-  const int q0 = head0 * args.group, heads = (head1 - head0) * args.group, total = count * heads;
+  // The queries that go with these heads: the lanes of a row take a few heads of a token in turn, with its rotation in registers.
+  const int q0 = head0 * args.group, heads = (head1 - head0) * args.group;
+  const int turn_heads = min(8, max(1, heads * count / kRowsAtOnce)), shares = (heads + turn_heads - 1) / turn_heads;
   constexpr int kAhead = 2;
-  for (int base = 0; base < total; base += kAhead * rows_at_once) {
-    HeadRaw<T, kVec, kScalarPairs> raw[kAhead];
-    int token[kAhead], head[kAhead];
+  for (int base = 0; base < count * shares; base += kRowsAtOnce) {
+    const int i = base + my_row, share = i % shares, token = i / shares;
+    const bool there = token < count;
+    const int from_head = share * turn_heads, mine = there ? min(turn_heads, heads - from_head) : 0;
+    float wx[kPairs], wy[kPairs];
+    head_weights<kNeighbours>(l, args.norm && args.q.weight != nullptr ? weights[0] : nullptr, wx, wy);
+    float2 cs[kPairs];
+    head_turns(l, turns + (there ? token : 0) * pairs, pairs, cs);
+    const HeadTurn<kPairs> turn(wx, wy, cs);
+    const long long row = row0 + (there ? token : 0);
+    const T* const some = static_cast<const T*>(args.q.x) + row * args.q.x_token + q0 * args.q.x_head;
+    const T* src = some + from_head * args.q.x_head;
+    T* dst = static_cast<T*>(args.q.y) + row * args.q.y_token + (q0 + from_head) * args.q.y_head;
+    for (int h = 0; h < turn_heads; h += kAhead) {
+      Raw raw[kAhead];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int i = base + u * rows_at_once + my_row;
-      const bool live = i < total;
-      token[u] = live ? i / heads : -1;
-      head[u] = live ? q0 + i - token[u] * heads : 0;
-      raw[u].load(static_cast<const T*>(args.q.x) + (live ? row0 + token[u] : row0) * args.q.x_token + head[u] * args.q.x_head, l, live);
-    }
+      for (int u = 0; u < kAhead; ++u) raw[u].load(h + u < mine ? src + u * args.q.x_head : some, l);
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      float a[kPairs], b[kPairs];
-      raw[u].values(a, b);
-      if (args.norm) head_norm(l, a, b, lanes, inv_columns, args.eps, args.q.weight != nullptr ? weights[0] : nullptr);
-      if (token[u] >= 0) {
-        head_turn(l, a, b, turns + token[u] * pairs, pairs);
-        head_store(static_cast<T*>(args.q.y) + (row0 + token[u]) * args.q.y_token + head[u] * args.q.y_head, l, a, b);
+      for (int u = 0; u < kAhead; ++u) {
+        float x[kPairs], y[kPairs];
+        raw[u].template values<kNeighbours>(l, x, y);
+        turn.apply(x, y, args.norm ? head_norm(l, x, y, inv_columns, args.eps) : 1.0f);
+        if (h + u < mine) head_store<kNeighbours>(dst + u * args.q.y_head, l, x, y);
       }
+      src += kAhead * args.q.x_head;
+      dst += kAhead * args.q.y_head;
     }
   }
 }

@@ -33,17 +33,6 @@ __host__ __device__ constexpr int kv_rows_smem_bytes() {
   return 1024 + 6 * 128 * kD * 2 + kKvRowsMeta * 8 * 16 + 256;
 }
 
-__device__ __forceinline__ uint64_t pack_f32x2(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void fma_f32x2(float& x, float& y, uint64_t factor, uint64_t addend) {
-  uint64_t v = pack_f32x2(x, y);
-  asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(v) : "l"(factor), "l"(addend));
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
-}
-
 // [q of tile 0, of tile 1][keys, 2 stages][values, 2 stages][scales][barriers]: operands as blocks of 64 columns, 128 rows of 128
 // bytes each, swizzled.
 template <typename T, int kD>
@@ -230,7 +219,7 @@ __global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid
 #pragma unroll
             for (int i = 0; i < 16; i += 2) {
               float x = __uint_as_float(s[16 * g + i]), y = __uint_as_float(s[16 * g + i + 1]);
-              fma_f32x2(x, y, mul2, add2);
+              unpack_f32x2(fma_f32x2(pack_f32x2(x, y), mul2, add2), x, y);
               if (masked) {
                 const int col = 32 * c + 16 * g + i;
                 if (!(col >= from && col < to)) x = -INFINITY;
