@@ -137,13 +137,16 @@ void kv_append_checked(const TraceaKvCache& cache, const TraceaSequences& seqs, 
   const int lanes = vec ? head_lanes(k.cols) : 32;
   const int size = 1 << a.cache.page_shift;
   a.turn_rows = a.seqs.starts != nullptr ? size : 1;
+  a.turn_lanes = 1;
+  while (a.turn_lanes < a.rot.pairs) a.turn_lanes *= 2;
   DeviceGuard guard(dev);
   DeviceState& st = device_state(dev);
   // Pages that get tokens: one a sequence, and with n tokens at most ceil((n - 1) / P) more.
   const long long pages = a.seqs.starts != nullptr ? std::min(k.tokens, k.tokens / size + 2LL * a.seqs.count) : a.seqs.count;
-  // All heads of a page share its angles; where the pages are few the heads are split over CTAs all the same.
+  // All heads of a page share its angles; where the pages would leave a quarter of the machine's two CTAs an SM idle the heads are split
+  // over CTAs all the same.
   a.heads_per_cta = a.cache.heads;
-  while (a.heads_per_cta > 1 && pages * ceil_div(a.cache.heads, a.heads_per_cta) < 4LL * st.num_sms) a.heads_per_cta = (a.heads_per_cta + 1) / 2;
+  while (a.heads_per_cta > 1 && pages * ceil_div(a.cache.heads, a.heads_per_cta) < 3LL * st.num_sms / 2) a.heads_per_cta = (a.heads_per_cta + 1) / 2;
   const dim3 grid(grid_of(pages), static_cast<unsigned>(ceil_div(a.cache.heads, a.heads_per_cta)));
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int rows = a.seqs.starts == nullptr ? 1 : std::max(1, size * lanes / tb200::kHeadThreads);

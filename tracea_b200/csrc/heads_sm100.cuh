@@ -30,21 +30,31 @@ struct Rotation {
   int interleaved;             // pair i is columns 2i and 2i + 1; else i and i + pairs
 };
 
-// Cosine and sine of position * frequency. The angle is taken in turns and in 64 bits, and so are the quarter turns that are cut
-// off: fp32 would be off by 2^-24 of an angle that grows with the position.
-__device__ __forceinline__ float2 rotation_of(int position, double frequency) {
-  const double quarters = static_cast<double>(position) * frequency * 0.63661977236758134308;   // 2 / pi
-  const double whole = rint(quarters);
-  const int quadrant = static_cast<int>(static_cast<long long>(whole) & 3);
-  float s, c;
-  sincospif(0.5f * static_cast<float>(quarters - whole), &s, &c);
-  if (quadrant & 1) {
-    const float t = c;
-    c = -s;
-    s = t;
+// Cosine and sine of position * frequency. The angle is taken in turns and in 64 bits, and so are the quarter turns that are cut off:
+// fp32 would be off by 2^-24 of an angle that grows with the position. Of what is left, x within +-pi/4, the Taylor polynomials up to
+// x^9 and x^10, whose next terms are below 2^-29 and 2^-31.
+struct Angle {
+  double quarters;                      // a step's, in quarter turns
+  __device__ __forceinline__ explicit Angle(double frequency) : quarters(frequency * 0.63661977236758134308) {}   // 2 / pi
+  __device__ __forceinline__ void turn(double position, float& c, float& s) const {
+    constexpr double kWhole = 6755399441055744.0;        // 1.5 * 2^52: adding it leaves a whole number in the low bits
+    const double all = position * quarters, whole = all + kWhole;
+    const int quadrant = __double2loint(whole);
+    const float x = static_cast<float>(all - (whole - kWhole)) * 1.57079633f, z = x * x;
+    float sine = fmaf(z, 1.0f / 362880, -1.0f / 5040), cosine = fmaf(z, -1.0f / 3628800, 1.0f / 40320);
+    sine = fmaf(z, sine, 1.0f / 120);
+    cosine = fmaf(z, cosine, -1.0f / 720);
+    sine = fmaf(z, sine, -1.0f / 6);
+    cosine = fmaf(z, cosine, 1.0f / 24);
+    sine = fmaf(x * z, sine, x);
+    cosine = fmaf(z, cosine, -0.5f);
+    cosine = fmaf(z, cosine, 1.0f);
+    c = (quadrant & 1) ? sine : cosine;
+    s = (quadrant & 1) ? cosine : sine;
+    if ((quadrant + 1) & 2) c = -c;
+    if (quadrant & 2) s = -s;
   }
-  return (quadrant & 2) ? make_float2(-c, -s) : make_float2(c, s);
-}
+};
 
 // ------------------------------------------------------------------ a lane's columns of a row
 // A lane holds kPairs pairs (x, y) of columns, which a rotation turns into (x cos - y sin, y cos + x sin).
@@ -240,39 +250,42 @@ __device__ __forceinline__ void head_weights(const HeadLane<kLanes, kScalarPairs
     }
   }
 }
-// A lane's cosines and sines; `turns`: a token's, from pair 0 on, in shared memory.
+// A lane's cosines and sines; `turns`: a token's, those of all pairs and then these, in shared memory.
 template <int kLanes, int kScalarPairs>
-__device__ __forceinline__ void head_turns(const HeadLane<kLanes, kScalarPairs>& l, const float2* turns, int pairs,
-                                           float2 (&cs)[HeadLane<kLanes, kScalarPairs>::kPairs]) {
+__device__ __forceinline__ void head_turns(const HeadLane<kLanes, kScalarPairs>& l, const float* turns, int pairs,
+                                           float (&c)[HeadLane<kLanes, kScalarPairs>::kPairs], float (&s)[HeadLane<kLanes, kScalarPairs>::kPairs]) {
 #pragma unroll
-  for (int i = 0; i < HeadLane<kLanes, kScalarPairs>::kPairs; ++i) cs[i] = make_float2(1.0f, 0.0f);
+  for (int i = 0; i < HeadLane<kLanes, kScalarPairs>::kPairs; ++i) {
+    c[i] = 1.0f;
+    s[i] = 0.0f;
+  }
   if constexpr (kLanes > 0) {
     if (l.turned) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float4 v = *reinterpret_cast<const float4*>(turns + l.angle + 2 * i);
-        cs[2 * i] = make_float2(v.x, v.y);
-        cs[2 * i + 1] = make_float2(v.z, v.w);
-      }
+      load8(turns + l.angle, c);
+      load8(turns + pairs + l.angle, s);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < kScalarPairs; ++i)
-      if (l.angle + 32 * i < pairs) cs[i] = turns[l.angle + 32 * i];
+    for (int i = 0; i < kScalarPairs; ++i) {
+      if (l.angle + 32 * i < pairs) {
+        c[i] = turns[l.angle + 32 * i];
+        s[i] = turns[pairs + l.angle + 32 * i];
+      }
+    }
   }
 }
 // Weights and rotation together, for rows of one token: (x, y) -> factor (x xx + y xy, y yy + x yx), two pairs at a time.
 template <int kPairs>
 struct HeadTurn {
   uint64_t xx[kPairs / 2], xy[kPairs / 2], yy[kPairs / 2], yx[kPairs / 2];
-  __device__ __forceinline__ HeadTurn(const float (&wx)[kPairs], const float (&wy)[kPairs], const float2 (&cs)[kPairs]) {
+  __device__ __forceinline__ HeadTurn(const float (&wx)[kPairs], const float (&wy)[kPairs], const float (&c)[kPairs], const float (&s)[kPairs]) {
 #pragma unroll
     for (int i = 0; i < kPairs / 2; ++i) {
       const int a = 2 * i, b = 2 * i + 1;
-      xx[i] = pack_f32x2(wx[a] * cs[a].x, wx[b] * cs[b].x);
-      xy[i] = pack_f32x2(-wy[a] * cs[a].y, -wy[b] * cs[b].y);
-      yy[i] = pack_f32x2(wy[a] * cs[a].x, wy[b] * cs[b].x);
-      yx[i] = pack_f32x2(wx[a] * cs[a].y, wx[b] * cs[b].y);
+      xx[i] = pack_f32x2(wx[a] * c[a], wx[b] * c[b]);
+      xy[i] = pack_f32x2(-wy[a] * s[a], -wy[b] * s[b]);
+      yy[i] = pack_f32x2(wy[a] * c[a], wy[b] * c[b]);
+      yx[i] = pack_f32x2(wx[a] * s[a], wx[b] * s[b]);
     }
   }
   __device__ __forceinline__ void apply(float (&x)[kPairs], float (&y)[kPairs], float factor) const {
@@ -319,23 +332,23 @@ __global__ void __launch_bounds__(kHeadThreads, 3) head_rotate_kernel(const __gr
   using Lane = HeadLane<kLanes, 4>;
   constexpr int kPairs = Lane::kPairs, kRowLanes = head_row_lanes(kLanes), kHeads = 32 / kRowLanes, kAhead = 2;
   __shared__ __align__(16) float weights[2][kHeadMaxColumns];
-  __shared__ __align__(16) float2 turns[kHeadThreads / 32][kHeadMaxColumns / 2];
+  __shared__ __align__(16) float turns[kHeadThreads / 32][kHeadMaxColumns];
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long token = static_cast<long long>(blockIdx.x) * (kHeadThreads / 32) + warp;
   for (int r = 0; r < 2; ++r) weights_to_shared<T>(weights[r], args.rows[r].weight, args.rows[r].weight_f32, args.D);
   if (token < args.tokens && args.rot.pairs > 0) {
-    const int position = args.positions[token];
-    for (int p = lane; p < args.rot.pairs; p += 32) turns[warp][p] = rotation_of(position, args.rot.frequencies[p]);
+    const double position = args.positions[token];
+    for (int p = lane; p < args.rot.pairs; p += 32) Angle(args.rot.frequencies[p]).turn(position, turns[warp][p], turns[warp][args.rot.pairs + p]);
   }
   __syncthreads();
   if (token >= args.tokens) return;
   const int group = lane / kRowLanes;
   const Lane l(lane % kRowLanes, args.D, args.rot);
   const float inv_columns = 1.0f / static_cast<float>(args.D);
-  float2 cs[kPairs];
-  head_turns(l, turns[warp], args.rot.pairs, cs);
+  float c[kPairs], s[kPairs];
+  head_turns(l, turns[warp], args.rot.pairs, c, s);
   const int split_begin = args.passes * static_cast<int>(blockIdx.y) / static_cast<int>(gridDim.y);
   const int split_end = args.passes * static_cast<int>(blockIdx.y + 1) / static_cast<int>(gridDim.y);
   int before = 0;
@@ -348,7 +361,7 @@ __global__ void __launch_bounds__(kHeadThreads, 3) head_rotate_kernel(const __gr
     if (begin >= end) continue;
     float wx[kPairs], wy[kPairs];
     head_weights<kNeighbours>(l, args.norm && rows.weight != nullptr ? weights[which] : nullptr, wx, wy);
-    const HeadTurn<kPairs> turn(wx, wy, cs);
+    const HeadTurn<kPairs> turn(wx, wy, c, s);
     const int heads = rows.heads;
     const long long x_step = kHeads * rows.x_head, y_step = kHeads * rows.y_head;
     const T* src = static_cast<const T*>(rows.x) + token * rows.x_token + (begin * kHeads + group) * rows.x_head;
@@ -488,6 +501,7 @@ struct KvAppendArgs {
   int group;                   // heads of q to one of k
   int heads_per_cta;           // of k
   int turn_rows;               // rows of angles in shared memory
+  int turn_lanes;              // threads that compute a row of them: a power of two, at least its pairs
   float eps;
 };
 
@@ -500,7 +514,7 @@ __global__ void __launch_bounds__(kHeadThreads, kLanes > 0 && kRows <= 2 ? 2 : 1
   using Lane = HeadLane<kLanes, kScalarPairs>;
   using Raw = HeadRaw<T, kLanes, kScalarPairs>;
   constexpr int kPairs = Lane::kPairs, kWarps = kHeadThreads / 32, kRowLanes = head_row_lanes(kLanes), kRowsAtOnce = kHeadThreads / kRowLanes;
-  extern __shared__ __align__(16) float2 turns[];          // [turn_rows][pairs]
+  extern __shared__ __align__(16) float turns[];           // [turn_rows][2][pairs]: cosines, sines
   __shared__ __align__(16) float weights[2][kCacheMaxColumns];
   __shared__ float peaks[2][2][kWarps];                    // two heads in turn: one barrier a head
   ptx::griddep_launch_dependents();
@@ -523,9 +537,12 @@ __global__ void __launch_bounds__(kHeadThreads, kLanes > 0 && kRows <= 2 ? 2 : 1
   weights_to_shared<T>(weights[0], args.q.weight, args.q.weight_f32, D);
   weights_to_shared<T>(weights[1], args.k.weight, args.k.weight_f32, D);
   const int pairs = args.rot.pairs;
-  for (int i = threadIdx.x; i < count * pairs; i += kHeadThreads) {
-    const int r = i / pairs, p = i - r * pairs;
-    turns[i] = rotation_of(from + r, args.rot.frequencies[p]);
+  const int my_pair = static_cast<int>(threadIdx.x) & (args.turn_lanes - 1);
+  if (my_pair < pairs) {
+    const Angle angle(args.rot.frequencies[my_pair]);
+    const int step = kHeadThreads / args.turn_lanes;
+    for (int r = static_cast<int>(threadIdx.x) / args.turn_lanes; r < count; r += step)
+      angle.turn(from + r, turns[2 * r * pairs + my_pair], turns[(2 * r + 1) * pairs + my_pair]);
   }
   __syncthreads();
 
@@ -562,16 +579,19 @@ __global__ void __launch_bounds__(kHeadThreads, kLanes > 0 && kRows <= 2 ? 2 : 1
         float wx[kPairs], wy[kPairs];
         head_weights<kNeighbours>(l, args.norm && args.k.weight != nullptr ? weights[1] : nullptr, wx, wy);
         const float factor = args.norm ? head_norm(l, kx[i], ky[i], inv_columns, args.eps) : 1.0f;
-        float2 cs[kPairs];
-        head_turns(l, turns + (r < count ? r : 0) * pairs, pairs, cs);
+        float c[kPairs], s[kPairs];
+        head_turns(l, turns + 2 * (r < count ? r : 0) * pairs, pairs, c, s);
         float mk = 0.0f, mv = 0.0f;                        // NaN if there is one among them
 #pragma unroll
-        for (int j = 0; j < kPairs; ++j) {
-          const float x = kx[i][j] * (factor * wx[j]), y = ky[i][j] * (factor * wy[j]);
-          kx[i][j] = x * cs[j].x - y * cs[j].y;
-          ky[i][j] = y * cs[j].x + x * cs[j].y;
-          mk = max_nan(mk, max_nan(fabsf(kx[i][j]), fabsf(ky[i][j])));
+        for (int j = 0; j < kPairs; j += 2) {
+          const uint64_t f = pack_f32x2(factor, factor), co = pack_f32x2(c[j], c[j + 1]), si = pack_f32x2(s[j], s[j + 1]);
+          const uint64_t x = mul_f32x2(mul_f32x2(pack_f32x2(kx[i][j], kx[i][j + 1]), f), pack_f32x2(wx[j], wx[j + 1]));
+          const uint64_t y = mul_f32x2(mul_f32x2(pack_f32x2(ky[i][j], ky[i][j + 1]), f), pack_f32x2(wy[j], wy[j + 1]));
+          unpack_f32x2(fma_f32x2(y, pack_f32x2(-s[j], -s[j + 1]), mul_f32x2(x, co)), kx[i][j], kx[i][j + 1]);
+          unpack_f32x2(fma_f32x2(x, si, mul_f32x2(y, co)), ky[i][j], ky[i][j + 1]);
         }
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) mk = max_nan(mk, max_nan(fabsf(kx[i][j]), fabsf(ky[i][j])));
         float vx[kPairs], vy[kPairs];
         rv[i].template values<false>(plain, vx, vy);
 #pragma unroll
@@ -689,9 +709,9 @@ __global__ void __launch_bounds__(kHeadThreads, kLanes > 0 && kRows <= 2 ? 2 : 1
     const int from_head = share * turn_heads, mine = there ? min(turn_heads, heads - from_head) : 0;
     float wx[kPairs], wy[kPairs];
     head_weights<kNeighbours>(l, args.norm && args.q.weight != nullptr ? weights[0] : nullptr, wx, wy);
-    float2 cs[kPairs];
-    head_turns(l, turns + (there ? token : 0) * pairs, pairs, cs);
-    const HeadTurn<kPairs> turn(wx, wy, cs);
+    float c[kPairs], s[kPairs];
+    head_turns(l, turns + 2 * (there ? token : 0) * pairs, pairs, c, s);
+    const HeadTurn<kPairs> turn(wx, wy, c, s);
     const long long row = row0 + (there ? token : 0);
     const T* const some = static_cast<const T*>(args.q.x) + row * args.q.x_token + q0 * args.q.x_head;
     const T* src = some + from_head * args.q.x_head;
