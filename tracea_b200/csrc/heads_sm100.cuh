@@ -702,7 +702,7 @@ __global__ void __launch_bounds__(kHeadThreads, kLanes > 0 && kRows <= 2 ? 2 : 1
   // The queries that go with these heads: the lanes of a row take a few heads of a token in turn, with its rotation in registers.
   const int q0 = head0 * args.group, heads = (head1 - head0) * args.group;
   const int turn_heads = min(8, max(1, heads * count / kRowsAtOnce)), shares = (heads + turn_heads - 1) / turn_heads;
-  constexpr int kAhead = 2;
+  constexpr int kAhead = kRows > 1 ? 4 : 2;                // small pages and single tokens give a row's lanes few heads
   for (int base = 0; base < count * shares; base += kRowsAtOnce) {
     const int i = base + my_row, share = i % shares, token = i / shares;
     const bool there = token < count;
