@@ -34,6 +34,11 @@ __device__ __forceinline__ float exp2_ftz(float x) {
   asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x));
   return x;
 }
+__device__ __forceinline__ float max_3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 __device__ __forceinline__ uint32_t pack_halves(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));

@@ -49,7 +49,7 @@ __global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid
   float4* const meta = reinterpret_cast<float4*>(smem_gen + 6 * kOperand);      // {keys' scale, values' exponent, 2^-that, -} of 16 tokens
   const uint32_t bars = smem_base + 6 * kOperand + kKvRowsMeta * 8 * 16;
   auto bar = [&](int i) { return bars + 8u * i; };
-  constexpr int kQFull = 0, kSFull = 2, kPFull = 4, kOFull = 6, kKFull = 8, kKEmpty = 10, kVFull = 12, kVEmpty = 14, kMetaFull = 16, kDrain = 20;
+  constexpr int kQFull = 0, kSFull = 2, kPFull = 4, kOFull = 6, kKFull = 8, kKEmpty = 10, kVFull = 12, kVEmpty = 14, kMetaFull = 16, kDrain = 20, kPFirst = 21;
   volatile uint32_t* const tmem_slot_p = reinterpret_cast<volatile uint32_t*>(smem_gen + 6 * kOperand + kKvRowsMeta * 8 * 16 + 8 * 24);
   volatile uint32_t* const abort_p = tmem_slot_p + 1;
 
@@ -81,6 +81,7 @@ __global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid
       mbar_init(bar(kQFull + i), kKvRowsTile);
       mbar_init(bar(kSFull + i), 1);
       mbar_init(bar(kPFull + i), kKvRowsTile);
+      mbar_init(bar(kPFirst + i), kKvRowsTile);
       mbar_init(bar(kOFull + i), 1);
       mbar_init(bar(kKFull + i), 128);
       mbar_init(bar(kKEmpty + i), 1);
@@ -130,7 +131,7 @@ __global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid
       }
       float back;
       const float up = args.sign * row_scale(peak, back);
-      const float factor = back * args.scale_log2;
+      const float factor = fmaxf(back * args.scale_log2, 1.17549435e-38f);     // not 0: a score of -infinity stays one
 #pragma unroll
       for (int d = 0; d < kD; d += 8) {
         float v[8];
@@ -163,29 +164,25 @@ __global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid
         // columns of this step that the row sees
         const int from = lo - t0, to = min(hi, see_hi) - t0;
         const bool masked = __any_sync(0xffffffffu, from > 0 || to < kKvRowsTokens);
+        uint32_t s[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_tmem + 32 * c, s[c]);
+        tmem_ld_wait();
+        if (masked) {
+#pragma unroll
+          for (int i = 0; i < kKvRowsTokens; ++i)
+            if (i < from || i >= to) s[i / 32][i % 32] = __float_as_uint(-INFINITY);
+        }
         float top = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t s[2][32];
-          tmem_ld_32x32(s_tmem + 64 * c, s[0]);
-          tmem_ld_32x32(s_tmem + 64 * c + 32, s[1]);
-          tmem_ld_wait();
+        for (int g = 0; g < 8; ++g) {
+          const uint32_t* const v = s[g / 2] + 16 * (g % 2);
+          float gm = __uint_as_float(v[0]);
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const float4 sc = scales[4 * c + g];
-            float gm = -INFINITY;
-            if (masked) {
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const int col = 64 * c + 16 * g + i;
-                if (col >= from && col < to) gm = fmaxf(gm, __uint_as_float(s[g >> 1][16 * (g & 1) + i]));
-              }
-            } else {
-#pragma unroll
-              for (int i = 0; i < 16; ++i) gm = fmaxf(gm, __uint_as_float(s[g >> 1][16 * (g & 1) + i]));
-            }
-            top = fmaxf(top, gm * (factor * sc.x) + sc.y);
-          }
+          for (int i = 1; i + 1 < 16; i += 2) gm = max_3(gm, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+          gm = fmaxf(gm, __uint_as_float(v[15]));
+          const float4 sc = scales[g];
+          top = fmaxf(top, gm * (factor * sc.x) + sc.y);
         }
         if (__any_sync(0xffffffffu, top > m + kSlack)) {
           const float next = fmaxf(m, top);
@@ -193,50 +190,47 @@ __global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid
           m = next;
           l *= shrink;
           if (j > 0) {
-#pragma unroll
-            for (int c = 0; c < kD; c += 32) {
-              uint32_t o[32];
-              tmem_ld_32x32(o_tmem + c, o);
+#pragma unroll 1
+            for (int c = 0; c < kD; c += 16) {
+              uint32_t o[16];
+              tmem_ld_32x16(o_tmem + c, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * shrink);
-              tmem_st_32x32(o_tmem + c, o);
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * shrink);
+              tmem_st_32x16(o_tmem + c, o);
             }
           }
         }
         const float base = m == -INFINITY ? 0.0f : m;                // a row that has seen nothing
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          uint32_t s[32], p[16];
-          tmem_ld_32x32(s_tmem + 32 * c, s);
-          tmem_ld_wait();
+          uint32_t p[16];
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
             const float4 sc = scales[2 * c + g];
             const float mul = factor * sc.x, add = sc.y - base;
             const uint64_t mul2 = pack_f32x2(mul, mul), add2 = pack_f32x2(add, add);
-            float sum = 0.0f;
+            uint64_t sum = 0;
 #pragma unroll
             for (int i = 0; i < 16; i += 2) {
-              float x = __uint_as_float(s[16 * g + i]), y = __uint_as_float(s[16 * g + i + 1]);
-              unpack_f32x2(fma_f32x2(pack_f32x2(x, y), mul2, add2), x, y);
-              if (masked) {
-                const int col = 32 * c + 16 * g + i;
-                if (!(col >= from && col < to)) x = -INFINITY;
-                if (!(col + 1 >= from && col + 1 < to)) y = -INFINITY;
-              }
+              float x, y;
+              unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[c][16 * g + i]), __uint_as_float(s[c][16 * g + i + 1])), mul2, add2), x, y);
               x = exp2_ftz(x);
               y = exp2_ftz(y);
-              sum += x + y;
+              sum = add_f32x2(sum, pack_f32x2(x, y));
               p[8 * g + i / 2] = pack_halves(x, y);
             }
-            l += sum * sc.z;
+            float x, y;
+            unpack_f32x2(sum, x, y);
+            l += (x + y) * sc.z;
           }
           tmem_st_32x16(s_tmem + 16 * c, p);
+          if (c % 2 == 1) {                                          // half of the weights: the product may begin
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(bar((c == 1 ? kPFirst : kPFull) + tile));
+          }
         }
-        tmem_st_wait();
-        tc_fence_before();
-        mbar_arrive(bar(kPFull + tile));
       }
       // results
       if (ok && steps > 0) {
@@ -291,7 +285,7 @@ __global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid
       return id >= 0 && id < args.cache.pages ? id : -1;
     };
     auto load_scales = [&] {
-      scale = make_float4(0.0f, -INFINITY, 0.0f, 0.0f);              // of a page that is not there: weights of 0
+      scale = make_float4(1.0f, -INFINITY, 0.0f, 0.0f);              // of a page that is not there: weights of 0
       if (w == 0 && ids >= 0) {
         const long long block = static_cast<long long>(ids) * args.cache.heads + head;
         const int ek = static_cast<int>(args.cache.k_scales[block]) - 127, ev = static_cast<int>(args.cache.v_scales[block]) - 127;
@@ -394,13 +388,17 @@ __global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid
       const uint32_t parity = (j >> 1) & 1, next_parity = ((j + 1) >> 1) & 1;
       for (int tile = 0; tile < tiles; ++tile) {
         if (tile == 0 && !wait(kVFull + slot, parity, j)) break;
-        if (!wait(kPFull + tile, j & 1, j)) break;
-        tc_fence_after();
         // v^ as it lies, its columns contiguous: 64 of them a block (the leading-dimension offset), 16 tokens 2048 bytes
         const uint32_t b = ((v_smem + slot * kOperand) >> 4) | ((kBlock >> 4) << 16);
 #pragma unroll
-        for (int k = 0; k < kKvRowsTokens / 16; ++k)
-          mma_tmem_a_if(issue, tmem + 256 + tile * 128, tmem + tile * 128 + 8 * k, b + 128 * k, kDescHi, kIdescO, j > 0 || k > 0 ? 1u : 0u);
+        for (int half = 0; half < 2; ++half) {
+          if (!wait((half == 0 ? kPFirst : kPFull) + tile, j & 1, j)) break;
+          tc_fence_after();
+#pragma unroll
+          for (int k = 4 * half; k < 4 * half + 4; ++k)
+            mma_tmem_a_if(issue, tmem + 256 + tile * 128, tmem + tile * 128 + 8 * k, b + 128 * k, kDescHi, kIdescO, j > 0 || k > 0 ? 1u : 0u);
+        }
+        if (!ok) break;
         if (j + 1 < steps) {
           if (tile == 0 && !wait(kKFull + next, next_parity, j)) break;
           tc_fence_after();
