@@ -5,15 +5,19 @@
 //
 //   S = q k^^T   128 x 128, q and k^ from shared memory        O += P v^   128 x D, P from tensor memory, v^ from shared memory
 //
-// Bound by the matrix instructions, 4 rows tokens D operations, and as much by the exponentials, of which an SM does 16 a cycle: two
-// tiles of 128 tokens take 2048 cycles of either at D = 128. So the tiles alternate: while one's softmax runs, the other's products
-// do. The elements of the cache are widened from e4m3 to halves, exactly, by warps of their own, once for both tiles; a row of q is a
-// thread's, scaled into halves on the way in. The weights P lie over the scores' columns, as halves. The pages' scales are applied to
-// scores and weights (kv_attention_sm100.cuh).
+// 4 rows tokens D operations, and an exponential for every row and token, of which an SM does 16 a cycle: two tiles of 128 tokens take
+// 2048 cycles of either at D = 128. What holds both up is shared memory: of its 128 bytes a cycle the operands of the products take 192 KB
+// a step and the widened keys and values 64 KB, 2048 cycles as well. So everything has to run beside everything else: the tiles alternate,
+// each with a warp of its own that issues its products; the elements of the cache are widened from e4m3 to halves, exactly, by warps of
+// their own, once for both tiles, whose loads are a step ahead; a row of q, scaled into halves on the way in, is a thread's. The weights P
+// lie over the scores' columns, as halves. The pages' scales are applied to scores and weights (kv_attention_sm100.cuh).
 //
-// Tensor memory: 2 x 128 columns of scores (and weights), 2 x 128 of results: all 512. Per step of 128 tokens and tile the issuer's
-// order is O += P v^, then the next S over the same P: an S that is complete says that the product in front of it is, and so that O may
-// be rescaled.
+// Tensor memory, all 512 columns: 128 of results a tile, and 128 of scores, as two buffers for 64 tokens each. A softmax goes from one
+// buffer to the other: while it works on 64 tokens, the product of the 64 in front is formed and then the scores of the next but one, over
+// these weights.
+//
+// A prompt of 8192 tokens, 32 heads to 8, D = 128: 540 us, 1.02 PFLOP/s (what the mask leaves counted); 395 without a softmax, of which 85
+// are the CTAs' beginnings and ends; the widening costs nothing beside it.
 #pragma once
 #include "kv_attention_sm100.cuh"
 
@@ -21,11 +25,11 @@ namespace tb200 {
 
 constexpr int kKvRowsTile = 128, kKvRowsTokens = 128;
 constexpr int kKvRowsOfCta = 2 * kKvRowsTile;
-constexpr int kKvRowsThreads = 512;            // warps 0..3 and 4..7 softmax of the two tiles, 8..11 widen, 12 issues the products
+constexpr int kKvRowsThreads = 512;            // warps 0..3 and 4..7 softmax of the two tiles, 8..11 widen, 12 and 13 issue the products
 constexpr int kKvRowsSoftmaxRegs = 176, kKvRowsWidenRegs = 104, kKvRowsMmaRegs = 56;
 static_assert(2 * kKvRowsSoftmaxRegs + kKvRowsWidenRegs + kKvRowsMmaRegs <= 4 * 128, "what the block is launched with, 128 a thread");
 constexpr int kKvRowsWidenWarp = 8, kKvRowsMmaWarp = 12;
-constexpr int kKvRowsMeta = 4;                 // steps whose scales are kept: a softmax is at most two steps behind the widening warps
+constexpr int kKvRowsMeta = 4;                 // steps whose scales are kept: a softmax is at most three steps behind the widening warps
 
 template <int kD>
 __host__ __device__ constexpr int kv_rows_smem_bytes() {
@@ -41,15 +45,16 @@ __global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid
   constexpr uint32_t kOperand = 128u * kD * 2u, kBlock = 128u * 128u;
   constexpr int kBlocks = kD / 64;
   constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);          // 8-row groups 1024 bytes apart, 128-byte swizzle
-  constexpr uint32_t kIdescS = make_idesc(0, 128, 128), kIdescO = make_idesc(0, 128, kD, 1);
+  constexpr uint32_t kIdescS = make_idesc(0, 128, 64), kIdescO = make_idesc(0, 128, kD, 1);
   extern __shared__ uint8_t smem_raw[];
+  __shared__ float row_factor[kKvRowsOfCta];
   const uint32_t smem_base = __shfl_sync(0xffffffffu, (smem_u32(smem_raw) + 1023u) & ~1023u, 0);
   uint8_t* const smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
   const uint32_t q_smem = smem_base, k_smem = smem_base + 2 * kOperand, v_smem = smem_base + 4 * kOperand;
   float4* const meta = reinterpret_cast<float4*>(smem_gen + 6 * kOperand);      // {keys' scale, values' exponent, 2^-that, -} of 16 tokens
   const uint32_t bars = smem_base + 6 * kOperand + kKvRowsMeta * 8 * 16;
   auto bar = [&](int i) { return bars + 8u * i; };
-  constexpr int kQFull = 0, kSFull = 2, kPFull = 4, kOFull = 6, kKFull = 8, kKEmpty = 10, kVFull = 12, kVEmpty = 14, kMetaFull = 16, kDrain = 20, kPFirst = 21;
+  constexpr int kQFull = 0, kSFull = 2, kPFull = 6, kKFull = 10, kKEmpty = 12, kVFull = 14, kVEmpty = 16, kMetaFull = 18, kDrain = 22;   // S, P: 2 tile + buffer
   volatile uint32_t* const tmem_slot_p = reinterpret_cast<volatile uint32_t*>(smem_gen + 6 * kOperand + kKvRowsMeta * 8 * 16 + 8 * 24);
   volatile uint32_t* const abort_p = tmem_slot_p + 1;
 
@@ -77,19 +82,20 @@ __global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid
   const int steps = max(0, (see_hi + kKvRowsTokens - 1) / kKvRowsTokens - step_lo);
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(bar(kQFull + i), kKvRowsTile);
+    for (int i = 0; i < 4; ++i) {
       mbar_init(bar(kSFull + i), 1);
       mbar_init(bar(kPFull + i), kKvRowsTile);
-      mbar_init(bar(kPFirst + i), kKvRowsTile);
-      mbar_init(bar(kOFull + i), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(kQFull + i), kKvRowsTile);
       mbar_init(bar(kKFull + i), 128);
-      mbar_init(bar(kKEmpty + i), 1);
+      mbar_init(bar(kKEmpty + i), tiles);
       mbar_init(bar(kVFull + i), 128);
-      mbar_init(bar(kVEmpty + i), 1);
+      mbar_init(bar(kVEmpty + i), tiles);
     }
     for (int i = 0; i < kKvRowsMeta; ++i) mbar_init(bar(kMetaFull + i), 1);
     mbar_init(bar(kDrain), 1);
+    mbar_init(bar(kDrain + 1), 1);
     *abort_p = 0u;
     fence_mbar_init();
   }
@@ -109,37 +115,43 @@ __global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid
     if (tile < tiles) {
       const bool live = my_row < rows;
       const int token = live ? (first_row + my_row) / group : 0, q_head = head * group + (live ? (first_row + my_row) % group : 0);
-      // q into halves, 64 columns at a time. The row is read twice: its largest value is needed first.
-      const T* const qp = static_cast<const T*>(args.q) + static_cast<long long>(at.first_row + token) * args.q_token + q_head * args.q_head;
-      auto read8 = [&](int d, float(&v)[8]) {
-        if (!live || d >= D) {
+      // q into halves: kD / 8 lanes a row, eight columns each, all of the warp's rows' loads under way together
+      constexpr int kRowLanes = kD / 8, kRowsAtOnce = 32 / kRowLanes, kLoads = 32 / kRowsAtOnce;
+      const int col = 8 * (lane % kRowLanes);
+      const T* const q0 = static_cast<const T*>(args.q) + static_cast<long long>(at.first_row) * args.q_token + head * group * args.q_head;
+      Vec8<T> raw[kLoads];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-        } else if (args.q_vec) {
-          load8(qp + d, v);
+      for (int i = 0; i < kLoads; ++i) {
+        const int row = first_row + min(tile * kKvRowsTile + (warp & 3) * 32 + i * kRowsAtOnce + lane / kRowLanes, rows - 1);
+        const T* const p = q0 + static_cast<long long>(row / group) * args.q_token + (row % group) * args.q_head + (col < D ? col : 0);
+        if (args.q_vec) {
+          fetch8(p, raw[i]);
         } else {
-          load8_upto(qp + d, 1, 8, v);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) reinterpret_cast<T*>(&raw[i])[k] = p[k];
         }
-      };
-      float peak = 0.0f;
-#pragma unroll
-      for (int d = 0; d < kD; d += 8) {
-        float v[8];
-        read8(d, v);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) peak = fmaxf(peak, fabsf(v[i]));
       }
-      float back;
-      const float up = args.sign * row_scale(peak, back);
-      const float factor = fmaxf(back * args.scale_log2, 1.17549435e-38f);     // not 0: a score of -infinity stays one
 #pragma unroll
-      for (int d = 0; d < kD; d += 8) {
-        float v[8];
-        read8(d, v);
-        st_shared_v4(q_smem + tile * kOperand + (d / 64) * kBlock + r * 128 + ((((d % 64) / 8) ^ (r & 7)) * 16),
+      for (int i = 0; i < kLoads; ++i) {
+        const int in_warp = i * kRowsAtOnce + lane / kRowLanes, in_tile = (warp & 3) * 32 + in_warp;
+        float v[8], peak = 0.0f;
+        widen8(raw[i], v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if (col >= D || tile * kKvRowsTile + in_tile >= rows) v[k] = 0.0f;
+          peak = fmaxf(peak, fabsf(v[k]));
+        }
+#pragma unroll
+        for (int o = kRowLanes / 2; o > 0; o >>= 1) peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, o));
+        float back;
+        const float up = args.sign * row_scale(peak, back);
+        if (lane % kRowLanes == 0) row_factor[tile * kKvRowsTile + in_tile] = back * args.scale_log2;
+        st_shared_v4(q_smem + tile * kOperand + (col / 64) * kBlock + in_tile * 128 + ((((col % 64) / 8) ^ (in_tile & 7)) * 16),
                      make_uint4(pack_halves(v[0] * up, v[1] * up), pack_halves(v[2] * up, v[3] * up), pack_halves(v[4] * up, v[5] * up),
                                 pack_halves(v[6] * up, v[7] * up)));
       }
+      __syncwarp();
+      const float factor = fmaxf(row_factor[my_row], 1.17549435e-38f);          // not 0: a score of -infinity stays one
       fence_proxy_async_smem();
       mbar_arrive(bar(kQFull + tile));
 
@@ -150,32 +162,41 @@ __global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid
       const uint32_t s_tmem = tmem + lanes + tile * 128, o_tmem = tmem + lanes + 256 + tile * 128;
       float m = -INFINITY, l = 0.0f;
       bool ok = true;
-      for (int j = 0; j < steps; ++j) {
-        const int t0 = (step_lo + j) * kKvRowsTokens;
-        const float4* const scales = meta + (j % kKvRowsMeta) * 8;
-        ok = mbar_wait_bounded(bar(kMetaFull + j % kKvRowsMeta), (j / kKvRowsMeta) & 1, abort_p, args.wait_limit) &&
-             mbar_wait_bounded(bar(kSFull + tile), j & 1, abort_p, args.wait_limit);
+      auto wait_scores = [&](int h) {                                // of half step h; it says too that the product of h - 2 is complete
+        ok = mbar_wait_bounded(bar(kSFull + 2 * tile + (h & 1)), (h >> 1) & 1, abort_p, args.wait_limit);
         if (__any_sync(0xffffffffu, !ok)) {
-          if (lane == 0) report_error_status(args.status, abort_p, kErrEpilogueWait, static_cast<uint32_t>(j));
+          if (lane == 0) report_error_status(args.status, abort_p, kErrEpilogueWait, static_cast<uint32_t>(h));
+          ok = false;
+        }
+        tc_fence_after();
+        return ok;
+      };
+      for (int h = 0; h < 2 * steps; ++h) {
+        const int j = h >> 1, t0 = (step_lo + j) * kKvRowsTokens + 64 * (h & 1);
+        const uint32_t buffer = s_tmem + 64 * (h & 1);
+        const float4* const scales = meta + (j % kKvRowsMeta) * 8 + 4 * (h & 1);
+        if (!wait_scores(h)) break;
+        uint32_t s[2][32];
+        tmem_ld_32x32(buffer, s[0]);
+        tmem_ld_32x32(buffer + 32, s[1]);
+        // columns that the row sees
+        const int from = lo - t0, to = min(hi, see_hi) - t0;
+        const bool masked = __any_sync(0xffffffffu, from > 0 || to < 64);
+        ok = mbar_wait_bounded(bar(kMetaFull + j % kKvRowsMeta), (j / kKvRowsMeta) & 1, abort_p, args.wait_limit);
+        if (__any_sync(0xffffffffu, !ok)) {
+          if (lane == 0) report_error_status(args.status, abort_p, kErrEpilogueWait, static_cast<uint32_t>(h));
           ok = false;
           break;
         }
-        tc_fence_after();
-        // columns of this step that the row sees
-        const int from = lo - t0, to = min(hi, see_hi) - t0;
-        const bool masked = __any_sync(0xffffffffu, from > 0 || to < kKvRowsTokens);
-        uint32_t s[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_tmem + 32 * c, s[c]);
         tmem_ld_wait();
         if (masked) {
 #pragma unroll
-          for (int i = 0; i < kKvRowsTokens; ++i)
+          for (int i = 0; i < 64; ++i)
             if (i < from || i >= to) s[i / 32][i % 32] = __float_as_uint(-INFINITY);
         }
         float top = -INFINITY;
 #pragma unroll
-        for (int g = 0; g < 8; ++g) {
+        for (int g = 0; g < 4; ++g) {
           const uint32_t* const v = s[g / 2] + 16 * (g % 2);
           float gm = __uint_as_float(v[0]);
 #pragma unroll
@@ -189,7 +210,8 @@ __global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid
           const float shrink = next == m ? 1.0f : exp2_ftz(m - next);
           m = next;
           l *= shrink;
-          if (j > 0) {
+          if (h > 0) {
+            if (!wait_scores(h + 1)) break;                          // the product of h - 1 is complete
 #pragma unroll 1
             for (int c = 0; c < kD; c += 16) {
               uint32_t o[16];
@@ -203,7 +225,7 @@ __global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid
         }
         const float base = m == -INFINITY ? 0.0f : m;                // a row that has seen nothing
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 2; ++c) {
           uint32_t p[16];
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
@@ -224,22 +246,14 @@ __global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid
             unpack_f32x2(sum, x, y);
             l += (x + y) * sc.z;
           }
-          tmem_st_32x16(s_tmem + 16 * c, p);
-          if (c % 2 == 1) {                                          // half of the weights: the product may begin
-            tmem_st_wait();
-            tc_fence_before();
-            mbar_arrive(bar((c == 1 ? kPFirst : kPFull) + tile));
-          }
+          tmem_st_32x16(buffer + 16 * c, p);
         }
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(bar(kPFull + 2 * tile + (h & 1)));
       }
       // results
-      if (ok && steps > 0) {
-        ok = mbar_wait_bounded(bar(kOFull + tile), 0, abort_p, args.wait_limit);
-        if (__any_sync(0xffffffffu, !ok)) {
-          if (lane == 0) report_error_status(args.status, abort_p, kErrEpilogueWait, 0xffffu);
-          ok = false;
-        }
-      }
+      if (ok && steps > 0) wait_scores(2 * steps + 1);               // the last product is complete
       if (ok) {
         tc_fence_after();
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -276,28 +290,37 @@ __global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid
     const long long page_bytes = (static_cast<long long>(args.cache.heads) << shift) * D;
     const long long head_bytes = (static_cast<long long>(head) << shift) * D;
     uint4 kr[kLoads], vr[kLoads];
+    // Places and scales are loaded steps ahead and looked at only when they are needed: what looks at a load waits for it.
     int ids = -1, next_ids = -1;                                     // of lane i < 8: page of tokens 16 i .. of a step
-    float4 scale;
+    uint32_t k_byte = 0, v_byte = 0;                                 // its scales
     auto load_ids = [&](int j) {
       const int token = (step_lo + j) * kKvRowsTokens + 16 * (lane & 7);
-      int id = -1;
-      if (j < steps && token < see_hi) id = args.seqs.table[at.sequence * args.seqs.table_stride + (token >> shift)];
-      return id >= 0 && id < args.cache.pages ? id : -1;
+      return j < steps && token < see_hi ? args.seqs.table[at.sequence * args.seqs.table_stride + (token >> shift)] : -1;
     };
+    auto there = [&](int id) { return id >= 0 && id < args.cache.pages; };
     auto load_scales = [&] {
-      scale = make_float4(1.0f, -INFINITY, 0.0f, 0.0f);              // of a page that is not there: weights of 0
-      if (w == 0 && ids >= 0) {
+      if (w == 0 && there(ids)) {
         const long long block = static_cast<long long>(ids) * args.cache.heads + head;
-        const int ek = static_cast<int>(args.cache.k_scales[block]) - 127, ev = static_cast<int>(args.cache.v_scales[block]) - 127;
+        k_byte = args.cache.k_scales[block];
+        v_byte = args.cache.v_scales[block];
+      }
+    };
+    auto put_scales = [&](int j) {
+      float4 scale = make_float4(1.0f, -INFINITY, 0.0f, 0.0f);       // of a page that is not there: weights of 0
+      if (there(ids)) {
+        const int ek = static_cast<int>(k_byte) - 127, ev = static_cast<int>(v_byte) - 127;
         scale = make_float4(power_of_two(ek), static_cast<float>(ev), power_of_two(-ev), 0.0f);
       }
+      if (lane < 8) meta[(j % kKvRowsMeta) * 8 + lane] = scale;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(kMetaFull + j % kKvRowsMeta));
     };
     auto fetch = [&](const uint8_t* from, int j, uint4(&raw)[kLoads]) {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const int row = kRowsOfLoad * i + my_row, token = (step_lo + j) * kKvRowsTokens + row;
         const int id = __shfl_sync(0xffffffffu, ids, row >> 4);
-        const bool here = id >= 0 && my_col < D && token < see_hi && token >= see_lo;
+        const bool here = there(id) && my_col < D && token < see_hi && token >= see_lo;
         raw[i] = make_uint4(0u, 0u, 0u, 0u);
         if (here)
           raw[i] = *reinterpret_cast<const uint4*>(from + id * page_bytes + head_bytes +
@@ -322,101 +345,95 @@ __global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid
     ids = load_ids(0);
     next_ids = load_ids(1);
     load_scales();
-    fetch(args.cache.k, 0, kr);
     fetch(args.cache.v, 0, vr);
-    for (int j = 0; j < steps; ++j) {
-      if (j == args.test_producer_stop) break;                       // test hook: go silent, leave normally
-      const int slot = j & 1;
-      const uint32_t free_parity = ((j >> 1) & 1) ^ 1;
-      if (j >= 2 && !mbar_wait_bounded(bar(kKEmpty + slot), free_parity, abort_p, args.wait_limit)) {
+    fetch(args.cache.k, 0, kr);
+    bool ok = true;
+    auto wait = [&](int b, int j) {                                  // for slot j % 2 to be free of step j - 2
+      if (j >= 2 && !mbar_wait_bounded(bar(b + (j & 1)), ((j >> 1) & 1) ^ 1, abort_p, args.wait_limit)) {
         report_error_status(args.status, abort_p, kErrProducerWait, static_cast<uint32_t>(j));
-        break;
+        ok = false;
       }
-      if (w == 0) {
-        if (lane < 8) meta[(j % kKvRowsMeta) * 8 + lane] = scale;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(kMetaFull + j % kKvRowsMeta));
+      return ok;
+    };
+    // keys, and the scales, a step ahead of the values: ids and scale are those of keys' step j
+    for (int j = 0; j <= steps && ok; ++j) {
+      if (j == args.test_producer_stop) break;                       // test hook: go silent, leave normally
+      if (j < steps) {
+        if (!wait(kKEmpty, j)) break;
+        if (w == 0) put_scales(j);
+        widen(k_smem + (j & 1) * kOperand, kr);
+        fence_proxy_async_smem();
+        mbar_arrive(bar(kKFull + (j & 1)));
       }
-      widen(k_smem + slot * kOperand, kr);
-      fence_proxy_async_smem();
-      mbar_arrive(bar(kKFull + slot));
+      if (j > 0) {
+        if (!wait(kVEmpty, j - 1)) break;
+        widen(v_smem + ((j - 1) & 1) * kOperand, vr);
+        fence_proxy_async_smem();
+        mbar_arrive(bar(kVFull + ((j - 1) & 1)));
+        if (j < steps) fetch(args.cache.v, j, vr);
+      }
       ids = next_ids;
       if (j + 1 < steps) {
         load_scales();
         fetch(args.cache.k, j + 1, kr);
       }
       next_ids = load_ids(j + 2);
-      if (j >= 2 && !mbar_wait_bounded(bar(kVEmpty + slot), free_parity, abort_p, args.wait_limit)) {
-        report_error_status(args.status, abort_p, kErrProducerWait, static_cast<uint32_t>(j));
-        break;
-      }
-      widen(v_smem + slot * kOperand, vr);
-      fence_proxy_async_smem();
-      mbar_arrive(bar(kVFull + slot));
-      if (j + 1 < steps) fetch(args.cache.v, j + 1, vr);
     }
     __syncwarp();
   } else {
     regs_down<kKvRowsMmaRegs>();
   }
-  if (warp == kKvRowsMmaWarp) {
-    // ------------------------------------------------------------ the products (uniform control flow, one lane issues)
+  if (warp >= kKvRowsMmaWarp && warp < kKvRowsMmaWarp + tiles) {
+    // ------------------------------------------------------------ a tile's products (uniform control flow, one lane issues)
     const uint32_t issue = elect_one_lane();
+    const int tile = warp - kKvRowsMmaWarp;
     bool ok = true;
     auto wait = [&](int b, uint32_t parity, int j) {
       ok = ok && mbar_wait_bounded_uniform(bar(b), parity, abort_p, args.wait_limit);
       if (!ok && issue) report_error_status(args.status, abort_p, kErrMmaWaitFull, static_cast<uint32_t>(j));
       return ok;
     };
-    auto scores = [&](int tile, int slot) {
-      const uint32_t a = (q_smem + tile * kOperand) >> 4, b = (k_smem + slot * kOperand) >> 4;
-      mma_step4<false, false>(tmem + tile * 128, a, a + 2, a + 4, a + 6, b, b + 2, b + 4, b + 6, kDescHi, kIdescS, issue);
+    // scores of half step h: 64 of the step's 128 rows of keys
+    auto scores = [&](int h) {
+      const uint32_t a = (q_smem + tile * kOperand) >> 4, b = (k_smem + ((h >> 1) & 1) * kOperand + (h & 1) * (64 * 128)) >> 4;
+      const uint32_t d = tmem + tile * 128 + 64 * (h & 1);
+      mma_step4<false, false>(d, a, a + 2, a + 4, a + 6, b, b + 2, b + 4, b + 6, kDescHi, kIdescS, issue);
       if constexpr (kBlocks == 2) {
         const uint32_t a1 = a + (kBlock >> 4), b1 = b + (kBlock >> 4);
-        mma_step4<false, true>(tmem + tile * 128, a1, a1 + 2, a1 + 4, a1 + 6, b1, b1 + 2, b1 + 4, b1 + 6, kDescHi, kIdescS, issue);
+        mma_step4<false, true>(d, a1, a1 + 2, a1 + 4, a1 + 6, b1, b1 + 2, b1 + 4, b1 + 6, kDescHi, kIdescS, issue);
       }
-      tcgen05_commit_if<false>(issue, bar(kSFull + tile));
     };
-    for (int tile = 0; tile < tiles && steps > 0; ++tile) {
-      if (!wait(kQFull + tile, 0, 0) || (tile == 0 && !wait(kKFull, 0, 0))) break;
+    if (steps > 0 && wait(kQFull + tile, 0, 0) && wait(kKFull, 0, 0)) {
       tc_fence_after();
-      scores(tile, 0);
-    }
-    if (ok && steps > 0) tcgen05_commit_if<false>(issue, bar(kKEmpty));
-    for (int j = 0; j < steps && ok; ++j) {
-      const int slot = j & 1, next = slot ^ 1;
-      const uint32_t parity = (j >> 1) & 1, next_parity = ((j + 1) >> 1) & 1;
-      for (int tile = 0; tile < tiles; ++tile) {
-        if (tile == 0 && !wait(kVFull + slot, parity, j)) break;
-        // v^ as it lies, its columns contiguous: 64 of them a block (the leading-dimension offset), 16 tokens 2048 bytes
-        const uint32_t b = ((v_smem + slot * kOperand) >> 4) | ((kBlock >> 4) << 16);
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          if (!wait((half == 0 ? kPFirst : kPFull) + tile, j & 1, j)) break;
-          tc_fence_after();
-#pragma unroll
-          for (int k = 4 * half; k < 4 * half + 4; ++k)
-            mma_tmem_a_if(issue, tmem + 256 + tile * 128, tmem + tile * 128 + 8 * k, b + 128 * k, kDescHi, kIdescO, j > 0 || k > 0 ? 1u : 0u);
-        }
-        if (!ok) break;
-        if (j + 1 < steps) {
-          if (tile == 0 && !wait(kKFull + next, next_parity, j)) break;
-          tc_fence_after();
-          scores(tile, next);
-        } else {
-          tcgen05_commit_if<false>(issue, bar(kOFull + tile));
-        }
+      for (int h = 0; h < 2; ++h) {
+        scores(h);
+        tcgen05_commit_if<false>(issue, bar(kSFull + 2 * tile + h));
       }
-      if (ok) {
+      tcgen05_commit_if<false>(issue, bar(kKEmpty));
+    }
+    for (int h = 0; h < 2 * steps && ok; ++h) {
+      const int j = h >> 1, slot = j & 1, next = slot ^ 1;
+      if (h % 2 == 0 && !wait(kVFull + slot, (j >> 1) & 1, j)) break;
+      if (h % 2 == 0 && j + 1 < steps && !wait(kKFull + next, ((j + 1) >> 1) & 1, j)) break;
+      if (!wait(kPFull + 2 * tile + (h & 1), j & 1, j)) break;
+      tc_fence_after();
+      // v^ as it lies, its columns contiguous: 64 of them a block (the leading-dimension offset), 16 tokens 2048 bytes
+      const uint32_t b = ((v_smem + slot * kOperand + (h & 1) * (64 * 128)) >> 4) | ((kBlock >> 4) << 16);
+      const uint32_t p = tmem + tile * 128 + 64 * (h & 1);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) mma_tmem_a_if(issue, tmem + 256 + tile * 128, p + 8 * k, b + 128 * k, kDescHi, kIdescO, h > 0 || k > 0 ? 1u : 0u);
+      if (h + 2 < 2 * steps) scores(h + 2);
+      tcgen05_commit_if<false>(issue, bar(kSFull + 2 * tile + (h & 1)));         // scores of h + 2, or that there are none
+      if (h % 2 == 1) {
         tcgen05_commit_if<false>(issue, bar(kVEmpty + slot));
         if (j + 1 < steps) tcgen05_commit_if<false>(issue, bar(kKEmpty + next));
       }
     }
     // never leave with products under way
-    tcgen05_commit_if<false>(issue, bar(kDrain));
+    tcgen05_commit_if<false>(issue, bar(kDrain + tile));
     __syncwarp();
     const long long t0 = clock64();
-    while (!mbar_try_wait(bar(kDrain), 0) && clock64() - t0 < args.wait_limit) {}
+    while (!mbar_try_wait(bar(kDrain + tile), 0) && clock64() - t0 < args.wait_limit) {}
     __syncwarp();
   }
   tc_fence_before();
