@@ -7,9 +7,6 @@ namespace {
 
 using namespace tb200_host;
 
-// Sequences of up to so many tokens are split over a cluster's CTAs, if that fills no more than the machine; one launch.
-constexpr long long kSharedTokens = 4096;
-
 template <typename Kernel>
 void allow_smem(Kernel kern, std::atomic<bool> (&done)[kMaxDevices], int dev, int bytes) {
   if (done[dev].load(std::memory_order_relaxed)) return;
@@ -27,13 +24,20 @@ void launch_tokens(tb200::KvTokensArgs& c, DeviceState& st, int dev, cudaStream_
   // The tokens that a sequence may have, as far as the host knows.
   long long most = static_cast<long long>(a.seqs.table_width) << a.cache.page_shift;
   if (a.window > 0) most = std::min<long long>(most, a.window + 16LL * tb200::kKvTokenTiles);
-  if (pairs * 8 <= slots && most <= kSharedTokens && heads <= 65535) {
+  // A cluster of up to eight CTAs to a sequence and head, more of them while they fill no more than the machine or have more than 2048
+  // tokens each; or one line of all steps, which costs a second launch and looks at all lengths first, 6 us in all, but splits a lone long
+  // sequence over every SM. us, cluster / line, for sequences x tokens (8 heads of keys, 32 of q, 128 columns): 1 x 300 5.6 / 12.4,
+  // 1 x 4000 9.3 / 13.4, 1 x 16000 20.7 / 17.5, 16 x 1000 10.7 / 17.4, 16 x 4000 27 / 33, 64 x 1000 27 / 35, 64 x 0..8191 90 / 95,
+  // 2 x 131000 208 / 84.
+  int splits = 1;
+  while (splits < 8 && splits * 16LL * tb200::kKvTokenWarps < most && (pairs * splits * 2 <= slots || most > 2048LL * splits)) splits *= 2;
+  const bool shared = most <= (2 * pairs * splits >= slots ? 2048LL : 1024LL) * splits && heads <= 65535;
+  if (shared) {
     auto kern = tb200::kv_tokens_kernel<T, kRows, kD, kExact, tb200::kShared>;
     allow_smem(kern, done[0], dev, kSmem);
-    c.splits = 8;
-    while (c.splits > 1 && c.splits * 16 * tb200::kKvTokenWarps >= 2 * most) c.splits /= 2;     // a step for every other warp at least
-    launch(kern, dim3(grid_of(static_cast<long long>(a.seqs.count) * c.splits), static_cast<unsigned>(heads)), tb200::kKvTokenThreads, kSmem,
-           c.splits, kLaunchKvTokens, stream, c);
+    c.splits = splits;
+    launch(kern, dim3(grid_of(static_cast<long long>(a.seqs.count) * splits), static_cast<unsigned>(heads)), tb200::kKvTokenThreads, kSmem, splits,
+           kLaunchKvTokens, stream, c);
     return;
   }
   auto kern = tb200::kv_tokens_kernel<T, kRows, kD, kExact, tb200::kFlat>;
