@@ -1,6 +1,6 @@
 """torch.nn front end of the conv path: the reference's `TraceaConv2d` / `patch_conv2d`
-(tracea-python/python/tracea/__init__.py:19-56), forward only; and of the 4-bit products, `MxLinear` and `MxFeedForward`, which
-the reference does not have.
+(tracea-python/python/tracea/__init__.py:19-56), forward only; and of the 4-bit products, `MxLinear`, `MxFeedForward` and
+`MxAttention`, which the reference does not have.
 
 Differences from the reference's module, all deliberate:
   * dilation > 1 is computed here (the reference falls back to PyTorch for it);
@@ -176,6 +176,61 @@ class MxFeedForward(torch.nn.Module):
         r = ops.block_norm_add(h, rows, self.post_weight.detach(), gate=gate, residual_scale=self.residual_scale, kind=self.norm,
                                eps=self.eps)
         return r.view(x.shape)
+
+
+class MxAttention(torch.nn.Module):
+    """An attention block on a paged cache in 8 bits, with a norm in front and one behind it, as MxFeedForward is for the other half of
+    a layer; for prompts, pieces of them and single tokens alike:
+
+        q, k, v = qkv(norm(x) * (1 + scale) + shift);  q, k normalised per head (``head_norm``) and rotated by position
+        r = residual_scale * x + gate * norm(out(attention(q, cache with k and v)))
+
+    Both projections are MxLinear; keys and values go into the cache, which the caller keeps (``cache`` makes one that fits), in the same
+    launch that rotates the queries. x: (T, dim), float16 or bfloat16, the last tokens of the sequences that ``pages``, ``lengths`` and
+    ``starts`` describe (``ops.kv_append``); gate, scale, shift: (G, dim) with G dividing T. Forward only."""
+
+    def __init__(self, dim, heads, kv_heads=None, head_dim=None, norm="rms", head_norm=True, eps=1e-6, base=10000.0, window=0,
+                 residual_scale=1.0, bias=False, device=None, dtype=None):
+        super().__init__()
+        self.heads, self.kv_heads = heads, kv_heads or heads
+        if self.heads % self.kv_heads != 0:
+            raise ValueError("heads must be a multiple of kv_heads")
+        if head_dim is None and dim % heads != 0:
+            raise ValueError("dim is no multiple of heads: give head_dim")
+        self.head_dim = head_dim or dim // heads
+        if self.head_dim % 16 != 0 or self.head_dim > 128:
+            raise ValueError("head_dim must be a multiple of 16 up to 128")
+        self.norm, self.eps, self.base, self.window, self.residual_scale = norm, eps, base, window, residual_scale
+        self.pre_weight = torch.nn.Parameter(torch.ones(dim, device=device))
+        self.post_weight = torch.nn.Parameter(torch.ones(dim, device=device))
+        self.q_weight = torch.nn.Parameter(torch.ones(self.head_dim, device=device)) if head_norm else None
+        self.k_weight = torch.nn.Parameter(torch.ones(self.head_dim, device=device)) if head_norm else None
+        self.qkv = MxLinear(dim, (self.heads + 2 * self.kv_heads) * self.head_dim, bias, None, device, dtype)
+        self.out = MxLinear(self.heads * self.head_dim, dim, bias, None, device, dtype)
+        self._frequencies = ops.rotary_frequencies(self.head_dim, base, self.pre_weight.device)
+
+    def _apply(self, fn, *args, **kwargs):
+        super()._apply(fn, *args, **kwargs)
+        # neither a parameter nor a buffer: a change of type would round them
+        self._frequencies = ops.rotary_frequencies(self.head_dim, self.base, self.pre_weight.device)
+        return self
+
+    def cache(self, pages, page_size=64):
+        """An empty ops.KvCache of ``pages`` pages for this block, on its device."""
+        return ops.KvCache.empty(pages, self.kv_heads, self.head_dim, page_size, self.pre_weight.device)
+
+    def forward(self, x, cache, pages, lengths, starts=None, gate=None, scale=None, shift=None):
+        rows = x.detach()
+        weights = [None if w is None else w.detach() for w in (self.q_weight, self.k_weight)]
+        normed = ops.block_norm(rows, self.pre_weight.detach(), None, scale, shift, self.norm, self.eps, quantize=True)
+        heads = self.qkv.product(normed, dtype=x.dtype).view(-1, self.heads + 2 * self.kv_heads, self.head_dim)
+        q, k, v = torch.split(heads, [self.heads, self.kv_heads, self.kv_heads], dim=1)
+        q = ops.kv_append(cache, k, v, pages, lengths, starts, self._frequencies, k_weight=weights[1], q=q, q_weight=weights[0],
+                          kind="rms" if self.q_weight is not None else "none", eps=self.eps)
+        a = ops.kv_attention(q, cache, pages, lengths, starts, window=self.window)
+        h = self.out.product(a.view(-1, self.heads * self.head_dim))
+        return ops.block_norm_add(h, rows, self.post_weight.detach(), gate=gate, residual_scale=self.residual_scale, kind=self.norm,
+                                  eps=self.eps)
 
 
 def patch_conv2d():
