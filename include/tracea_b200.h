@@ -351,7 +351,7 @@ typedef struct {
  * included, token j in row j % P of page pages[s][j / P]; rows starts[s] .. starts[s + 1] - 1 of the call are its last ones. starts
  * ([sequences + 1], not decreasing, from 0 to the rows) may be NULL: row s is the last token of sequence s. An entry of `pages` outside
  * the cache is a page that is not there, and so is what the table is too short for: nothing is written to it and nothing of it is
- * attended to. Sequences share pages only where no call writes to them. */
+ * attended to. A page that a call writes to stands in one place of one sequence. */
 typedef struct {
   TraceaTensorView pages;   /* [sequences, width] */
   TraceaTensorView lengths; /* [sequences] */

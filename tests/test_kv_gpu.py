@@ -346,3 +346,19 @@ def test_offsets_beyond_32_bits():
     check_attention(q, sub, [[2, 0, 1]], [300], [0, 300],
                     got=ops.kv_attention(q, cache, ints(table), ints([300]), ints([0, 300])))
     check_attention(q[:1], sub, [[2, 0, 1]], [300], None, got=ops.kv_attention(q[:1], cache, ints(table), ints([300])))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("h, kv, d, size, sequences", [(8, 2, 128, 64, [(4000, 130)]), (4, 1, 64, 32, [(0, 2500), (3000, 70)]),
+                                                       (6, 2, 80, 128, [(9000, 45), (100, 3), (2000, 90)])])
+def test_attention_of_pieces_of_prompts_behind_long_ones(h, kv, d, size, sequences, dtype):
+    """Few blocks of rows and many tokens: the tokens are split over CTAs, and some of a block's parts are seen by none of its rows."""
+    lengths = [a + b for a, b in sequences]
+    starts = [sum(n for _, n in sequences[:i]) for i in range(len(sequences) + 1)]
+    total = sum(-(-n // size) for n in lengths) + 2
+    pages = tables(lengths, size, total, h, extra=20)
+    pages[0][3] = -1
+    cache = random_cache(total, kv, size, d, d + h)
+    q = rows(starts[-1], h, d, dtype, 1)
+    for causal, window in ((True, 0), (False, 0), (True, 900), (True, 33)):
+        check_attention(q, cache, pages, lengths, starts, causal, window)

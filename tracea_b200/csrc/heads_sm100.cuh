@@ -535,9 +535,27 @@ __global__ void __launch_bounds__(kHeadThreads, kLanes > 0 && kRows <= 2 ? 2 : 1
   const int from = max(begin, slot << shift), to = min(at.length, (slot + 1) << shift);
   const int count = to - from, first = from - (slot << shift);
   const int row0 = at.first_row + from - begin;
-  long long page = -1;
-  if (slot >= 0 && slot < args.seqs.table_width) page = args.seqs.table[at.sequence * args.seqs.table_stride + slot];
-  if (page >= args.cache.pages) page = -1;
+  int entry = -1;                                          // looked at below, when it has arrived
+  if (slot >= 0 && slot < args.seqs.table_width) entry = args.seqs.table[at.sequence * args.seqs.table_stride + slot];
+
+  const int my_row = static_cast<int>(threadIdx.x) / kRowLanes, my_lane = static_cast<int>(threadIdx.x) % kRowLanes;
+  const Lane l(my_lane, D, args.rot);
+  const Lane plain(my_lane, D, Rotation{nullptr, 0, 0});   // values are not rotated: their columns in order
+  const float inv_columns = 1.0f / static_cast<float>(D);
+  const int head0 = static_cast<int>(blockIdx.y) * args.heads_per_cta, head1 = min(args.cache.heads, head0 + args.heads_per_cta);
+
+  // the first head's keys and values, on their way while the angles are computed
+  Raw rk[kRows], rv[kRows];
+  const T *k_row[kRows], *v_row[kRows];
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const int r = my_row + i * kRowsAtOnce;
+    const long long row = row0 + (r < count ? r : 0);
+    k_row[i] = static_cast<const T*>(args.k.x) + row * args.k.x_token + head0 * args.k.x_head;
+    v_row[i] = static_cast<const T*>(args.v) + row * args.v_token + head0 * args.v_head;
+    rk[i].load(k_row[i], l);
+    rv[i].load(v_row[i], plain);
+  }
 
   weights_to_shared<T>(weights[0], args.q.weight, args.q.weight_f32, D);
   weights_to_shared<T>(weights[1], args.k.weight, args.k.weight_f32, D);
@@ -551,24 +569,8 @@ __global__ void __launch_bounds__(kHeadThreads, kLanes > 0 && kRows <= 2 ? 2 : 1
   }
   __syncthreads();
 
-  const int my_row = static_cast<int>(threadIdx.x) / kRowLanes, my_lane = static_cast<int>(threadIdx.x) % kRowLanes;
-  const Lane l(my_lane, D, args.rot);
-  const Lane plain(my_lane, D, Rotation{nullptr, 0, 0});   // values are not rotated: their columns in order
-  const float inv_columns = 1.0f / static_cast<float>(D);
-  const int head0 = static_cast<int>(blockIdx.y) * args.heads_per_cta, head1 = min(args.cache.heads, head0 + args.heads_per_cta);
-
+  const long long page = entry >= 0 && entry < args.cache.pages ? entry : -1;
   if (page >= 0) {
-    Raw rk[kRows], rv[kRows];
-    const T *k_row[kRows], *v_row[kRows];
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      const int r = my_row + i * kRowsAtOnce;
-      const long long row = row0 + (r < count ? r : 0);
-      k_row[i] = static_cast<const T*>(args.k.x) + row * args.k.x_token + head0 * args.k.x_head;
-      v_row[i] = static_cast<const T*>(args.v) + row * args.v_token + head0 * args.v_head;
-      rk[i].load(k_row[i], l);
-      rv[i].load(v_row[i], plain);
-    }
     for (int head = head0; head < head1; ++head) {
       const long long block = page * args.cache.heads + head;
       uint8_t* ck = args.cache.k + (block << shift) * D;

@@ -55,7 +55,7 @@ void launch_tokens(tb200::KvTokensArgs& c, DeviceState& st, int dev, cudaStream_
 }
 
 template <typename T, int kD>
-void launch_rows(const tb200::KvAttentionArgs& a, long long items, int dev, cudaStream_t stream) {
+void launch_rows(const tb200::KvAttentionArgs& a, long long items, DeviceState& st, int dev, cudaStream_t stream) {
   constexpr int kSmem = tb200::kv_rows_smem_bytes<kD>();
   auto kern = tb200::kv_rows_kernel<T, kD>;
   static std::atomic<bool> done[kMaxDevices];
@@ -66,7 +66,25 @@ void launch_rows(const tb200::KvAttentionArgs& a, long long items, int dev, cuda
     TB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
     done[dev].store(true, std::memory_order_relaxed);
   }
-  launch(kern, grid_of(items * a.cache.heads), tb200::kKvRowsThreads, kSmem, 1, kLaunchKvRows, stream, a);
+  tb200::KvRowsArgs c;
+  memset(&c, 0, sizeof(c));
+  c.a = a;
+  // Few blocks of rows leave SMs idle: their tokens are split, as long as a part has four steps where the sequences are as long as they
+  // may be.
+  long long most = static_cast<long long>(a.seqs.table_width) << a.cache.page_shift;
+  if (a.window > 0) most = std::min<long long>(most, a.window + static_cast<long long>(tb200::kKvRowsOfCta));
+  const long long blocks = items * a.cache.heads;
+  c.splits = static_cast<int>(std::max(1LL, std::min({st.num_sms / blocks, most / (4 * tb200::kKvRowsTokens), 8LL})));
+  Scratch scratch;
+  if (c.splits > 1) {
+    const size_t rows = static_cast<size_t>(c.splits) * a.seqs.rows * a.cache.heads * a.group;
+    scratch.alloc(st, rows * (kD * sizeof(float) + sizeof(float2)), stream);
+    c.sums = static_cast<float*>(scratch.ptr);
+    c.tops = reinterpret_cast<float2*>(c.sums + rows * kD);
+  }
+  launch(kern, grid_of(blocks * c.splits), tb200::kKvRowsThreads, kSmem, 1, kLaunchKvRows, stream, c);
+  if (c.splits > 1)
+    launch(tb200::kv_rows_join_kernel<T, kD>, dim3(grid_of(blocks), 8), 32 * tb200::kKvRowsJoinWarps, 0, 1, kLaunchKvRows, stream, c);
 }
 
 template <typename F>
@@ -95,6 +113,7 @@ void kv_attention_checked(const TraceaTensorView& qv, const TraceaKvCache& cache
   a.seqs = load_sequences(seqs, dev, q.tokens);
   if (q.tokens * (q.heads / a.cache.heads) > 0x7fffff00LL) TB_FAIL(TRACEA_UNSUPPORTED_CONFIG, "q: too many rows");
   if (q.tokens == 0 || a.seqs.count == 0) return;
+  if (a.cache.pages == 0) a.cache.k = a.cache.v = reinterpret_cast<uint8_t*>(q.ptr);   // what copies of no bytes point to
   a.q = q.ptr;
   a.out = out.ptr;
   a.q_token = q.token_stride;
@@ -127,8 +146,8 @@ void kv_attention_checked(const TraceaTensorView& qv, const TraceaKvCache& cache
       a.fewest = only_many ? 1 : kFew + 1;
       a.most = 0x7fffffff;
       const long long items = all_rows / tb200::kKvRowsOfCta + std::min<long long>(a.seqs.count, ceil_div(all_rows, a.fewest));
-      if (a.cache.D <= 64) launch_rows<T, 64>(a, items, dev, stream);
-      else launch_rows<T, 128>(a, items, dev, stream);
+      if (a.cache.D <= 64) launch_rows<T, 64>(a, items, st, dev, stream);
+      else launch_rows<T, 128>(a, items, st, dev, stream);
     }
     if (!only_many) {
       a.fewest = 1;

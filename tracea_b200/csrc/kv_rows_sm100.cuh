@@ -37,11 +37,37 @@ __host__ __device__ constexpr int kv_rows_smem_bytes() {
   return 1024 + 6 * 128 * kD * 2 + kKvRowsMeta * 8 * 16 + 256;
 }
 
+struct KvRowsArgs {
+  KvAttentionArgs a;
+  int splits;                    // CTAs that share a block of rows, each a part of the tokens
+  float* sums;                   // splits > 1: [splits][rows * H][kD] results in the making,
+  float2* tops;                  // and [splits][rows * H] of {maximum, denominator}
+};
+
+// 256 rows of a sequence and a head of keys.
+struct RowsItem {
+  SequenceItem at;
+  int first_row, rows;
+};
+__device__ __forceinline__ bool rows_item(const KvAttentionArgs& a, int index, RowsItem& item) {
+  const int group = a.group;
+  if (!find_sequence(a.seqs, index, item.at, [&](int n, int) {
+        const long long all = static_cast<long long>(n) * group;
+        return all < a.fewest || all > a.most ? 0 : static_cast<int>((all + kKvRowsOfCta - 1) / kKvRowsOfCta);
+      }))
+    return false;
+  const int all_rows = item.at.rows * group, last = (all_rows + kKvRowsOfCta - 1) / kKvRowsOfCta - 1;
+  item.first_row = (last - item.at.item) * kKvRowsOfCta;            // the last rows see most: they come first
+  item.rows = min(kKvRowsOfCta, all_rows - item.first_row);
+  return true;
+}
+
 // [q of tile 0, of tile 1][keys, 2 stages][values, 2 stages][scales][barriers]: operands as blocks of 64 columns, 128 rows of 128
 // bytes each, swizzled.
 template <typename T, int kD>
-__global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid_constant__ KvAttentionArgs args) {
+__global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid_constant__ KvRowsArgs call) {
   using namespace ptx;
+  const KvAttentionArgs& args = call.a;
   constexpr uint32_t kOperand = 128u * kD * 2u, kBlock = 128u * 128u;
   constexpr int kBlocks = kD / 64;
   constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);          // 8-row groups 1024 bytes apart, 128-byte swizzle
@@ -59,27 +85,34 @@ __global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid
   volatile uint32_t* const abort_p = tmem_slot_p + 1;
 
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  // Tensor memory first: a dependent grid that is let in before may take the columns and wait for this one.
+  if (warp == kKvRowsMmaWarp) {
+    tmem_alloc<512>(bars + 8 * 24);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot_p, 0);
   griddep_launch_dependents();
   griddep_wait();
-  const int head = static_cast<int>(blockIdx.x) % args.cache.heads;
-  SequenceItem at;
-  const int group = args.group;
-  if (!find_sequence(args.seqs, static_cast<int>(blockIdx.x) / args.cache.heads, at, [&](int n, int) {
-        const long long all = static_cast<long long>(n) * group;
-        return all < args.fewest || all > args.most ? 0 : static_cast<int>((all + kKvRowsOfCta - 1) / kKvRowsOfCta);
-      }))
+  const int split = static_cast<int>(blockIdx.x) % call.splits, id = static_cast<int>(blockIdx.x) / call.splits;
+  const int head = id % args.cache.heads, group = args.group;
+  RowsItem item;
+  if (!rows_item(args, id / args.cache.heads, item)) {
+    if (warp == kKvRowsMmaWarp) tmem_dealloc<512>(tmem);
     return;
-  const int all_rows = at.rows * group;
-  const int last_item = (all_rows + kKvRowsOfCta - 1) / kKvRowsOfCta - 1;
-  const int first_row = (last_item - at.item) * kKvRowsOfCta;       // the last rows see most: they come first
-  const int rows = min(kKvRowsOfCta, all_rows - first_row), tiles = rows > kKvRowsTile ? 2 : 1;
+  }
+  const SequenceItem& at = item.at;
+  const int first_row = item.first_row, rows = item.rows, tiles = rows > kKvRowsTile ? 2 : 1;
   const int D = args.cache.D, shift = args.cache.page_shift;
   const int begin = at.length - at.rows;
   const int pos_lo = begin + first_row / group, pos_hi = begin + (first_row + rows - 1) / group;
   const int see_lo = args.window > 0 ? max(0, pos_lo - args.window + 1) : 0;
   const int see_hi = min(args.causal ? max(0, pos_hi + 1) : at.length, args.seqs.table_width << shift);
-  const int step_lo = see_lo / kKvRowsTokens;
-  const int steps = max(0, (see_hi + kKvRowsTokens - 1) / kKvRowsTokens - step_lo);
+  const int all_steps = max(0, (see_hi + kKvRowsTokens - 1) / kKvRowsTokens - see_lo / kKvRowsTokens);
+  const int step_lo = see_lo / kKvRowsTokens + all_steps * split / call.splits;
+  const int steps = see_lo / kKvRowsTokens + all_steps * (split + 1) / call.splits - step_lo;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 4; ++i) {
@@ -99,14 +132,7 @@ __global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid
     *abort_p = 0u;
     fence_mbar_init();
   }
-  if (warp == kKvRowsMmaWarp) {
-    tmem_alloc<512>(bars + 8 * 24);
-    tmem_relinquish();
-  }
-  tc_fence_before();
   __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot_p, 0);
 
   if (warp < kKvRowsWidenWarp) {
     regs_up<kKvRowsSoftmaxRegs>();
@@ -256,8 +282,12 @@ __global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid
       if (ok && steps > 0) wait_scores(2 * steps + 1);               // the last product is complete
       if (ok) {
         tc_fence_after();
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const bool whole = call.splits == 1;
+        const float inv = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
         T* const op = static_cast<T*>(args.out) + static_cast<long long>(at.first_row + token) * args.out_token + q_head * args.out_head;
+        const long long heads = static_cast<long long>(args.cache.heads) * group;
+        const long long part = (split * static_cast<long long>(args.seqs.rows) + at.first_row + token) * heads + q_head;
+        if (!whole && live) call.tops[part] = make_float2(m, l);
 #pragma unroll
         for (int c = 0; c < kD; c += 32) {
           uint32_t o[32];
@@ -271,7 +301,8 @@ __global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = l == 0.0f ? 0.0f : __uint_as_float(o[d + i]) * inv;
             if (live && c + d < D) {
-              if (args.out_vec == 8) store8(op + c + d, v);
+              if (!whole) store8(call.sums + part * kD + c + d, v);
+              else if (args.out_vec == 8) store8(op + c + d, v);
               else store8_upto(op + c + d, 1, 8, v);
             }
           }
@@ -440,6 +471,36 @@ __global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid
   __syncthreads();
   tc_fence_after();
   if (warp == kKvRowsMmaWarp) tmem_dealloc<512>(tmem);
+}
+
+// The sums of rows whose tokens were split: a warp to a row, a CTA to 256 rows as above, a lane four columns.
+constexpr int kKvRowsJoinWarps = 8;
+template <typename T, int kD>
+__global__ void __launch_bounds__(32 * kKvRowsJoinWarps) kv_rows_join_kernel(const __grid_constant__ KvRowsArgs call) {
+  using namespace ptx;
+  const KvAttentionArgs& args = call.a;
+  griddep_launch_dependents();
+  griddep_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int id = static_cast<int>(blockIdx.x), head = id % args.cache.heads, group = args.group;
+  RowsItem item;
+  if (!rows_item(args, id / args.cache.heads, item)) return;
+  const long long heads = static_cast<long long>(args.cache.heads) * group, all = args.seqs.rows * heads;
+  for (int r = static_cast<int>(blockIdx.y) * kKvRowsJoinWarps + warp; r < item.rows; r += kKvRowsJoinWarps * static_cast<int>(gridDim.y)) {
+    const int row = item.first_row + r, token = item.at.first_row + row / group, q_head = head * group + row % group;
+    const long long part = token * heads + q_head;
+    float top = -INFINITY, total = 0.0f;
+    for (int s = 0; s < call.splits; ++s) top = fmaxf(top, call.tops[s * all + part].x);
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int s = 0; s < call.splits; ++s) {
+      const float2 t = call.tops[s * all + part];
+      const float f = part_factor(t.x, t.y, top);
+      total += f * t.y;
+      if (4 * lane < args.cache.D) add_scaled(sum, *reinterpret_cast<const float4*>(call.sums + (s * all + part) * kD + 4 * lane), f);
+    }
+    T* const p = static_cast<T*>(args.out) + token * args.out_token + q_head * args.out_head + 4 * lane;
+    if (4 * lane < args.cache.D) store_4(p, sum, total == 0.0f ? 0.0f : 1.0f / total, args.out_vec);
+  }
 }
 
 }  // namespace tb200
