@@ -70,11 +70,12 @@ void launch_rows(const tb200::KvAttentionArgs& a, long long items, DeviceState& 
   memset(&c, 0, sizeof(c));
   c.a = a;
   // Few blocks of rows leave SMs idle: their tokens are split, as long as a part has four steps where the sequences are as long as they
-  // may be.
+  // may be. us, one part / split, 32 heads to 8 of 128 columns: 256 tokens behind 8000 144 / 56, 256 behind 2000 48 / 33, 128 behind
+  // 30000 496 / 86; 8 heads to 2, 500 behind 4000 82 / 34.
   long long most = static_cast<long long>(a.seqs.table_width) << a.cache.page_shift;
   if (a.window > 0) most = std::min<long long>(most, a.window + static_cast<long long>(tb200::kKvRowsOfCta));
   const long long blocks = items * a.cache.heads;
-  c.splits = static_cast<int>(std::max(1LL, std::min({st.num_sms / blocks, most / (4 * tb200::kKvRowsTokens), 8LL})));
+  c.splits = static_cast<int>(std::max(1LL, std::min({st.num_sms / blocks, most / (4 * tb200::kKvRowsTokens), 16LL})));
   Scratch scratch;
   if (c.splits > 1) {
     const size_t rows = static_cast<size_t>(c.splits) * a.seqs.rows * a.cache.heads * a.group;
@@ -145,7 +146,9 @@ void kv_attention_checked(const TraceaTensorView& qv, const TraceaKvCache& cache
     if (!only_few) {
       a.fewest = only_many ? 1 : kFew + 1;
       a.most = 0x7fffffff;
-      const long long items = all_rows / tb200::kKvRowsOfCta + std::min<long long>(a.seqs.count, ceil_div(all_rows, a.fewest));
+      // blocks of rows: a sequence's last one may be short
+      const long long items = std::min(ceil_div(all_rows, tb200::kKvRowsOfCta) + a.seqs.count - 1,
+                                       all_rows / tb200::kKvRowsOfCta + ceil_div(all_rows, a.fewest));
       if (a.cache.D <= 64) launch_rows<T, 64>(a, items, st, dev, stream);
       else launch_rows<T, 128>(a, items, st, dev, stream);
     }
