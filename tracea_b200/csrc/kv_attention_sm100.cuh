@@ -9,7 +9,8 @@
 
 namespace tb200 {
 
-constexpr float kSlack = 8.0f;   // weights up to 2^8 in halves, which reach 2^16
+constexpr float kSlack = 8.0f;
+constexpr float kLift = 7.0f;    // the weights are 2^7 times the above, up to 2^15: halves reach 2^16, and lose bits below 2^-14
 
 struct KvAttentionArgs {
   CacheRef cache;

@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid
             }
           }
         }
-        const float base = m == -INFINITY ? 0.0f : m;                // a row that has seen nothing
+        const float base = m == -INFINITY ? 0.0f : m - kLift;        // a row that has seen nothing
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t p[16];

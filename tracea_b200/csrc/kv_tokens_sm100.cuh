@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(kKvTokenThreads, kv_token_ctas(kRows)) kv_toke
         for (int n = 0; n < kN; ++n) {
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const float base = m[n][j] == -INFINITY ? 0.0f : m[n][j];      // a row that has seen nothing
+            const float base = m[n][j] == -INFINITY ? 0.0f : m[n][j] - kLift;      // a row that has seen nothing
             s[n][j] = exp2_ftz(s[n][j] - base);
             s[n][2 + j] = exp2_ftz(s[n][2 + j] - base);
             l[n][j] += (s[n][j] + s[n][2 + j]) * unscale;
