@@ -46,12 +46,12 @@ def copies(cache):
     return [t.clone() for t in (cache.k, cache.v, cache.k_scales, cache.v_scales)]
 
 
-def check_append(cache, before, k, v, pages, lengths, starts, rotation=None, weight=None, kind="none"):
+def check_append(cache, before, k, v, pages, lengths, starts, rotation=None, weight=None, kind="none", interleaved=False):
     """The whole cache after appending, from the one before."""
     size, total = cache.page_size, cache.k.shape[0]
     where = kvref.places(pages, lengths, starts, k.shape[0], size, total)
     positions = torch.tensor([w[1] for w in where], device="cuda")
-    vk, ek = kvref.rotate(k, positions, rotation, False, weight, kind)
+    vk, ek = kvref.rotate(k, positions, rotation, interleaved, weight, kind)
     vv, ev = v.double(), torch.zeros_like(v, dtype=torch.float64)
     bad = ~(torch.isfinite(vk) & torch.isfinite(vv)).all(-1)
     exact = rotation is None and kind == "none"
