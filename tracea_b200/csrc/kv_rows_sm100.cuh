@@ -73,7 +73,6 @@ __global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid
   constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);          // 8-row groups 1024 bytes apart, 128-byte swizzle
   constexpr uint32_t kIdescS = make_idesc(0, 128, 64), kIdescO = make_idesc(0, 128, kD, 1);
   extern __shared__ uint8_t smem_raw[];
-  __shared__ float row_factor[kKvRowsOfCta];
   const uint32_t smem_base = __shfl_sync(0xffffffffu, (smem_u32(smem_raw) + 1023u) & ~1023u, 0);
   uint8_t* const smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
   const uint32_t q_smem = smem_base, k_smem = smem_base + 2 * kOperand, v_smem = smem_base + 4 * kOperand;
@@ -142,42 +141,67 @@ __global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid
       const bool live = my_row < rows;
       const int token = live ? (first_row + my_row) / group : 0, q_head = head * group + (live ? (first_row + my_row) % group : 0);
       // q into halves: kD / 8 lanes a row, eight columns each, all of the warp's rows' loads under way together
-      constexpr int kRowLanes = kD / 8, kRowsAtOnce = 32 / kRowLanes, kLoads = 32 / kRowsAtOnce;
-      const int col = 8 * (lane % kRowLanes);
-      const T* const q0 = static_cast<const T*>(args.q) + static_cast<long long>(at.first_row) * args.q_token + head * group * args.q_head;
+      constexpr int kRowLanes = kD / 8, kRowsAtOnce = 32 / kRowLanes, kLoads = kRowLanes;
+      const int col = 8 * (lane % kRowLanes), first = tile * kKvRowsTile + (warp & 3) * 32 + lane / kRowLanes;
+      const T* const q0 = static_cast<const T*>(args.q) + static_cast<long long>(at.first_row) * args.q_token + head * group * args.q_head + col;
       Vec8<T> raw[kLoads];
+      auto load_rows = [&](auto fetch_row) {
+        // a division for the first row's token and head, steps from there
+        const int step_token = kRowsAtOnce / group, step_head = kRowsAtOnce % group;
+        int q_tok = (first_row + first) / group, q_sub = (first_row + first) % group;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+          raw[i] = Vec8<T>{};
+          if (col < D && first + i * kRowsAtOnce < rows) fetch_row(q0 + q_tok * args.q_token + q_sub * args.q_head, raw[i]);
+          q_tok += step_token;
+          q_sub += step_head;
+          if (q_sub >= group) {
+            q_sub -= group;
+            ++q_tok;
+          }
+        }
+      };
+      if (args.q_vec) {
+        load_rows([](const T* p, Vec8<T>& v) { fetch8(p, v); });
+      } else {
+        load_rows([](const T* p, Vec8<T>& v) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) reinterpret_cast<T*>(&v)[k] = p[k];
+        });
+      }
+      // Peaks of the rows: every exchange halves the rows that a lane holds, until lane i of a row's lanes has that of load i.
+      float peak[kLoads];
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
-        const int row = first_row + min(tile * kKvRowsTile + (warp & 3) * 32 + i * kRowsAtOnce + lane / kRowLanes, rows - 1);
-        const T* const p = q0 + static_cast<long long>(row / group) * args.q_token + (row % group) * args.q_head + (col < D ? col : 0);
-        if (args.q_vec) {
-          fetch8(p, raw[i]);
-        } else {
+        float v[8];
+        widen8(raw[i], v);
+        peak[i] = 0.0f;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) reinterpret_cast<T*>(&raw[i])[k] = p[k];
-        }
+        for (int k = 0; k < 8; ++k) peak[i] = fmaxf(peak[i], fabsf(v[k]));
       }
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int in_warp = i * kRowsAtOnce + lane / kRowLanes, in_tile = (warp & 3) * 32 + in_warp;
-        float v[8], peak = 0.0f;
-        widen8(raw[i], v);
+      for (int o = kRowLanes / 2; o > 0; o >>= 1) {
+        const bool upper = (lane & o) != 0;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          if (col >= D || tile * kKvRowsTile + in_tile >= rows) v[k] = 0.0f;
-          peak = fmaxf(peak, fabsf(v[k]));
+        for (int i = 0; i < o; ++i) {
+          const float other = __shfl_xor_sync(0xffffffffu, upper ? peak[i] : peak[i + o], o);
+          peak[i] = fmaxf(upper ? peak[i + o] : peak[i], other);
         }
+      }
+      float back;
+      const float up_of_lane = args.sign * row_scale(peak[0], back);
 #pragma unroll
-        for (int o = kRowLanes / 2; o > 0; o >>= 1) peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, o));
-        float back;
-        const float up = args.sign * row_scale(peak, back);
-        if (lane % kRowLanes == 0) row_factor[tile * kKvRowsTile + in_tile] = back * args.scale_log2;
+      for (int i = 0; i < kLoads; ++i) {
+        const int in_tile = (warp & 3) * 32 + i * kRowsAtOnce + lane / kRowLanes;
+        const float up = __shfl_sync(0xffffffffu, up_of_lane, i, kRowLanes);
+        float v[8];
+        widen8(raw[i], v);
         st_shared_v4(q_smem + tile * kOperand + (col / 64) * kBlock + in_tile * 128 + ((((col % 64) / 8) ^ (in_tile & 7)) * 16),
                      make_uint4(pack_halves(v[0] * up, v[1] * up), pack_halves(v[2] * up, v[3] * up), pack_halves(v[4] * up, v[5] * up),
                                 pack_halves(v[6] * up, v[7] * up)));
       }
-      __syncwarp();
-      const float factor = fmaxf(row_factor[my_row], 1.17549435e-38f);          // not 0: a score of -infinity stays one
+      // This thread's row is row lane / kRowsAtOnce of the loads. Not 0: a score of -infinity stays one.
+      const float factor = fmaxf(__shfl_sync(0xffffffffu, back, (lane % kRowsAtOnce) * kRowLanes + lane / kRowsAtOnce) * args.scale_log2, 1.17549435e-38f);
       fence_proxy_async_smem();
       mbar_arrive(bar(kQFull + tile));
 
