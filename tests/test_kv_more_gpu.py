@@ -119,3 +119,51 @@ def test_random_batches(seed):
     for causal, window in ((True, 0), (r.random() < 0.5, r.randint(1, 400))):
         check_attention(q, cache, pages, lengths, starts, causal, window)
     status_ok()
+
+
+@pytest.mark.parametrize("h, kv", [(8, 2), (48, 1)])
+def test_sequences_that_share_pages(h, kv):
+    """A prefix that several sequences have in common, and a page that stands twice in one of them, are only read."""
+    cache = random_cache(12, kv, 32, 64, 9)
+    pages = [[3, 4, 5, 0], [3, 4, 6, 7], [3, 3, 4, -1], [5, 4, 3, 2]]
+    lengths = [100, 128, 70, 96]
+    check_attention(rows(4, h, 64, "f16", 1), cache, pages, lengths, None)
+    check_attention(rows(185, h, 64, "f16", 2), cache, pages, lengths, [0, 90, 91, 155, 185], window=77)
+
+
+@pytest.mark.parametrize("n, old", [(1, 500), (1, 30000), (20, 100), (150, 30), (100, 6000)])
+def test_attention_in_place_with_rows_behind_the_last_sequence(n, old):
+    """Every form reads what it needs of q before it writes there, and leaves the rows that belong to no sequence."""
+    cache = random_cache(520, 2, 64, 128, 4)
+    lengths, pages = [old + n], tables([old + n], 64, 520, 5)
+    q = rows(n + 3, 10, 128, "bf16", 6)
+    out = q.clone()
+    s, alive = c_sequences(ints(pages), ints(lengths), ints([0, n]))
+    v = ops._view(out)
+    st = ffi.load().tracea_kv_attention(v.c, c_cache(cache), s, ctypes.byref(v.c), ffi.KvAttentionParams(128 ** -0.5, 1, 0, stream()))
+    assert st == ffi.SUCCESS, ffi.last_error()
+    check_attention(q[:n], cache, pages, lengths, [0, n], got=out[:n])
+    assert torch.equal(out[n:], q[n:])
+    status_ok()
+
+
+def test_many_sequences_few_of_which_have_rows():
+    new = [0] * 150
+    new[3], new[31], new[32], new[100], new[149] = 40, 1, 200, 7, 1
+    lengths = [n + 20 * (i % 3) for i, n in enumerate(new)]
+    starts = [sum(new[:i]) for i in range(151)]
+    pages = tables([max(n, 1) for n in lengths], 16, 1000, 2)
+    cache = random_cache(1000, 2, 16, 80, 7)
+    check_attention(rows(starts[-1], 8, 80, "f16", 3), cache, pages, lengths, starts)
+
+
+def test_calls_of_no_rows_and_no_sequences():
+    cache = random_cache(4, 2, 16, 64, 1)
+    before = copies(cache)
+    none, x, kv = ints([]), torch.empty(0, 4, 64, dtype=torch.float16, device="cuda"), torch.empty(0, 2, 64, dtype=torch.float16, device="cuda")
+    for pages, lengths, starts in ((ints([[0], [1]]), ints([3, 0]), ints([0, 0, 0])), (torch.empty(0, 3, dtype=torch.int32, device="cuda"), none, None)):
+        assert ops.kv_append(cache, kv, kv, pages, lengths, starts, q=x).shape == x.shape
+        assert ops.kv_attention(x, cache, pages, lengths, starts).shape == x.shape
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(copies(cache), before))
+    q, k = ops.head_norm_rotate(x, kv)
+    assert q.shape == x.shape and k.shape == kv.shape

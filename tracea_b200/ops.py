@@ -392,7 +392,8 @@ def kv_append(cache, k, v, pages, lengths, starts=None, frequencies=None, interl
     k, v (T, heads, D): the last tokens of the sequences. int32 tensors, read on the device: ``lengths`` (B), each sequence's tokens, the
     new ones included; ``pages`` (B, width), its pages: token j lies in row j % page_size of page pages[s, j // page_size], and is dropped
     where that is no page of the cache; ``starts`` (B + 1): rows starts[s] .. starts[s + 1] - 1 belong to sequence s -- None: row s is
-    the one new token of sequence s.
+    the one new token of sequence s. A page that a call writes to stands in one place of one sequence; such as are only read may be shared.
+    Rows of no sequence are not read, and not set in the result.
 
     A block, the tokens of a page and head, has one scale: the smallest power of two 2^e of which 448 reach its largest value,
     -40 <= e <= 40. It grows when a larger value is appended, and the block's older tokens are then rounded anew; a page's first token
