@@ -409,7 +409,8 @@ uint32_t tracea_b200_device_status(int32_t device_id);
  * record a code, the CTA unwind and the kernel return normally. wait_limit_cycles > 0 replaces the limit of a single
  * wait (default about two seconds) for the launches that follow; producer_stop_after >= 0 makes the TMA producer of
  * every CTA of those launches stop after that many pipeline stages and leave normally, so that the waits downstream
- * of it run out -- nothing faults, traps or spins without limit. (0, -1) restores normal operation. Process-wide.
+ * of it run out -- nothing faults, traps or spins without limit. In attention for many rows the producers are four warps;
+ * 65536 more than the number of steps stops the last of them alone. (0, -1) restores normal operation. Process-wide.
  * No counterpart in the reference (its kernels wait without limit, src/backend/cuda/primitives.rs:70-121). */
 void tracea_b200_test_hooks(int64_t wait_limit_cycles, int32_t producer_stop_after);
 

@@ -31,6 +31,7 @@ constexpr int kKvRowsThreads = 512;            // warps 0..3 and 4..7 softmax of
 constexpr int kKvRowsSoftmaxRegs = 176, kKvRowsWidenRegs = 104, kKvRowsMmaRegs = 56;
 static_assert(2 * kKvRowsSoftmaxRegs + kKvRowsWidenRegs + kKvRowsMmaRegs <= 4 * 128, "what the block is launched with, 128 a thread");
 constexpr int kKvRowsWidenWarp = 8, kKvRowsMmaWarp = 12;
+constexpr int kTestStopOneWarp = 1 << 16;      // test hook: see tracea_b200_test_hooks
 constexpr int kKvRowsMeta = 4;                 // steps whose scales are kept: a softmax is at most three steps behind the widening warps
 
 template <int kD>
@@ -405,16 +406,18 @@ __global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid
     fetch(args.cache.v, 0, vr);
     fetch(args.cache.k, 0, kr);
     bool ok = true;
-    auto wait = [&](int b, int j) {                                  // for slot j % 2 to be free of step j - 2
-      if (j >= 2 && !mbar_wait_bounded(bar(b + (j & 1)), ((j >> 1) & 1) ^ 1, abort_p, args.wait_limit)) {
-        report_error_status(args.status, abort_p, kErrProducerWait, static_cast<uint32_t>(j));
+    // For slot j % 2 to be free of step j - 2. The whole warp goes on or gives up: what follows exchanges values between its lanes.
+    auto wait = [&](int b, int j) {
+      if (j >= 2 && !mbar_wait_bounded_uniform(bar(b + (j & 1)), ((j >> 1) & 1) ^ 1, abort_p, args.wait_limit)) {
+        if (lane == 0) report_error_status(args.status, abort_p, kErrProducerWait, static_cast<uint32_t>(j));
         ok = false;
       }
       return ok;
     };
     // keys, and the scales, a step ahead of the values: ids and scale are those of keys' step j
     for (int j = 0; j <= steps && ok; ++j) {
-      if (j == args.test_producer_stop) break;                       // test hook: go silent, leave normally
+      // test hook: all four warps, or the last of them alone, go silent and leave normally
+      if (j == args.test_producer_stop || (w == 3 && j + kTestStopOneWarp == args.test_producer_stop)) break;
       if (j < steps) {
         if (!wait(kKEmpty, j)) break;
         if (w == 0) put_scales(j);
