@@ -326,7 +326,7 @@ typedef struct {
 } TraceaRotation;
 
 /* y = rotate(norm(x) * weight) for queries and keys (either may be NULL) of the same tokens and D, even and at most 256: norm per head
- * (TRACEA_NORM_NONE or TRACEA_NORM_RMS), in fp32, rounded once. positions: [tokens], INT32, needed with a rotation (NULL: none). */
+ * (TRACEA_NORM_RMS; TRACEA_NORM_NONE: norm(x) = x, its weight counts all the same), in fp32, rounded once. positions: [tokens], INT32, needed with a rotation (NULL: none). */
 TraceaStatus tracea_head_norm_rotate(const TraceaHeads *q, const TraceaHeads *k, TraceaNormKind kind, float eps,
                                      const TraceaRotation *rotation, const TraceaTensorView *positions, void *stream);
 

@@ -1,9 +1,11 @@
 """Heads, the cache and attention on a B200 where single values, rows or warps go their own way: waits that run out for some warps of a
-block and not for others."""
+block and not for others, weights without a norm."""
 import pytest
 import torch
 
-from test_kv_gpu import check_attention, ints, random_cache, rows
+import kvref
+from test_heads_gpu import DT, assert_near, make, weights
+from test_kv_gpu import check_append, check_attention, copies, ints, random_cache, rows, tables
 from tracea_b200 import ffi, ops
 
 pytestmark = pytest.mark.gpu
@@ -27,3 +29,46 @@ def test_waits_that_run_out_behind_one_silent_warp(stop):
     assert lib.tracea_b200_device_status(0) != 0
     assert lib.tracea_b200_device_status(0) == 0
     check_attention(q, cache, pages, lengths, starts)
+
+
+def weighted(x, weight, positions=None, frequencies=None, interleaved=False):
+    """kvref.rotate of the weighted rows: the weight's product, rounded, is a half step more of what its bound of 32 counts 5 of."""
+    return kvref.rotate(x.double() * weight.double(), positions, frequencies, interleaved)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("t, h, kv, d, rotated", [(1, 32, 8, 128, 128), (9, 3, 2, 64, 32), (7, 4, 1, 72, 40), (5, 2, 1, 250, 0), (33, 6, 3, 80, 0)])
+def test_a_weight_counts_without_a_norm(t, h, kv, d, rotated, dtype):
+    """Lanes of 16 columns and column by column, all, some and none of them rotated."""
+    q, k, _ = make(t, h, kv, d, dtype, 11)
+    positions = torch.arange(t, dtype=torch.int32).cuda() * 1001 + 5
+    freq = ops.rotary_frequencies(rotated, device="cuda") if rotated else None
+    for w in (weights(d, torch.float32, 2), weights(d, DT[dtype], 3)):
+        for interleaved in (False, True):
+            got = ops.head_norm_rotate(q, k, positions, freq, interleaved, *w, kind="none")
+            for x, y, weight in zip((q, k), got, w):
+                assert_near(y, *weighted(x, weight, positions, freq, interleaved))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_a_weight_counts_without_a_norm_when_appending(shift, dtype):
+    """What kv_append does by default; rows on a 16-byte boundary and off it."""
+    heads, d, size = 2, 64, 32
+    lengths, starts = [40, 3, 101], [0, 40, 41, 100]
+    pages = tables(lengths, size, 12, 1)
+    part = lambda n, seed: rows(100, n, d + 8, dtype, seed)[:, :, shift:shift + d]      # noqa: E731
+    k, v, q = part(heads, 1), part(heads, 2), part(3 * heads, 3)
+    kw, qw = weights(d, torch.float32, 4)
+    freq = ops.rotary_frequencies(48, device="cuda")
+    where = torch.tensor([w[1] for w in kvref.places(pages, lengths, starts, 100, size, 12)], device="cuda")
+    cache = random_cache(12, heads, size, d, 5)
+    before = copies(cache)
+    got = ops.kv_append(cache, k, v, ints(pages), ints(lengths), ints(starts), freq, k_weight=kw, q=q, q_weight=qw)
+    check_append(cache, before, k.double() * kw.double(), v, pages, lengths, starts, freq)
+    assert_near(got, *weighted(q, qw, where, freq))
+    one = random_cache(12, heads, size, d, 6)
+    before = copies(one)
+    got = ops.kv_append(one, k[:3], v[:3], ints(pages), ints(lengths), None, None, k_weight=torch.full_like(kw, 0.5), q=q[:3], q_weight=qw)
+    check_append(one, before, k[:3].double() * 0.5, v[:3], pages, lengths, None)      # by a power of two: exactly
+    assert_near(got, *weighted(q[:3], qw))

@@ -365,7 +365,7 @@ __global__ void __launch_bounds__(kHeadThreads, 3) head_rotate_kernel(const __gr
     before += passes;
     if (begin >= end) continue;
     float wx[kPairs], wy[kPairs];
-    head_weights<kNeighbours>(l, args.norm && rows.weight != nullptr ? weights[which] : nullptr, wx, wy);
+    head_weights<kNeighbours>(l, rows.weight != nullptr ? weights[which] : nullptr, wx, wy);
     const HeadTurn<kPairs> turn(wx, wy, c, s);
     const int heads = rows.heads;
     const long long x_step = kHeads * rows.x_head, y_step = kHeads * rows.y_head;
@@ -584,7 +584,7 @@ __global__ void __launch_bounds__(kHeadThreads, kLanes > 0 && kRows <= 2 ? 2 : 1
         const int r = my_row + i * kRowsAtOnce;
         rk[i].template values<kNeighbours>(l, kx[i], ky[i]);
         float wx[kPairs], wy[kPairs];
-        head_weights<kNeighbours>(l, args.norm && args.k.weight != nullptr ? weights[1] : nullptr, wx, wy);
+        head_weights<kNeighbours>(l, args.k.weight != nullptr ? weights[1] : nullptr, wx, wy);
         const float factor = args.norm ? head_norm(l, kx[i], ky[i], inv_columns, args.eps) : 1.0f;
         float c[kPairs], s[kPairs];
         head_turns(l, turns + 2 * (r < count ? r : 0) * pairs, pairs, c, s);
@@ -715,7 +715,7 @@ __global__ void __launch_bounds__(kHeadThreads, kLanes > 0 && kRows <= 2 ? 2 : 1
     const bool there = token < count;
     const int from_head = share * turn_heads, mine = there ? min(turn_heads, heads - from_head) : 0;
     float wx[kPairs], wy[kPairs];
-    head_weights<kNeighbours>(l, args.norm && args.q.weight != nullptr ? weights[0] : nullptr, wx, wy);
+    head_weights<kNeighbours>(l, args.q.weight != nullptr ? weights[0] : nullptr, wx, wy);
     float c[kPairs], s[kPairs];
     head_turns(l, turns + 2 * (there ? token : 0) * pairs, pairs, c, s);
     const HeadTurn<kPairs> turn(wx, wy, c, s);

@@ -342,10 +342,10 @@ def head_norm_rotate(q, k, positions=None, frequencies=None, interleaved=False, 
     token's position, in one pass. Returns new (q, k).
 
     q (T, H, D) and k (T, H', D), either may be None; their columns are contiguous, other strides any (slices of one projection, say);
-    float32, float16 or bfloat16, D even and at most 256. kind "rms" or "none"; weights (D), float32 or the rows' type. positions (T),
-    int32, and frequencies, float64 radians per position (``rotary_frequencies``): pair i of the first 2 * len(frequencies) columns,
-    columns 2i and 2i + 1 if ``interleaved`` and i and i + len(frequencies) if not, is turned by positions * frequencies[i], an angle
-    that is computed in 64 bits."""
+    float32, float16 or bfloat16, D even and at most 256. kind "rms" or "none"; weights (D), float32 or the rows' type, with either kind.
+    positions (T), int32, and frequencies, float64 radians per position (``rotary_frequencies``): pair i of the first
+    2 * len(frequencies) columns, columns 2i and 2i + 1 if ``interleaved`` and i and i + len(frequencies) if not, is turned by
+    positions * frequencies[i], an angle that is computed in 64 bits."""
     return _native().head_norm_rotate(q, k, positions, frequencies, interleaved, q_weight, k_weight, _norm_kind(kind), eps)
 
 
