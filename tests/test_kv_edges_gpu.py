@@ -1,5 +1,6 @@
 """Heads, the cache and attention on a B200 where single values, rows or warps go their own way: waits that run out for some warps of a
-block and not for others, weights without a norm."""
+block and not for others, weights without a norm, scores that
+vanish beside masked ones."""
 import pytest
 import torch
 
@@ -72,3 +73,22 @@ def test_a_weight_counts_without_a_norm_when_appending(shift, dtype):
     got = ops.kv_append(one, k[:3], v[:3], ints(pages), ints(lengths), None, None, k_weight=torch.full_like(kw, 0.5), q=q[:3], q_weight=qw)
     check_append(one, before, k[:3].double() * 0.5, v[:3], pages, lengths, None)      # by a power of two: exactly
     assert_near(got, *weighted(q[:3], qw))
+
+
+@pytest.mark.parametrize("d", [64, 80, 128])
+@pytest.mark.parametrize("n, old", [(3, 40), (70, 0), (150, 90), (100, 6000)])
+def test_scores_that_vanish_and_masks(n, old, d):
+    """A scale of zero, or queries so small that all products underflow, over pages of the smallest scale and of zeros: the mean of what
+    a row sees, and no NaN out of what it does not. Few rows, many, and many with their tokens split."""
+    length = old + n
+    total = -(-length // 16) + 1
+    cache = random_cache(total, 2, 16, d, 7)
+    cache.k_scales[::2] = 87
+    cache.k[::4] = 0
+    pages, starts = tables([length], 16, total, 3), [0, n]
+    for dtype in ("f16", "bf16"):
+        q = rows(n, 8, d, dtype, 8)
+        smallest = (q.float() * (1e-37 if dtype == "bf16" else 1e-6)).to(q.dtype)
+        for window in (0, 33):
+            for x, scale in ((q, 0.0), (q, -0.2), (q, 1e-30), (smallest, 0.1), (smallest, 0.0), (torch.zeros_like(q), 0.1)):
+                check_attention(x, cache, pages, [length], starts, window=window, scale=scale)

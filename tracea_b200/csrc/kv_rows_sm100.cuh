@@ -203,8 +203,10 @@ __global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid
                      make_uint4(pack_halves(v[0] * up, v[1] * up), pack_halves(v[2] * up, v[3] * up), pack_halves(v[4] * up, v[5] * up),
                                 pack_halves(v[6] * up, v[7] * up)));
       }
-      // This thread's row is row lane / kRowsAtOnce of the loads. Not 0: a score of -infinity stays one.
-      const float factor = fmaxf(__shfl_sync(0xffffffffu, back, (lane % kRowsAtOnce) * kRowLanes + lane / kRowsAtOnce) * args.scale_log2, 1.17549435e-38f);
+      // This thread's row is row lane / kRowsAtOnce of the loads. Times a page's scale, 2^-40 or more, it must not vanish: masked scores are
+      // -infinity before that product. Where 2^-86 is more than the row's own factor, scores, which are below 2^17 2^40 times it, move by
+      // less than 2^-29.
+      const float factor = fmaxf(__shfl_sync(0xffffffffu, back, (lane % kRowsAtOnce) * kRowLanes + lane / kRowsAtOnce) * args.scale_log2, 0x1p-86f);
       fence_proxy_async_smem();
       mbar_arrive(bar(kQFull + tile));
 
