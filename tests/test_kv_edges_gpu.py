@@ -1,6 +1,6 @@
 """Heads, the cache and attention on a B200 where single values, rows or warps go their own way: waits that run out for some warps of a
 block and not for others, weights without a norm, scores that
-vanish beside masked ones."""
+vanish beside masked ones, rows that are not finite and see nothing."""
 import pytest
 import torch
 
@@ -92,3 +92,28 @@ def test_scores_that_vanish_and_masks(n, old, d):
         for window in (0, 33):
             for x, scale in ((q, 0.0), (q, -0.2), (q, 1e-30), (smallest, 0.1), (smallest, 0.0), (torch.zeros_like(q), 0.1)):
                 check_attention(x, cache, pages, [length], starts, window=window, scale=scale)
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("n", [1, 90, 300])
+def test_rows_of_anything_that_see_no_page_are_zero(n, value):
+    """Pages that are not there, under rows that are not finite (what a padded batch may hold): 0, in every form; NaN where there is one."""
+    size, d = 16, 64
+    cache = random_cache(300, 2, size, d, 9)
+    cache.k[7] = 1.0
+    width = 400
+    pages = [[-1] * width, [-1, 3] + [300] * (width - 2), [-1] * width]
+    pages[2][250] = 7
+    lengths, starts = [n + 5, 2 * size + n, 300 * size], [0, n, 2 * n, 3 * n]
+    for dtype in ("f16", "bf16"):
+        q = rows(3 * n, 4, d, dtype, 2)
+        q[:, 1] = value
+        q[:, 3, 5] = value
+        got = ops.kv_attention(q, cache, ints(pages), ints(lengths), ints(starts))
+        assert not got[:n].any()
+        clean = torch.nan_to_num(q, nan=0.0, posinf=0.0)
+        check_attention(clean[:, ::2], cache, pages, lengths, starts, got=got[:, ::2])
+        if value != value:
+            assert torch.isnan(got[n:, 1::2]).all()
+        near = ops.kv_attention(q, cache, ints(pages), ints(lengths), ints(starts), window=size)
+        assert not near[:n].any() and not near[n + size:2 * n].any() and not near[2 * n:].any()

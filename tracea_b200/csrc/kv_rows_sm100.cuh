@@ -65,6 +65,20 @@ __device__ __forceinline__ bool rows_item(const KvAttentionArgs& a, int index, R
   return true;
 }
 
+// Whether a row, token `token` of its sequence's in this call, sees a page that is there; `kept`, in shared memory: the sequence, the
+// position of its first row, and the tokens that the CTA looks at, from .. to.
+__device__ __forceinline__ bool sees_a_page(const KvAttentionArgs& args, uint32_t kept_at, int token) {
+  const float4 kept = ptx::ld_shared_f4(kept_at);
+  const int p = __float_as_int(kept.y) + token, shift = args.cache.page_shift;
+  const int end = args.causal ? min(__float_as_int(kept.w), p + 1) : __float_as_int(kept.w);
+  bool sees = false;
+  for (int t = max(__float_as_int(kept.z), args.window > 0 ? p - args.window + 1 : 0); t < end && !sees; t = ((t >> shift) + 1) << shift) {
+    const int id = args.seqs.table[__float_as_int(kept.x) * args.seqs.table_stride + (t >> shift)];
+    sees = id >= 0 && id < args.cache.pages;
+  }
+  return sees;
+}
+
 // [q of tile 0, of tile 1][keys, 2 stages][values, 2 stages][scales][barriers]: operands as blocks of 64 columns, 128 rows of 128
 // bytes each, swizzled.
 template <typename T, int kD>
@@ -132,6 +146,7 @@ __global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid
     mbar_init(bar(kDrain), 1);
     mbar_init(bar(kDrain + 1), 1);
     *abort_p = 0u;
+    st_shared_v4(bars + 8 * 26, make_uint4(at.sequence, begin, step_lo * kKvRowsTokens, min(see_hi, (step_lo + steps) * kKvRowsTokens)));
     fence_mbar_init();
   }
   __syncthreads();
@@ -311,6 +326,10 @@ __global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid
       if (ok && steps > 0) wait_scores(2 * steps + 1);               // the last product is complete
       if (ok) {
         tc_fence_after();
+        // A row of q that is not finite takes NaN from pages that are not there, too, whose scores no mask hides; it is NaN only if it sees
+        // a token. (m is -infinity as long as all scores are NaN or of such pages. What this takes waits in shared memory: no register is
+        // left for it.)
+        if (live && m == -INFINITY && l != l && !sees_a_page(args, bars + 8 * 26, token)) l = 0.0f;
         const bool whole = call.splits == 1;
         const float inv = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
         T* const op = static_cast<T*>(args.out) + static_cast<long long>(at.first_row + token) * args.out_token + q_head * args.out_head;
