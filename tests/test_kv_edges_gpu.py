@@ -1,6 +1,6 @@
 """Heads, the cache and attention on a B200 where single values, rows or warps go their own way: waits that run out for some warps of a
-block and not for others, weights without a norm, scores that
-vanish beside masked ones, rows that are not finite and see nothing."""
+block and not for others, weights without a norm, scores that vanish beside masked ones, rows that are not finite and see nothing,
+values that are not finite beside columns that are copied."""
 import pytest
 import torch
 
@@ -117,3 +117,33 @@ def test_rows_of_anything_that_see_no_page_are_zero(n, value):
             assert torch.isnan(got[n:, 1::2]).all()
         near = ops.kv_attention(q, cache, ints(pages), ints(lengths), ints(starts), window=size)
         assert not near[:n].any() and not near[n + size:2 * n].any() and not near[2 * n:].any()
+
+
+def same(got, y, err):
+    """As assert_near, element by element where the formula gives no finite value."""
+    assert torch.equal(torch.isnan(got), torch.isnan(y))
+    assert torch.equal(torch.isinf(got), torch.isinf(y)) and torch.equal(got[torch.isinf(got)].double(), y[torch.isinf(y)])
+    finite = torch.isfinite(y)
+    assert_near(got[finite], y[finite], err[finite])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d, rotated", [(64, 32), (64, 0), (128, 128), (72, 40), (250, 0), (80, 16), (96, 2)])
+def test_columns_that_are_not_rotated_keep_to_themselves(d, rotated, dtype):
+    q, k, _ = make(40, 2, 1, d, dtype, 12)
+    positions = torch.arange(40, dtype=torch.int32).cuda() + 1
+    freq = ops.rotary_frequencies(rotated, device="cuda") if rotated else None
+    for i in range(40):
+        q[i, i % 2, (7 * i) % d] = (float("nan"), float("inf"), -float("inf"))[i % 3]
+        k[i, 0, d - 1 - i] = (float("inf"), float("nan"))[i % 2]
+    w = weights(d, torch.float32, 5)
+    for interleaved in (False, True):
+        for qw, kw in ((None, None), w):
+            got = ops.head_norm_rotate(q, k, positions, freq, interleaved, qw, kw, kind="none")
+            for x, y, weight in zip((q, k), got, (qw, kw)):
+                same(y, *kvref.rotate(x if weight is None else x.double() * weight.double(), positions, freq, interleaved))
+    if d % 16 == 0:
+        cache = ops.KvCache.empty(10, 1, min(d, 128), 16)
+        got = ops.kv_append(cache, k.nan_to_num(0.0, 0.0, 0.0), k.nan_to_num(0.0, 0.0, 0.0), ints([list(range(10))]), ints([41]), ints([0, 40]),
+                            freq, q=q)
+        same(got, *kvref.rotate(q, positions, freq))

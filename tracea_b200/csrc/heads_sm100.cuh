@@ -279,7 +279,8 @@ __device__ __forceinline__ void head_turns(const HeadLane<kLanes, kScalarPairs>&
     }
   }
 }
-// Weights and rotation together, for rows of one token: (x, y) -> factor (x xx + y xy, y yy + x yx), two pairs at a time.
+// Weights and rotation together, for rows of one token: (x, y) -> factor (x xx + y xy, y yy + x yx), two pairs at a time. Columns that are
+// not rotated are only multiplied: 0 times a partner that is not finite would be NaN.
 template <int kPairs>
 struct HeadTurn {
   uint64_t xx[kPairs / 2], xy[kPairs / 2], yy[kPairs / 2], yx[kPairs / 2];
@@ -293,13 +294,34 @@ struct HeadTurn {
       yx[i] = pack_f32x2(wx[a] * s[a], wx[b] * s[b]);
     }
   }
-  __device__ __forceinline__ void apply(float (&x)[kPairs], float (&y)[kPairs], float factor) const {
+  // pairs: those of the whole rotation
+  template <typename Lane>
+  __device__ __forceinline__ void apply(const Lane& l, int pairs, float (&x)[kPairs], float (&y)[kPairs], float factor) const {
     const uint64_t f = pack_f32x2(factor, factor);
 #pragma unroll
     for (int i = 0; i < kPairs / 2; ++i) {
       const uint64_t u = mul_f32x2(pack_f32x2(x[2 * i], x[2 * i + 1]), f), v = mul_f32x2(pack_f32x2(y[2 * i], y[2 * i + 1]), f);
-      unpack_f32x2(fma_f32x2(v, xy[i], mul_f32x2(u, xx[i])), x[2 * i], x[2 * i + 1]);
-      unpack_f32x2(fma_f32x2(u, yx[i], mul_f32x2(v, yy[i])), y[2 * i], y[2 * i + 1]);
+      uint64_t a = mul_f32x2(u, xx[i]), b = mul_f32x2(v, yy[i]);
+      if constexpr (Lane::kVec) {
+        if (l.turned) {
+          a = fma_f32x2(v, xy[i], a);
+          b = fma_f32x2(u, yx[i], b);
+        }
+        unpack_f32x2(a, x[2 * i], x[2 * i + 1]);
+        unpack_f32x2(b, y[2 * i], y[2 * i + 1]);
+      } else {
+        float p[4], q[4];                                    // multiplied only, rotated
+        unpack_f32x2(a, p[0], p[1]);
+        unpack_f32x2(b, p[2], p[3]);
+        unpack_f32x2(fma_f32x2(v, xy[i], a), q[0], q[1]);
+        unpack_f32x2(fma_f32x2(u, yx[i], b), q[2], q[3]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const bool turned = l.angle + 32 * (2 * i + j) < pairs;
+          x[2 * i + j] = turned ? q[j] : p[j];
+          y[2 * i + j] = turned ? q[2 + j] : p[2 + j];
+        }
+      }
     }
   }
 };
@@ -384,7 +406,7 @@ __global__ void __launch_bounds__(kHeadThreads, 3) head_rotate_kernel(const __gr
       for (int u = 0; u < kAhead; ++u) {
         float x[kPairs], y[kPairs];
         raw[u].template values<kNeighbours>(l, x, y);
-        turn.apply(x, y, args.norm ? head_norm(l, x, y, inv_columns, args.eps) : 1.0f);
+        turn.apply(l, args.rot.pairs, x, y, args.norm ? head_norm(l, x, y, inv_columns, args.eps) : 1.0f);
         if (here[u]) head_store<kNeighbours>(dst + u * y_step, l, x, y);
       }
       src += kAhead * x_step;
@@ -731,7 +753,7 @@ __global__ void __launch_bounds__(kHeadThreads, kLanes > 0 && kRows <= 2 ? 2 : 1
       for (int u = 0; u < kAhead; ++u) {
         float x[kPairs], y[kPairs];
         raw[u].template values<kNeighbours>(l, x, y);
-        turn.apply(x, y, args.norm ? head_norm(l, x, y, inv_columns, args.eps) : 1.0f);
+        turn.apply(l, args.rot.pairs, x, y, args.norm ? head_norm(l, x, y, inv_columns, args.eps) : 1.0f);
         if (h + u < mine) head_store<kNeighbours>(dst + u * args.q.y_head, l, x, y);
       }
       src += kAhead * args.q.x_head;
