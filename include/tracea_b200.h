@@ -362,8 +362,8 @@ typedef struct {
  * gets tokens gets the scale that reaches its largest value, the smallest 2^e with |values| <= 448 * 2^e, -40 <= e <= 40 -- or keeps the
  * one it has, if that is larger and the block holds older tokens; where theirs grows, they are rounded to it. Elements are rounded to
  * nearest, ties to even, and saturate. A token whose key or value in a head is not finite becomes a NaN key and a zero value there, and
- * counts for no scale. Rows of a page behind the sequence's last token are left as they are. q, if given ([rows, a multiple of heads, D]),
- * is normalised and rotated into q->y in the same launch, and so are the rows whose page is not there. */
+ * counts for no scale. Rows of a page behind the sequence's last token are left as they are. q, if given ([rows, a multiple of heads, up
+ * to 2^23 of them, D]), is normalised and rotated into q->y in the same launch, and so are the rows whose page is not there. */
 TraceaStatus tracea_kv_append(TraceaKvCache cache, TraceaSequences sequences, TraceaTensorView k, TraceaTensorView v,
                               const TraceaTensorView *k_weight, const TraceaHeads *q, TraceaNormKind kind, float eps,
                               const TraceaRotation *rotation, void *stream);

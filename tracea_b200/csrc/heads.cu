@@ -123,6 +123,7 @@ void kv_append_checked(const TraceaKvCache& cache, const TraceaSequences& seqs, 
     check_like(y, "the output", x, "q");
     if (y.heads != x.heads) TB_FAIL(TRACEA_INVALID_PARAMS, "the output has %lld heads, q has %lld", y.heads, x.heads);
     if (x.heads % k.heads != 0) TB_FAIL(TRACEA_INVALID_PARAMS, "%lld heads of q are no multiple of the %lld of k", x.heads, k.heads);
+    if (x.heads > tb200::kCacheMostQueryHeads) TB_FAIL(TRACEA_UNSUPPORTED_CONFIG, "%lld heads of q: up to %lld", x.heads, tb200::kCacheMostQueryHeads);
     check_heads_output(y, "the output");
     w = load_head_weight(q->weight, "q_weight", dev, k.cols, k.dtype, f32);
     a.q = load_head_rows(x, &y, w, f32);

@@ -22,6 +22,7 @@ constexpr int kHeadMaxColumns = 256;
 constexpr int kCacheMaxColumns = 128;
 constexpr int kCacheMaxPage = 128;
 constexpr int kMaxTokens = 1 << 30;        // of a sequence
+constexpr long long kCacheMostQueryHeads = 1 << 23;   // times the rows of a page: 2^30, which kv_append_kernel counts in 32 bits
 constexpr int kCacheMinExponent = -40, kCacheMaxExponent = 40;
 
 struct Rotation {
