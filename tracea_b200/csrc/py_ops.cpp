@@ -70,6 +70,12 @@ long int_arg(PyObject* o) {
   return v;
 }
 
+bool bool_arg(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw PyError{};
+  return v != 0;
+}
+
 // Raises tracea_b200.ffi.TraceaError(status, last error text, entry).
 [[noreturn]] void raise_status(TraceaStatus st, const char* entry) {
   char text[1024];
@@ -131,7 +137,7 @@ PyObject* py_conv2d(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     const at::Tensor &x = tensor_arg(a[0], "x"), &w = tensor_arg(a[1], "w"), &out = tensor_arg(a[4], "out");
     const at::Tensor *bias = optional_tensor(a[2], "bias"), *res = optional_tensor(a[3], "residual");
-    const int* order = PyObject_IsTrue(a[5]) ? kChannelsLast : nullptr;
+    const int* order = bool_arg(a[5]) ? kChannelsLast : nullptr;
     if (order != nullptr && (x.dim() != 4 || w.dim() != 4 || out.dim() != 4 || (res != nullptr && res->dim() != 4))) {
       PyErr_SetString(PyExc_ValueError, "x, w, residual and out must have four dimensions");
       throw PyError{};
@@ -388,7 +394,7 @@ PyObject* py_block_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
       const TraceaStatus st = without_gil([&] { return tracea_block_norm(vx.v, &args.norm, y, y_mx, stream); });
       if (st != TRACEA_SUCCESS) raise_status(st, "tracea_block_norm");
     };
-    if (PyObject_IsTrue(a[7])) {
+    if (bool_arg(a[7])) {
       NewMx out(x.size(0), x.size(1), x);
       call(nullptr, &out.m);
       return out.release();
@@ -509,7 +515,7 @@ PyObject* py_head_norm_rotate(PyObject*, PyObject* const* a, Py_ssize_t n) {
     c10::optional<HeadsArg> hq, hk;
     if (q != nullptr) hq.emplace(*q, a[5], "q", "q_weight");
     if (k != nullptr) hk.emplace(*k, a[6], "k", "k_weight");
-    const RotationArg rot(a[3], PyObject_IsTrue(a[4]), first);
+    const RotationArg rot(a[3], bool_arg(a[4]), first);
     View vp;
     const TraceaTensorView* pp = opt(pos, vp);
     const auto kind = static_cast<TraceaNormKind>(int_arg(a[7]));
@@ -588,7 +594,7 @@ PyObject* py_kv_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const TraceaTensorView* pw = opt(optional_tensor(a[9], "k_weight"), vw);
     c10::optional<HeadsArg> hq;
     if (q != nullptr) hq.emplace(*q, a[11], "q", "q_weight");
-    const RotationArg rot(a[12], PyObject_IsTrue(a[13]), k);
+    const RotationArg rot(a[12], bool_arg(a[13]), k);
     const auto kind = static_cast<TraceaNormKind>(int_arg(a[14]));
     const float eps = float_arg(a[15]);
     void* stream = stream_of(k);
@@ -610,7 +616,7 @@ PyObject* py_kv_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const SequencesArg seqs(a + 5);
     TraceaKvAttentionParams p;
     p.scale = float_arg(a[8]);
-    p.causal = PyObject_IsTrue(a[9]) ? 1 : 0;
+    p.causal = bool_arg(a[9]) ? 1 : 0;
     const long window = int_arg(a[10]);
     if (window < 0 || window > 0x7fffffffL) {
       PyErr_SetString(PyExc_ValueError, "window must be 0 (none) or a number of tokens");
