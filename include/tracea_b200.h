@@ -371,7 +371,10 @@ TraceaStatus tracea_kv_append(TraceaKvCache cache, TraceaSequences sequences, Tr
 /* out = softmax(scale * q k^T) v over the tokens of the cache that each row sees: those of its sequence, if `causal` up to its own
  * position, if window > 0 none more than window - 1 positions in front of its own. q and out: [rows, H, D],
  * FLOAT16 or BFLOAT16, H a multiple of the cache's heads, which H / heads consecutive ones share. A row that sees nothing becomes 0;
- * one that sees a NaN key, NaN (values of the cache hold none). Scores, maxima, sums and the result are held in fp32; the weights of the values are rounded to 11 bits. */
+ * one that sees a NaN key, NaN (values of the cache hold none). Scores, maxima, sums and the result are held in fp32. Two factors are
+ * rounded to halves: elements of q, where they are below 2^-14 of their row's largest, by up to 2^-25 of that; and a token's weight times
+ * its values' scale to 11 bits, or by up to 2^-32 of the row's largest such product, so that what a page adds whose products are all
+ * smaller than that is lost. */
 typedef struct {
   float scale;
   int32_t causal;

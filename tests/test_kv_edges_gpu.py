@@ -1,6 +1,6 @@
 """Heads, the cache and attention on a B200 where single values, rows or warps go their own way: waits that run out for some warps of a
 block and not for others, weights without a norm, scores that vanish beside masked ones, rows that are not finite and see nothing,
-values that are not finite beside columns that are copied."""
+values that are not finite beside columns that are copied, small weights beside large ones."""
 import pytest
 import torch
 
@@ -147,3 +147,28 @@ def test_columns_that_are_not_rotated_keep_to_themselves(d, rotated, dtype):
         got = ops.kv_append(cache, k.nan_to_num(0.0, 0.0, 0.0), k.nan_to_num(0.0, 0.0, 0.0), ints([list(range(10))]), ints([41]), ints([0, 40]),
                             freq, q=q)
         same(got, *kvref.rotate(q, positions, freq))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("n, d", [(1, 64), (3, 128), (100, 64), (100, 128)])
+def test_small_weights_count(n, d, dtype):
+    """Weights of 2^-24.5 beside largest ones whose values are 0: as halves that reach no lower than 2^-24 they would be off by a third.
+    Bound: 2^-11 of a weight's rounding, 2^-20 of exponential and sums, twice a score's 24.5 times 8 half steps of 2^-24 (q, scale and
+    key are exact but for the scale's own rounding and its product with log2 e); and 2^-32 of the largest weight for each token."""
+    size, length = 64, 8192
+    cache = ops.KvCache.empty(length // size, 1, d, size)
+    cache.k_scales.fill_(127)
+    cache.v_scales.fill_(127)
+    one = torch.tensor(1.0, device="cuda").to(torch.float8_e4m3fn).view(torch.uint8)
+    k, v = cache.k.view(torch.uint8), cache.v.view(torch.uint8)
+    k[..., 3] = one | 128
+    v.fill_(int(one))
+    k[:, :, ::16], v[:, :, ::16] = 0, 0
+    q = torch.zeros(n, 2, d, dtype=DT[dtype], device="cuda")
+    q[:, :, 3] = 24.5
+    got = ops.kv_attention(q, cache, ints([list(range(length // size))]), ints([length]), ints([0, n]), scale=0.6931471805599453, causal=False)
+    low = length * 15 / 16 * 2.0 ** -24.5
+    want = low / (length / 16 + low)
+    bound = (2.0 ** -11 + 2.0 ** -20 + 2 * 24.5 * 2.0 ** -21) * want + 2.0 ** -32 * length * 15 / 16 / (length / 16)
+    f = torch.finfo(got.dtype)
+    assert float((got.double() - want).abs().max()) <= bound + f.eps / 2 * (want + bound) + f.smallest_normal * f.eps
