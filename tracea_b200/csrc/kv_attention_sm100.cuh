@@ -2,7 +2,8 @@
 //
 // One maximum serves the softmax and the values' scales: with s the score in powers of two and m >= s + ev for all tokens so far, up to
 // a slack, the weights 2^(s + ev - m) need no scaling of v^ and fit halves, whatever the pages' scales are; the softmax's denominator
-// is the sum of 2^(s + ev - m) 2^-ev. Since |ev| <= 40, neither can leave the range of fp32. The slack: m moves only when a score
+// is the sum of 2^(s + ev - m) 2^-ev. Since |ev| <= 40, neither can leave the range of fp32. The weights are halves because the matrix
+// instructions take 16 bits of both operands; the denominator is summed from them before they are rounded. The slack: m moves only when a score
 // passes it by 2^kSlack, so the sums are rescaled a few times a sequence and not every step.
 #pragma once
 #include "heads_sm100.cuh"

@@ -6,20 +6,21 @@
 //   S = q k^^T   128 x 128, q and k^ from shared memory        O += P v^   128 x D, P from tensor memory, v^ from shared memory
 //
 // 4 rows tokens D operations, and an exponential for every row and token, of which an SM does 16 a cycle: two tiles of 128 tokens take
-// 2048 cycles of either at D = 128. What holds both up is shared memory: of its 128 bytes a cycle the operands of the products take 192 KB
-// a step and the widened keys and values 64 KB, 2048 cycles as well. So everything has to run beside everything else: the tiles alternate,
-// each with a warp of its own that issues its products; the elements of the cache are widened from e4m3 to halves, exactly, by warps of
-// their own, once for both tiles, whose loads are a step ahead; a row of q, scaled into halves on the way in, is a thread's. The weights P
-// lie over the scores' columns, as halves. The pages' scales are applied to scores and weights (kv_attention_sm100.cuh).
+// 2048 cycles of either at D = 128. What holds both up is shared memory: of its 128 bytes a cycle the operands of the products take 256 KB
+// a step (128 of q, which every 64 tokens' scores read anew, 64 of keys and 64 of values) and the widened keys and values 64 KB, 2560
+// cycles. So everything has to run beside everything else: the tiles alternate, each with a warp of its own that issues its products; the
+// elements of the cache are widened from e4m3 to halves, exactly, by warps of their own, once for both tiles, whose loads are a step ahead;
+// a row of q, scaled into halves on the way in, is a thread's. The weights P lie over the scores' columns, as halves. The pages' scales are
+// applied to scores and weights (kv_attention_sm100.cuh).
 //
 // Tensor memory, all 512 columns: 128 of results a tile, and 128 of scores, as two buffers for 64 tokens each. A softmax goes from one
 // buffer to the other: while it works on 64 tokens, the product of the 64 in front is formed and then the scores of the next but one, over
 // these weights.
 //
-// A prompt of 8192 tokens, 32 heads to 8, D = 128: 530 us, 1.04 PFLOP/s (what the mask leaves counted), and 570 once power is short; 395
-// without a softmax, of which 75 are the CTAs' beginnings and ends; the widening costs nothing beside it. Blocks that take over the work
-// of those not launched yet, with q of the next in before the results of the last go out, were slower (560 -> 588): the softmax's
-// registers no longer held what it needs.
+// A prompt of 8192 tokens, 32 heads to 8, D = 128: 548 us in a row on the same inputs, 1.0 PFLOP/s (what the mask leaves counted), and
+// 575 - 590 on others each time; 395 without a softmax, of which 75 are the CTAs' beginnings and ends; the widening costs nothing beside
+// it. Blocks that take over the work of those not launched yet, with q of the next in before the results of the last go out, were slower
+// (560 -> 588): the softmax's registers no longer held what it needs.
 #pragma once
 #include "kv_attention_sm100.cuh"
 
