@@ -1,6 +1,7 @@
 """Heads, the cache and attention on a B200 where single values, rows or warps go their own way: waits that run out for some warps of a
 block and not for others, weights without a norm, scores that vanish beside masked ones, rows that are not finite and see nothing,
-values that are not finite beside columns that are copied, small weights beside large ones."""
+values that are not finite beside columns that are copied, small weights beside large ones, scores of
+any size."""
 import pytest
 import torch
 
@@ -172,3 +173,46 @@ def test_small_weights_count(n, d, dtype):
     bound = (2.0 ** -11 + 2.0 ** -20 + 2 * 24.5 * 2.0 ** -21) * want + 2.0 ** -32 * length * 15 / 16 / (length / 16)
     f = torch.finfo(got.dtype)
     assert float((got.double() - want).abs().max()) <= bound + f.eps / 2 * (want + bound) + f.smallest_normal * f.eps
+
+
+@pytest.mark.parametrize("n, length", [(1, 300), (1, 4096), (2, 30000), (3, 700), (200, 300), (100, 6000), (600, 600)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_scores_of_any_size(n, length, d):
+    """Values that are all 1: whatever the scores, every row's result is 1, a weighted mean. Weights in halves are off by 2^-11 at most,
+    the denominator, of as many exponentials in fp32, by less, the result's rounding by half a step."""
+    size = 64
+    total = -(-length // size)
+    cache = random_cache(total, 2, size, d, 3, 0.0)
+    cache.v[:] = 1.0
+    cache.v_scales.fill_(127)
+    table = ints([list(range(total))])
+    for dtype in ("f16", "bf16"):
+        q = rows(n, 8, d, dtype, 4)
+        off = 2.0 ** -11 + 2.0 ** -20 + torch.finfo(q.dtype).eps / 2
+        for e in (0, 10, 18, 20, 21, 22, 24, 26, 28, 30, 34, 40, 60):
+            for sign in (1, -1):
+                got = ops.kv_attention(q, cache, table, ints([length]), ints([0, n]), scale=sign * 2.0 ** e * d ** -0.5)
+                assert float((got.double() - 1).abs().max()) <= off, (dtype, e, sign)
+
+
+@pytest.mark.parametrize("n, length", [(1, 4096), (3, 30000), (100, 4196)])
+@pytest.mark.parametrize("power", [18, 20, 24, 26, 27, 28])
+def test_maxima_a_step_of_fp32_apart(n, length, power):
+    """Scores of 1.5 2^power in 64 tokens and a step of 8 or more, up to 2^5, above that in the 64 behind them, and so on: the larger ones'
+    values are 1, the others' 0. scale log2(e) is 1 in fp32, and all scores, sums and differences are exact."""
+    size, d = 64, 64
+    total = -(-length // size)
+    cache = ops.KvCache.empty(total, 1, d, size)
+    cache.k_scales.fill_(127)
+    cache.v_scales.fill_(127)
+    cache.k[:, :, :, 0] = 1.0
+    cache.k[1::2, :, :, 1] = 1.0
+    cache.v[1::2] = 1.0
+    step = max(8.0, 2.0 ** (power - 23))
+    q = torch.zeros(n, 2, d, dtype=torch.bfloat16, device="cuda")
+    q[:, :, 0], q[:, :, 1] = 1.5 * 2.0 ** power, step
+    got = ops.kv_attention(q, cache, ints([list(range(total))]), ints([length]), ints([0, n]), scale=0.6931471824645996, causal=False)
+    full = 64 * (total // 2) - (64 * total - length if total % 2 == 0 else 0)      # tokens of the larger score
+    less = length - full
+    want = full / (full + less * 2.0 ** -step)
+    assert float((got.double() - want).abs().max()) <= 2.0 ** -11 + 2.0 ** -20 + 2.0 ** -8

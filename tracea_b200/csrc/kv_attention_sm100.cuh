@@ -11,6 +11,9 @@
 namespace tb200 {
 
 constexpr float kSlack = 8.0f;
+// Beyond 2^20 steps of fp32 are no longer small beside 1: there the maximum is taken from a score before anything is added to it, which is
+// exact for scores near it, and follows it without slack, or weights would leave halves. A warp does so for all its rows if one has to.
+constexpr float kFar = 1048576.0f;
 constexpr float kLift = 7.0f;    // the weights are 2^7 times the above, up to 2^15: halves reach 2^16, and lose bits below 2^-14
 
 struct KvAttentionArgs {
@@ -57,6 +60,7 @@ __device__ __forceinline__ void mma_16x8x16(float (&c)[4], const uint32_t (&a)[4
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ bool is_far(float m) { return fabsf(m) >= kFar && m != -INFINITY; }
 // By what sums with the maximum m and the denominator l are taken in where the maximum of all is `top`: 0 for a part that has seen
 // nothing, but for one that has seen nothing but NaN.
 __device__ __forceinline__ float part_factor(float m, float l, float top) {

@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
       const uint32_t s_tmem = tmem + lanes + tile * 128, o_tmem = tmem + lanes + 256 + tile * 128;
       float m = -INFINITY, l = 0.0f;
-      bool ok = true;
+      bool ok = true, far = false;                                   // far: a maximum of the warp's rows is (kFar)
       auto wait_scores = [&](int h) {                                // of half step h; it says too that the product of h - 2 is complete
         ok = mbar_wait_bounded(bar(kSFull + 2 * tile + (h & 1)), (h >> 1) & 1, abort_p, args.wait_limit);
         if (__any_sync(0xffffffffu, !ok)) {
@@ -274,10 +274,11 @@ __global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid
           for (int i = 1; i + 1 < 16; i += 2) gm = max_3(gm, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
           gm = fmaxf(gm, __uint_as_float(v[15]));
           const float4 sc = scales[g];
-          top = fmaxf(top, gm * (factor * sc.x) + sc.y);
+          top = fmaxf(top, fmaf(gm, factor * sc.x, sc.y));
         }
-        if (__any_sync(0xffffffffu, top > m + kSlack)) {
+        if (far || __any_sync(0xffffffffu, top > m + kSlack)) {
           const float next = fmaxf(m, top);
+          far = __any_sync(0xffffffffu, is_far(next));
           const float shrink = next == m ? 1.0f : exp2_ftz(m - next);
           m = next;
           l *= shrink;
@@ -294,31 +295,40 @@ __global__ void __launch_bounds__(kKvRowsThreads, 1) kv_rows_kernel(const __grid
             }
           }
         }
-        const float base = m == -INFINITY ? 0.0f : m - kLift;        // a row that has seen nothing
+        auto weights = [&](auto is_far_form) {
+          constexpr bool kFarForm = decltype(is_far_form)::value;
+          const float base = m == -INFINITY ? 0.0f : kFarForm ? m : m - kLift;         // 0: a row that has seen nothing
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t p[16];
+          for (int c = 0; c < 2; ++c) {
+            uint32_t p[16];
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const float4 sc = scales[2 * c + g];
-            const float mul = factor * sc.x, add = sc.y - base;
-            const uint64_t mul2 = pack_f32x2(mul, mul), add2 = pack_f32x2(add, add);
-            uint64_t sum = 0;
+            for (int g = 0; g < 2; ++g) {
+              const float4 sc = scales[2 * c + g];
+              const float mul = factor * sc.x, add = kFarForm ? sc.y : sc.y - base;
+              const uint64_t mul2 = pack_f32x2(mul, mul), add2 = pack_f32x2(add, add);
+              uint64_t sum = 0;
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) {
+              for (int i = 0; i < 16; i += 2) {
+                float x, y;
+                unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[c][16 * g + i]), __uint_as_float(s[c][16 * g + i + 1])), mul2, add2), x, y);
+                if constexpr (kFarForm) {        // the score, then what it is from the maximum, then the lift
+                  x = x - base + kLift;
+                  y = y - base + kLift;
+                }
+                x = exp2_ftz(x);
+                y = exp2_ftz(y);
+                sum = add_f32x2(sum, pack_f32x2(x, y));
+                p[8 * g + i / 2] = pack_halves(x, y);
+              }
               float x, y;
-              unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[c][16 * g + i]), __uint_as_float(s[c][16 * g + i + 1])), mul2, add2), x, y);
-              x = exp2_ftz(x);
-              y = exp2_ftz(y);
-              sum = add_f32x2(sum, pack_f32x2(x, y));
-              p[8 * g + i / 2] = pack_halves(x, y);
+              unpack_f32x2(sum, x, y);
+              l += (x + y) * sc.z;
             }
-            float x, y;
-            unpack_f32x2(sum, x, y);
-            l += (x + y) * sc.z;
+            tmem_st_32x16(buffer + 16 * c, p);
           }
-          tmem_st_32x16(buffer + 16 * c, p);
-        }
+        };
+        if (far) weights(std::true_type{});
+        else weights(std::false_type{});
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(bar(kPFull + 2 * tile + (h & 1)));

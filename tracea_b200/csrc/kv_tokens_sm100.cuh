@@ -221,6 +221,7 @@ __global__ void __launch_bounds__(kKvTokenThreads, kv_token_ctas(kRows)) kv_toke
     int pos[kN][2];
     uint32_t qb[kN][kSegments][4][2];
     float m[kN][2], l[kN][2], o[kN][kTilesV][4];
+    bool far = false;                            // a maximum of the warp's rows is (kFar)
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
       m[n][0] = m[n][1] = -INFINITY;
@@ -384,12 +385,13 @@ __global__ void __launch_bounds__(kKvTokenThreads, kv_token_ctas(kRows)) kv_toke
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[n][i] = s[n][i] * (factor[n][i & 1] * k_scale) + ev;
         }
-        bool grown = false;
+        bool grown = far;
 #pragma unroll
         for (int n = 0; n < kN; ++n)
 #pragma unroll
           for (int j = 0; j < 2; ++j) grown = grown || fmaxf(s[n][j], s[n][2 + j]) > m[n][j] + kSlack;
         if (__any_sync(0xffffffffu, grown)) {
+          bool mine = false;
 #pragma unroll
           for (int n = 0; n < kN; ++n)
 #pragma unroll
@@ -399,6 +401,7 @@ __global__ void __launch_bounds__(kKvTokenThreads, kv_token_ctas(kRows)) kv_toke
               for (int x = 4; x < 32; x <<= 1) p = fmaxf(p, __shfl_xor_sync(0xffffffffu, p, x));
               const float shrink = p == m[n][j] ? 1.0f : exp2_ftz(m[n][j] - p);
               m[n][j] = p;
+              mine = mine || is_far(p);
               l[n][j] *= shrink;
 #pragma unroll
               for (int v = 0; v < kTilesV; ++v) {
@@ -406,6 +409,13 @@ __global__ void __launch_bounds__(kKvTokenThreads, kv_token_ctas(kRows)) kv_toke
                 o[n][v][2 + j] *= shrink;
               }
             }
+          far = __any_sync(0xffffffffu, mine);
+        }
+        if (far) {
+#pragma unroll
+          for (int n = 0; n < kN; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[n][i] = m[n][i & 1] == -INFINITY ? s[n][i] : s[n][i] - m[n][i & 1] + kLift;
         }
         const float unscale = power_of_two(127 - static_cast<int>(scales >> 8));
         uint32_t pb[kN][2];
@@ -413,7 +423,7 @@ __global__ void __launch_bounds__(kKvTokenThreads, kv_token_ctas(kRows)) kv_toke
         for (int n = 0; n < kN; ++n) {
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const float base = m[n][j] == -INFINITY ? 0.0f : m[n][j] - kLift;      // a row that has seen nothing
+            const float base = m[n][j] == -INFINITY || far ? 0.0f : m[n][j] - kLift;      // 0: a row that has seen nothing, or see above
             s[n][j] = exp2_ftz(s[n][j] - base);
             s[n][2 + j] = exp2_ftz(s[n][2 + j] - base);
             l[n][j] += (s[n][j] + s[n][2 + j]) * unscale;
