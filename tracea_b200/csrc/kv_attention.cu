@@ -29,7 +29,7 @@ void launch_tokens(tb200::KvTokensArgs& c, DeviceState& st, int dev, cudaStream_
   // sequence over every SM. us, cluster / line, for sequences x tokens (8 heads of keys, 32 of q, 128 columns): 1 x 300 5.6 / 12.4,
   // 1 x 4000 9.3 / 13.4, 1 x 16000 20.7 / 17.5, 16 x 1000 10.7 / 17.4, 16 x 4000 27 / 33, 64 x 1000 27 / 35, 64 x 0..8191 90 / 95,
   // 2 x 131000 208 / 84. All with tables that just fit: the lengths are on the device, and a table for 131072 tokens, as a captured step may
-  // want, takes the line for all of them (1 x 300 12.3, 64 x 1000 35), one for 16384 splits 64 x 1000 over clusters of eight (63).
+  // want, takes the line for all of them (1 x 300 12.6, 64 x 1000 35), one for 16384 splits 64 x 1000 over clusters of eight (64).
   int splits = 1;
   while (splits < 8 && splits * 16LL * tb200::kKvTokenWarps < most && (pairs * splits * 2 <= slots || most > 2048LL * splits)) splits *= 2;
   const bool shared = most <= (2 * pairs * splits >= slots ? 2048LL : 1024LL) * splits && heads <= 65535;
@@ -73,7 +73,7 @@ void launch_rows(const tb200::KvAttentionArgs& a, long long items, DeviceState& 
   // Few blocks of rows leave SMs idle: their tokens are split, as long as a part has four steps where the sequences are as long as they
   // may be. us, one part / split, 32 heads to 8 of 128 columns: 256 tokens behind 8000 144 / 56, 256 behind 2000 48 / 33, 128 behind
   // 30000 496 / 86; 8 heads to 2, 500 behind 4000 82 / 34. With a table that just fits; a wider one splits short prompts as well (500 tokens
-  // 18.3 -> 29.8).
+  // 18.7 -> 30.1).
   long long most = static_cast<long long>(a.seqs.table_width) << a.cache.page_shift;
   if (a.window > 0) most = std::min<long long>(most, a.window + static_cast<long long>(tb200::kKvRowsOfCta));
   const long long blocks = items * a.cache.heads;

@@ -17,8 +17,8 @@
 // buffer to the other: while it works on 64 tokens, the product of the 64 in front is formed and then the scores of the next but one, over
 // these weights.
 //
-// A prompt of 8192 tokens, 32 heads to 8, D = 128: 548 us in a row on the same inputs, 1.0 PFLOP/s (what the mask leaves counted), and
-// 575 - 590 on others each time; 395 without a softmax, of which 75 are the CTAs' beginnings and ends; the widening costs nothing beside
+// A prompt of 8192 tokens, 32 heads to 8, D = 128: 561 us in a row on the same inputs, 0.98 PFLOP/s (what the mask leaves counted), and
+// 590 - 597 on others each time; 395 without a softmax, of which 75 are the CTAs' beginnings and ends; the widening costs nothing beside
 // it. Blocks that take over the work of those not launched yet, with q of the next in before the results of the last go out, were slower
 // (560 -> 588): the softmax's registers no longer held what it needs.
 #pragma once

@@ -9,8 +9,8 @@
 // 512 consecutive bytes each: copies by the lanes of what each multiplies, 64 bytes of eight rows, stop at 4.9 TB/s where these reach
 // 6.7. In shared memory the 16-byte columns of a row are exchanged so that no two lanes meet on a bank (see below). Several CTAs of four
 // warps share an SM, so that one's first loads, each of which waits for the one in front of it -- the lengths, the places of the pages,
-// the pages -- and its sums' meeting lie beside the others' work. 64 sequences of 0 - 8191 tokens, 32 heads to 8 of 128: 90 - 96 us, 5.2 TB/s;
-// 2 of 105000: 84 - 87 us, of which 14 are the line's set-up (below), its join and the launch of that.
+// the pages -- and its sums' meeting lie beside the others' work. 64 sequences of 0 - 8191 tokens, 32 heads to 8 of 128: 92 - 96 us, 5.2 TB/s;
+// 2 of 105000: 85 - 87 us, of which 14 are the line's set-up (below), its join and the launch of that.
 //
 // The work is split along the cache in one of two ways:
 //   kShared    the CTAs of a cluster share a sequence and head and add up their sums through shared memory: one launch, for few tokens
